@@ -433,6 +433,85 @@ int wdrz_kv_fill(int dtype, const void* k_src, const void* v_src, const int64_t*
 int wdrz_median_filter(const float* x, int64_t x_stride, float* y, int64_t y_stride, int64_t rows,
                        int64_t N, int width, void* stream);
 
+/*
+ * The slot cache held in 8 bits. Positions are held in blocks of 32; n_blocks = ceil(max_seq / 32).
+ * A block of one (slot, head) is 32 x 64 codes (OCP e4m3) and one scale for its keys and one for its
+ * values: 2^e with e the least whole number of [-100, 100] under which the block's largest finite value
+ * is at most 448; code = round to nearest even of clamp(x 2^-e, -448, 448), what is not finite is NaN.
+ * With a ring (k_ring and v_ring given) only complete blocks are codes, and the newest positions stand as
+ * they came: position p in ring row p % 64, for the last complete block and the one behind it. Reads take
+ * positions below 32 floor(length / 32) from the codes, the rest from the ring. A length may therefore
+ * be set back by up to 32 positions, or to any multiple of 32, without another write. Without a
+ * ring every position is a code (a cache that is filled at once).
+ * No counterpart in the reference, whose caches are 16-bit (FlashKVCache, src/whisperdrz/model.py:98-192).
+ */
+typedef struct wdrz_kv8 {
+  void* k_codes; /* uint8 [n_slots, n_heads, n_blocks * 32, 64], contiguous, as are the others */
+  void* v_codes;
+  float* k_scales; /* [n_slots, n_heads, n_blocks] */
+  float* v_scales;
+  void* k_ring; /* 16-bit [n_slots, n_heads, 64, 64], the calls' dtype; both NULL: no ring */
+  void* v_ring;
+  int64_t n_slots, n_heads, max_seq;
+} wdrz_kv8;
+
+/*
+ * Rows into a cache: k_src / v_src [B, T, n_heads, 64] (16-bit, element strides of b, t, h) to positions
+ * start_pos .. start_pos + T - 1 of slot slot_indices[b] (int64, NULL: slot b). With a ring: an append at
+ * length start_pos, whose block's older positions are taken from the ring. Without: start_pos is a
+ * multiple of 32, and the last block is closed with zeros behind its rows.
+ * Slots outside [0, n_slots) are skipped; of rows that name one slot the last is written.
+ * The counterpart of wdrz_kv_fill.
+ */
+int wdrz_kv8_write(int dtype, const wdrz_kv8* cache, const void* k_src, const int64_t* k_strides,
+                   const void* v_src, const int64_t* v_strides, const int64_t* slot_indices, int64_t B,
+                   int64_t T, int64_t start_pos, void* stream);
+
+/* Workspace (bytes) of wdrz_attn_kvcache8; zeroed and kept as wdrz_attn_kvcache's. */
+size_t wdrz_attn_kvcache8_workspace_size(int64_t B, int64_t sq, int64_t n_heads, int64_t max_seq);
+
+/*
+ * Attention against a slot cache held in 8 bits: the counterpart of wdrz_attn_kvcache.
+ *
+ * q, o: [B, sq, n_heads, 64] of a 16-bit dtype. cache_batch_idx: int32 [B] row -> slot (NULL: identity).
+ * k_new, v_new [B, sq, n_heads, 64] given (a cache with a ring): appended at cache_seqlens[b]; query t
+ *   attends positions j <= cache_seqlens[b] + t, the new rows as they are. The lengths are not
+ *   modified. Rows that name one slot have to name one length too; then the new rows of the last of them
+ *   are appended and attended by all. Rows that do not give NaN, and nothing is appended to their slot.
+ * Both NULL: every query attends the first cache_seqlens[b] positions (NULL: max_seq); none: zeros.
+ * A slot or length out of range gives NaN rows and writes nothing.
+ */
+int wdrz_attn_kvcache8(int dtype, const wdrz_kv8* cache, const void* q, const int64_t* q_strides,
+                       const void* k_new, const int64_t* kn_strides, const void* v_new,
+                       const int64_t* vn_strides, const int32_t* cache_seqlens,
+                       const int32_t* cache_batch_idx, void* o, const int64_t* o_strides, int64_t B,
+                       int64_t sq, float softmax_scale, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/*
+ * A Linear with 4-bit weights: Y = act(X (s Q)^T + b), the counterpart of wdrz_linear.
+ *
+ * x: [M, K] 16-bit rows (stride x_stride); y: [M, N] rows (stride y_stride); bias: [N] or NULL.
+ * Q: whole numbers -7..7; s: a 16-bit scale for each output feature and group of `group` inputs (32,
+ * 64 or 128, K a multiple of it). fp32 accumulation, bias and activation (0 none, 1 GELU), one rounding.
+ * w_packed: [ceil(N / 16)][ceil(K / 128)] tiles of 1024 bytes. In a tile the byte 16 (16 g + n) + 4 s + i
+ *   (n 0..15, g and s and i 0..3) holds feature n's inputs 32 s + 8 g + i (low half) and 32 s + 8 g + 4
+ *   + i (high half), each as sign (bit 3) and magnitude; zeros past N and K.
+ * scales_packed: [ceil(N / 16)][K / group][16] of dtype, zeros past N.
+ * Pointers 16-byte aligned (bias and y 2-byte), x_stride a multiple of 8.
+ */
+int wdrz_linear4(int dtype, const void* x, int64_t x_stride, const void* w_packed,
+                 const void* scales_packed, const void* bias, void* y, int64_t y_stride, int64_t M,
+                 int64_t N, int64_t K, int64_t group, int activation, void* stream);
+
+/*
+ * The same split along K: fp32 partials [n_split][M][N], contiguous, no bias, for
+ * wdrz_add_layernorm_partials; their sum over the first dimension is X (s Q)^T. n_split 2 or 4.
+ */
+int wdrz_linear4_partials(int dtype, const void* x, int64_t x_stride, const void* w_packed,
+                          const void* scales_packed, float* partials, int64_t M, int64_t N, int64_t K,
+                          int64_t group, int n_split, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,15 +9,18 @@ from . import _lib
 from .attention import (
     WorkspaceCache,
     flash_attn_with_kvcache,
+    flash_attn_with_kvcache8,
+    kvcache8_workspace_size,
     kvcache_workspace_size,
     qkv_attention,
     scaled_dot_product_attention,
 )
 from .audio import LogMelSpectrogram, log_mel_spectrogram
-from .decode_ops import (add_layernorm_, add_layernorm_partials_, layer_norm, linear, linear_gelu, linear_partials,
-                         ln_linear, masked_argmax)
+from .decode_ops import (QuantLinear4, add_layernorm_, add_layernorm_partials_, layer_norm, linear, linear4,
+                         linear4_partials, linear_gelu, linear_partials, ln_linear, masked_argmax)
 from .dtw import (compute_attention, dtw_attention_prep, dtw_prep, dtw_prep_batch, dtw_prep_workspace_size,
                   median_filter)
+from .kv_cache import FlashKVCache8
 
 from .debug import check_kvcache_metadata, force_torch, probe
 
@@ -30,11 +33,15 @@ __all__ = [
     "check_kvcache_metadata",
     "force_torch",
     "probe",
+    "FlashKVCache8",
     "LogMelSpectrogram",
+    "QuantLinear4",
     "add_layernorm_",
     "add_layernorm_partials_",
     "layer_norm",
     "linear",
+    "linear4",
+    "linear4_partials",
     "linear_gelu",
     "linear_partials",
     "ln_linear",
@@ -48,6 +55,8 @@ __all__ = [
     "dtw_prep_workspace_size",
     "WorkspaceCache",
     "flash_attn_with_kvcache",
+    "flash_attn_with_kvcache8",
+    "kvcache8_workspace_size",
     "kvcache_workspace_size",
     "qkv_attention",
     "scaled_dot_product_attention",

@@ -50,6 +50,11 @@ EXPORTED_SYMBOLS = (
     "wdrz_dtw_attention_prep",
     "wdrz_kv_fill",
     "wdrz_median_filter",
+    "wdrz_kv8_write",
+    "wdrz_attn_kvcache8_workspace_size",
+    "wdrz_attn_kvcache8",
+    "wdrz_linear4",
+    "wdrz_linear4_partials",
 )
 ABI_VERSION = 1
 
@@ -61,6 +66,13 @@ _i64 = ctypes.c_int64
 _p = ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _i32p = ctypes.c_void_p
+
+
+class Kv8(ctypes.Structure):
+    """``wdrz_kv8``: the buffers and sizes of one 8-bit slot cache."""
+
+    _fields_ = [(n, _p) for n in ("k_codes", "v_codes", "k_scales", "v_scales", "k_ring", "v_ring")] + \
+               [(n, _i64) for n in ("n_slots", "n_heads", "max_seq")]
 
 
 def _declare(lib: ctypes.CDLL) -> None:
@@ -172,6 +184,30 @@ def _declare(lib: ctypes.CDLL) -> None:
 
     lib.wdrz_median_filter.restype = ctypes.c_int
     lib.wdrz_median_filter.argtypes = [_p, _i64, _p, _i64, _i64, _i64, ctypes.c_int, _p]
+    kv8p = ctypes.POINTER(Kv8)
+    lib.wdrz_kv8_write.restype = ctypes.c_int
+    lib.wdrz_kv8_write.argtypes = [
+        ctypes.c_int, kv8p, _p, _i64p, _p, _i64p,  # dtype, cache, k, strides, v, strides
+        _p, _i64, _i64, _i64, _p,  # slot_indices, B, T, start_pos, stream
+    ]
+    lib.wdrz_attn_kvcache8_workspace_size.restype = ctypes.c_size_t
+    lib.wdrz_attn_kvcache8_workspace_size.argtypes = [_i64, _i64, _i64, _i64]
+    lib.wdrz_attn_kvcache8.restype = ctypes.c_int
+    lib.wdrz_attn_kvcache8.argtypes = [
+        ctypes.c_int, kv8p, _p, _i64p, _p, _i64p, _p, _i64p,  # dtype, cache, q, k_new, v_new with strides
+        _i32p, _i32p, _p, _i64p,  # cache_seqlens, cache_batch_idx, out, strides
+        _i64, _i64, ctypes.c_float, _p, ctypes.c_size_t, _p,  # B, sq, softmax_scale, workspace, bytes, stream
+    ]
+    lib.wdrz_linear4.restype = ctypes.c_int
+    lib.wdrz_linear4.argtypes = [
+        ctypes.c_int, _p, _i64, _p, _p, _p,  # dtype, x, x stride, w, scales, bias
+        _p, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, _p,  # y, y stride, M, N, K, group, activation, stream
+    ]
+    lib.wdrz_linear4_partials.restype = ctypes.c_int
+    lib.wdrz_linear4_partials.argtypes = [
+        ctypes.c_int, _p, _i64, _p, _p, _p,  # dtype, x, x stride, w, scales, partials
+        _i64, _i64, _i64, _i64, ctypes.c_int, _p,  # M, N, K, group, n_split, stream
+    ]
 
 
 def load() -> ctypes.CDLL:
@@ -224,6 +260,10 @@ def available() -> bool:
 
 def last_error() -> str:
     return load().wdrz_last_error().decode()
+
+
+def strides3(s) -> ctypes.Array:
+    return (ctypes.c_int64 * 3)(s[0], s[1], s[2])
 
 
 def strides4(s) -> ctypes.Array:

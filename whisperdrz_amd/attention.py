@@ -27,13 +27,16 @@ from . import _lib
 
 __all__ = [
     "flash_attn_with_kvcache",
+    "flash_attn_with_kvcache8",
     "scaled_dot_product_attention",
     "qkv_attention",
     "kvcache_workspace_size",
+    "kvcache8_workspace_size",
     "WorkspaceCache",
 ]
 
 _DTYPES = {torch.float32: _lib.WDRZ_F32, torch.float16: _lib.WDRZ_F16, torch.bfloat16: _lib.WDRZ_BF16}
+_DTYPES16 = {torch.float16: _lib.WDRZ_F16, torch.bfloat16: _lib.WDRZ_BF16}
 HEAD_DIM = 64
 
 
@@ -58,6 +61,26 @@ def _check_cuda(name: str, t: torch.Tensor, device: torch.device) -> None:
 
 def _stream_handle() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+class _on:
+    """``with _on(device) as stream``: the handle of ``device``'s current stream, with that device current."""
+
+    __slots__ = ("index", "other")
+
+    def __init__(self, device: torch.device) -> None:
+        current = torch.cuda.current_device()
+        self.index = current if device.index is None else device.index
+        self.other = None if self.index == current else torch.cuda.device(self.index)
+
+    def __enter__(self) -> int:
+        if self.other is not None:
+            self.other.__enter__()
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc) -> None:
+        if self.other is not None:
+            self.other.__exit__(*exc)
 
 
 def _raise(rc: int, what: str) -> None:
@@ -232,6 +255,120 @@ def flash_attn_with_kvcache(
     )
     if rc != _lib.WDRZ_OK:
         _raise(rc, "flash_attn_with_kvcache")
+    return out
+
+
+def _check_ids(name: str, t: torch.Tensor, B: int, device: torch.device) -> torch.Tensor:
+    """An int32 [B] tensor on ``device`` as it is, anything else as :func:`_as_int32` takes it."""
+    if t.__class__ is torch.Tensor and t.dtype is torch.int32 and t.device == device and t.shape == (B,) and t.is_contiguous():
+        return t
+    return _as_int32(name, t, B, device)
+
+
+def kvcache8_workspace_size(batch: int, sq: int, n_heads: int, max_seq: int) -> int:
+    """Bytes of split-KV workspace :func:`flash_attn_with_kvcache8` needs for these sizes."""
+    return int(_lib.load().wdrz_attn_kvcache8_workspace_size(batch, sq, n_heads, max_seq))
+
+
+def flash_attn_with_kvcache8(
+    q: torch.Tensor,
+    cache,
+    k: Optional[torch.Tensor] = None,
+    v: Optional[torch.Tensor] = None,
+    cache_seqlens=None,
+    cache_batch_idx: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+    *,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """:func:`flash_attn_with_kvcache` against a slot cache held in 8 bits (a ``FlashKVCache8``).
+
+    ``q`` ``[B, sq, H, 64]`` in bf16 or fp16; ``cache_batch_idx`` ``[B]`` row -> slot (identity if None).
+
+    With ``k`` / ``v`` ``[B, sq, H, 64]`` (a cache with a ring): they are appended at ``cache_seqlens[b]`` of
+    the row's slot and query ``t`` attends positions ``j <= cache_seqlens[b] + t``: those below the last
+    multiple of 32 as the codes' values, the newer ones as they came. The lengths are not modified. Rows
+    that name one slot must name one length; the last row's ``k`` / ``v`` then count for all of them (rows
+    that disagree give NaN and append nothing; ``WDRZ_DEBUG=1`` raises).
+    Without them every query attends the first ``cache_seqlens[b]`` positions of the slot, by default all
+    of them (a cache with a ring needs the lengths); a row of no positions gives zeros.
+    A slot or length out of range gives NaN rows and writes nothing.
+
+    ``out`` is a preallocated output, ``workspace`` a caller-owned split-KV workspace (zero-filled before
+    its first use; :func:`kvcache8_workspace_size`). Without it calls of one stream share a cached one, and
+    a call that is captured into a graph gets its own, cleared by every replay.
+    """
+    if not (isinstance(q, torch.Tensor) and q.is_cuda):
+        _check_cuda("q", q, q.device if isinstance(q, torch.Tensor) else None)
+    device = q.device
+    if cache.device != device:
+        raise RuntimeError(f"the cache is on {cache.device}, expected {device}")
+    if q.dim() != 4:
+        raise ValueError("q must be 4-D ([B, sq, H, 64])")
+    B, sq, H, D = q.shape
+    if H != cache.n_heads or D != cache.head_dim:
+        raise ValueError(f"cache heads/head_dim {(cache.n_heads, cache.head_dim)} do not match q {(H, D)}")
+    dt = _DTYPES16.get(q.dtype)
+    if dt is None:
+        raise TypeError(f"q: dtype {q.dtype} is not supported (bfloat16, float16)")
+    if cache.has_ring and q.dtype != cache.dtype:
+        raise TypeError(f"q must have the cache's dtype {cache.dtype}")
+    has_new = k is not None or v is not None
+    if has_new:
+        if k is None or v is None:
+            raise ValueError("k and v must be given together")
+        _check_cuda("k", k, device)
+        _check_cuda("v", v, device)
+        if k.shape != q.shape or v.shape != q.shape:
+            raise ValueError(f"k/v must have shape {(B, sq, H, D)}")
+        if k.dtype != q.dtype or v.dtype != q.dtype:
+            raise TypeError("k and v must have q's dtype")
+        if not cache.has_ring:
+            raise ValueError("appending needs a cache with a ring")
+    if cache_seqlens is None:
+        if has_new or cache.has_ring:
+            raise ValueError("cache_seqlens is required when k/v are given and for a cache with a ring")
+        seqlens = None
+    else:
+        seqlens = _check_ids("cache_seqlens", cache_seqlens, B, device)
+    if cache_batch_idx is not None:
+        cache_batch_idx = _check_ids("cache_batch_idx", cache_batch_idx, B, device)
+    if out is None:
+        out = torch.empty((B, sq, H, D), dtype=q.dtype, device=device)
+    else:
+        _check_cuda("out", out, device)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out must match q's shape and dtype")
+    if B == 0 or sq == 0:
+        return out
+    lib = _lib.load()
+    with _on(device) as stream:
+        nbytes = lib.wdrz_attn_kvcache8_workspace_size(B, sq, H, cache.max_seq_length)
+        ws_ptr, ws_bytes = None, 0
+        if nbytes:
+            if workspace is None:
+                if torch.cuda.is_current_stream_capturing():
+                    # another graph captured on this stream may be replayed beside this one
+                    workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+                else:
+                    workspace = _WORKSPACES.get(device, nbytes)
+            else:
+                _check_cuda("workspace", workspace, device)
+            ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+            if ws_bytes < nbytes:
+                raise ValueError(f"workspace too small: need {nbytes} bytes")
+        rc = lib.wdrz_attn_kvcache8(
+            dt, cache.struct, q.data_ptr(), _lib.strides4(q.stride()),
+            k.data_ptr() if has_new else None, _lib.strides4(k.stride()) if has_new else None,
+            v.data_ptr() if has_new else None, _lib.strides4(v.stride()) if has_new else None,
+            seqlens.data_ptr() if seqlens is not None else None,
+            cache_batch_idx.data_ptr() if cache_batch_idx is not None else None,
+            out.data_ptr(), _lib.strides4(out.stride()), B, sq,
+            D ** -0.5 if softmax_scale is None else float(softmax_scale), ws_ptr, ws_bytes, stream,
+        )
+    if rc != _lib.WDRZ_OK:
+        _raise(rc, "flash_attn_with_kvcache8")
     return out
 
 

@@ -154,6 +154,29 @@ int debug_check_kv_metadata(const int32_t* seqlens, const int32_t* bidx, bool ha
   }
   return WDRZ_OK;
 }
+
+// The same for a call on the 8-bit cache, whose reads take lengths too and whose appending rows that name
+// one slot have to name one length.
+int debug_check_kv8_metadata(const int32_t* seqlens, const int32_t* bidx, bool has_new, int64_t B, int64_t sq,
+                             int64_t n_slots, int64_t Lmax) {
+  int rc = debug_check_kv_metadata(seqlens, bidx, has_new, B, sq, n_slots, Lmax);
+  if (rc || !seqlens) return rc;
+  std::vector<int32_t> hs(B, 0), hb(B), first(n_slots, -1);
+  for (int64_t i = 0; i < B; ++i) hb[i] = (int32_t)i;
+  if ((bidx && hipMemcpy(hb.data(), bidx, B * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess) ||
+      hipMemcpy(hs.data(), seqlens, B * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess)
+    return fail(WDRZ_ELAUNCH, "debug check: reading the rows' slots and lengths failed");
+  for (int64_t i = 0; i < B; ++i) {
+    if (!has_new && (hs[i] < 0 || hs[i] > Lmax))
+      return fail(WDRZ_EINVAL, "debug check: row %lld reads %d positions of %lld", (long long)i, hs[i], (long long)Lmax);
+    int32_t& f = first[hb[i]];
+    if (has_new && f >= 0 && hs[f] != hs[i])
+      return fail(WDRZ_EINVAL, "debug check: rows %d and %lld append to slot %d at lengths %d and %d", f, (long long)i,
+                  hb[i], hs[f], hs[i]);
+    f = (int32_t)i;
+  }
+  return WDRZ_OK;
+}
 #endif
 
 }  // namespace
@@ -819,6 +842,196 @@ int wdrz_dtw_attention_prep(int dtype, const void* const* q_heads, const int64_t
   if (rc == -1) return WDRZ_OK;
   if (rc != WDRZ_OK) return rc;
   hipError_t err = wdrz::launch_dtw_qk_prep(dtype, a, q, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  return WDRZ_OK;
+}
+
+// ---- the 8-bit cache and the 4-bit linears ----
+
+static int check_dtype16(int dtype) {
+  if (dtype == WDRZ_BF16 || dtype == WDRZ_F16) return WDRZ_OK;
+  return fail(dtype == WDRZ_F32 ? WDRZ_EUNSUPPORTED : WDRZ_EINVAL, "dtype %d: only WDRZ_BF16 / WDRZ_F16", dtype);
+}
+
+static int kv8_cache(const wdrz_kv8* c, wdrz::Kv8Cache* out) {
+  if (!c) return fail(WDRZ_EINVAL, "cache is NULL");
+  if (c->n_slots <= 0 || c->n_heads <= 0 || c->max_seq <= 0)
+    return fail(WDRZ_EINVAL, "bad cache sizes n_slots=%lld n_heads=%lld max_seq=%lld", (long long)c->n_slots,
+                (long long)c->n_heads, (long long)c->max_seq);
+  if (c->n_heads > 65535 || c->max_seq > (1 << 24) || c->n_slots > (1 << 24))
+    return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  int rc;
+  if ((rc = check_ptr("k_codes", c->k_codes)) || (rc = check_ptr("v_codes", c->v_codes)) ||
+      (rc = check_ptr("k_scales", c->k_scales)) || (rc = check_ptr("v_scales", c->v_scales)))
+    return rc;
+  if (!c->k_ring != !c->v_ring) return fail(WDRZ_EINVAL, "k_ring and v_ring must be given together");
+  if (c->k_ring && ((rc = check_ptr("k_ring", c->k_ring)) || (rc = check_ptr("v_ring", c->v_ring)))) return rc;
+  out->kc = static_cast<uint8_t*>(c->k_codes);
+  out->vc = static_cast<uint8_t*>(c->v_codes);
+  out->ks = c->k_scales;
+  out->vs = c->v_scales;
+  out->kr = static_cast<char*>(c->k_ring);
+  out->vr = static_cast<char*>(c->v_ring);
+  out->n_slots = (int)c->n_slots;
+  out->H = (int)c->n_heads;
+  out->Lk = (int)c->max_seq;
+  out->n_blk = (int)((c->max_seq + 31) / 32);
+  return WDRZ_OK;
+}
+
+// [B, T, H, 64] rows of a 16-bit type: pointer and the strides of b, t, h, in bytes.
+static int rows16(const char* name, const void* p, const int64_t* s, int64_t* bytes) {
+  int rc;
+  if ((rc = check_ptr(name, p)) || (rc = check_strides(name, s, 2))) return rc;
+  for (int i = 0; i < 3; ++i) bytes[i] = s[i] * 2;
+  return WDRZ_OK;
+}
+
+int wdrz_kv8_write(int dtype, const wdrz_kv8* cache, const void* k_src, const int64_t* k_strides, const void* v_src,
+                   const int64_t* v_strides, const int64_t* slot_indices, int64_t B, int64_t T, int64_t start_pos,
+                   void* stream) {
+  g_last_error.clear();
+  int rc;
+  wdrz::Kv8Cache c{};
+  if ((rc = check_dtype16(dtype)) || (rc = kv8_cache(cache, &c))) return rc;
+  if (B < 0 || T < 0 || start_pos < 0)
+    return fail(WDRZ_EINVAL, "bad sizes B=%lld T=%lld start_pos=%lld", (long long)B, (long long)T, (long long)start_pos);
+  if (B > 65535) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (T > c.Lk || start_pos > c.Lk - T)
+    return fail(WDRZ_EINVAL, "rows [%lld, %lld) exceed the cache length %d", (long long)start_pos,
+                (long long)(start_pos + T), c.Lk);
+  if (!c.kr && start_pos % 32 != 0)
+    return fail(WDRZ_EINVAL, "start_pos=%lld: a cache without a ring is written from multiples of 32", (long long)start_pos);
+  if (!slot_indices && B > c.n_slots)
+    return fail(WDRZ_EINVAL, "%lld rows exceed the %d slots", (long long)B, c.n_slots);
+  if (B == 0 || T == 0) return WDRZ_OK;
+  wdrz::Kv8WriteArgs a{};
+  if ((rc = rows16("k", k_src, k_strides, a.ks)) || (rc = rows16("v", v_src, v_strides, a.vs))) return rc;
+  a.k = static_cast<const char*>(k_src);
+  a.v = static_cast<const char*>(v_src);
+  a.B = (int)B;
+  a.T = (int)T;
+  a.start = (int)start_pos;
+  hipError_t err = wdrz::launch_kv8_write(dtype, c, a, nullptr, slot_indices, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  return WDRZ_OK;
+}
+
+size_t wdrz_attn_kvcache8_workspace_size(int64_t B, int64_t sq, int64_t n_heads, int64_t max_seq) {
+  if (B <= 0 || sq <= 0 || n_heads <= 0 || max_seq <= 0) return 0;
+  return wdrz::kv8_workspace_bytes(B, sq, n_heads, max_seq);
+}
+
+int wdrz_attn_kvcache8(int dtype, const wdrz_kv8* cache, const void* q, const int64_t* q_strides, const void* k_new,
+                       const int64_t* kn_strides, const void* v_new, const int64_t* vn_strides,
+                       const int32_t* cache_seqlens, const int32_t* cache_batch_idx, void* o, const int64_t* o_strides,
+                       int64_t B, int64_t sq, float softmax_scale, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  g_last_error.clear();
+  int rc;
+  wdrz::Kv8Cache c{};
+  if ((rc = check_dtype16(dtype)) || (rc = kv8_cache(cache, &c))) return rc;
+  if (B < 0 || sq <= 0) return fail(WDRZ_EINVAL, "bad sizes B=%lld sq=%lld", (long long)B, (long long)sq);
+  if (B > 65535 || sq > 4096) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (!(softmax_scale > 0.f) || softmax_scale > 3.0e38f) return fail(WDRZ_EINVAL, "softmax_scale must be a positive finite number");
+  const bool has_new = k_new || v_new;
+  if (has_new && (!k_new || !v_new)) return fail(WDRZ_EINVAL, "k and v must be given together");
+  if (has_new && !c.kr) return fail(WDRZ_EINVAL, "appending needs a cache with a ring");
+  if ((has_new || c.kr) && !cache_seqlens)
+    return fail(WDRZ_EINVAL, "cache_seqlens is required when k/v are given and for a cache with a ring");
+  if (has_new && sq > c.Lk) return fail(WDRZ_EINVAL, "sq=%lld exceeds cache length %d", (long long)sq, c.Lk);
+  if (B == 0) return WDRZ_OK;
+  wdrz::Kv8Args a{};
+  if ((rc = rows16("q", q, q_strides, a.qs)) || (rc = rows16("out", o, o_strides, a.os))) return rc;
+  if (has_new && ((rc = rows16("k", k_new, kn_strides, a.kns)) || (rc = rows16("v", v_new, vn_strides, a.vns)))) return rc;
+#ifdef WDRZ_DEBUG_CHECKS
+  if ((rc = debug_check_kv8_metadata(cache_seqlens, cache_batch_idx, has_new, B, sq, c.n_slots, c.Lk))) return rc;
+#endif
+  a.q = static_cast<const char*>(q);
+  a.kn = has_new ? static_cast<const char*>(k_new) : nullptr;
+  a.vn = has_new ? static_cast<const char*>(v_new) : nullptr;
+  a.seqlens = cache_seqlens;
+  a.bidx = cache_batch_idx;
+  a.o = static_cast<char*>(o);
+  a.B = (int)B;
+  a.sq = (int)sq;
+  a.H = c.H;
+  a.append = sq <= wdrz::kKv8FusedAppend;
+  a.c = softmax_scale * 1.4426950408889634f;
+  wdrz::kv8_plan(B, sq, c.H, c.Lk, &a);
+  const int64_t units = B * a.n_qblocks * c.H;
+  if (units > 0x7fffffff) return fail(WDRZ_EUNSUPPORTED, "B * ceil(sq / rows per block) * H exceeds 2^31 - 1");
+  const size_t need = wdrz::kv8_workspace_bytes(B, sq, c.H, c.Lk);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return fail(WDRZ_EWORKSPACE, "workspace of %zu bytes required (got %zu)", need, workspace ? workspace_bytes : 0);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+      return fail(WDRZ_EINVAL, "workspace is not 256-byte aligned");
+    const size_t counters = ((size_t)units * sizeof(int) + 255) / 256 * 256;
+    a.ws_count = static_cast<int*>(workspace);
+    a.ws_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + counters);
+  }
+  hipError_t err = wdrz::launch_kv8_attn(dtype, c, a, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  return WDRZ_OK;
+}
+
+// What the two 4-bit linears share. Returns WDRZ_OK, an error code, or -1 for "nothing to do".
+static int linear4_args(int dtype, const void* x, int64_t x_stride, const void* w, const void* scales, int64_t M,
+                        int64_t N, int64_t K, int64_t group, wdrz::Linear4Args* a) {
+  int rc;
+  if ((rc = check_dtype16(dtype))) return rc;
+  if (M < 0 || N <= 0 || K <= 0) return fail(WDRZ_EINVAL, "bad sizes M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  if (group != 32 && group != 64 && group != 128) return fail(WDRZ_EUNSUPPORTED, "group %lld is not 32, 64 or 128", (long long)group);
+  if (K % group != 0)
+    return fail(WDRZ_EUNSUPPORTED, "K=%lld must be a multiple of the group of %lld", (long long)K, (long long)group);
+  if (M > 65535 * 64 || N > (1 << 24) || K > (1 << 20)) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (M == 0) return -1;  // nothing to read or write (an empty tensor's pointer may be NULL)
+  if ((rc = check_ptr("x", x)) || (rc = check_ptr("w_packed", w)) || (rc = check_ptr("scales_packed", scales))) return rc;
+  if (x_stride < K) return fail(WDRZ_EINVAL, "row strides shorter than the rows");
+  if (x_stride % 8) return fail(WDRZ_EINVAL, "row strides are not 16-byte aligned");
+  a->x = x;
+  a->w = w;
+  a->scales = scales;
+  a->x_stride = x_stride;
+  a->M = (int)M;
+  a->N = (int)N;
+  a->K = (int)K;
+  a->group = (int)group;
+  return WDRZ_OK;
+}
+
+int wdrz_linear4(int dtype, const void* x, int64_t x_stride, const void* w_packed, const void* scales_packed,
+                 const void* bias, void* y, int64_t y_stride, int64_t M, int64_t N, int64_t K, int64_t group,
+                 int activation, void* stream) {
+  g_last_error.clear();
+  wdrz::Linear4Args a{};
+  if (activation != 0 && activation != 1) return fail(WDRZ_EINVAL, "activation %d is not 0 (none) or 1 (GELU)", activation);
+  int rc = linear4_args(dtype, x, x_stride, w_packed, scales_packed, M, N, K, group, &a);
+  if (rc) return rc < 0 ? WDRZ_OK : rc;
+  if (!y) return fail(WDRZ_EINVAL, "y is NULL");
+  if ((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(y)) & 1) return fail(WDRZ_EINVAL, "bias or y is not 2-byte aligned");
+  if (y_stride < N) return fail(WDRZ_EINVAL, "row strides shorter than the rows");
+  a.bias = bias;
+  a.y = y;
+  a.y_stride = y_stride;
+  a.act = activation;
+  hipError_t err = wdrz::launch_linear4(dtype, a, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  return WDRZ_OK;
+}
+
+int wdrz_linear4_partials(int dtype, const void* x, int64_t x_stride, const void* w_packed, const void* scales_packed,
+                          float* partials, int64_t M, int64_t N, int64_t K, int64_t group, int n_split, void* stream) {
+  g_last_error.clear();
+  wdrz::Linear4Args a{};
+  if (n_split != 2 && n_split != 4) return fail(WDRZ_EUNSUPPORTED, "n_split %d is not 2 or 4", n_split);
+  int rc = linear4_args(dtype, x, x_stride, w_packed, scales_packed, M, N, K, group, &a);
+  if (rc) return rc < 0 ? WDRZ_OK : rc;
+  if ((rc = check_ptr("partials", partials))) return rc;
+  a.part = partials;
+  a.n_split = n_split;
+  hipError_t err = wdrz::launch_linear4(dtype, a, reinterpret_cast<hipStream_t>(stream));
   if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
   return WDRZ_OK;
 }

@@ -51,6 +51,47 @@ hipError_t launch_kv_attn(int dtype, const KvArgs& a, hipStream_t stream);
 // new rows appended. Cross (no new rows): all Lk cache rows, nothing appended.
 hipError_t launch_kv_prefill(int dtype, const KvArgs& a, hipStream_t stream);
 
+// The cache held in 8 bits (kv8.hip). Buffers are contiguous: codes [n_slots, H, n_blk * 32, 64], scales
+// [n_slots, H, n_blk], ring rows [n_slots, H, 64, 64] of 16 bits (nullptr: a cache without a ring).
+struct Kv8Cache {
+  uint8_t* kc;
+  uint8_t* vc;
+  float* ks;
+  float* vs;
+  char* kr;
+  char* vr;
+  int n_slots, H, Lk, n_blk;
+};
+// Strides in BYTES of b, t, h; the head_dim is contiguous.
+struct Kv8Args {
+  const char* q;
+  const char* kn;  // new rows (nullptr: nothing is appended)
+  const char* vn;
+  const int32_t* seqlens;  // with kn: lengths before the append; without: keys to read (nullptr: Lk)
+  const int32_t* bidx;     // batch row -> slot (nullptr: identity)
+  char* o;
+  float* ws_part;
+  int* ws_count;
+  int B, sq, n_qblocks, n_splits, split_len;
+  int H;       // as the cache's
+  int append;  // the attention launch writes the new rows (sq <= 32)
+  int64_t qs[3], kns[3], vns[3], os[3];
+  float c;  // softmax scale * log2(e)
+};
+struct Kv8WriteArgs {
+  const char* k;
+  const char* v;
+  int64_t ks[3], vs[3];
+  const int32_t* starts;  // [B] first position of each row (nullptr: start)
+  int B, T, start;
+};
+constexpr int kKv8FusedAppend = 32;  // new rows that the attention launch appends itself
+void kv8_plan(int64_t B, int64_t sq, int64_t H, int64_t Lk, Kv8Args* a);
+size_t kv8_workspace_bytes(int64_t B, int64_t sq, int64_t H, int64_t Lk);
+hipError_t launch_kv8_attn(int dtype, const Kv8Cache& c, const Kv8Args& a, hipStream_t stream);
+hipError_t launch_kv8_write(int dtype, const Kv8Cache& c, const Kv8WriteArgs& a, const int32_t* slots32,
+                            const int64_t* slots64, hipStream_t stream);
+
 // Dense MFMA attention (bf16 / fp16). Strides in ELEMENTS in [B, H, L, D] order.
 struct DenseArgs {
   const void* q;
@@ -193,6 +234,20 @@ struct LinearArgs {
   int n_split = 1;
 };
 hipError_t launch_linear(int dtype, const LinearArgs& a, hipStream_t stream);
+
+// Y = act(X (s Q)^T + b), Q 4-bit weights packed as linear4.hip says, s 16-bit scales a feature and group.
+struct Linear4Args {
+  const void* x;
+  const void* w;       // [ceil(N / 16)][ceil(K / 128)][64 lanes][16 bytes]
+  const void* scales;  // [ceil(N / 16)][K / group][16]
+  const void* bias;    // nullptr: no bias
+  void* y;
+  int64_t x_stride, y_stride;
+  int M, N, K, group, act;
+  float* part;  // split form: fp32 sums [n_split][M][N] instead of y
+  int n_split;
+};
+hipError_t launch_linear4(int dtype, const Linear4Args& a, hipStream_t stream);
 
 // Y = act(LayerNorm(x + delta) W^T + b) for M <= 4 rows of K <= 1536: ln gives x, the delta's
 // partials and the LayerNorm's parameters; the new residual goes to x_out.

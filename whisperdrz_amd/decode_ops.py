@@ -9,6 +9,7 @@
   additive -65504 mask, repetition penalty, argmax, one launch instead of six.
 * :func:`linear_gelu` — the MLP's ``Linear(n_state, 4 n_state)`` + ``GELU`` (``model.py:388-391``,
   applied at ``model.py:434``): GEMM, bias, rounding and exact GELU in one launch.
+* :func:`linear4` — the same with 4-bit weights and group scales (:class:`QuantLinear4`).
 
 There is no fallback: CPU tensors, fp32 LayerNorm inputs and a missing library raise.
 """
@@ -20,9 +21,10 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .attention import _check_cuda, _dtype_code, _raise, _stream_handle
+from .attention import _check_cuda, _dtype_code, _on, _raise, _stream_handle
 
-__all__ = ["add_layernorm_", "layer_norm", "linear_gelu", "ln_linear", "masked_argmax"]
+__all__ = ["QuantLinear4", "add_layernorm_", "layer_norm", "linear4", "linear4_partials", "linear_gelu", "ln_linear",
+           "masked_argmax"]
 
 _LN16 = {torch.bfloat16: _lib.WDRZ_BF16, torch.float16: _lib.WDRZ_F16}
 
@@ -181,6 +183,131 @@ def add_layernorm_partials_(x: torch.Tensor, partials: torch.Tensor, lin: nn.Lin
     if rc != _lib.WDRZ_OK:
         _raise(rc, "add_layernorm_partials_")
     return y.view(x.shape)
+
+
+class QuantLinear4(nn.Module):
+    """A Linear with 4-bit weights: ``weight[n, k] = codes[n, k] * scales[n, k // group]``, codes whole
+    numbers -7..7 and scales of the activations' 16-bit type, packed once for :func:`linear4`.
+
+    ``from_linear`` rounds a 16-bit Linear, ``from_codes`` takes codes and scales from elsewhere. ``group`` is
+    32, 64 or 128 and divides the inputs. Inference only: the weights are buffers without gradients."""
+
+    GROUPS = (32, 64, 128)
+
+    def __init__(self, in_features: int, out_features: int, group: int, packed: torch.Tensor, scales: torch.Tensor,
+                 bias: Optional[torch.Tensor]):
+        super().__init__()
+        self.in_features, self.out_features, self.group = in_features, out_features, group
+        self.register_buffer("packed", packed)
+        self.register_buffer("scales", scales)
+        self.register_buffer("bias", bias)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "QuantLinear4":
+        """``codes`` ``[N, K]`` whole numbers -7..7, ``scales`` ``[N, K / group]`` (bf16 or fp16), ``bias`` ``[N]``."""
+        if codes.dim() != 2 or scales.dim() != 2 or scales.shape[0] != codes.shape[0] or codes.shape[0] == 0 \
+                or scales.shape[1] == 0 or codes.shape[1] % scales.shape[1]:
+            raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} must be [N, K] and [N, K / group]")
+        N, K = (int(n) for n in codes.shape)
+        group = K // int(scales.shape[1])
+        if group not in cls.GROUPS:
+            raise NotImplementedError(f"group {group} is not one of {cls.GROUPS}")
+        if scales.dtype not in _LN16 or (bias is not None and (bias.dtype != scales.dtype or tuple(bias.shape) != (N,))):
+            raise TypeError("scales and bias must share a 16-bit dtype (bfloat16, float16), bias [N]")
+        if codes.is_floating_point() or codes.is_complex() or codes.dtype == torch.bool:
+            raise TypeError(f"codes: dtype {codes.dtype} is not a whole type")
+        codes = codes.detach()
+        if bool(((codes < -7) | (codes > 7)).any()):
+            raise ValueError("codes must lie in -7..7")
+        tiles, chunks = -(-N // 16), -(-K // 128)
+        nib = codes.abs().to(torch.uint8) | ((codes < 0).to(torch.uint8) << 3)
+        full = torch.zeros(tiles * 16, chunks * 128, dtype=torch.uint8, device=codes.device)
+        full[:N, :K] = nib
+        # [tile, n, chunk, s, g, half, i] -> [tile, chunk, g, n, s, i], the halves in one byte
+        full = full.view(tiles, 16, chunks, 4, 4, 2, 4).permute(0, 2, 4, 1, 3, 6, 5)
+        packed = (full[..., 0] | (full[..., 1] << 4)).reshape(tiles, chunks, 1024).contiguous()
+        s = torch.zeros(tiles * 16, K // group, dtype=scales.dtype, device=scales.device)
+        s[:N] = scales.detach()
+        s = s.view(tiles, 16, K // group).transpose(1, 2).contiguous()
+        return cls(K, N, group, packed, s, None if bias is None else bias.detach().contiguous())
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, group: int = 64) -> "QuantLinear4":
+        """Rounds ``weight`` ``[N, K]``: a group's scale is its largest magnitude / 7 (in the weight's type),
+        its codes the nearest whole numbers."""
+        if weight.dim() != 2 or weight.dtype not in _LN16:
+            raise TypeError("weight must be 2-D, bfloat16 or float16")
+        N, K = (int(n) for n in weight.shape)
+        if group not in cls.GROUPS or K % group:
+            raise NotImplementedError(f"group {group} must be one of {cls.GROUPS} and divide the {K} inputs")
+        w = weight.detach().float().view(N, K // group, group)
+        scales = (w.abs().amax(-1) / 7).to(weight.dtype)
+        s = scales.float()
+        codes = torch.where(s[..., None] > 0, w / s[..., None], torch.zeros_like(w)).round_().clamp_(-7, 7)
+        return cls.from_codes(codes.view(N, K).to(torch.int8), scales, bias)
+
+    @classmethod
+    def from_linear(cls, lin: nn.Linear, group: int = 64) -> "QuantLinear4":
+        return cls.from_weight(lin.weight, lin.bias, group)
+
+    def dequantize(self) -> torch.Tensor:
+        """The fp32 weight ``[N, K]`` that the codes and scales stand for."""
+        tiles, chunks, _ = self.packed.shape
+        p = self.packed.view(tiles, chunks, 4, 16, 4, 4)
+        nib = torch.stack([p & 15, p >> 4], -1).permute(0, 3, 1, 4, 2, 6, 5).reshape(tiles * 16, chunks * 128)
+        codes = (nib & 7).float() * (1 - 2 * (nib >> 3).float())
+        s = self.scales.transpose(1, 2).reshape(tiles * 16, -1).float().repeat_interleave(self.group, 1)
+        return codes[: self.out_features, : self.in_features] * s[: self.out_features]
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return linear4(x, self)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, group={self.group}, bias={self.bias is not None}"
+
+
+def _linear4_rows(x: torch.Tensor, lin: QuantLinear4) -> torch.Tensor:
+    """The checked rows ``[M, K]`` of ``x``."""
+    if x.dtype not in _LN16:
+        raise TypeError(f"x: dtype {x.dtype} is not supported (bfloat16, float16)")
+    _check_cuda("x", x, lin.packed.device)
+    if lin.scales.dtype != x.dtype or lin.scales.device != x.device or (
+            lin.bias is not None and (lin.bias.dtype != x.dtype or lin.bias.device != x.device)):
+        raise TypeError("the Linear's scales and bias must have the activations' dtype and device")
+    if x.shape[-1] != lin.in_features:
+        raise ValueError(f"x must have {lin.in_features} features, got {tuple(x.shape)}")
+    return x if x.dim() == 2 and x.stride(1) == 1 else _rows(x, "x")
+
+
+def linear4(x: torch.Tensor, lin: QuantLinear4, gelu: bool = False) -> torch.Tensor:
+    """``lin(x)`` (``gelu``: then the exact GELU) for 16-bit ``x [..., K]``: fp32 accumulation, bias and
+    activation, one rounding."""
+    xr = _linear4_rows(x, lin)
+    M, N = xr.shape[0], lin.out_features
+    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    with _on(x.device) as stream:
+        rc = _lib.load().wdrz_linear4(
+            _LN16[x.dtype], xr.data_ptr(), xr.stride(0) if M > 1 else lin.in_features, lin.packed.data_ptr(),
+            lin.scales.data_ptr(), lin.bias.data_ptr() if lin.bias is not None else None, y.data_ptr(), N, M, N,
+            lin.in_features, lin.group, 1 if gelu else 0, stream)
+    if rc != _lib.WDRZ_OK:
+        _raise(rc, "linear4")
+    return y
+
+
+def linear4_partials(x: torch.Tensor, lin: QuantLinear4, n_split: int = 4) -> torch.Tensor:
+    """:func:`linear_partials` of a Linear with 4-bit weights: fp32 ``[n_split, rows, N]`` whose sum over the
+    first dimension is ``x @ weight.T`` (no bias), for :func:`add_layernorm_partials_`."""
+    xr = _linear4_rows(x, lin)
+    M, N = xr.shape[0], lin.out_features
+    part = torch.empty(n_split, M, N, dtype=torch.float32, device=x.device)
+    with _on(x.device) as stream:
+        rc = _lib.load().wdrz_linear4_partials(
+            _LN16[x.dtype], xr.data_ptr(), xr.stride(0) if M > 1 else lin.in_features, lin.packed.data_ptr(),
+            lin.scales.data_ptr(), part.data_ptr(), M, N, lin.in_features, lin.group, n_split, stream)
+    if rc != _lib.WDRZ_OK:
+        _raise(rc, "linear4_partials")
+    return part
 
 
 LN_LINEAR_ROWS = 4  # rows ln_linear takes (every workgroup repeats their LayerNorm)

@@ -161,6 +161,137 @@ class FlashKVCache:
         self.cross_attn_len = 0
 
 
+class FlashKVCache8:
+    """The slot cache held in 8 bits: ``FlashKVCache``'s methods over e4m3 codes, for
+    ``flash_attn_with_kvcache8``.
+
+    Positions are held in blocks of 32; a complete block of one (slot, head) is codes with one power-of-two
+    scale for its keys and one for its values (:meth:`dequantize` says what they stand for). With ``ring``
+    (a self cache) the newest positions also stand as they came, in 64 rows a (slot, head), and the block
+    that is not complete is read from there: a position is rounded once, when its block completes, however
+    the tokens were cut into calls. ``seq_lens`` may be set back by up to 32 positions (a draft that was
+    rejected) or to any multiple of 32; anything else needs the positions written again.
+    Without ``ring`` (a cross cache) the cache is filled by :meth:`set_cross_attention`.
+
+    Buffers: ``k_codes`` / ``v_codes`` ``[batch_size, n_heads, blocks * 32, 64]`` (``float8_e4m3fn``),
+    ``k_scales`` / ``v_scales`` ``[batch_size, n_heads, blocks]`` fp32, ``k_ring`` / ``v_ring``
+    ``[batch_size, n_heads, 64, 64]`` of ``dtype``; ``storage`` places them in given (contiguous) tensors.
+    Per slot and head 128 bytes a position and 16 KB of ring, against 256 bytes a position in 16 bits.
+    """
+
+    BLOCK = 32
+    RING = 64
+
+    def __init__(self, batch_size: int, max_seq_length: int, n_heads: int, head_dim: int = 64, dtype=torch.bfloat16,
+                 device=None, *, ring: bool = True, storage: Optional[dict[str, Tensor]] = None,
+                 seq_lens: Optional[Tensor] = None):
+        if head_dim != 64:
+            raise NotImplementedError(f"head_dim {head_dim} is not supported (only 64)")
+        if dtype not in _FILL_DTYPES:
+            raise TypeError(f"dtype {dtype} is not supported (bfloat16, float16)")
+        self.batch_size, self.max_seq_length = batch_size, max_seq_length
+        self.n_heads, self.head_dim, self.dtype, self.has_ring = n_heads, head_dim, dtype, bool(ring)
+        layout = self.layout(batch_size, max_seq_length, n_heads, dtype, ring)
+        if storage is None:
+            storage = {n: torch.zeros(shape, dtype=torch.uint8, device=device).view(dt) if dt is torch.float8_e4m3fn
+                       else torch.zeros(shape, dtype=dt, device=device) for n, (shape, dt) in layout.items()}
+        for n, (shape, dt) in layout.items():
+            t = storage.get(n)
+            if t is None or tuple(t.shape) != shape or t.dtype != dt or not t.is_contiguous():
+                raise ValueError(f"storage[{n!r}] must be a contiguous {dt} tensor of shape {shape}")
+            if t.device != storage["k_codes"].device:
+                raise ValueError("the buffers must be on one device")
+            setattr(self, n, t)
+        if not ring:
+            self.k_ring = self.v_ring = None
+        self.device = self.k_codes.device
+        self.struct = _lib.Kv8(*(storage[n].data_ptr() if n in layout else None for n in
+                                 ("k_codes", "v_codes", "k_scales", "v_scales", "k_ring", "v_ring")),
+                               batch_size, n_heads, max_seq_length)
+        self.seq_lens = torch.zeros(batch_size, dtype=torch.int32, device=self.device) if seq_lens is None else seq_lens
+        self.done = False
+        self.cross_attn_len = 0
+
+    @classmethod
+    def layout(cls, batch_size: int, max_seq_length: int, n_heads: int, dtype, ring: bool) -> dict:
+        """Shape and dtype of every buffer."""
+        blocks = -(-max_seq_length // cls.BLOCK)
+        res = {}
+        for n in "kv":
+            res[n + "_codes"] = ((batch_size, n_heads, blocks * cls.BLOCK, 64), torch.float8_e4m3fn)
+            res[n + "_scales"] = ((batch_size, n_heads, blocks), torch.float32)
+            if ring:
+                res[n + "_ring"] = ((batch_size, n_heads, cls.RING, 64), dtype)
+        return res
+
+    def _write(self, k: Tensor, v: Tensor, slot_indices: Optional[Tensor], start_pos: int) -> None:
+        from .attention import _check_cuda, _on, _raise
+
+        for name, t in (("k", k), ("v", v)):
+            _check_cuda(name, t, self.device)
+            if t.dim() != 4 or tuple(t.shape[2:]) != (self.n_heads, self.head_dim) or t.shape != k.shape:
+                raise ValueError(f"{name} must be [B, T, {self.n_heads}, {self.head_dim}], got {tuple(t.shape)}")
+            if t.dtype not in _FILL_DTYPES or t.dtype != k.dtype or (self.has_ring and t.dtype != self.dtype):
+                raise TypeError(f"{name}: dtype {t.dtype} does not match the cache's")
+        B, T = int(k.shape[0]), int(k.shape[1])
+        slots = None
+        if slot_indices is not None:
+            _check_cuda("slot_indices", slot_indices, self.device)
+            slots = slot_indices.to(torch.int64)
+            if slots.dim() != 1 or slots.shape[0] != B:
+                raise ValueError(f"slot_indices must be [{B}]")
+            slots = slots.contiguous()
+        if B == 0 or T == 0:
+            return
+        with _on(self.device) as stream:
+            rc = _lib.load().wdrz_kv8_write(
+                _FILL_DTYPES[k.dtype], self.struct, k.data_ptr(), _lib.strides4(k.stride()), v.data_ptr(),
+                _lib.strides4(v.stride()), slots.data_ptr() if slots is not None else None, B, T, int(start_pos), stream)
+        if rc != _lib.WDRZ_OK:
+            _raise(rc, "kv8_write")
+
+    def prefill(self, k: Tensor, v: Tensor, start_pos: int = 0, slot_indices: Optional[Tensor] = None):
+        """Append ``k, v`` ``[B, seq, heads, 64]`` at length ``start_pos`` and set ``seq_lens`` to the end."""
+        if not self.has_ring:
+            raise ValueError("prefill needs a cache with a ring")
+        self._write(k, v, slot_indices, start_pos)
+        if slot_indices is not None:
+            self.seq_lens[slot_indices] = start_pos + k.shape[1]
+        else:
+            self.seq_lens[: k.shape[0]] = start_pos + k.shape[1]
+
+    def set_cross_attention(self, k: Tensor, v: Tensor, slot_indices: Optional[Tensor] = None):
+        """Fill the slots with the encoder-side ``k, v`` ``[B, seq, heads, 64]``."""
+        if self.has_ring:
+            raise ValueError("set_cross_attention needs a cache without a ring")
+        self._write(k, v, slot_indices, 0)
+        self.cross_attn_len = k.shape[1]
+        self.done = True
+
+    def dequantize(self, lengths: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+        """fp32 ``[batch_size, max_seq_length, n_heads, 64]`` keys and values of every slot, as the attention
+        reads them at ``lengths`` ``[batch_size]`` (``seq_lens`` if None; a cache without a ring has none)."""
+        L, res = self.max_seq_length, []
+        pos = torch.arange(L, device=self.device)
+        for codes, scales, ring in ((self.k_codes, self.k_scales, self.k_ring), (self.v_codes, self.v_scales, self.v_ring)):
+            x = codes.float()[:, :, :L] * scales.repeat_interleave(self.BLOCK, -1)[:, :, :L, None]
+            if ring is not None:
+                n = self.seq_lens if lengths is None else lengths
+                x = torch.where((pos < (n // self.BLOCK * self.BLOCK)[:, None])[:, None, :, None], x,
+                                ring.float()[:, :, pos % self.RING])
+            res.append(x.permute(0, 2, 1, 3))
+        return res[0], res[1]
+
+    def reset(self, slot_indices: Optional[Tensor] = None):
+        """Zero the lengths of ``slot_indices`` (all slots if None); nothing is cleared."""
+        if slot_indices is not None:
+            self.seq_lens[slot_indices] = 0
+        else:
+            self.seq_lens.zero_()
+        self.done = False
+        self.cross_attn_len = 0
+
+
 @dataclass(frozen=True)
 class SlotPlan:
     n_slots: int
