@@ -17,13 +17,19 @@
 // [c0, len + sq) are at most 63, so no new row shares a ring row with an old one that is still read,
 // and the append rides in the attention launch. Longer prompts append in a launch of their own behind it.
 //
-// One wavefront takes a block of 32 keys and up to 16 queries a step, as kv_mq_kernel does:
+// One query: four lanes a key, dot products and sums on the VALU (kv8_row_kernel). More: a wavefront takes a
+// block of 32 keys and up to 16 queries a step on the matrix cores (kv8_attn_kernel):
 //   S^T (32 keys x 16 queries) = K Q^T with 4 v_mfma_f32_16x16x32, O^T (64 dims x 16 queries) += V^T P^T
 // with 8 more, P in two 16-bit parts. Codes become bf16 (fp16 queries: fp16 for K, whose products are
 // then exact too) two an instruction; the keys' scale multiplies the scores in fp32, the values' scale
 // is the conversion's own, exact in bf16. A lane's 16-byte load is 16 dimensions of one key: the matrix
-// product sums over the dimensions in that order, for K and Q alike. V goes through an LDS tile and
-// comes back transposed.
+// product sums over the dimensions in that order, for K and Q alike. V goes through an LDS tile, as
+// codes, and comes back transposed. Both read their codes two blocks ahead.
+//
+// Bound: the stream of codes. 52 streams, one fp16 query over 1500 positions: 36 us for 200 MB (5.6 TB/s
+// with the launch). One query on the matrix cores instead took 59: eight exponentials and a pack for two
+// a key, the LDS round trip and 128 registers. Small calls: launch, the trip for the row's metadata, one
+// for its keys; 1 stream 6.2 us over 1500, append at 200 4.4 us.
 #include <algorithm>
 
 #include "kv_merge.h"
@@ -48,6 +54,10 @@ template <> struct Ops<Bf16> {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
   static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
   static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
+  typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, a), __builtin_bit_cast(v2, b), c, false);
+  }
   static constexpr uint32_t kExp = 0x7f80u;  // exponent bits: all set in what is not finite
 };
 template <> struct Ops<F16> {
@@ -58,6 +68,10 @@ template <> struct Ops<F16> {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
   static __device__ __forceinline__ float lo(uint32_t w) { return f16_lo(w); }
   static __device__ __forceinline__ float hi(uint32_t w) { return f16_hi(w); }
+  typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, a), __builtin_bit_cast(v2, b), c, false);
+  }
   static constexpr uint32_t kExp = 0x7c00u;
 };
 
@@ -236,39 +250,273 @@ __device__ __forceinline__ float group4_max(float x) {
   return fmaxf(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
 }
 
-// O^T += V^T P^T over 32 keys, the probabilities as two operands of type E (the rounded value and what
-// the rounding left, so that they count with 16 bits or more).
+// ---- one query -----------------------------------------------------------------------------------
+// Four lanes take a key, 16 dimensions each: q.k on v_dot2 (codes widened to the queries' type, exactly),
+// P.V in fp32. A step is 32 keys of codes (a block) or 16 keys of 16-bit rows, 16 registers of raw data
+// either way, and two steps are in flight while one is computed. The block that is read from the ring
+// and the new row comes first, as two steps of the wavefront that has the fewest blocks.
+
+// The append of a call with sq <= 32 new rows, by one workgroup of every (row, head).
+template <typename T, int kThreads>
+__device__ __forceinline__ void append_rows(const Kv8Cache& c, const Kv8Args& a, int64_t sh, int len, const char* kn,
+                                            const char* vn, uint32_t (&red)[2][4]) {
+  const int tid = threadIdx.x, end = len + a.sq, done = len / kBlk;
+  char* kr = c.kr + sh * (kRing * kRowBytes16);
+  char* vr = c.vr + sh * (kRing * kRowBytes16);
+  for (int i = tid; i < a.sq * 16; i += kThreads) {
+    const int t = i >> 4, which = (i >> 3) & 1, ch = i & 7;
+    const char* src = (which ? vn + (int64_t)t * a.vns[1] : kn + (int64_t)t * a.kns[1]) + ch * 16;
+    store16((which ? vr : kr) + ((len + t) % kRing) * kRowBytes16 + ch * 16, load16(src));
+  }
+  if (end / kBlk == done) return;  // block `done` is not complete yet
+  u32x4 w[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  if (tid < 256) {
+    const int p = done * kBlk + (tid >> 3), ch = (tid & 7) * 16;
+    w[0] = load16((p >= len ? kn + (int64_t)(p - len) * a.kns[1] : kr + (p % kRing) * kRowBytes16) + ch);
+    w[1] = load16((p >= len ? vn + (int64_t)(p - len) * a.vns[1] : vr + (p % kRing) * kRowBytes16) + ch);
+  }
+  const int64_t blk = sh * c.n_blk + done;
+  quantize_block<T>(w[0], w[1], c.kc + blk * (kBlk * kHeadDim), c.vc + blk * (kBlk * kHeadDim), c.ks + blk, c.vs + blk, red);
+}
+
+template <typename T, bool RING, bool HAS_NEW, int kWaves>
+__global__ __launch_bounds__(kWaves * 64) void kv8_row_kernel(Kv8Cache c, Kv8Args a) {
+  static_assert(!HAS_NEW || (RING && kWaves >= 4), "appends need a ring and 256 threads");
+  __shared__ float sm_acc[kWaves][1][kHeadDim];
+  __shared__ float sm_m[kWaves][1];
+  __shared__ float sm_l[kWaves][1];
+  __shared__ uint32_t sm_red[2][4];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int kg = lane >> 2, r = lane & 3;  // key of a group of 16, quarter of its row
+
+  const int h = (int)(blockIdx.x % (unsigned)c.H);  // heads fastest: neighbours in the cache run together
+  const int b = (int)(blockIdx.x / (unsigned)c.H);
+  const int split = blockIdx.z;
+  const int slot = a.bidx ? a.bidx[b] : b;
+  const int len = a.seqlens ? a.seqlens[b] : c.Lk;
+  u32x4 q[2];
+  {
+    const char* qrow = a.q + b * a.qs[0] + h * a.qs[2] + r * 32;
+    q[0] = load16(qrow);
+    q[1] = load16(qrow + 16);
+  }
+  SlotRows rows{b, false};
+  if (HAS_NEW && a.bidx)
+    rows = slot_rows(a.B, slot, len, [&](int i) { return a.bidx[i]; }, [&](int i) { return a.seqlens[i]; });
+  const bool bad = slot < 0 || slot >= c.n_slots || len < 0 || len > c.Lk - (HAS_NEW ? 1 : 0) || rows.conflict;
+  const int key_lim = HAS_NEW ? len + 1 : len;
+  const int n_split_b = bad ? 1 : max(1, (key_lim + a.split_len - 1) / a.split_len);
+  if (split >= n_split_b) return;
+  if (!HAS_NEW && key_lim == 0 && !bad) {  // a row without keys
+    if (tid < kHeadDim / 2) *reinterpret_cast<uint32_t*>(a.o + b * a.os[0] + h * a.os[2] + tid * 4) = 0;
+    return;
+  }
+  const int k_begin = split * a.split_len;
+  const int k_end = bad ? k_begin : min(key_lim, k_begin + a.split_len);
+  const int k_last = k_end - 1;
+  const int64_t sh = slot_head(c, bad ? 0 : slot, h);
+  const uint8_t* kc = c.kc + sh * c.n_blk * (kBlk * kHeadDim) + r * 16;
+  const uint8_t* vc = c.vc + sh * c.n_blk * (kBlk * kHeadDim) + r * 16;
+  const float* ks = c.ks + sh * c.n_blk;
+  const float* vs = c.vs + sh * c.n_blk;
+  const char* kn = HAS_NEW ? a.kn + rows.src * a.kns[0] + h * a.kns[2] : nullptr;
+  const char* vn = HAS_NEW ? a.vn + rows.src * a.vns[0] + h * a.vns[2] : nullptr;
+  // blocks of this split: codes [blk0, blk1), then, where the ring begins inside it, one of 16-bit rows
+  const int blk0 = k_begin / kBlk;
+  const int blk1 = RING ? min(len, k_end) / kBlk : (k_end + kBlk - 1) / kBlk;
+  const int tail0 = blk1 * kBlk;
+  const int tails = RING && (blk1 - blk0) % kWaves == wave ? (k_end - tail0 + 15) / 16 : 0;  // 16-key steps, at most 2
+  const int codes = max(0, (blk1 - blk0 - wave + kWaves - 1) / kWaves);
+  const int steps = bad ? 0 : tails + codes;
+
+  struct Step {
+    u32x4 k[2], v[2];
+    float ks, vs;
+  };
+  auto row16 = [&](int p, const char* ring, const char* nw) __attribute__((always_inline)) {
+    return (HAS_NEW && p >= len ? nw : ring + sh * (kRing * kRowBytes16) + (p % kRing) * kRowBytes16) + r * 32;
+  };
+  auto load_step = [&](int i, Step& s) __attribute__((always_inline)) {
+    if (RING && i < tails) {
+      const int p = min(tail0 + 16 * i + kg, k_last);
+      const char* kp = row16(p, c.kr, kn);
+      const char* vp = row16(p, c.vr, vn);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s.k[u] = load16(kp + 16 * u);
+        s.v[u] = load16(vp + 16 * u);
+      }
+    } else {
+      const int blk = blk0 + wave + (i - tails) * kWaves;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int64_t at = (int64_t)min(blk * kBlk + 16 * u + kg, k_last) * kHeadDim;
+        s.k[u] = load16_stream(kc + at);
+        s.v[u] = load16_stream(vc + at);
+      }
+      s.ks = ks[blk];
+      s.vs = vs[blk];
+    }
+  };
+  float m = kNegBig, l = 0.f, acc[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  auto grow = [&](float s) __attribute__((always_inline)) {  // move the reference when a score exceeds it by > kTau
+    if (__any(s > m + kTau)) {
+      const float mn = s > m + kTau ? s : m;
+      const float alpha = fast_exp2(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] *= alpha;
+    }
+  };
+  auto quad_sum = [](float x) __attribute__((always_inline)) {
+    x += dpp_xor1(x);
+    return x + dpp_xor2(x);
+  };
+  auto compute_step = [&](int i, const Step& s) __attribute__((always_inline)) {
+    if (RING && i < tails) {
+      const bool seen = tail0 + 16 * i + kg <= k_last;
+      float d = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d = Ops<T>::dot2(q[j / 4][j % 4], s.k[j / 4][j % 4], d);
+      const float x = seen ? quad_sum(d) * a.c : -INFINITY;
+      grow(x);
+      const float p = fast_exp2(x - m);
+      l += p;
+      if (seen) {  // a masked key's value may not be finite: 0 times it would count
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          acc[2 * j] = __builtin_fmaf(p, Ops<T>::lo(s.v[j / 4][j % 4]), acc[2 * j]);
+          acc[2 * j + 1] = __builtin_fmaf(p, Ops<T>::hi(s.v[j / 4][j % 4]), acc[2 * j + 1]);
+        }
+      }
+    } else {
+      const int p0 = (blk0 + wave + (i - tails) * kWaves) * kBlk + kg;
+      const float ksc = a.c * s.ks;
+      float x[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const u32x4 k0 = widen8<T>(s.k[u][0], s.k[u][1], 1.f), k1 = widen8<T>(s.k[u][2], s.k[u][3], 1.f);
+        float d = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d = Ops<T>::dot2(q[0][j], k0[j], d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d = Ops<T>::dot2(q[1][j], k1[j], d);
+        x[u] = p0 + 16 * u <= k_last ? quad_sum(d) * ksc : -INFINITY;
+      }
+      grow(fmaxf(x[0], x[1]));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float e = fast_exp2(x[u] - m);
+        l += e;
+        const float p = e * s.vs;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(s.v[u][j], false);
+          const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(s.v[u][j], true);
+          acc[4 * j] = __builtin_fmaf(p, lo[0], acc[4 * j]);
+          acc[4 * j + 1] = __builtin_fmaf(p, lo[1], acc[4 * j + 1]);
+          acc[4 * j + 2] = __builtin_fmaf(p, hi[0], acc[4 * j + 2]);
+          acc[4 * j + 3] = __builtin_fmaf(p, hi[1], acc[4 * j + 3]);
+        }
+      }
+    }
+  };
+  Step A, B;
+  if (steps > 0) load_step(0, A);
+  if (steps > 1) load_step(1, B);
+  for (int i = 0; i < steps; i += 2) {
+    compute_step(i, A);
+    if (i + 2 < steps) load_step(i + 2, A);
+    if (i + 1 < steps) compute_step(i + 1, B);
+    if (i + 3 < steps) load_step(i + 3, B);
+  }
+
+  // The 16 key groups of the wavefront: a common maximum, then every halving of the lanes keeps half of the
+  // 16 sums, until each lane holds one dimension.
+  float mx = fmaxf(m, __shfl_xor(m, 4));
+  mx = group4_max(fmaxf(mx, __shfl_xor(mx, 8)));
+  const float f = fast_exp2(m - mx);
+  l *= f;
+#pragma unroll
+  for (int off = 4; off <= 32; off *= 2) l += __shfl_xor(l, off);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] *= f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[e]), __float_as_uint(acc[e + 8]), false, false);
+    acc[e] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[e]), __float_as_uint(acc[e + 4]), false, false);
+    acc[e] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float give = lane & 8 ? acc[e] : acc[e + 2];
+    acc[e] = (lane & 8 ? acc[e + 2] : acc[e]) + __shfl_xor(give, 8);
+  }
+  const float give = lane & 4 ? acc[0] : acc[1];
+  const float one = (lane & 4 ? acc[1] : acc[0]) + __shfl_xor(give, 4);
+  const int dim = 16 * r + 8 * (lane >> 5) + 4 * ((lane >> 4) & 1) + 2 * ((lane >> 3) & 1) + ((lane >> 2) & 1);
+  sm_acc[wave][0][dim] = one;
+  if (lane == 0) {
+    sm_m[wave][0] = mx;
+    sm_l[wave][0] = l;
+  }
+  __syncthreads();
+  kv_finish<T, 1, kWaves>(a, b, 0, 1, 1, h, split, n_split_b, bad, sm_acc, sm_m, sm_l);
+  if constexpr (HAS_NEW) {
+    if (!bad && rows.src == b && split == n_split_b - 1) append_rows<T, kWaves * 64>(c, a, sh, len, kn, vn, sm_red);
+  }
+}
+
+// ---- 2 and more queries ----------------------------------------------------------------------------
+
+// Transposing LDS read of bytes (ds_read_b64_tr_b8): within each 16-lane group, lane i receives byte i%8
+// of the 8-byte chunks read by lanes 2c + i/8 (c = 0..7), in the order of c.
+__device__ __forceinline__ u32x2 read_tr8(const uint8_t* p) {
+#if __HIP_DEVICE_COMPILE__
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(uint32_t)(uintptr_t)p));
+#else
+  (void)p;
+  return u32x2{0, 0};
+#endif
+}
+
+// The lane's 8 probabilities as two operands of type E: the rounded values and what the rounding left,
+// so that they count with 16 bits or more.
 template <typename E>
-__device__ __forceinline__ void pv_step(const uint16_t* vt_lane, const float (&p)[8], f32x4 (&o)[4]) {
-  u32x4 ph, pl;
+__device__ __forceinline__ void split_p(const float (&p)[8], u32x4& ph, u32x4& pl) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     ph[j] = Ops<E>::pack(p[2 * j], p[2 * j + 1]);
     pl[j] = Ops<E>::pack(p[2 * j] - Ops<E>::lo(ph[j]), p[2 * j + 1] - Ops<E>::hi(ph[j]));
   }
-#pragma unroll
-  for (int db = 0; db < 4; ++db) {
-    const u32x2 lo = read_tr16(vt_lane + 16 * db);
-    const u32x2 hi = read_tr16(vt_lane + 16 * kVPitch + 16 * db);
-    const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
-    o[db] = Ops<E>::mfma(v, pl, o[db]);
-    o[db] = Ops<E>::mfma(v, ph, o[db]);
-  }
 }
 
-// SQ: query rows a workgroup (1, 8 or 16). HAS_NEW: the call appends.
-template <typename T, int SQ, bool HAS_NEW, int kWaves>
+constexpr int kV8Pitch = kHeadDim + 16;  // row pitch (bytes) of a tile of codes
+
+// SQ: query rows a workgroup (8 or 16). RING: the cache has one; HAS_NEW: the call appends.
+template <typename T, int SQ, bool RING, bool HAS_NEW, int kWaves>
 __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv8Args a) {
+  static_assert(!HAS_NEW || RING, "appends need a ring");
   __shared__ float sm_acc[kWaves][SQ][kHeadDim];
   __shared__ float sm_m[kWaves][SQ];
   __shared__ float sm_l[kWaves][SQ];
-  __shared__ __attribute__((aligned(16))) uint16_t sm_v[kWaves][kBlk * kVPitch];
+  // one V tile a wavefront: 32 rows of codes, or of 16-bit values
+  __shared__ __attribute__((aligned(16))) uint8_t sm_v[kWaves][RING ? kBlk * kVPitch * 2 : kBlk * kV8Pitch];
   __shared__ uint32_t sm_red[2][4];
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int qi = lane & 15, gq = lane >> 4;  // query slot (and key row) of this lane, 16-lane group
 
-  const int h = (int)(blockIdx.x % (unsigned)c.H);  // heads fastest: neighbours in the cache run together
+  const int h = (int)(blockIdx.x % (unsigned)c.H);
   const int bq = (int)(blockIdx.x / (unsigned)c.H);
   const int b = bq / a.n_qblocks;
   const int t0 = (bq % a.n_qblocks) * SQ;
@@ -277,6 +525,13 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
 
   const int slot = a.bidx ? a.bidx[b] : b;
   const int len = a.seqlens ? a.seqlens[b] : c.Lk;
+  // Q^T operand halves: query t0 + qi, dims 16 gq + 8 dh .. + 7
+  u32x4 qop[2];
+  {
+    const char* qrow = a.q + b * a.qs[0] + (t0 + min(qi, nq - 1)) * a.qs[1] + h * a.qs[2] + gq * 32;
+    qop[0] = load16(qrow);
+    qop[1] = load16(qrow + 16);
+  }
   SlotRows rows{b, false};
   if (HAS_NEW && a.bidx)
     rows = slot_rows(a.B, slot, len, [&](int i) { return a.bidx[i]; }, [&](int i) { return a.seqlens[i]; });
@@ -293,171 +548,183 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
   const int k_begin = split * a.split_len;  // a multiple of 32
   const int k_end = bad ? k_begin : min(key_lim, k_begin + a.split_len);
   const int k_last = k_end - 1;
-  int lim = k_last;  // last key this lane's query may see (slots past the block's rows see none)
-  if (HAS_NEW) lim = min(lim, len + t0 + qi);
-  if (qi >= nq) lim = -1;
-
-  // Q^T operand halves: query t0 + qi, dims 16 gq + 8 dh .. + 7
-  u32x4 qop[2];
-  {
-    const char* qrow = a.q + b * a.qs[0] + (t0 + min(qi, nq - 1)) * a.qs[1] + h * a.qs[2] + gq * 32;
-    qop[0] = load16(qrow);
-    qop[1] = load16(qrow + 16);
-  }
+  // last key this lane's query may see
+  const int lim = HAS_NEW ? min(k_last, len + t0 + qi) : k_last;
 
   const int64_t sh = slot_head(c, bad ? 0 : slot, h);
   const uint8_t* kc = c.kc + sh * c.n_blk * (kBlk * kHeadDim);
   const uint8_t* vc = c.vc + sh * c.n_blk * (kBlk * kHeadDim);
   const float* ks = c.ks + sh * c.n_blk;
   const float* vs = c.vs + sh * c.n_blk;
-  char* kr = c.kr + sh * (kRing * kRowBytes16);
-  char* vr = c.vr + sh * (kRing * kRowBytes16);
   const char* kn = HAS_NEW ? a.kn + rows.src * a.kns[0] + h * a.kns[2] : nullptr;
   const char* vn = HAS_NEW ? a.vn + rows.src * a.vns[0] + h * a.vns[2] : nullptr;
-  const int code_blks = c.kr ? len / kBlk : 0x7fffffff;  // blocks below are read as codes
-  auto row16 = [&](int p, const char* ring, const char* nw, int64_t step) __attribute__((always_inline)) {
-    return HAS_NEW && p >= len ? nw + (int64_t)(p - len) * step : ring + (p % kRing) * kRowBytes16;
+  // blocks of this split: codes [blk0, blk1), then 16-bit rows, dealt on to the wavefronts in turn
+  const int blk0 = k_begin / kBlk;
+  const int blk1 = bad ? blk0 : RING ? min(len, k_end) / kBlk : (k_end + kBlk - 1) / kBlk;
+  const int blk2 = (k_end + kBlk - 1) / kBlk;
+
+  uint8_t* vt = sm_v[wave];
+  float m = kNegBig, l = 0.f;
+  f32x4 o[4];  // O^T blocks: dims 16 db + 4 gq + i, query qi
+#pragma unroll
+  for (int db = 0; db < 4; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // The running maximum and the probabilities of one block's scores (times `scale`, log2 units): keys
+  // 16 kb + 4 gq + i of it; those past `last` do not count.
+  auto softmax = [&](const f32x4 (&s)[2], float scale, int last, float (&p)[8]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3];
+    if (__any(last < kBlk - 1)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if ((j >> 2) * 16 + 4 * gq + (j & 3) > last) p[j] = -INFINITY;
+    }
+    float mb = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+    mb = group4_max(mb) * scale;
+    if (__any(mb > m + kTau)) {
+      const float mn = mb > m + kTau ? mb : m;
+      const float alpha = fast_exp2(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int db = 0; db < 4; ++db) o[db] *= alpha;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = fast_exp2(__builtin_fmaf(p[j], scale, -m));
+      l += p[j];
+    }
   };
 
-  // Loads of block blk. Codes: kw[kb] is key 16 kb + qi, dims 16 gq ..; vw[i] piece lane + 64 i of the
-  // tile's 128 (row piece / 4). 16-bit rows: kw[2 kb + half], vw[i] piece lane + 64 i of 256.
-  // Rows past the end re-read the last key.
-  u32x4 kw[4], vw[4];
-  float kscale = 0.f, vscale = 0.f;
-  auto load_block = [&](int blk) __attribute__((always_inline)) {
-    const int p0 = blk * kBlk;
-    if (blk < code_blks) {
+  // ---- blocks of codes: kw[i] is key 16 i + qi, dims 16 gq ..; vw[i] piece lane + 64 i of the tile's 128
+  // (row piece / 4). Two blocks in flight while one is computed. Rows past the end re-read the last key.
+  struct Codes {
+    u32x4 k[2], v[2];
+    float ks, vs;
+  };
+  auto load_codes = [&](int blk, Codes& x) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        kw[i] = load16_stream(kc + (int64_t)min(p0 + 16 * i + qi, k_last) * kHeadDim + 16 * gq);
-        const int piece = lane + 64 * i;
-        vw[i] = load16_stream(vc + (int64_t)min(p0 + (piece >> 2), k_last) * kHeadDim + (piece & 3) * 16);
-      }
-      kscale = ks[blk];
-      vscale = vs[blk];
-    } else {
+    for (int i = 0; i < 2; ++i) {
+      const int piece = lane + 64 * i;
+      x.k[i] = load16_stream(kc + (int64_t)min(blk * kBlk + 16 * i + qi, k_last) * kHeadDim + 16 * gq);
+      x.v[i] = load16_stream(vc + (int64_t)min(blk * kBlk + (piece >> 2), k_last) * kHeadDim + (piece & 3) * 16);
+    }
+    x.ks = ks[blk];
+    x.vs = vs[blk];
+  };
+  auto compute_codes = [&](int blk, const Codes& x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int piece = lane + 64 * i;
+      *reinterpret_cast<u32x4*>(vt + (piece >> 2) * kV8Pitch + (piece & 3) * 16) = x.v[i];
+    }
+    f32x4 s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      s[kb] = Ops<T>::mfma(widen8<T>(x.k[kb][0], x.k[kb][1], 1.f), qop[0], f32x4{0.f, 0.f, 0.f, 0.f});
+      s[kb] = Ops<T>::mfma(widen8<T>(x.k[kb][2], x.k[kb][3], 1.f), qop[1], s[kb]);
+    }
+    float p[8];
+    softmax(s, a.c * x.ks, k_last - blk * kBlk, p);
+    u32x4 ph, pl;
+    split_p<Bf16>(p, ph, pl);
+    // V^T operands in the scores' key order: keys 4 gq + (0..3) and 16 + 4 gq + (0..3), dims 16 db + qi
+    const int row = (qi >> 1) < 4 ? 4 * gq + (qi >> 1) : 12 + 4 * gq + (qi >> 1);
+    const uint8_t* at = vt + row * kV8Pitch + (qi & 1) * 8;
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+      const u32x2 w = read_tr8(at + 16 * db);
+      const u32x4 v = widen8<Bf16>(w[0], w[1], x.vs);
+      o[db] = Ops<Bf16>::mfma(v, pl, o[db]);
+      o[db] = Ops<Bf16>::mfma(v, ph, o[db]);
+    }
+  };
+  int blk = blk0 + wave;
+  Codes A, B;
+  if (blk < blk1) load_codes(blk, A);
+  if (blk + kWaves < blk1) load_codes(blk + kWaves, B);
+
+  // ---- blocks of 16-bit rows: the ring's, then the new ones. Values that are not finite stay out of the
+  // matrix product, where a masked key's 0 times NaN would be NaN (and an infinity times the two parts of P
+  // too), and count for the queries that see their key, one by one.
+  if constexpr (RING) {
+    auto row16 = [&](int p, const char* ring, const char* nw, int64_t step) __attribute__((always_inline)) {
+      return HAS_NEW && p >= len ? nw + (int64_t)(p - len) * step : ring + sh * (kRing * kRowBytes16) + (p % kRing) * kRowBytes16;
+    };
+    const int64_t kstep = HAS_NEW ? a.kns[1] : 0, vstep = HAS_NEW ? a.vns[1] : 0;
+    uint16_t* vt16 = reinterpret_cast<uint16_t*>(vt);
+    for (int tb = blk1 + (wave + kWaves - (blk1 - blk0) % kWaves) % kWaves; tb < blk2; tb += kWaves) {
+      const int p0 = tb * kBlk;
+      u32x4 kw[4], vw[4];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        const char* kp = row16(min(p0 + 16 * kb + qi, k_last), kr, kn, HAS_NEW ? a.kns[1] : 0) + gq * 32;
+        const char* kp = row16(min(p0 + 16 * kb + qi, k_last), c.kr, kn, kstep) + gq * 32;
         kw[2 * kb] = load16(kp);
         kw[2 * kb + 1] = load16(kp + 16);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int piece = lane + 64 * i;
-        vw[i] = load16(row16(min(p0 + (piece >> 3), k_last), vr, vn, HAS_NEW ? a.vns[1] : 0) + (piece & 7) * 16);
+        vw[i] = load16(row16(min(p0 + (piece >> 3), k_last), c.vr, vn, vstep) + (piece & 7) * 16);
       }
-    }
-  };
-
-  uint16_t* vt = sm_v[wave];
-  const uint16_t* vt_lane = vt + (4 * gq + (qi >> 2)) * kVPitch + 4 * (qi & 3);
-  float m, l;
-  f32x4 o[4];  // O^T blocks: dims 16 db + 4 gq + i, query qi
-
-  // SAFE: 16-bit values that are not finite count for the queries that see their key, and for no other
-  // (a masked key's probability of 0 times NaN is NaN, and an infinity times the two parts of P also).
-  bool safe = false;
-  for (;;) {
-    m = kNegBig;
-    l = 0.f;
-#pragma unroll
-    for (int db = 0; db < 4; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int blk = k_begin / kBlk + wave;
-    if (blk * kBlk < k_end) load_block(blk);
-    for (; blk * kBlk < k_end; blk += kWaves) {
-      const int p0 = blk * kBlk;
-      const bool codes = blk < code_blks;
       f32x4 s[2];
-      float sscale = a.c;
-      const float vsc = vscale;
-      if (codes) {
-        sscale = a.c * kscale;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          s[kb] = Ops<T>::mfma(widen8<T>(kw[kb][0], kw[kb][1], 1.f), qop[0], f32x4{0.f, 0.f, 0.f, 0.f});
-          s[kb] = Ops<T>::mfma(widen8<T>(kw[kb][2], kw[kb][3], 1.f), qop[1], s[kb]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int piece = lane + 64 * i;
-          uint16_t* dst = &vt[(piece >> 2) * kVPitch + (piece & 3) * 16];
-          *reinterpret_cast<u32x4*>(dst) = widen8<Bf16>(vw[i][0], vw[i][1], vsc);
-          *reinterpret_cast<u32x4*>(dst + 8) = widen8<Bf16>(vw[i][2], vw[i][3], vsc);
-        }
-      } else {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          s[kb] = Ops<T>::mfma(kw[2 * kb], qop[0], f32x4{0.f, 0.f, 0.f, 0.f});
-          s[kb] = Ops<T>::mfma(kw[2 * kb + 1], qop[1], s[kb]);
-        }
-        if (safe) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              if ((vw[i][w] & Ops<T>::kExp) == Ops<T>::kExp) vw[i][w] &= 0xffff0000u;
-              if (((vw[i][w] >> 16) & Ops<T>::kExp) == Ops<T>::kExp) vw[i][w] &= 0xffffu;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int piece = lane + 64 * i;
-          *reinterpret_cast<u32x4*>(&vt[(piece >> 3) * kVPitch + (piece & 7) * 8]) = vw[i];
-        }
+      for (int kb = 0; kb < 2; ++kb) {
+        s[kb] = Ops<T>::mfma(kw[2 * kb], qop[0], f32x4{0.f, 0.f, 0.f, 0.f});
+        s[kb] = Ops<T>::mfma(kw[2 * kb + 1], qop[1], s[kb]);
       }
-      if ((blk + kWaves) * kBlk < k_end) load_block(blk + kWaves);
-      // ---- softmax of the lane's 8 scores (log2 units): keys 16 kb + 4 gq + i ----
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const bool lo = (vw[i][w] & Ops<T>::kExp) == Ops<T>::kExp;
+          const bool hi = ((vw[i][w] >> 16) & Ops<T>::kExp) == Ops<T>::kExp;
+          odd = odd || lo || hi;
+          vw[i][w] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0xffffu : 0xffffffffu);
+        }
+        const int piece = lane + 64 * i;
+        *reinterpret_cast<u32x4*>(&vt16[(piece >> 3) * kVPitch + (piece & 7) * 8]) = vw[i];
+      }
       float p[8];
+      softmax(s, a.c, lim - p0, p);
+      u32x4 ph, pl;
+      split_p<T>(p, ph, pl);
+      const uint16_t* at = vt16 + (4 * gq + (qi >> 2)) * kVPitch + 4 * (qi & 3);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          p[kb * 4 + i] = p0 + kb * 16 + 4 * gq + i <= lim ? s[kb][i] * sscale : -INFINITY;
-      float mb = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-      mb = group4_max(mb);
-      if (__any(mb > m + kTau)) {
-        const float mn = mb > m + kTau ? mb : m;
-        const float alpha = fast_exp2(m - mn);
-        m = mn;
-        l *= alpha;
-#pragma unroll
-        for (int db = 0; db < 4; ++db) o[db] *= alpha;
+      for (int db = 0; db < 4; ++db) {
+        const u32x2 v0 = read_tr16(at + 16 * db), v1 = read_tr16(at + 16 * kVPitch + 16 * db);
+        const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
+        o[db] = Ops<T>::mfma(v, pl, o[db]);
+        o[db] = Ops<T>::mfma(v, ph, o[db]);
       }
+      if (__any(odd)) {
+        for (int j = 0; j < kBlk; ++j) {
+          float pj = 0.f;  // the probability of key j, from the lane and register that hold it
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = fast_exp2(p[j] - m);
-        l += p[j];
-      }
-      if (codes) {
-        pv_step<Bf16>(vt_lane, p, o);
-      } else {
-        pv_step<T>(vt_lane, p, o);
-        if (safe) {
-          for (int j = 0; j < kBlk; ++j) {
-            const float pj = __shfl(p[(j >> 4) * 4 + (j & 3)], qi + 16 * ((j & 15) >> 2));
-            const char* row = row16(min(p0 + j, k_last), vr, vn, HAS_NEW ? a.vns[1] : 0);
+          for (int r = 0; r < 8; ++r) {
+            const float x = __shfl(p[r], qi + 16 * ((j & 15) >> 2));
+            if (r == (j >> 4) * 4 + (j & 3)) pj = x;
+          }
+          if (p0 + j > lim) continue;
+          const char* row = row16(min(p0 + j, k_last), c.vr, vn, vstep);
 #pragma unroll
-            for (int db = 0; db < 4; ++db) {
-              const uint2 w = *reinterpret_cast<const uint2*>(row + (16 * db + 4 * gq) * 2);
+          for (int db = 0; db < 4; ++db) {
+            const uint2 w = *reinterpret_cast<const uint2*>(row + (16 * db + 4 * gq) * 2);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t x = ((i & 2) ? w.y : w.x) >> (16 * (i & 1)) & 0xffffu;
-                if ((x & Ops<T>::kExp) == Ops<T>::kExp && p0 + j <= lim) o[db][i] += pj * Ops<T>::lo(x);
-              }
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t x = ((i & 2) ? w.y : w.x) >> (16 * (i & 1)) & 0xffffu;
+              if ((x & Ops<T>::kExp) == Ops<T>::kExp) o[db][i] += pj * Ops<T>::lo(x);
             }
           }
         }
       }
     }
-    if (safe) break;
-    bool nan = false;
-#pragma unroll
-    for (int db = 0; db < 4; ++db)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) nan = nan || o[db][i] != o[db][i];
-    if (!__any(nan && qi < nq)) break;
-    safe = true;
+  }
+  for (; blk < blk1; blk += 2 * kWaves) {
+    compute_codes(blk, A);
+    if (blk + 2 * kWaves < blk1) load_codes(blk + 2 * kWaves, A);
+    if (blk + kWaves < blk1) compute_codes(blk + kWaves, B);
+    if (blk + 3 * kWaves < blk1) load_codes(blk + 3 * kWaves, B);
   }
 
   // row sums: the four lane groups hold different keys of the same query
@@ -466,8 +733,7 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
   if (qi < nq) {
 #pragma unroll
     for (int db = 0; db < 4; ++db)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sm_acc[wave][qi][16 * db + 4 * gq + i] = o[db][i];
+      *reinterpret_cast<f32x4*>(&sm_acc[wave][qi][16 * db + 4 * gq]) = o[db];
     if (gq == 0) {
       sm_m[wave][qi] = m;
       sm_l[wave][qi] = l;
@@ -476,39 +742,41 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
   __syncthreads();
   kv_finish<T, SQ, kWaves>(a, b, t0, nq, a.n_qblocks > 1 ? SQ : nq, h, split, n_split_b, bad, sm_acc, sm_m, sm_l);
 
-  // ---- the append (sq <= 32): by the last query block's last split of the row that gives the new rows ----
-  if constexpr (HAS_NEW) {
-    if (!a.append || bad || rows.src != b || t0 + nq != a.sq || split != n_split_b - 1) return;
-    const int end = len + a.sq, done = len / kBlk;
-    for (int i = tid; i < a.sq * 16; i += kWaves * 64) {
-      const int t = i >> 4, which = (i >> 3) & 1, ch = i & 7;
-      const char* src = (which ? vn + (int64_t)t * a.vns[1] : kn + (int64_t)t * a.kns[1]) + ch * 16;
-      store16((which ? vr : kr) + ((len + t) % kRing) * kRowBytes16 + ch * 16, load16(src));
-    }
-    if (end / kBlk > done) {  // block `done` is complete
-      u32x4 w[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-      if (tid < 256) {
-        const int p = done * kBlk + (tid >> 3);
-        w[0] = load16(row16(p, kr, kn, a.kns[1]) + (tid & 7) * 16);
-        w[1] = load16(row16(p, vr, vn, a.vns[1]) + (tid & 7) * 16);
-      }
-      const int64_t code = (sh * c.n_blk + done) * (kBlk * kHeadDim);
-      quantize_block<T>(w[0], w[1], c.kc + code, c.vc + code, c.ks + sh * c.n_blk + done, c.vs + sh * c.n_blk + done, sm_red);
-    }
+  if constexpr (HAS_NEW) {  // the last query block's last split of the row that gives the new rows
+    if (a.append && !bad && rows.src == b && t0 + nq == a.sq && split == n_split_b - 1)
+      append_rows<T, kWaves * 64>(c, a, sh, len, kn, vn, sm_red);
   }
 }
 
 template <typename T, int SQ, int W>
 void launch_attn(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.B * a.n_qblocks * c.H), 1, a.n_splits), block(W * 64);
-  if (a.kn) hipLaunchKernelGGL((kv8_attn_kernel<T, SQ, true, W>), grid, block, 0, stream, c, a);
-  else hipLaunchKernelGGL((kv8_attn_kernel<T, SQ, false, W>), grid, block, 0, stream, c, a);
+  if (a.kn) hipLaunchKernelGGL((kv8_attn_kernel<T, SQ, true, true, W>), grid, block, 0, stream, c, a);
+  else if (c.kr) hipLaunchKernelGGL((kv8_attn_kernel<T, SQ, true, false, W>), grid, block, 0, stream, c, a);
+  else hipLaunchKernelGGL((kv8_attn_kernel<T, SQ, false, false, W>), grid, block, 0, stream, c, a);
+}
+
+template <typename T, int W>
+void launch_row(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)a.B * c.H), 1, a.n_splits), block(W * 64);
+  if (a.kn) hipLaunchKernelGGL((kv8_row_kernel<T, true, true, W>), grid, block, 0, stream, c, a);
+  else if (c.kr) hipLaunchKernelGGL((kv8_row_kernel<T, true, false, W>), grid, block, 0, stream, c, a);
+  else hipLaunchKernelGGL((kv8_row_kernel<T, false, false, W>), grid, block, 0, stream, c, a);
+}
+
+template <typename T>
+void launch_row_t(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
+  if (a.waves == 16) launch_row<T, 16>(c, a, stream);
+  else if (a.waves == 8) launch_row<T, 8>(c, a, stream);
+  else launch_row<T, 4>(c, a, stream);
 }
 
 template <typename T>
 void launch_attn_t(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
-  if (a.sq == 1) launch_attn<T, 1, 4>(c, a, stream);
+  if (a.sq == 1) launch_row_t<T>(c, a, stream);
+  else if (a.sq <= 8 && a.waves == 8) launch_attn<T, 8, 8>(c, a, stream);
   else if (a.sq <= 8) launch_attn<T, 8, 4>(c, a, stream);
+  else if (a.waves == 8) launch_attn<T, 16, 8>(c, a, stream);
   else launch_attn<T, 16, 4>(c, a, stream);
 }
 
@@ -522,20 +790,33 @@ void launch_write_t(const Kv8Cache& c, const Kv8WriteArgs& a, const Id* slots, h
 
 }  // namespace
 
-// Splits of a row's keys (see launch_kv8_attn's callers for the workspace): rows that are fewer than
-// half the CUs and hold 768 keys or more.
+// One workgroup walks a row unless few long rows leave most of the chip idle: merging splits costs about
+// 2 us (publish, count, read back). One query, bf16, cold caches in a graph, us, unsplit / split:
+//   1 stream of 20 heads: 500 positions 4.6 / 6.0, 1000 5.3 / 6.3, 1500 6.4 / 6.9, 3000 11.8 / 7.6, 6000
+//   19.1 / 8.9, 20000 58.3 / 14.8; 2 streams: 1500 7.8 / 7.2, 3000 12.0 / 8.4; 4: 1500 8.1 / 8.2, 3000
+//   12.2 / 9.7, 6000 22.7 / 14.8; 6: 1500 8.4 / 8.7, 6000 24.0 / 19.7; 8: 1500 9.0 / 10.2.
+// More splits than fill the CUs once gain nothing (4 streams of 3000: 3 splits 9.7, 4 10.7).
+constexpr int64_t kCus = 256;
+constexpr int64_t kSplitMinLk = 2048;
+constexpr int64_t kSplitMinKeys = 512;
+// Eight wavefronts a workgroup while the launch has no more workgroups than CUs, else four. Us, eight /
+// four: cross over 1500, 1 stream 6.4 / 7.7, 8 9.0 / 11.2, 13 (260 workgroups) 14.6 / 13.0, 32 22.6 / 23.2;
+// self of 440, 4 streams 6.0 / 6.9, 52 of 447 14.8 / 12.9. Sixteen are slower from 8 streams on. Five
+// queries follow the same lines: cross over 1500, 1 stream 7.6 / 9.2, 8 10.1 / 12.3, 16 16.3 / 16.0; 6000
+// positions, 1 stream, 1 / 8 splits 23.3 / 9.6.
 void kv8_plan(int64_t B, int64_t sq, int64_t H, int64_t Lk, Kv8Args* a) {
   const int block = sq == 1 ? 1 : sq <= 8 ? 8 : 16;
   a->n_qblocks = (int)((sq + block - 1) / block);
   a->n_splits = 1;
   a->split_len = (int)((Lk + kBlk - 1) / kBlk * kBlk);
   const int64_t units = B * a->n_qblocks * H;
-  if (units <= 128 && Lk >= 768) {
-    const int64_t want = std::min<int64_t>(std::min<int64_t>((160 + units - 1) / units, (Lk + 191) / 192), kMaxMergeSplits);
-    const int64_t len = ((Lk + want - 1) / want + 63) / 64 * 64;
+  if (units <= kCus / 2 && Lk >= kSplitMinLk) {
+    const int64_t want = std::min<int64_t>(std::min<int64_t>(kCus / units, Lk / kSplitMinKeys), kMaxMergeSplits);
+    const int64_t len = ((Lk + want - 1) / want + kBlk - 1) / kBlk * kBlk;
     a->split_len = (int)len;
     a->n_splits = (int)((Lk + len - 1) / len);
   }
+  a->waves = units * a->n_splits <= kCus ? 8 : 4;
 }
 
 size_t kv8_workspace_bytes(int64_t B, int64_t sq, int64_t H, int64_t Lk) {
