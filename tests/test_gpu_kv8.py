@@ -179,7 +179,8 @@ def test_cross_attention(cuda, dtype, sq, L):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B,sq,H,L", [(1, 1, 20, 1500), (3, 1, 4, 1500), (1, 5, 20, 1500), (2, 12, 3, 1499), (1, 1, 2, 6000),
-                                      (7, 1, 20, 1500), (1, 224, 2, 1500), (1, 33, 1, 20000)])
+                                      (7, 1, 20, 1500), (1, 224, 2, 1500), (1, 33, 1, 20000), (3, 1, 20, 3001),
+                                      (2, 5, 4, 6000), (1, 1, 1, 40000)])
 def test_long_cross_attention(cuda, dtype, B, sq, H, L):
     """Rows whose keys are split over workgroups, ragged so that some splits have nothing; called twice."""
     from whisperdrz_amd import flash_attn_with_kvcache8
@@ -247,7 +248,8 @@ def test_append(cuda, dtype, sq):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("B,sq,H,L,filled", [(1, 1, 20, 1500, 1300), (2, 5, 3, 2000, 1991), (1, 20, 4, 900, 850)])
+@pytest.mark.parametrize("B,sq,H,L,filled", [(1, 1, 20, 1500, 1300), (2, 5, 3, 3000, 2991), (1, 20, 4, 900, 850), (1, 1, 2, 4000, 3999),
+                                             (2, 30, 1, 2100, 2065)])
 def test_append_behind_long_histories(cuda, dtype, B, sq, H, L, filled):
     """Split rows that append."""
     from whisperdrz_amd import flash_attn_with_kvcache8
@@ -496,7 +498,7 @@ def test_cache_past_32_bit_offsets(cuda):
     assert not c.k_codes[: S - 2].view(torch.uint8).any()
 
 
-@pytest.mark.parametrize("B,sq,L", [(2, 1, 200), (1, 3, 1500), (2, 40, 200)])
+@pytest.mark.parametrize("B,sq,L", [(2, 1, 200), (1, 3, 3000), (2, 40, 200)])
 def test_graph_replays(cuda, B, sq, L):
     """A captured append whose inputs change between replays, eager work between them; two graphs of split
     rows share no workspace."""
@@ -533,7 +535,7 @@ def test_graph_replays(cuda, B, sq, L):
 def test_calls_on_two_streams(cuda):
     from whisperdrz_amd import flash_attn_with_kvcache8
 
-    c = _cache(cuda, torch.float16, 1, 1500, 20, False, 5)
+    c = _cache(cuda, torch.float16, 1, 4000, 20, False, 5)
     g = _gen(cuda, 3)
     qs = [_randn(g, 1, 1, 20, 64, dtype=torch.float16) for _ in range(2)]
     want = [flash_attn_with_kvcache8(q, c) for q in qs]

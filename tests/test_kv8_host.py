@@ -162,8 +162,8 @@ def _attn(cache="default", dtype=2, q=P, qs=(128, 128, 64, 1), k=P, ks=(128, 128
     (dict(sq=101), 1, "exceeds"), (dict(q=None), 1, "q is NULL"), (dict(q=P + 2), 1, "aligned"),
     (dict(qs=(128, 128, 64, 2)), 1, "stride"), (dict(ks=(128, 4, 64, 1)), 1, "aligned"), (dict(vs=None), 1, "NULL"),
     (dict(os=(3, 128, 64, 1)), 1, "aligned"), (dict(o=None), 1, "out is NULL"),
-    (dict(k=None, v=None, k_ring=None, v_ring=None, max_seq=1500, B=1), 4, "workspace"),
-    (dict(k=None, v=None, k_ring=None, v_ring=None, max_seq=1500, B=1, ws=P + 16, nbytes=1 << 20), 1, "256-byte"),
+    (dict(k=None, v=None, k_ring=None, v_ring=None, max_seq=3000, B=1), 4, "workspace"),
+    (dict(k=None, v=None, k_ring=None, v_ring=None, max_seq=3000, B=1, ws=P + 16, nbytes=1 << 20), 1, "256-byte"),
 ])
 def test_attention_refusals(kw, code, word):
     rc, msg = _attn(**kw)

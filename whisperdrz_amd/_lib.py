@@ -6,6 +6,7 @@ missing or fails to load, every compute entry point raises ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 from pathlib import Path
@@ -262,8 +263,10 @@ def last_error() -> str:
     return load().wdrz_last_error().decode()
 
 
-def strides3(s) -> ctypes.Array:
-    return (ctypes.c_int64 * 3)(s[0], s[1], s[2])
+@functools.lru_cache(maxsize=4096)
+def strides(s: tuple) -> ctypes.Array:
+    """:func:`strides4` of a tuple, built once per value (the entry points only read it)."""
+    return (ctypes.c_int64 * 4)(*s)
 
 
 def strides4(s) -> ctypes.Array:

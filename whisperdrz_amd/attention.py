@@ -18,6 +18,7 @@ only routes ``q.is_cuda`` calls to the accelerated implementation).
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
@@ -63,24 +64,11 @@ def _stream_handle() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-class _on:
-    """``with _on(device) as stream``: the handle of ``device``'s current stream, with that device current."""
-
-    __slots__ = ("index", "other")
-
-    def __init__(self, device: torch.device) -> None:
-        current = torch.cuda.current_device()
-        self.index = current if device.index is None else device.index
-        self.other = None if self.index == current else torch.cuda.device(self.index)
-
-    def __enter__(self) -> int:
-        if self.other is not None:
-            self.other.__enter__()
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.other is not None:
-            self.other.__exit__(*exc)
+# The handle of a device's current stream and the current device's index. The public calls build a Stream
+# object and look at the initialisation each time: 1 us of a 7 us call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _raise(rc: int, what: str) -> None:
@@ -260,11 +248,12 @@ def flash_attn_with_kvcache(
 
 def _check_ids(name: str, t: torch.Tensor, B: int, device: torch.device) -> torch.Tensor:
     """An int32 [B] tensor on ``device`` as it is, anything else as :func:`_as_int32` takes it."""
-    if t.__class__ is torch.Tensor and t.dtype is torch.int32 and t.device == device and t.shape == (B,) and t.is_contiguous():
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == device and t.shape == (B,) and t.is_contiguous():
         return t
     return _as_int32(name, t, B, device)
 
 
+@functools.lru_cache(maxsize=1024)
 def kvcache8_workspace_size(batch: int, sq: int, n_heads: int, max_seq: int) -> int:
     """Bytes of split-KV workspace :func:`flash_attn_with_kvcache8` needs for these sizes."""
     return int(_lib.load().wdrz_attn_kvcache8_workspace_size(batch, sq, n_heads, max_seq))
@@ -301,72 +290,70 @@ def flash_attn_with_kvcache8(
     """
     if not (isinstance(q, torch.Tensor) and q.is_cuda):
         _check_cuda("q", q, q.device if isinstance(q, torch.Tensor) else None)
-    device = q.device
+    device, shape, dtype = q.device, q.shape, q.dtype
     if cache.device != device:
         raise RuntimeError(f"the cache is on {cache.device}, expected {device}")
-    if q.dim() != 4:
+    if len(shape) != 4:
         raise ValueError("q must be 4-D ([B, sq, H, 64])")
-    B, sq, H, D = q.shape
+    B, sq, H, D = shape
     if H != cache.n_heads or D != cache.head_dim:
         raise ValueError(f"cache heads/head_dim {(cache.n_heads, cache.head_dim)} do not match q {(H, D)}")
-    dt = _DTYPES16.get(q.dtype)
+    dt = _DTYPES16.get(dtype)
     if dt is None:
-        raise TypeError(f"q: dtype {q.dtype} is not supported (bfloat16, float16)")
-    if cache.has_ring and q.dtype != cache.dtype:
+        raise TypeError(f"q: dtype {dtype} is not supported (bfloat16, float16)")
+    if cache.has_ring and dtype != cache.dtype:
         raise TypeError(f"q must have the cache's dtype {cache.dtype}")
-    has_new = k is not None or v is not None
-    if has_new:
+    k_ptr = k_strides = v_ptr = v_strides = len_ptr = idx_ptr = ws_ptr = None
+    if k is not None or v is not None:
         if k is None or v is None:
             raise ValueError("k and v must be given together")
         _check_cuda("k", k, device)
         _check_cuda("v", v, device)
-        if k.shape != q.shape or v.shape != q.shape:
+        if k.shape != shape or v.shape != shape:
             raise ValueError(f"k/v must have shape {(B, sq, H, D)}")
-        if k.dtype != q.dtype or v.dtype != q.dtype:
+        if k.dtype != dtype or v.dtype != dtype:
             raise TypeError("k and v must have q's dtype")
         if not cache.has_ring:
             raise ValueError("appending needs a cache with a ring")
-    if cache_seqlens is None:
-        if has_new or cache.has_ring:
-            raise ValueError("cache_seqlens is required when k/v are given and for a cache with a ring")
-        seqlens = None
-    else:
-        seqlens = _check_ids("cache_seqlens", cache_seqlens, B, device)
+        k_ptr, k_strides, v_ptr, v_strides = k.data_ptr(), _lib.strides(k.stride()), v.data_ptr(), _lib.strides(v.stride())
+    if cache_seqlens is not None:
+        cache_seqlens = _check_ids("cache_seqlens", cache_seqlens, B, device)
+        len_ptr = cache_seqlens.data_ptr()
+    elif cache.has_ring:
+        raise ValueError("cache_seqlens is required when k/v are given and for a cache with a ring")
     if cache_batch_idx is not None:
         cache_batch_idx = _check_ids("cache_batch_idx", cache_batch_idx, B, device)
+        idx_ptr = cache_batch_idx.data_ptr()
     if out is None:
-        out = torch.empty((B, sq, H, D), dtype=q.dtype, device=device)
+        out = torch.empty(shape, dtype=dtype, device=device)
     else:
         _check_cuda("out", out, device)
-        if out.shape != q.shape or out.dtype != q.dtype:
+        if out.shape != shape or out.dtype != dtype:
             raise ValueError("out must match q's shape and dtype")
     if B == 0 or sq == 0:
         return out
-    lib = _lib.load()
-    with _on(device) as stream:
-        nbytes = lib.wdrz_attn_kvcache8_workspace_size(B, sq, H, cache.max_seq_length)
-        ws_ptr, ws_bytes = None, 0
-        if nbytes:
-            if workspace is None:
-                if torch.cuda.is_current_stream_capturing():
-                    # another graph captured on this stream may be replayed beside this one
-                    workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-                else:
-                    workspace = _WORKSPACES.get(device, nbytes)
-            else:
-                _check_cuda("workspace", workspace, device)
-            ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-            if ws_bytes < nbytes:
-                raise ValueError(f"workspace too small: need {nbytes} bytes")
-        rc = lib.wdrz_attn_kvcache8(
-            dt, cache.struct, q.data_ptr(), _lib.strides4(q.stride()),
-            k.data_ptr() if has_new else None, _lib.strides4(k.stride()) if has_new else None,
-            v.data_ptr() if has_new else None, _lib.strides4(v.stride()) if has_new else None,
-            seqlens.data_ptr() if seqlens is not None else None,
-            cache_batch_idx.data_ptr() if cache_batch_idx is not None else None,
-            out.data_ptr(), _lib.strides4(out.stride()), B, sq,
-            D ** -0.5 if softmax_scale is None else float(softmax_scale), ws_ptr, ws_bytes, stream,
-        )
+    index = device.index
+    if index != _current_device():  # launches go to the current device
+        with torch.cuda.device(index):
+            return flash_attn_with_kvcache8(q, cache, k, v, cache_seqlens, cache_batch_idx, softmax_scale, out=out,
+                                            workspace=workspace)
+    lib, ws_bytes = _lib.load(), 0
+    nbytes = kvcache8_workspace_size(B, sq, H, cache.max_seq_length)
+    if nbytes:
+        if workspace is None:
+            # a captured call's own: another graph captured on this stream may be replayed beside its graph
+            workspace = (torch.zeros(nbytes, dtype=torch.uint8, device=device)
+                         if torch.cuda.is_current_stream_capturing() else _WORKSPACES.get(device, nbytes))
+        else:
+            _check_cuda("workspace", workspace, device)
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if ws_bytes < nbytes:
+            raise ValueError(f"workspace too small: need {nbytes} bytes")
+    rc = lib.wdrz_attn_kvcache8(
+        dt, cache.struct, q.data_ptr(), _lib.strides(q.stride()), k_ptr, k_strides, v_ptr, v_strides, len_ptr, idx_ptr,
+        out.data_ptr(), _lib.strides(out.stride()), B, sq, 0.125 if softmax_scale is None else softmax_scale, ws_ptr,
+        ws_bytes, _raw_stream(index),
+    )
     if rc != _lib.WDRZ_OK:
         _raise(rc, "flash_attn_with_kvcache8")
     return out

@@ -21,7 +21,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .attention import _check_cuda, _dtype_code, _on, _raise, _stream_handle
+from .attention import (_check_cuda, _current_device, _dtype_code, _raise, _raw_stream, _stream_handle)
 
 __all__ = ["QuantLinear4", "add_layernorm_", "layer_norm", "linear4", "linear4_partials", "linear_gelu", "ln_linear",
            "masked_argmax"]
@@ -266,30 +266,35 @@ class QuantLinear4(nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, group={self.group}, bias={self.bias is not None}"
 
 
-def _linear4_rows(x: torch.Tensor, lin: QuantLinear4) -> torch.Tensor:
-    """The checked rows ``[M, K]`` of ``x``."""
-    if x.dtype not in _LN16:
-        raise TypeError(f"x: dtype {x.dtype} is not supported (bfloat16, float16)")
-    _check_cuda("x", x, lin.packed.device)
-    if lin.scales.dtype != x.dtype or lin.scales.device != x.device or (
-            lin.bias is not None and (lin.bias.dtype != x.dtype or lin.bias.device != x.device)):
+def _linear4_operands(x: torch.Tensor, lin: QuantLinear4):
+    """The checked rows ``[M, K]`` of ``x`` and the layer's packed weights, scales and bias."""
+    dtype = x.dtype
+    if dtype not in _LN16:
+        raise TypeError(f"x: dtype {dtype} is not supported (bfloat16, float16)")
+    own = lin._buffers  # nn.Module's attribute lookup costs 0.15 us a name
+    packed, scales, bias = own["packed"], own["scales"], own["bias"]
+    _check_cuda("x", x, packed.device)
+    if scales.dtype != dtype or scales.device != x.device or (
+            bias is not None and (bias.dtype != dtype or bias.device != x.device)):
         raise TypeError("the Linear's scales and bias must have the activations' dtype and device")
-    if x.shape[-1] != lin.in_features:
+    if x.dim() == 0 or x.shape[-1] != lin.in_features:
         raise ValueError(f"x must have {lin.in_features} features, got {tuple(x.shape)}")
-    return x if x.dim() == 2 and x.stride(1) == 1 else _rows(x, "x")
+    return x if x.dim() == 2 and x.stride(1) == 1 else _rows(x, "x"), packed, scales, bias
 
 
 def linear4(x: torch.Tensor, lin: QuantLinear4, gelu: bool = False) -> torch.Tensor:
     """``lin(x)`` (``gelu``: then the exact GELU) for 16-bit ``x [..., K]``: fp32 accumulation, bias and
     activation, one rounding."""
-    xr = _linear4_rows(x, lin)
-    M, N = xr.shape[0], lin.out_features
+    xr, packed, scales, bias = _linear4_operands(x, lin)
+    index = x.device.index
+    if index != _current_device():  # launches go to the current device
+        with torch.cuda.device(index):
+            return linear4(x, lin, gelu)
+    M, K, N = xr.shape[0], lin.in_features, lin.out_features
     y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
-    with _on(x.device) as stream:
-        rc = _lib.load().wdrz_linear4(
-            _LN16[x.dtype], xr.data_ptr(), xr.stride(0) if M > 1 else lin.in_features, lin.packed.data_ptr(),
-            lin.scales.data_ptr(), lin.bias.data_ptr() if lin.bias is not None else None, y.data_ptr(), N, M, N,
-            lin.in_features, lin.group, 1 if gelu else 0, stream)
+    rc = _lib.load().wdrz_linear4(
+        _LN16[x.dtype], xr.data_ptr(), xr.stride(0) if M > 1 else K, packed.data_ptr(), scales.data_ptr(),
+        None if bias is None else bias.data_ptr(), y.data_ptr(), N, M, N, K, lin.group, 1 if gelu else 0, _raw_stream(index))
     if rc != _lib.WDRZ_OK:
         _raise(rc, "linear4")
     return y
@@ -298,13 +303,16 @@ def linear4(x: torch.Tensor, lin: QuantLinear4, gelu: bool = False) -> torch.Ten
 def linear4_partials(x: torch.Tensor, lin: QuantLinear4, n_split: int = 4) -> torch.Tensor:
     """:func:`linear_partials` of a Linear with 4-bit weights: fp32 ``[n_split, rows, N]`` whose sum over the
     first dimension is ``x @ weight.T`` (no bias), for :func:`add_layernorm_partials_`."""
-    xr = _linear4_rows(x, lin)
-    M, N = xr.shape[0], lin.out_features
+    xr, packed, scales, _ = _linear4_operands(x, lin)
+    index = x.device.index
+    if index != _current_device():  # launches go to the current device
+        with torch.cuda.device(index):
+            return linear4_partials(x, lin, n_split)
+    M, K, N = xr.shape[0], lin.in_features, lin.out_features
     part = torch.empty(n_split, M, N, dtype=torch.float32, device=x.device)
-    with _on(x.device) as stream:
-        rc = _lib.load().wdrz_linear4_partials(
-            _LN16[x.dtype], xr.data_ptr(), xr.stride(0) if M > 1 else lin.in_features, lin.packed.data_ptr(),
-            lin.scales.data_ptr(), part.data_ptr(), M, N, lin.in_features, lin.group, n_split, stream)
+    rc = _lib.load().wdrz_linear4_partials(
+        _LN16[x.dtype], xr.data_ptr(), xr.stride(0) if M > 1 else K, packed.data_ptr(), scales.data_ptr(),
+        part.data_ptr(), M, N, K, lin.group, n_split, _raw_stream(index))
     if rc != _lib.WDRZ_OK:
         _raise(rc, "linear4_partials")
     return part

@@ -225,28 +225,30 @@ class FlashKVCache8:
         return res
 
     def _write(self, k: Tensor, v: Tensor, slot_indices: Optional[Tensor], start_pos: int) -> None:
-        from .attention import _check_cuda, _on, _raise
+        from .attention import _check_cuda, _current_device, _raise, _raw_stream
 
-        for name, t in (("k", k), ("v", v)):
-            _check_cuda(name, t, self.device)
-            if t.dim() != 4 or tuple(t.shape[2:]) != (self.n_heads, self.head_dim) or t.shape != k.shape:
-                raise ValueError(f"{name} must be [B, T, {self.n_heads}, {self.head_dim}], got {tuple(t.shape)}")
-            if t.dtype not in _FILL_DTYPES or t.dtype != k.dtype or (self.has_ring and t.dtype != self.dtype):
-                raise TypeError(f"{name}: dtype {t.dtype} does not match the cache's")
-        B, T = int(k.shape[0]), int(k.shape[1])
+        _check_cuda("k", k, self.device)
+        _check_cuda("v", v, self.device)
+        if k.dim() != 4 or k.shape[2:] != (self.n_heads, self.head_dim) or v.shape != k.shape:
+            raise ValueError(f"k and v must be [B, T, {self.n_heads}, {self.head_dim}], got {tuple(k.shape)} and {tuple(v.shape)}")
+        if k.dtype not in _FILL_DTYPES or v.dtype != k.dtype or (self.has_ring and k.dtype != self.dtype):
+            raise TypeError(f"k and v: dtypes {k.dtype} and {v.dtype} do not match the cache's")
+        B, T = k.shape[0], k.shape[1]
         slots = None
         if slot_indices is not None:
             _check_cuda("slot_indices", slot_indices, self.device)
-            slots = slot_indices.to(torch.int64)
-            if slots.dim() != 1 or slots.shape[0] != B:
-                raise ValueError(f"slot_indices must be [{B}]")
-            slots = slots.contiguous()
+            if slot_indices.is_floating_point() or slot_indices.shape != (B,):
+                raise ValueError(f"slot_indices must be whole numbers [{B}]")
+            slots = slot_indices.to(torch.int64).contiguous()
         if B == 0 or T == 0:
             return
-        with _on(self.device) as stream:
-            rc = _lib.load().wdrz_kv8_write(
-                _FILL_DTYPES[k.dtype], self.struct, k.data_ptr(), _lib.strides4(k.stride()), v.data_ptr(),
-                _lib.strides4(v.stride()), slots.data_ptr() if slots is not None else None, B, T, int(start_pos), stream)
+        index = self.device.index
+        if index != _current_device():  # launches go to the current device
+            with torch.cuda.device(index):
+                return self._write(k, v, slots, start_pos)
+        rc = _lib.load().wdrz_kv8_write(
+            _FILL_DTYPES[k.dtype], self.struct, k.data_ptr(), _lib.strides(k.stride()), v.data_ptr(),
+            _lib.strides(v.stride()), None if slots is None else slots.data_ptr(), B, T, start_pos, _raw_stream(index))
         if rc != _lib.WDRZ_OK:
             _raise(rc, "kv8_write")
 
