@@ -49,7 +49,10 @@ def test_linear4(cuda, dtype, M, N, K, group):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N,K,group", [(1, 5120, 1280, 32), (52, 3840, 1280, 64), (4, 1280, 5120, 128), (500, 1280, 1280, 32),
-                                         (1000, 1000, 5120, 64), (3, 51866, 1280, 128), (257, 2048, 512, 128)])
+                                         (1000, 1000, 5120, 64), (3, 51866, 1280, 128), (257, 2048, 512, 128),
+                                         # tiles of 64 x 128 and of 128 x 160, whole and with all three ends inside a tile
+                                         (2048, 1280, 1280, 128), (2047, 1100, 1312, 32), (2040, 1111, 1344, 64),
+                                         (3584, 1280, 5120, 128), (3500, 1234, 2080, 32), (3333, 1249, 2112, 64)])
 def test_linear4_at_the_decoders_sizes(cuda, dtype, M, N, K, group):
     from whisperdrz_amd import linear4
 
@@ -60,7 +63,8 @@ def test_linear4_at_the_decoders_sizes(cuda, dtype, M, N, K, group):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N,K,group,n_split", [(1, 1280, 1280, 64, 2), (5, 1280, 5120, 32, 4), (64, 1000, 640, 128, 4),
-                                                 (17, 40, 96, 32, 4), (70, 33, 256, 64, 2), (600, 1280, 5120, 64, 4)])
+                                                 (17, 40, 96, 32, 4), (70, 33, 256, 64, 2), (600, 1280, 5120, 64, 4),
+                                                 (900, 1240, 1376, 32, 2), (3584, 1280, 5120, 128, 2), (100, 2000, 160, 32, 4)])
 def test_linear4_partials(cuda, dtype, M, N, K, group, n_split):
     from whisperdrz_amd import linear4_partials
 
@@ -102,6 +106,36 @@ def test_strided_rows_and_shapes(cuda):
             linear4(bad, lin)
     with pytest.raises(NotImplementedError, match="n_split 3"):
         linear4_partials(x, lin, 3)
+
+
+def test_rows_far_apart(cuda):
+    """Rows more than 2^22 elements apart: beyond the tiles' 31-bit offsets."""
+    from whisperdrz_amd import linear4
+
+    dtype = torch.bfloat16
+    lin, w, g = _layer(cuda, dtype, 512, 256, 64, 3)
+    big = torch.empty(600, (1 << 22) + 8, dtype=dtype, device=cuda)
+    x = big[:, 64:320]
+    x.copy_(torch.randn(600, 256, generator=g, device=cuda))
+    _check(linear4(x, lin), x, w, lin.bias, False, dtype)
+
+
+@pytest.mark.parametrize("M,K", [(200, 256), (700, 288), (3000, 1312), (3000, 160)])
+def test_infinities_in_tiles(cuda, M, K):
+    """An infinity in the last inputs of a K that ends inside a chunk counts once, in its row."""
+    from whisperdrz_amd import linear4
+
+    dtype = torch.bfloat16
+    lin, w, g = _layer(cuda, dtype, 1280, K, 32, 9)
+    x = torch.randn(M, K, generator=g, device=cuda).to(dtype)
+    y = linear4(x, lin)
+    x[M // 2, K - 1] = float("inf")
+    x[M - 1, K - 8] = float("nan")
+    z = linear4(x, lin)
+    want = x[M // 2].double() @ w.T + lin.bias.double()
+    rest = [i for i in range(M) if i not in (M // 2, M - 1)]
+    assert torch.equal(y[rest], z[rest]) and torch.isnan(z[M - 1]).all()
+    assert torch.equal(torch.isnan(z[M // 2]), torch.isnan(want)) and torch.equal(torch.isinf(z[M // 2]), torch.isinf(want))
 
 
 @pytest.mark.parametrize("M", [1, 20, 200])

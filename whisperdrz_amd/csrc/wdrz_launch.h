@@ -247,8 +247,9 @@ struct Linear4Args {
   int M, N, K, group, act;
   float* part;  // split form: fp32 sums [n_split][M][N] instead of y
   int n_split;
+  int vec;  // whole feature tiles, aligned rows: results in one store of four (set by the launcher)
 };
-hipError_t launch_linear4(int dtype, const Linear4Args& a, hipStream_t stream);
+hipError_t launch_linear4(int dtype, Linear4Args a, hipStream_t stream);
 
 // Y = act(LayerNorm(x + delta) W^T + b) for M <= 4 rows of K <= 1536: ln gives x, the delta's
 // partials and the LayerNorm's parameters; the new residual goes to x_out.
