@@ -210,6 +210,55 @@ def test_read_only_call_on_a_cache_with_a_ring(cuda, dtype, sq):
     _rows(q, _oracle(c), list(range(8)), [[n] * sq for n in lens], dtype, out)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,sq,H,L,ring", [(20, 40, 20, 70, False), (20, 64, 20, 96, False), (20, 65, 20, 33, True),
+                                           (20, 130, 10, 130, True), (26, 33, 20, 1, False)])
+def test_many_prompts(cuda, dtype, B, sq, H, L, ring):
+    """More than 1024 blocks of 16 queries: blocks of 64. Lengths from none to all."""
+    from whisperdrz_amd import flash_attn_with_kvcache8
+
+    c = _cache(cuda, dtype, B, L, H, ring, 31)
+    q = _randn(_gen(cuda, 3), B, sq, H, 64, dtype=dtype, std=2.0)
+    lens = [L - (L * b) // (B - 1) for b in range(B)]
+    lens[1], bad = -1, [1]
+    out = flash_attn_with_kvcache8(q, c, cache_seqlens=torch.tensor(lens, dtype=torch.int32, device=cuda))
+    torch.cuda.synchronize()
+    ref = _oracle(c)
+    assert torch.isnan(out[1]).all() and not out[B - 1].any()
+    for b in (0, 2, 5, B // 2, B - 2):
+        want, mag, big = o8.attend(_np(q[b]), ref.read(0, b, lens[b]), ref.read(1, b, lens[b]), [lens[b]] * sq, SCALE)
+        _check(out[b], want, mag, big, lens[b], dtype, f"row {b}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,sq,H,L", [(18, 40, 20, 200), (18, 65, 20, 200), (30, 33, 20, 140), (9, 130, 13, 200)])
+def test_many_prompts_append(cuda, dtype, B, sq, H, L):
+    from whisperdrz_amd import flash_attn_with_kvcache8
+
+    c = _cache(cuda, dtype, B, L, H, True, 41)
+    ref = _oracle(c)
+    g = _gen(cuda, 13)
+    q, k, v = (_randn(g, B, sq, H, 64, dtype=dtype) for _ in range(3))
+    k[0, sq - 1, 0, 3] = float("nan")  # seen by the last query alone
+    v[0, sq - 2, 1, 5] = float("inf")  # ... by the last two
+    v[1, 0, 2, 7] = -float("inf")  # by all
+    lens = [(17 * b) % (L - sq + 1) for b in range(B)]
+    out = flash_attn_with_kvcache8(q, c, k, v, cache_seqlens=torch.tensor(lens, dtype=torch.int32, device=cuda))
+    torch.cuda.synchronize()
+    got = _np(out)
+    assert np.isnan(got[0, -1, 0]).all() and np.isfinite(got[0, :-1, 0]).all()
+    assert np.isposinf(got[0, -2:, 1, 5]).all() and np.isfinite(got[0, :-2, 1]).all() and np.isfinite(got[0, :, 1, :5]).all()
+    assert np.isneginf(got[1, :, 2, 7]).all() and np.isfinite(got[1, :, 2, 8:]).all()
+    for b in (2, 3, B // 2, B - 1):
+        kk = np.concatenate([ref.read(0, b, lens[b]), _np(k[b]).transpose(1, 0, 2)], 1)
+        vv = np.concatenate([ref.read(1, b, lens[b]), _np(v[b]).transpose(1, 0, 2)], 1)
+        want, mag, big = o8.attend(_np(q[b]), kk, vv, [lens[b] + t + 1 for t in range(sq)], SCALE)
+        _check(out[b], want, mag, big, lens[b] + sq, dtype, f"row {b}")
+    for b in range(B):
+        ref.append(b, lens[b], _np(k[b]), _np(v[b]))
+    _same_state(c, ref)
+
+
 # ---- append -------------------------------------------------------------------------------------
 
 

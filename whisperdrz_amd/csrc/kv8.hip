@@ -211,11 +211,12 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Cache c, Kv8WriteArgs
   }
   if (!c.kr) return;
   const int keep = end / kBlk - 1;  // blocks from here on stand in the ring
-  if (blk >= keep && p >= start && p < end && (blk == first || (blk - first) % 2 != 0)) {
+  const bool shared = start % kBlk != 0;  // the first block has old rows in the ring
+  if (blk >= keep && p >= start && p < end && (blk == first || !shared || (blk - first) % 2 != 0)) {
 #pragma unroll
     for (int n = 0; n < 2; ++n) store16(rings[n] + (p % kRing) * kRowBytes16, w[n]);
   }
-  if (blk == first) {
+  if (shared && blk == first) {
     __syncthreads();  // every old row has been read
     for (int j = first + 2; j <= last; j += 2) {
       const int q = j * kBlk + row;
@@ -242,12 +243,23 @@ __device__ __forceinline__ u32x2 read_tr16(const uint16_t* p) {
 #endif
 }
 
+// The larger of two values. (fmaxf would first quiet each: three instructions.)
+__device__ __forceinline__ float max2(float x, float y) {
+#if __HIP_DEVICE_COMPILE__
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
+  return r;
+#else
+  return x > y ? x : y;
+#endif
+}
+
 // max of x over lanes l, l^16, l^32, l^48, in every lane
 __device__ __forceinline__ float group4_max(float x) {
   const auto r32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(r32[0]), __uint_as_float(r32[1]));
+  x = max2(__uint_as_float(r32[0]), __uint_as_float(r32[1]));
   const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
+  return max2(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
 }
 
 // ---- one query -----------------------------------------------------------------------------------
@@ -489,6 +501,19 @@ __device__ __forceinline__ u32x2 read_tr8(const uint8_t* p) {
 #endif
 }
 
+// The largest of a lane's 8 scores, in four instructions.
+__device__ __forceinline__ float max8(const float (&x)[8]) {
+#if __HIP_DEVICE_COMPILE__
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x[0]), "v"(x[1]), "v"(x[2]));
+  asm("v_max3_f32 %0, %0, %1, %2" : "+v"(r) : "v"(x[3]), "v"(x[4]));
+  asm("v_max3_f32 %0, %0, %1, %2" : "+v"(r) : "v"(x[5]), "v"(x[6]));
+  return max2(r, x[7]);
+#else
+  return x[0];
+#endif
+}
+
 // The lane's 8 probabilities as two operands of type E: the rounded values and what the rounding left,
 // so that they count with 16 bits or more.
 template <typename E>
@@ -496,6 +521,7 @@ __device__ __forceinline__ void split_p(const float (&p)[8], u32x4& ph, u32x4& p
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     ph[j] = Ops<E>::pack(p[2 * j], p[2 * j + 1]);
+    asm("" : "+v"(ph[j]));  // else its halves are rounded a second time
     pl[j] = Ops<E>::pack(p[2 * j] - Ops<E>::lo(ph[j]), p[2 * j + 1] - Ops<E>::hi(ph[j]));
   }
 }
@@ -577,9 +603,10 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if ((j >> 2) * 16 + 4 * gq + (j & 3) > last) p[j] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(p[j]));  // keep this rare path a branch
     }
-    float mb = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-    mb = group4_max(mb) * scale;
+    const float mb = group4_max(max8(p)) * scale;
     if (__any(mb > m + kTau)) {
       const float mn = mb > m + kTau ? mb : m;
       const float alpha = fast_exp2(m - mn);
@@ -748,12 +775,245 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
   }
 }
 
+// ---- prompts ---------------------------------------------------------------------------------------
+// 64 queries a workgroup, 16 a wavefront. Stages of up to 64 keys are widened to 16 bits once for the
+// four wavefronts, into one of two LDS buffers while the other is computed; no partial leaves a wavefront.
+// First the stages of codes, then those of 16-bit rows (the ring's and the new ones). The probabilities'
+// sums come from the matrix cores too. Bound: issue, 28 matrix products of 16 cycles and about 145 VALU
+// instructions a wavefront and stage; a third of both is the probabilities' second part.
+// 16 prompts of 224 over 1500 bf16 positions 68 us, in blocks of 16 queries 93; 32 queries a wavefront 70
+// (fewer wavefronts hide less), stages of 32 keys 74.
+constexpr int kStageKeys = 2 * kBlk;
+
+constexpr int kPromptQueries = 64;
+
+template <typename T, bool RING, bool HAS_NEW>
+__global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args a) {
+  static_assert(!HAS_NEW || RING, "appends need a ring");
+  __shared__ __attribute__((aligned(16))) uint16_t sm_k[2][kStageKeys * kVPitch], sm_v[2][kStageKeys * kVPitch];
+  __shared__ float sm_ks[2][2];
+  __shared__ int sm_odd[2];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int qi = lane & 15, gq = lane >> 4;
+
+  const int h = (int)(blockIdx.x % (unsigned)c.H);
+  const int bq = (int)(blockIdx.x / (unsigned)c.H);
+  // the last queries of a causal prompt see the most keys: they start first
+  const int b = bq / a.n_qblocks, t0 = (a.n_qblocks - 1 - bq % a.n_qblocks) * kPromptQueries;
+  const int nq = min(kPromptQueries, a.sq - t0);
+  const int slot = a.bidx ? a.bidx[b] : b;
+  const int len = a.seqlens ? a.seqlens[b] : c.Lk;
+  const int w0 = t0 + wave * 16;  // this wavefront's first query
+  u32x4 qop[2];  // Q^T halves: query w0 + qi, dims 32 dh + 8 gq ..
+  {
+    const char* qrow = a.q + b * a.qs[0] + min(w0 + qi, a.sq - 1) * a.qs[1] + h * a.qs[2] + gq * 16;
+    qop[0] = load16(qrow);
+    qop[1] = load16(qrow + 64);
+  }
+  SlotRows rows{b, false};
+  if (HAS_NEW && a.bidx)
+    rows = slot_rows(a.B, slot, len, [&](int i) { return a.bidx[i]; }, [&](int i) { return a.seqlens[i]; });
+  const bool bad = slot < 0 || slot >= c.n_slots || len < 0 || len > c.Lk - (HAS_NEW ? a.sq : 0) || rows.conflict;
+  const int k_end = bad ? 0 : HAS_NEW ? len + t0 + nq : len, k_last = k_end - 1;
+  // the last key that any query of this wavefront sees
+  const int w_end = HAS_NEW ? min(k_end, len + w0 + 16) : k_end;
+  const int64_t sh = slot_head(c, bad ? 0 : slot, h);
+  const uint8_t* codes = (tid < 128 ? c.kc : c.vc) + sh * c.n_blk * (kBlk * kHeadDim) + (tid & 3) * 16;
+  const float* ks = c.ks + sh * c.n_blk;
+  const float* vs = c.vs + sh * c.n_blk;
+  const char* kn = HAS_NEW ? a.kn + rows.src * a.kns[0] + h * a.kns[2] : nullptr;
+  const char* vn = HAS_NEW ? a.vn + rows.src * a.vns[0] + h * a.vns[2] : nullptr;
+  const int64_t kstep = HAS_NEW ? a.kns[1] : 0, vstep = HAS_NEW ? a.vns[1] : 0;
+  const int blk1 = bad ? 0 : RING ? min(len, k_end) / kBlk : (k_end + kBlk - 1) / kBlk, blk2 = (k_end + kBlk - 1) / kBlk;
+
+  float m = kNegBig;
+  f32x4 o[5];  // O^T blocks: dims 16 db + 4 gq + i, query qi; the last one the query's sum of probabilities
+#pragma unroll
+  for (int db = 0; db < 5; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto row16 = [&](int p, const char* ring, const char* nw, int64_t step) __attribute__((always_inline)) {
+    return HAS_NEW && p >= len ? nw + (int64_t)(p - len) * step : ring + sh * (kRing * kRowBytes16) + (p % kRing) * kRowBytes16;
+  };
+  // One stage: rows of buffer `buf`, positions p0 .. p0 + 63 below `end`; scale[half] of the scores of each 32 of them,
+  // E the values' type. Both blocks go through each step together: one maximum, one branch, twice the
+  // independent work.
+  auto compute = [&](int buf, int p0, int end, const float (&scale)[2], bool odd, auto etag) __attribute__((always_inline)) {
+    typedef decltype(etag) E;
+    if (p0 >= w_end) return;  // no query of this wavefront sees the stage
+    float p[2][8];
+    {
+      const uint16_t* kt = &sm_k[buf][qi * kVPitch + 8 * gq];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        f32x4 s = Ops<T>::mfma(*reinterpret_cast<const u32x4*>(kt + 16 * kb * kVPitch), qop[0], f32x4{0.f, 0.f, 0.f, 0.f});
+        s = Ops<T>::mfma(*reinterpret_cast<const u32x4*>(kt + 16 * kb * kVPitch + 32), qop[1], s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[kb >> 1][(kb & 1) * 4 + i] = s[i];
+      }
+    }
+    // the last key of the stage that this query sees
+    const int lim = min(HAS_NEW ? min(k_last, len + w0 + qi) : k_last, end - 1) - p0;
+    if (p0 + kStageKeys > min(w_end - (HAS_NEW ? 16 : 0), end)) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float& x = p[j >> 3][j & 7];
+        if ((j >> 2) * 16 + 4 * gq + (j & 3) > lim) x = -INFINITY;
+        asm volatile("" : "+v"(x));  // keep this rare path a branch
+      }
+    }
+    const float mb = group4_max(max2(max8(p[0]) * scale[0], max8(p[1]) * scale[1]));
+    if (__any(mb > m + kTau)) {
+      const float mn = mb > m + kTau ? mb : m;
+      const float alpha = fast_exp2(m - mn);
+      m = mn;
+#pragma unroll
+      for (int db = 0; db < 5; ++db) o[db] *= alpha;
+    }
+    constexpr uint32_t kOne = __is_same(E, Bf16) ? 0x3f803f80u : 0x3c003c00u;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[half][j] = fast_exp2(__builtin_fmaf(p[half][j], scale[half], -m));
+      u32x4 ph, pl;
+      split_p<E>(p[half], ph, pl);
+      const uint16_t* at = &sm_v[buf][(half * kBlk + 4 * gq + (qi >> 2)) * kVPitch + 4 * (qi & 3)];
+#pragma unroll
+      for (int db = 0; db < 5; ++db) {
+        u32x4 v = {kOne, kOne, kOne, kOne};
+        if (db < 4) {
+          const u32x2 v0 = read_tr16(at + 16 * db), v1 = read_tr16(at + 16 * kVPitch + 16 * db);
+          v = u32x4{v0[0], v0[1], v1[0], v1[1]};
+        }
+        o[db] = Ops<E>::mfma(v, pl, o[db]);
+        o[db] = Ops<E>::mfma(v, ph, o[db]);
+      }
+    }
+    if (odd) {  // values that are not finite, one by one (see kv8_attn_kernel)
+      for (int j = 0; j < kStageKeys; ++j) {
+        const char* row = row16(min(p0 + j, k_last), c.vr, vn, vstep);
+        float pj = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = __shfl(p[r >> 3][r & 7], qi + 16 * ((j & 15) >> 2));
+          if (r == (j >> 4) * 4 + (j & 3)) pj = x;
+        }
+        if (j > lim) continue;
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          const uint2 w = *reinterpret_cast<const uint2*>(row + (16 * db + 4 * gq) * 2);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = ((i & 2) ? w.y : w.x) >> (16 * (i & 1)) & 0xffffu;
+            if ((x & Ops<T>::kExp) == Ops<T>::kExp) o[db][i] += pj * Ops<T>::lo(x);
+          }
+        }
+      }
+    }
+  };
+
+  // ---- codes: threads 0..127 move K, the others V, a 16-byte piece (a quarter row) of each block ----
+  if (blk1 > 0) {
+    u32x4 raw[2];
+    float sc[2];  // the values' scale, or the keys' (which goes to the scores)
+    const float* scales = tid < 128 ? ks : vs;
+    auto fetch = [&](int blk) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int x = min(blk + i, blk1 - 1);
+        raw[i] = load16(codes + (int64_t)min(x * kBlk + (tid >> 2 & 31), k_last) * kHeadDim);
+        sc[i] = scales[x];
+      }
+    };
+    auto stage = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint16_t* to = (tid < 128 ? sm_k : sm_v)[buf] + (i * kBlk + (tid >> 2 & 31)) * kVPitch + (tid & 3) * 16;
+        if (tid < 128) {
+          *reinterpret_cast<u32x4*>(to) = widen8<T>(raw[i][0], raw[i][1], 1.f);
+          *reinterpret_cast<u32x4*>(to + 8) = widen8<T>(raw[i][2], raw[i][3], 1.f);
+        } else {
+          *reinterpret_cast<u32x4*>(to) = widen8<Bf16>(raw[i][0], raw[i][1], sc[i]);
+          *reinterpret_cast<u32x4*>(to + 8) = widen8<Bf16>(raw[i][2], raw[i][3], sc[i]);
+        }
+        if (tid == 0) sm_ks[buf][i] = sc[i];
+      }
+    };
+    fetch(0);
+    stage(0);
+    __syncthreads();
+    for (int blk = 0, buf = 0; blk < blk1; blk += 2, buf ^= 1) {
+      fetch(blk + 2);
+      const float scale[2] = {a.c * sm_ks[buf][0], a.c * sm_ks[buf][1]};
+      compute(buf, blk * kBlk, blk1 * kBlk, scale, false, Bf16{});
+      stage(buf ^ 1);  // last read before the barrier that ended the stage before
+      __syncthreads();
+    }
+  }
+  // ---- 16-bit rows: a 16-byte piece of K and of V a thread and block ----
+  if (RING && blk2 > blk1) {
+    u32x4 rk[2], rv[2];
+    auto fetch = [&](int blk) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int p = min((blk + i) * kBlk + (tid >> 3), k_last);
+        rk[i] = load16(row16(p, c.kr, kn, kstep) + (tid & 7) * 16);
+        rv[i] = load16(row16(p, c.vr, vn, vstep) + (tid & 7) * 16);
+      }
+    };
+    auto stage = [&](int buf) __attribute__((always_inline)) {
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = (i * kBlk + (tid >> 3)) * kVPitch + (tid & 7) * 8;
+        *reinterpret_cast<u32x4*>(&sm_k[buf][at]) = rk[i];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const bool lo = (rv[i][w] & Ops<T>::kExp) == Ops<T>::kExp, hi = ((rv[i][w] >> 16) & Ops<T>::kExp) == Ops<T>::kExp;
+          odd = odd || lo || hi;
+          rv[i][w] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0xffffu : 0xffffffffu);
+        }
+        *reinterpret_cast<u32x4*>(&sm_v[buf][at]) = rv[i];
+      }
+      if (odd) sm_odd[buf] = 1;
+    };
+    if (tid < 2) sm_odd[tid] = 0;
+    __syncthreads();
+    fetch(blk1);
+    stage(0);
+    __syncthreads();
+    for (int blk = blk1, buf = 0; blk < blk2; blk += 2, buf ^= 1) {
+      fetch(blk + 2);
+      const float scale[2] = {a.c, a.c};
+      compute(buf, blk * kBlk, blk2 * kBlk, scale, sm_odd[buf] != 0, T{});
+      stage(buf ^ 1);
+      __syncthreads();
+    }
+  }
+  const int t = w0 + qi;
+  if (t >= a.sq) return;
+  char* op = a.o + b * a.os[0] + t * a.os[1] + h * a.os[2] + gq * 8;
+#pragma unroll
+  for (int db = 0; db < 4; ++db) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = bad ? quiet_nan() : k_end == 0 ? 0.f : o[db][i] / o[4][0];
+    *reinterpret_cast<u32x2*>(op + db * 32) = u32x2{Ops<T>::pack(v[0], v[1]), Ops<T>::pack(v[2], v[3])};
+  }
+}
+
 template <typename T, int SQ, int W>
 void launch_attn(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.B * a.n_qblocks * c.H), 1, a.n_splits), block(W * 64);
   if (a.kn) hipLaunchKernelGGL((kv8_attn_kernel<T, SQ, true, true, W>), grid, block, 0, stream, c, a);
   else if (c.kr) hipLaunchKernelGGL((kv8_attn_kernel<T, SQ, true, false, W>), grid, block, 0, stream, c, a);
   else hipLaunchKernelGGL((kv8_attn_kernel<T, SQ, false, false, W>), grid, block, 0, stream, c, a);
+}
+
+template <typename T>
+void launch_prompt(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)a.B * a.n_qblocks * c.H)), block(256);
+  if (a.kn) hipLaunchKernelGGL((kv8_prompt_kernel<T, true, true>), grid, block, 0, stream, c, a);
+  else if (c.kr) hipLaunchKernelGGL((kv8_prompt_kernel<T, true, false>), grid, block, 0, stream, c, a);
+  else hipLaunchKernelGGL((kv8_prompt_kernel<T, false, false>), grid, block, 0, stream, c, a);
 }
 
 template <typename T, int W>
@@ -774,6 +1034,7 @@ void launch_row_t(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
 template <typename T>
 void launch_attn_t(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
   if (a.sq == 1) launch_row_t<T>(c, a, stream);
+  else if (a.block == kPromptQueries) launch_prompt<T>(c, a, stream);
   else if (a.sq <= 8 && a.waves == 8) launch_attn<T, 8, 8>(c, a, stream);
   else if (a.sq <= 8) launch_attn<T, 8, 4>(c, a, stream);
   else if (a.waves == 8) launch_attn<T, 16, 8>(c, a, stream);
@@ -804,13 +1065,20 @@ constexpr int64_t kSplitMinKeys = 512;
 // self of 440, 4 streams 6.0 / 6.9, 52 of 447 14.8 / 12.9. Sixteen are slower from 8 streams on. Five
 // queries follow the same lines: cross over 1500, 1 stream 7.6 / 9.2, 8 10.1 / 12.3, 16 16.3 / 16.0; 6000
 // positions, 1 stream, 1 / 8 splits 23.3 / 9.6.
+// 64 queries a workgroup instead of 16 once blocks of 16 would be more than four workgroups a CU. Us, 16 / 64:
+// over 1500 positions 4 prompts of 224 (1120 blocks of 16) 28.6 / 32.7, 8 of 224 (2240) 48.5 / 42.1, 16 of 64
+// (1280) 37.8 / 33.7, 8 of 40 (480) 16.9 / 24.2; over themselves 4 of 224 19.8 / 16.8, 16 of 224 46.7 / 31.5,
+// 16 of 64 18.2 / 13.2. Up to 32 queries blocks of 16 append in the same launch (52 of 17: 68.8 / 74.3).
+constexpr int64_t kPromptWgs = 1024;
 void kv8_plan(int64_t B, int64_t sq, int64_t H, int64_t Lk, Kv8Args* a) {
-  const int block = sq == 1 ? 1 : sq <= 8 ? 8 : 16;
+  const int block = sq == 1 ? 1 : sq <= 8 ? 8 : sq <= kKv8FusedAppend || B * ((sq + 15) / 16) * H <= kPromptWgs ? 16 : kPromptQueries;
+  a->block = block;
+  a->append = sq <= kKv8FusedAppend;
   a->n_qblocks = (int)((sq + block - 1) / block);
   a->n_splits = 1;
   a->split_len = (int)((Lk + kBlk - 1) / kBlk * kBlk);
   const int64_t units = B * a->n_qblocks * H;
-  if (units <= kCus / 2 && Lk >= kSplitMinLk) {
+  if (block < kPromptQueries && units <= kCus / 2 && Lk >= kSplitMinLk) {
     const int64_t want = std::min<int64_t>(std::min<int64_t>(kCus / units, Lk / kSplitMinKeys), kMaxMergeSplits);
     const int64_t len = ((Lk + want - 1) / want + kBlk - 1) / kBlk * kBlk;
     a->split_len = (int)len;

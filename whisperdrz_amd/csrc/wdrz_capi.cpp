@@ -956,7 +956,6 @@ int wdrz_attn_kvcache8(int dtype, const wdrz_kv8* cache, const void* q, const in
   a.B = (int)B;
   a.sq = (int)sq;
   a.H = c.H;
-  a.append = sq <= wdrz::kKv8FusedAppend;
   a.c = softmax_scale * 1.4426950408889634f;
   wdrz::kv8_plan(B, sq, c.H, c.Lk, &a);
   const int64_t units = B * a.n_qblocks * c.H;
