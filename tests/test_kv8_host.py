@@ -218,3 +218,24 @@ def test_partials_refuse_other_splits():
     lib = _lib.load()
     assert lib.wdrz_linear4_partials(2, P, 64, P, P, P, 2, 8, 64, 32, 3, None) == 2
     assert lib.wdrz_linear4_partials(2, None, 64, None, None, None, 0, 8, 64, 32, 2, None) == 0
+
+
+def test_pool_of_8_bit_caches():
+    from whisperdrz_amd.kv_cache import FlashKVCache8, KVSlotPool, cache_bytes_per_slot, plan_slots
+
+    pool = KVSlotPool(2, 5, 2, 64, self_len=40, cross_len=33, dtype=torch.float16, cache_bits=8)
+    ptrs = []
+    for s, x in zip(pool.self_kv, pool.cross_kv):
+        assert isinstance(s, FlashKVCache8) and s.has_ring and not x.has_ring and s.dtype == torch.float16
+        assert s.k_codes.shape == (5, 2, 64, 64) and x.v_codes.shape == (5, 2, 64, 64) and s.max_seq_length == 40
+        ptrs += [t.data_ptr() for t in (s.k_codes, s.v_codes, s.k_scales, s.v_scales, s.k_ring, s.v_ring, x.k_codes, x.v_scales)]
+    base = pool.arena.data_ptr()
+    assert len(set(ptrs)) == len(ptrs) and all(base <= p < base + pool.arena.numel() and (p - base) % (2 << 20) == 0 for p in ptrs)
+    assert pool.self_kv[1].seq_lens.data_ptr() == pool.self_seq_lens[1].data_ptr()
+    per = cache_bytes_per_slot(32, 20, 64, 448, 1500, torch.bfloat16, 8)
+    assert per == 32 * 20 * (2 * (448 * 64 + 14 * 4 + 64 * 128) + 2 * (1504 * 64 + 47 * 4))
+    plan = plan_slots(272 * 10**9, cache_bits=8)
+    assert plan.bytes_per_slot == per and plan.total_bytes <= 272 * 10**9
+    assert KVSlotPool.arena_bytes(plan.n_slots + 1, 32, 20, 64, 448, 1500, torch.bfloat16, 8) > 272 * 10**9
+    with pytest.raises(ValueError, match="cache_bits"):
+        KVSlotPool(1, 1, 1, 64, self_len=8, cross_len=8, cache_bits=4)

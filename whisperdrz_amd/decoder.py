@@ -19,6 +19,8 @@ cached attention, so the HIP kernels can be exercised exactly as WhisperDRZ driv
   (``linear_gelu``), and the attention output projections and fc2 as split-K partials summed by
   the residual add (``linear_partials`` + ``add_layernorm_partials_``); the default for 16-bit
   GPU activations.
+* 8-bit caches (``KVSlotPool(cache_bits=8)``) and 4-bit Linears (``TextDecoderStack.quantize_linears_``) run on
+  their own kernels in the same step.
 * ``BucketedDecodeGraphs`` — one captured decode step per batch bucket, replayed with static
   token / position / slot buffers (reference ``transcriber.py:18-173``); on ROCm
   ``torch.cuda.CUDAGraph`` is a hipGraph.
@@ -36,10 +38,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
-from .attention import flash_attn_with_kvcache, scaled_dot_product_attention
-from .decode_ops import (LN_LINEAR_MAX_K, LN_LINEAR_ROWS, add_layernorm_, add_layernorm_partials_, layer_norm, linear,
-                         linear_gelu, linear_partials, ln_linear, step_begin, step_end_)
-from .kv_cache import FlashKVCache, KVSlotPool
+from .attention import flash_attn_with_kvcache, flash_attn_with_kvcache8, scaled_dot_product_attention
+from .decode_ops import (LN_LINEAR_MAX_K, LN_LINEAR_ROWS, QuantLinear4, add_layernorm_, add_layernorm_partials_, layer_norm,
+                         linear, linear4, linear4_partials, linear_gelu, linear_partials, ln_linear, step_begin, step_end_)
+from .kv_cache import FlashKVCache, FlashKVCache8, KVSlotPool
 
 # Batch buckets of the captured decode step (reference transcriber.py:18).
 GRAPH_BUCKETS = [1, 2, 4, 8, 16, 32, 42, 52, 54]
@@ -58,7 +60,10 @@ def _out_add_layernorm(x: Tensor, o: Tensor, out: nn.Linear, ln: nn.LayerNorm) -
     420-432 and the next sub-layer's LayerNorm): the
     attention's output projection as 2 split-K fp32 partials summed by the residual add (K a
     multiple of 256, n_state <= 1536), else torch's Linear and the fused add + LayerNorm."""
-    if out.in_features % 256 == 0 and out.out_features <= 1536 and out.bias is not None:
+    if isinstance(out, QuantLinear4):
+        if out.out_features <= 1536 and out.bias is not None:
+            return add_layernorm_partials_(x, linear4_partials(o, out, 2), out, ln)
+    elif out.in_features % 256 == 0 and out.out_features <= 1536 and out.bias is not None:
         return add_layernorm_partials_(x, linear_partials(o, out, 2), out, ln)
     return add_layernorm_(x, out(o), ln)
 
@@ -135,7 +140,9 @@ class MultiHeadAttention(nn.Module):
         cross-attention's query projection). Same arithmetic per output element.
         ``project_out=False`` returns the attention output before ``out`` (the caller applies it,
         fused with the residual add)."""
-        if is_cross_attn:
+        if isinstance(self.query, QuantLinear4):
+            proj = linear4(x, self.query if is_cross_attn else self.qkv4)
+        elif is_cross_attn:
             # the query projection on the same kernels as the others (K % 128 == 0)
             proj = linear(x, self.query.weight, self.query.bias) if self.n_state % 128 == 0 else self.query(x)
         else:
@@ -151,16 +158,45 @@ class MultiHeadAttention(nn.Module):
         B, seq_len, _ = proj.shape
         d = self.n_state // self.n_head
         if is_cross_attn:
-            o = self.attn_kvcache(proj.view(B, seq_len, self.n_head, d), kv_cache.k_cache, kv_cache.v_cache,
-                                  cache_batch_idx=batch_idx, softmax_scale=d ** -0.5, causal=False)
+            o = self.cached(proj.view(B, seq_len, self.n_head, d), kv_cache, None, None, None, batch_idx)
         else:
             qkv = proj.view(B, seq_len, 3, self.n_head, d)
-            o = self.attn_kvcache(qkv[:, :, 0], kv_cache.k_cache, kv_cache.v_cache, k=qkv[:, :, 1], v=qkv[:, :, 2],
-                                  cache_seqlens=cache_seqlens, cache_batch_idx=batch_idx, softmax_scale=d ** -0.5,
-                                  causal=self.causal)
+            o = self.cached(qkv[:, :, 0], kv_cache, qkv[:, :, 1], qkv[:, :, 2], cache_seqlens, batch_idx)
         return o.reshape(B, seq_len, self.n_state)
 
-    def forward_flash(self, x: Tensor, kv_cache: FlashKVCache, is_cross_attn: bool = False,
+    def cached(self, q: Tensor, kv_cache: FlashKVCache | FlashKVCache8, k: Optional[Tensor], v: Optional[Tensor],
+               seqlens: Optional[Tensor], batch_idx: Optional[Tensor]) -> Tensor:
+        """The cached attention of ``[B, sq, H, d]`` rows, appending ``k`` / ``v`` (self) or not (cross), on
+        the cache's own kernels."""
+        scale = (self.n_state // self.n_head) ** -0.5
+        if isinstance(kv_cache, FlashKVCache8):
+            return flash_attn_with_kvcache8(q, kv_cache, k, v, cache_seqlens=seqlens, cache_batch_idx=batch_idx,
+                                            softmax_scale=scale)
+        if k is None:
+            return self.attn_kvcache(q, kv_cache.k_cache, kv_cache.v_cache, cache_batch_idx=batch_idx, softmax_scale=scale,
+                                     causal=False)
+        return self.attn_kvcache(q, kv_cache.k_cache, kv_cache.v_cache, k=k, v=v, cache_seqlens=seqlens,
+                                 cache_batch_idx=batch_idx, softmax_scale=scale, causal=self.causal)
+
+    def quantize_linears_(self, group: int) -> None:
+        """The projections of the activations in 4 bits: query (self: query, key and value, also as one
+        layer of whole feature tiles whose parts share its memory) and out."""
+        n = self.n_state
+        if self.causal and n % 16 == 0:
+            w, b = self.qkv_weight()
+            self.qkv4 = whole = QuantLinear4.from_weight(w, b, group)
+            part = lambda i, bias: QuantLinear4(n, n, group, whole.packed[i * n // 16:(i + 1) * n // 16],
+                                                whole.scales[i * n // 16:(i + 1) * n // 16],
+                                                whole.bias[i * n:(i + 1) * n] if bias else None)
+            self.query, self.key, self.value = part(0, True), part(1, False), part(2, True)
+            self._qkv_cache = None
+        elif self.causal:
+            raise NotImplementedError(f"n_state {n} is not a multiple of 16")
+        else:
+            self.query = QuantLinear4.from_linear(self.query, group)
+        self.out = QuantLinear4.from_linear(self.out, group)
+
+    def forward_flash(self, x: Tensor, kv_cache: FlashKVCache | FlashKVCache8, is_cross_attn: bool = False,
                       slot_indices: Optional[Tensor] = None) -> Tensor:
         B, seq_len, _ = x.shape
         d = self.n_state // self.n_head
@@ -168,13 +204,11 @@ class MultiHeadAttention(nn.Module):
         seqlens = kv_cache.seq_lens if slot_indices is None else kv_cache.seq_lens[slot_indices]
         batch_idx = None if slot_indices is None else slot_indices.to(torch.int32)
         if is_cross_attn:
-            o = self.attn_kvcache(q, kv_cache.k_cache, kv_cache.v_cache, cache_batch_idx=batch_idx,
-                                  softmax_scale=d ** -0.5, causal=False)
+            o = self.cached(q, kv_cache, None, None, None, batch_idx)
         else:
             k_new = self.key(x).view(B, seq_len, self.n_head, d)
             v_new = self.value(x).view(B, seq_len, self.n_head, d)
-            o = self.attn_kvcache(q, kv_cache.k_cache, kv_cache.v_cache, k=k_new, v=v_new, cache_seqlens=seqlens,
-                                  cache_batch_idx=batch_idx, softmax_scale=d ** -0.5, causal=self.causal)
+            o = self.cached(q, kv_cache, k_new, v_new, seqlens, batch_idx)
         return self.out(o.reshape(B, seq_len, self.n_state))
 
 
@@ -214,13 +248,34 @@ class TextDecoderStack(nn.Module):
         # Cached steps on 16-bit GPU activations fuse every residual add with the LayerNorm that
         # follows it (one kernel instead of two); False keeps torch's separate ops.
         self.fused_small_ops = True
+        self.logits4: Optional[QuantLinear4] = None
+
+    @torch.no_grad()
+    def quantize_linears_(self, group: int = 64, logits: bool = False) -> "TextDecoderStack":
+        """Every Linear of the decode step in 4 bits with group scales (``QuantLinear4``), in place: the blocks'
+        query / key / value, out and MLP projections, with ``logits`` the output projection too (the embedding
+        keeps its table). The cross-attention's key and value projections, which see each window once, stay
+        as they are. 16-bit weights; inference only."""
+        for block in self.blocks:
+            block.attn.quantize_linears_(group)
+            block.cross_attn.quantize_linears_(group)
+            for i in (0, 2):
+                block.mlp[i] = QuantLinear4.from_linear(block.mlp[i], group)
+        if logits:
+            self.logits4 = QuantLinear4.from_weight(self.token_embedding.weight, None, group)
+        return self
+
+    def _logits(self, h: Tensor) -> Tensor:
+        if self.logits4 is not None:
+            return linear4(h, self.logits4)
+        return h @ self.token_embedding.weight.to(h.dtype).T
 
     def forward(self, tokens: Tensor, xa: Tensor) -> Tensor:
         """Uncached forward over all tokens (the DTW-alignment path, model.py:547-568)."""
         x = self.token_embedding(tokens) + self.positional_embedding[: tokens.shape[1]]
         for block in self.blocks:
             x = block(x, xa)
-        return self.ln(x) @ self.token_embedding.weight.to(x.dtype).T
+        return self._logits(self.ln(x))
 
     def forward_flash(self, tokens: Tensor, self_kv: list[FlashKVCache], cross_kv: list[FlashKVCache],
                       positions: Tensor, slot_indices: Optional[Tensor] = None) -> Tensor:
@@ -234,7 +289,7 @@ class TextDecoderStack(nn.Module):
             h = self._fused_blocks(x, h, self_kv, cross_kv, batch_idx, list(seqlens.unbind(0)))
             # the attention never bumps lengths; the caller does, after all layers
             step_end_(lens, seqlens, slot_indices, seq_len)
-            return h @ self.token_embedding.weight.to(h.dtype).T
+            return self._logits(h)
         x = self.token_embedding(tokens) + self.positional_embedding[positions]
         if self.fused_small_ops and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16):
             x = x.contiguous()
@@ -261,7 +316,7 @@ class TextDecoderStack(nn.Module):
                     s_kv.seq_lens[slot_indices] += seq_len
                 else:
                     s_kv.seq_lens[:B] += seq_len
-        return h @ self.token_embedding.weight.to(h.dtype).T
+        return self._logits(h)
 
     def _fused_prologue(self, tokens: Tensor, positions: Tensor, slot_indices: Optional[Tensor], lens: Tensor) -> bool:
         """Whether ``step_begin`` / ``step_end_`` take this step: 16-bit, 16-byte aligned tables of up
@@ -290,7 +345,8 @@ class TextDecoderStack(nn.Module):
         blocks = list(self.blocks)
         # a small step: every add + LayerNorm inside the projection that follows it
         n = self.n_state
-        if (x.numel() // n if n else 0) <= LN_LINEAR_ROWS and n % 256 == 0 and n <= LN_LINEAR_MAX_K and all(
+        quantized = isinstance(blocks[0].mlp[0], QuantLinear4) if blocks else False
+        if not quantized and (x.numel() // n if n else 0) <= LN_LINEAR_ROWS and n % 256 == 0 and n <= LN_LINEAR_MAX_K and all(
                 m.bias is not None for b in blocks for m in (b.attn.out, b.cross_attn.out, b.mlp[2])) and all(
                 b.mlp[2].in_features % 512 == 0 for b in blocks):
             part = lin = None
@@ -318,7 +374,9 @@ class TextDecoderStack(nn.Module):
             # fused fc1 + GELU, then fc2 as 4 split-K fp32 partials that the residual add sums
             # (with fc2's bias and rounding) before the next LayerNorm: every Whisper width
             # (K % 128 == 0, 4 K % 512 == 0, n <= 1536); other widths keep torch's MLP
-            if fc1.in_features % 128 == 0 and fc2.in_features % 512 == 0 and fc2.out_features <= 1536 \
+            if quantized and fc2.out_features <= 1536 and fc2.bias is not None:
+                h = add_layernorm_partials_(x, linear4_partials(linear4(h, fc1, gelu=True), fc2, 4), fc2, ln_next)
+            elif not quantized and fc1.in_features % 128 == 0 and fc2.in_features % 512 == 0 and fc2.out_features <= 1536 \
                     and fc2.bias is not None:
                 h = add_layernorm_partials_(x, linear_partials(linear_gelu(h, fc1), fc2, 4), fc2, ln_next)
             else:
