@@ -95,10 +95,15 @@ def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, limits, scale: float):
     return out, mag, big
 
 
-def bound(out, mag, big, n_keys: int, half_step: float) -> np.ndarray:
+def bound(out, mag, big, n_keys: int, half_step: float, one_part: bool = False) -> np.ndarray:
     """How far a kernel may be from ``attend``: the result's own rounding (half a step of its type), and in
     units of sum p |v|: twice the error of a score (64 products and a few factors in fp32; it counts in
     the probability and in the sum), the probability's two 16-bit parts (2^-16) with its exp2 (2^-22),
-    and the fp32 sums over the keys."""
+    and the fp32 sums over the keys. ``one_part``: the probabilities are one fp16 value each, p (1 + e) with
+    |e| <= 2^-11, above and below the line alike: sum p e v - out sum p e over sum p, at most
+    2^-11 (sum p |v| + |out|) <= 2^-10 sum p |v|; those under fp16's normal range, 2^-14 against a largest
+    of at least 1, are off by 2^-25 instead, n_keys 2^-25 in all twice."""
     rel = 2 * 72 * 2.0 ** -24 * big + 2.0 ** -16 + 2.0 ** -20 + (n_keys + 64) * 2.0 ** -24
+    if one_part:
+        rel = rel + 2.0 ** -10 + n_keys * 2.0 ** -24
     return half_step * np.abs(out) + rel * mag + 2.0 ** -25

@@ -65,9 +65,14 @@ def _same_state(c, ref):
         assert np.array_equal(_np(got), want, equal_nan=True), name
 
 
-def _check(out, want, mag, big, n_keys, dtype, what=""):
+def _one_part(dtype, B, sq, H):
+    """Whether a call's codes meet probabilities of one fp16 value: many bf16 prompts, in blocks of 64 queries."""
+    return dtype is torch.bfloat16 and sq > 32 and B * -(-sq // 16) * H > 1024
+
+
+def _check(out, want, mag, big, n_keys, dtype, what="", one_part=False):
     got = _np(out)
-    err = np.abs(got - want) - o8.bound(want, mag, big, n_keys, HALF[dtype])
+    err = np.abs(got - want) - o8.bound(want, mag, big, n_keys, HALF[dtype], one_part)
     assert np.isfinite(got).all() and err.max() <= 0, f"{what}: {err.max():.3e} over the bound"
 
 
@@ -227,7 +232,7 @@ def test_many_prompts(cuda, dtype, B, sq, H, L, ring):
     assert torch.isnan(out[1]).all() and not out[B - 1].any()
     for b in (0, 2, 5, B // 2, B - 2):
         want, mag, big = o8.attend(_np(q[b]), ref.read(0, b, lens[b]), ref.read(1, b, lens[b]), [lens[b]] * sq, SCALE)
-        _check(out[b], want, mag, big, lens[b], dtype, f"row {b}")
+        _check(out[b], want, mag, big, lens[b], dtype, f"row {b}", _one_part(dtype, B, sq, H))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -253,10 +258,46 @@ def test_many_prompts_append(cuda, dtype, B, sq, H, L):
         kk = np.concatenate([ref.read(0, b, lens[b]), _np(k[b]).transpose(1, 0, 2)], 1)
         vv = np.concatenate([ref.read(1, b, lens[b]), _np(v[b]).transpose(1, 0, 2)], 1)
         want, mag, big = o8.attend(_np(q[b]), kk, vv, [lens[b] + t + 1 for t in range(sq)], SCALE)
-        _check(out[b], want, mag, big, lens[b] + sq, dtype, f"row {b}")
+        _check(out[b], want, mag, big, lens[b] + sq, dtype, f"row {b}", _one_part(dtype, B, sq, H))
     for b in range(B):
         ref.append(b, lens[b], _np(k[b]), _np(v[b]))
     _same_state(c, ref)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sq", [1, 5, 64])
+@pytest.mark.parametrize("span", [4, 14, 40, 90])
+def test_scales_of_any_size(cuda, dtype, sq, span):
+    """Values' scales 2^span apart, the attention on one block at a time: a small block's result is not
+    rounded in a large one's units. K of each block points along one axis that a query picks."""
+    from whisperdrz_amd import flash_attn_with_kvcache8
+
+    B, H, blocks = 17, 16, 9
+    c = _cache(cuda, dtype, B, blocks * 32, H, False, 51)
+    g = _gen(cuda, 5)
+    e = torch.randint(-span // 2, span // 2 + 1, c.v_scales.shape, generator=g, device=cuda)
+    e[0, :, :] = torch.linspace(-span / 2, span / 2, blocks, device=cuda).round().int()
+    e[1] = e[0].flip(-1)
+    c.v_scales.copy_(((e.int() + 127) << 23).view(torch.float32))
+    kc = torch.zeros(B, H, blocks, 32, 64, device=cuda)
+    for j in range(blocks):
+        kc[:, :, j, :, j] = 64.0
+    c.k_codes.copy_(kc.view(B, H, -1, 64).to(torch.float8_e4m3fn))
+    c.k_scales.fill_(1.0)
+    pick = torch.randint(0, blocks, (B, sq, H), generator=g, device=cuda)
+    q = torch.nn.functional.one_hot(pick, 64).to(dtype) * 40.0  # scores 320 against 0: other blocks weigh e^-320
+    out = flash_attn_with_kvcache8(q, c)
+    torch.cuda.synchronize()
+    ref = _oracle(c)
+    rows = range(B) if sq < 64 else (0, 1, 7)
+    for b in rows:
+        want, mag, big = o8.attend(_np(q[b]), ref.read(0, b, blocks * 32), ref.read(1, b, blocks * 32), [blocks * 32] * sq, SCALE)
+        top = 60000.0 if dtype is torch.float16 else 3e38
+        keep = np.abs(want) < top  # what the output's type holds
+        lim = o8.bound(want, mag, big, 288, HALF[dtype], _one_part(dtype, B, sq, H))
+        if dtype is torch.bfloat16:
+            lim = lim - 2.0 ** -25 + 1e-30  # the last term is fp16's smallest step: bf16 rounds small results too
+        assert (np.abs(_np(out[b]) - want) <= lim)[keep].all(), b
 
 
 # ---- append -------------------------------------------------------------------------------------
