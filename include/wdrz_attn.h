@@ -441,8 +441,9 @@ int wdrz_median_filter(const float* x, int64_t x_stride, float* y, int64_t y_str
  * With a ring (k_ring and v_ring given) only complete blocks are codes, and the newest positions stand as
  * they came: position p in ring row p % 64, for the last complete block and the one behind it. Reads take
  * positions below 32 floor(length / 32) from the codes, the rest from the ring. A length may therefore
- * be set back by up to 32 positions, or to any multiple of 32, without another write. Without a
- * ring every position is a code (a cache that is filled at once).
+ * be set back to 32 below the furthest position written, or to any multiple of 32 (from where that count
+ * starts anew), without another write. Without a ring every position is a code (a cache that is filled
+ * at once). Scales are powers of two: the kernels read no more of them than the exponent.
  * No counterpart in the reference, whose caches are 16-bit (FlashKVCache, src/whisperdrz/model.py:98-192).
  */
 typedef struct wdrz_kv8 {

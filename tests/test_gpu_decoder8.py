@@ -160,3 +160,17 @@ def test_quantized_layers_share_the_fused_projection(cuda):
     xa = torch.randn(2, CROSS_LEN, N_STATE, device=cuda).to(torch.bfloat16)
     with torch.no_grad():
         assert torch.isfinite(hip(toks, xa)).all()
+
+
+def test_quantize_refusals(cuda):
+    from whisperdrz_amd.decoder import TextDecoderStack
+
+    hip, _ = _make(cuda, torch.bfloat16, 1, 16, 64)
+    with pytest.raises(ValueError, match="already"):
+        hip.quantize_linears_(64)
+    odd = TextDecoderStack(64, 16, 192, 3, 1).to(cuda, torch.bfloat16)
+    with pytest.raises(NotImplementedError, match="group"):
+        odd.quantize_linears_(128)
+    assert isinstance(odd.blocks[0].attn.query, nn.Linear)  # nothing was changed
+    with pytest.raises(TypeError):
+        TextDecoderStack(64, 16, 192, 3, 1).quantize_linears_(64)

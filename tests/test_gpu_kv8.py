@@ -509,6 +509,26 @@ def test_masked_places_do_not_count(cuda, dtype):
     assert np.isinf(got[0, 2, 1, 7]) and np.isnan(got[0, 3, 0, 5]) and np.isfinite(got[0, :2]).all() and np.isfinite(got[1, :5]).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,sq", [(2, 1), (2, 5), (2, 20), (18, 64)])
+@pytest.mark.parametrize("at", [0, 40, 69])
+def test_nan_codes(cuda, dtype, B, sq, at):
+    """What was not finite when it was stored: a key makes its rows NaN, a value its dimension."""
+    from whisperdrz_amd import flash_attn_with_kvcache8
+
+    H = 16
+    c = _cache(cuda, dtype, B, 70, H, False, 61)
+    q = _randn(_gen(cuda, 2), B, sq, H, 64, dtype=dtype)
+    clean = flash_attn_with_kvcache8(q, c)
+    c.k_codes.view(torch.uint8)[0, 1, at, 7] = 0x7F
+    c.v_codes.view(torch.uint8)[1, 2, at, 9] = 0xFF
+    out = flash_attn_with_kvcache8(q, c)
+    torch.cuda.synchronize()
+    nan = torch.zeros_like(out, dtype=torch.bool)
+    nan[0, :, 1], nan[1, :, 2, 9] = True, True
+    assert torch.equal(torch.isnan(out), nan) and torch.equal(out[~nan], clean[~nan])
+
+
 # ---- layouts, streams, graphs ---------------------------------------------------------------------
 
 
@@ -640,3 +660,34 @@ def test_calls_on_two_streams(cuda):
     for i in range(2):
         for o in got[i]:
             assert torch.equal(o, want[i])
+
+
+# ---- the library with host checks -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("case,word", [("slot", "slot 3"), ("overflow", "outside the cache"), ("negative", "outside the cache"),
+                                       ("differ", "lengths 5 and 6"), ("read", "positions of 100"), ("good", "")])
+def test_debug_library_checks_the_metadata(cuda, case, word):
+    import ctypes
+
+    from whisperdrz_amd import _lib
+
+    lib = ctypes.CDLL(str(_lib.DEBUG_LIB_PATH))
+    _lib._declare(lib)
+    c = _cache(cuda, torch.bfloat16, 3, 100, 2, True, 1)
+    before = _bits(c)
+    q = _randn(_gen(cuda, 2), 3, 2, 2, 64, dtype=torch.bfloat16)
+    out = torch.zeros_like(q)
+    idx, lens = {"slot": ([1, 3, 0], [5, 5, 5]), "overflow": ([1, 0, 2], [5, 99, 1]), "negative": ([1, 0, 2], [5, -1, 1]),
+                 "differ": ([1, 0, 1], [5, 9, 6]), "read": ([1, 0, 2], [5, 101, 6]), "good": ([1, 0, 1], [5, 9, 5])}[case]
+    idx, lens = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in (idx, lens))
+    new, st = (None, None) if case == "read" else (q.data_ptr(), _lib.strides(q.stride()))
+    rc = lib.wdrz_attn_kvcache8(_lib.WDRZ_BF16, c.struct, q.data_ptr(), _lib.strides(q.stride()), new, st, new, st,
+                                lens.data_ptr(), idx.data_ptr(), out.data_ptr(), _lib.strides(q.stride()), 3, 2, 0.125, None, 0,
+                                torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    if case == "good":
+        assert rc == _lib.WDRZ_OK and out.any()
+        return
+    assert rc == _lib.WDRZ_EINVAL and word in lib.wdrz_last_error().decode(), lib.wdrz_last_error()
+    assert not out.any() and all(torch.equal(x, y) for x, y in zip(before, _bits(c)))

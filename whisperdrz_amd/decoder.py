@@ -180,9 +180,9 @@ class MultiHeadAttention(nn.Module):
 
     def quantize_linears_(self, group: int) -> None:
         """The projections of the activations in 4 bits: query (self: query, key and value, also as one
-        layer of whole feature tiles whose parts share its memory) and out."""
+        layer of whole feature tiles whose parts share its memory) and out. ``n_state`` a multiple of 16."""
         n = self.n_state
-        if self.causal and n % 16 == 0:
+        if self.causal:
             w, b = self.qkv_weight()
             self.qkv4 = whole = QuantLinear4.from_weight(w, b, group)
             part = lambda i, bias: QuantLinear4(n, n, group, whole.packed[i * n // 16:(i + 1) * n // 16],
@@ -190,8 +190,6 @@ class MultiHeadAttention(nn.Module):
                                                 whole.bias[i * n:(i + 1) * n] if bias else None)
             self.query, self.key, self.value = part(0, True), part(1, False), part(2, True)
             self._qkv_cache = None
-        elif self.causal:
-            raise NotImplementedError(f"n_state {n} is not a multiple of 16")
         else:
             self.query = QuantLinear4.from_linear(self.query, group)
         self.out = QuantLinear4.from_linear(self.out, group)
@@ -256,6 +254,13 @@ class TextDecoderStack(nn.Module):
         query / key / value, out and MLP projections, with ``logits`` the output projection too (the embedding
         keeps its table). The cross-attention's key and value projections, which see each window once, stay
         as they are. 16-bit weights; inference only."""
+        if any(isinstance(m, QuantLinear4) for m in self.modules()):
+            raise ValueError("the Linears are quantized already")
+        if self.n_state % 16 or group not in QuantLinear4.GROUPS or self.n_state % group:
+            raise NotImplementedError(f"n_state {self.n_state} must be a multiple of 16 and of the group, {group}, one of "
+                                      f"{QuantLinear4.GROUPS}")
+        if self.token_embedding.weight.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"weights of {self.token_embedding.weight.dtype} are not supported (bfloat16, float16)")
         for block in self.blocks:
             block.attn.quantize_linears_(group)
             block.cross_attn.quantize_linears_(group)

@@ -169,13 +169,15 @@ class FlashKVCache8:
     scale for its keys and one for its values (:meth:`dequantize` says what they stand for). With ``ring``
     (a self cache) the newest positions also stand as they came, in 64 rows a (slot, head), and the block
     that is not complete is read from there: a position is rounded once, when its block completes, however
-    the tokens were cut into calls. ``seq_lens`` may be set back by up to 32 positions (a draft that was
-    rejected) or to any multiple of 32; anything else needs the positions written again.
+    the tokens were cut into calls. A slot's length may be set back to 32 below the furthest position that
+    was written (a draft that was rejected), or to any multiple of 32, from where that count starts anew;
+    anywhere else the ring's rows are others.
     Without ``ring`` (a cross cache) the cache is filled by :meth:`set_cross_attention`.
 
     Buffers: ``k_codes`` / ``v_codes`` ``[batch_size, n_heads, blocks * 32, 64]`` (``float8_e4m3fn``),
     ``k_scales`` / ``v_scales`` ``[batch_size, n_heads, blocks]`` fp32, ``k_ring`` / ``v_ring``
-    ``[batch_size, n_heads, 64, 64]`` of ``dtype``; ``storage`` places them in given (contiguous) tensors.
+    ``[batch_size, n_heads, 64, 64]`` of ``dtype``; ``storage`` places them in given (contiguous) tensors, which
+    the cache then keeps. Scales are powers of two.
     Per slot and head 128 bytes a position and 16 KB of ring, against 256 bytes a position in 16 bits.
     """
 
