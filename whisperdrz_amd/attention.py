@@ -307,12 +307,13 @@ def flash_attn_with_kvcache8(
     if k is not None or v is not None:
         if k is None or v is None:
             raise ValueError("k and v must be given together")
-        _check_cuda("k", k, device)
-        _check_cuda("v", v, device)
-        if k.shape != shape or v.shape != shape:
-            raise ValueError(f"k/v must have shape {(B, sq, H, D)}")
-        if k.dtype != dtype or v.dtype != dtype:
-            raise TypeError("k and v must have q's dtype")
+        for name, t in (("k", k), ("v", v)):
+            if not isinstance(t, torch.Tensor) or t.device != device:
+                _check_cuda(name, t, device)
+            if t.shape != shape:
+                raise ValueError(f"{name} must have shape {(B, sq, H, D)}")
+            if t.dtype is not dtype:
+                raise TypeError("k and v must have q's dtype")
         if not cache.has_ring:
             raise ValueError("appending needs a cache with a ring")
         k_ptr, k_strides, v_ptr, v_strides = k.data_ptr(), _lib.strides(k.stride()), v.data_ptr(), _lib.strides(v.stride())
@@ -324,8 +325,8 @@ def flash_attn_with_kvcache8(
     if cache_batch_idx is not None:
         cache_batch_idx = _check_ids("cache_batch_idx", cache_batch_idx, B, device)
         idx_ptr = cache_batch_idx.data_ptr()
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+    if out is None:  # like a contiguous q: 1.2 us on the host, empty 2.2
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=device)
     else:
         _check_cuda("out", out, device)
         if out.shape != shape or out.dtype != dtype:

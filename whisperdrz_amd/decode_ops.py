@@ -291,7 +291,7 @@ def linear4(x: torch.Tensor, lin: QuantLinear4, gelu: bool = False) -> torch.Ten
         with torch.cuda.device(index):
             return linear4(x, lin, gelu)
     M, K, N = xr.shape[0], lin.in_features, lin.out_features
-    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], N))
     rc = _lib.load().wdrz_linear4(
         _LN16[x.dtype], xr.data_ptr(), xr.stride(0) if M > 1 else K, packed.data_ptr(), scales.data_ptr(),
         None if bias is None else bias.data_ptr(), y.data_ptr(), N, M, N, K, lin.group, 1 if gelu else 0, _raw_stream(index))
