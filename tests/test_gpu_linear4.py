@@ -62,6 +62,20 @@ def test_linear4_at_the_decoders_sizes(cuda, dtype, M, N, K, group):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [1, 5, 16])
+@pytest.mark.parametrize("N,K,group", [(7169, 160, 32), (7300, 1280, 64), (16393, 288, 32), (20001, 1280, 128), (32769, 1376, 32), (51865, 640, 64)])
+def test_many_features_and_few_rows(cuda, dtype, M, N, K, group):
+    """One, two and four feature tiles a workgroup, the last ones part of a group or past the features."""
+    from whisperdrz_amd import linear4
+
+    lin, w, g = _layer(cuda, dtype, N, K, group, M + N)
+    x = torch.randn(M, K, generator=g, device=cuda).to(dtype)
+    _check(linear4(x, lin), x, w, lin.bias, False, dtype)
+    if M > 1:
+        assert torch.equal(linear4(x, lin)[:1], linear4(x[:1], lin))  # a row's result is its own
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N,K,group,n_split", [(1, 1280, 1280, 64, 2), (5, 1280, 5120, 32, 4), (64, 1000, 640, 128, 4),
                                                  (17, 40, 96, 32, 4), (70, 33, 256, 64, 2), (600, 1280, 5120, 64, 4),
                                                  (900, 1240, 1376, 32, 2), (3584, 1280, 5120, 128, 2), (100, 2000, 160, 32, 4)])

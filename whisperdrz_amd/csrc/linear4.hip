@@ -15,7 +15,7 @@
 //
 // Bound: few rows, launch and one trip to memory (1 row of 1280 x 5120 4.2-4.7 us for 3.5 MB; in turn
 // instead of together the trips took 6.6); a large vocabulary, the weights' stream (1 row of 1280 x 51866
-// 12.8 us, 2.7 TB/s); many rows, matrix products and lookups issued in turn (3584 rows of 5120 x 1280 60 us,
+// 12.4 us, 2.8 TB/s); many rows, matrix products and lookups issued in turn (3584 rows of 5120 x 1280 60 us,
 // 780 TFLOP/s, where the 16-bit library product takes 59).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -110,36 +110,47 @@ __device__ __forceinline__ void put4(const Linear4Args& a, int z, int64_t m, int
 }
 
 // ---- few rows -------------------------------------------------------------------------------------
-// A workgroup takes 16 features and 16 MT rows; its wavefronts take the 128-input chunks in turn and
+// A workgroup takes 16 NT features and 16 MT rows; its wavefronts take the 128-input chunks in turn and
 // add up through LDS. NB chunks' weights, activations and scales are requested together, so a short K
 // is one trip to memory. GS: 32-input steps a group. PART: the chunks of split z only, fp32 sums to
 // part[z][m][n].
-template <typename T, int ACT, bool PART, int GS, int MT, int NB, int kWaves>
+template <typename T, int ACT, bool PART, int GS, int MT, int NT, int NB, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void linear4_rows_kernel(Linear4Args a) {
-  __shared__ f32x4 red[kWaves][MT][64];
+  __shared__ f32x4 red[kWaves][NT * MT][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nt = blockIdx.x, m0 = blockIdx.y * 16 * MT;
+  const int nt0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT;
   const int li = lane & 15, g = lane >> 4;
-  const int steps = a.K / 32, chunks = (a.K + 127) / 128, groups = steps / GS;
+  const int steps = a.K / 32, chunks = (a.K + 127) / 128, groups = steps / GS, tiles = (a.N + 15) / 16;
   const int c0 = PART ? (int)((int64_t)chunks * blockIdx.z / a.n_split) : 0;
   const int c1 = PART ? (int)((int64_t)chunks * (blockIdx.z + 1) / a.n_split) : chunks;
-  const u32x4* w = static_cast<const u32x4*>(a.w) + (int64_t)nt * chunks * 64 + lane;
-  const uint16_t* sc = static_cast<const uint16_t*>(a.scales) + (int64_t)nt * groups * 16 + 4 * g;
+  const u32x4* w[NT];
+  const uint16_t* sc[NT];
+  f32x4 bias[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {  // tiles past N re-read the last one and are not stored
+    const int64_t nt = NT == 1 ? nt0 : min(nt0 + j, tiles - 1);
+    w[j] = static_cast<const u32x4*>(a.w) + nt * chunks * 64 + lane;
+    sc[j] = static_cast<const uint16_t*>(a.scales) + nt * groups * 16 + 4 * g;
+    bias[j] = bias4<T>(a, (int)nt * 16 + 4 * g);
+  }
   const uint16_t* x[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
     x[t] = static_cast<const uint16_t*>(a.x) + (int64_t)min(m0 + 16 * t + li, a.M - 1) * a.x_stride + 8 * g;
-  const f32x4 bias = bias4<T>(a, nt * 16 + 4 * g);
-  f32x4 acc[MT];
+  f32x4 acc[NT][MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int cb = c0 + wave; cb < c1; cb += kWaves * NB) {
-    u32x4 wq[NB], xv[NB][4][MT];
-    uint2 sq[NB][4 / GS];
+    u32x4 wq[NB][NT], xv[NB][4][MT];
+    uint2 sq[NB][NT][4 / GS];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int c = cb + i * kWaves;
-      if (c < c1) wq[i] = load16_stream(w + (int64_t)c * 64);
+      if (c < c1)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) wq[i][j] = load16_stream(w[j] + (int64_t)c * 64);
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
@@ -150,29 +161,34 @@ __global__ __launch_bounds__(64 * kWaves) void linear4_rows_kernel(Linear4Args a
 #pragma unroll
           for (int t = 0; t < MT; ++t) xv[i][s][t] = load16(x[t] + min(4 * c + s, steps - 1) * 32);
 #pragma unroll
-        for (int j = 0; j < 4 / GS; ++j)
-          sq[i][j] = *reinterpret_cast<const uint2*>(sc + (int64_t)min(c * (4 / GS) + j, groups - 1) * 16);
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int q = 0; q < 4 / GS; ++q)
+            sq[i][j][q] = *reinterpret_cast<const uint2*>(sc[j] + (int64_t)min(c * (4 / GS) + q, groups - 1) * 16);
       }
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int c = cb + i * kWaves;
       if (c < c1) {
-        f32x4 part[MT];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          if (4 * c + s < steps) {
-            const u32x4 wop = unpack8<T>(wq[i][s]);
+        for (int j = 0; j < NT; ++j) {
+          f32x4 part[MT];
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-              part[t] = L4<T>::mfma(wop, xv[i][s][t], s % GS == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : part[t]);
-            if (s % GS == GS - 1) {
-              const uint2 q = sq[i][s / GS];
-              const float f[4] = {L4<T>::lo(q.x), L4<T>::hi(q.x), L4<T>::lo(q.y), L4<T>::hi(q.y)};
+          for (int s = 0; s < 4; ++s) {
+            if (4 * c + s < steps) {
+              const u32x4 wop = unpack8<T>(wq[i][j][s]);
 #pragma unroll
               for (int t = 0; t < MT; ++t)
+                part[t] = L4<T>::mfma(wop, xv[i][s][t], s % GS == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : part[t]);
+              if (s % GS == GS - 1) {
+                const uint2 q = sq[i][j][s / GS];
+                const float f[4] = {L4<T>::lo(q.x), L4<T>::hi(q.x), L4<T>::lo(q.y), L4<T>::hi(q.y)};
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[t][r] = __builtin_fmaf(f[r], part[t][r], acc[t][r]);
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) acc[j][t][r] = __builtin_fmaf(f[r], part[t][r], acc[j][t][r]);
+              }
             }
           }
         }
@@ -180,16 +196,22 @@ __global__ __launch_bounds__(64 * kWaves) void linear4_rows_kernel(Linear4Args a
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
-  __syncthreads();
-  // red[w][t][lane][r]: feature 4 g + r, row 16 t + li, over wavefront w's chunks
-  for (int t = wave; t < MT; t += kWaves) {
-    f32x4 s = red[0][t][lane];
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int v = 1; v < kWaves; ++v) s += red[v][t][lane];
-    const int m = m0 + 16 * t + li;
-    if (m < a.M) put4<T, ACT, PART>(a, blockIdx.z, m, nt * 16 + 4 * g, s, bias);
-  }
+    for (int t = 0; t < MT; ++t) red[wave][j * MT + t][lane] = acc[j][t];
+  __syncthreads();
+  // red[w][j MT + t][lane][r]: feature 16 j + 4 g + r, row 16 t + li, over wavefront w's chunks
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      if ((j * MT + t) % kWaves != wave || nt0 + j >= tiles) continue;
+      f32x4 s = red[0][j * MT + t][lane];
+#pragma unroll
+      for (int v = 1; v < kWaves; ++v) s += red[v][j * MT + t][lane];
+      const int m = m0 + 16 * t + li;
+      if (m < a.M) put4<T, ACT, PART>(a, blockIdx.z, m, (nt0 + j) * 16 + 4 * g, s, bias[j]);
+    }
 }
 
 // ---- many rows --------------------------------------------------------------------------------------
@@ -356,10 +378,11 @@ void launch_tile(const Linear4Args& a, hipStream_t stream) {
   hipLaunchKernelGGL((linear4_tile_kernel<T, ACT, PART, GS, WM, WN, KH, NT>), grid, dim3(64 * WM * WN * KH), 0, stream, a);
 }
 
-template <typename T, int ACT, bool PART, int GS, int MT, int NB, int W>
+template <typename T, int ACT, bool PART, int GS, int MT, int NT, int NB, int W>
 void launch_rows(const Linear4Args& a, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)), (unsigned)(PART ? a.n_split : 1));
-  hipLaunchKernelGGL((linear4_rows_kernel<T, ACT, PART, GS, MT, NB, W>), grid, dim3(64 * W), 0, stream, a);
+  const dim3 grid((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)),
+                  (unsigned)(PART ? a.n_split : 1));
+  hipLaunchKernelGGL((linear4_rows_kernel<T, ACT, PART, GS, MT, NT, NB, W>), grid, dim3(64 * W), 0, stream, a);
 }
 
 // Time of a tile launch in us, from how many workgroups run at once and how long one takes over `chunks`
@@ -372,8 +395,11 @@ double tile_cost(int64_t wgs, double fixed, double step, double chunks, bool bot
 }
 
 // Which kernel, by what it takes at these sizes (bf16, cold weights in a graph, us):
-//   * up to 16 rows: one row tile; eight wavefronts share a short K, sixteen a long one, four where there are
-//     tiles enough (1 row: 1280 x 1280 3.7, 1280 x 5120 4.4-5.0, 5120 x 1280 5.5-6.4, 1280 x 51866 13-17);
+//   * up to 16 rows: one row tile; eight wavefronts share a short K, sixteen a long one (1 row: 1280 x 1280
+//     3.7, 1280 x 5120 4.4-5.0, 5120 x 1280 5.5-6.4). From some 450 tiles of features on a workgroup takes two
+//     of them, and above 2048 four, which share its activations (1 / 16 rows, one tile a workgroup of four
+//     wavefronts, then as here: 2560 x 7680 6.6 / 8.9, 6.5 / 7.2; 1280 x 24576 8.9 / 13.9, 7.9 / 9.8;
+//     1280 x 51866 13.2 / 23.6, 12.4 / 16.4). Below, two cost more: 1280 x 3840 4.3, and 5.4 with two;
 //   * blocks of 32 rows while the launch has about as many workgroups as CUs, up to twice as many for a
 //     short K: 52 rows 1280 x 1280 5.2, x 3840 7.2, 5120 x 1280 12.4; 128 rows of 5120 x 1280 (320
 //     workgroups) 23.4, and 18.8 in tiles; 64 rows of 1280 x 5120 (640) 10.9, and 8.0 in tiles;
@@ -385,15 +411,18 @@ void launch_g(const Linear4Args& a, hipStream_t stream) {
   const int64_t tiles = (a.N + 15) / 16, splits = PART ? a.n_split : 1;
   const int chunks = (int)((a.K + 127) / 128 / splits);
   if (a.M <= 16) {
-    if (tiles * splits > 1024) launch_rows<T, ACT, PART, GS, 1, 3, 4>(a, stream);
-    else if (chunks <= 16) launch_rows<T, ACT, PART, GS, 1, 3, 8>(a, stream);
-    else launch_rows<T, ACT, PART, GS, 1, 3, 16>(a, stream);
+    const int64_t wgs = tiles * splits;
+    if (wgs > 2048) launch_rows<T, ACT, PART, GS, 1, 4, 1, 4>(a, stream);
+    else if (wgs > 1024) launch_rows<T, ACT, PART, GS, 1, 2, 2, 4>(a, stream);
+    else if (wgs > 448) launch_rows<T, ACT, PART, GS, 1, 2, 2, 8>(a, stream);
+    else if (chunks <= 16) launch_rows<T, ACT, PART, GS, 1, 1, 3, 8>(a, stream);
+    else launch_rows<T, ACT, PART, GS, 1, 1, 3, 16>(a, stream);
     return;
   }
   const int64_t blocks32 = (a.M + 31) / 32 * tiles * splits;
   // a tile's rows are addressed by 31-bit offsets
   if (blocks32 <= 256 || (blocks32 <= 512 && a.K <= 2048) || a.x_stride > (1 << 22)) {
-    launch_rows<T, ACT, PART, GS, 2, 2, 8>(a, stream);
+    launch_rows<T, ACT, PART, GS, 2, 1, 2, 8>(a, stream);
     return;
   }
   auto wgs = [&](int rows, int feats) { return (int64_t)((a.M + rows - 1) / rows) * ((a.N + feats - 1) / feats) * splits; };
