@@ -1060,8 +1060,7 @@ void launch_row(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
 
 template <typename T>
 void launch_row_t(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
-  if (a.waves == 16) launch_row<T, 16>(c, a, stream);
-  else if (a.waves == 8) launch_row<T, 8>(c, a, stream);
+  if (a.waves == 8) launch_row<T, 8>(c, a, stream);
   else launch_row<T, 4>(c, a, stream);
 }
 
