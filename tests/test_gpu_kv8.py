@@ -265,6 +265,36 @@ def test_many_prompts_append(cuda, dtype, B, sq, H, L):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sq", [64, 70, 130])
+def test_many_prompts_append_to_named_slots(cuda, dtype, sq):
+    """Lengths at and off multiples of 32 (ring rows written with the attention and behind it), a slot named
+    twice, rows that disagree, and rows out of range, in one call of blocks of 64 queries."""
+    from whisperdrz_amd import flash_attn_with_kvcache8
+
+    B, H, L = 18, 20, 288
+    c = _cache(cuda, dtype, 30, L, H, True, sq)
+    ref = _oracle(c)
+    g = _gen(cuda, 15)
+    q, k, v = (_randn(g, B, sq, H, 64, dtype=dtype) for _ in range(3))
+    lens = [0, 32, 64, 96, 1, 31, 33, 63, 95, 128, L - sq, 64, 7, 40, 41, 0, L - sq + 1, -1]
+    slots = [29, 3, 7, 12, 1, 0, 5, 20, 21, 22, 23, 7, 24, 9, 9, 30, 25, 26]  # 7 twice alike, 9 disagrees
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    out = flash_attn_with_kvcache8(q, c, k, v, cache_seqlens=i32(lens), cache_batch_idx=i32(slots))
+    torch.cuda.synchronize()
+    assert torch.isnan(out[13:]).all()
+    for b in (0, 1, 2, 6, 10, 11, 12):
+        src = 11 if slots[b] == 7 else b
+        kk = np.concatenate([ref.read(0, slots[b], lens[b]), _np(k[src]).transpose(1, 0, 2)], 1)
+        vv = np.concatenate([ref.read(1, slots[b], lens[b]), _np(v[src]).transpose(1, 0, 2)], 1)
+        want, mag, big = o8.attend(_np(q[b]), kk, vv, [lens[b] + t + 1 for t in range(sq)], SCALE)
+        _check(out[b], want, mag, big, lens[b] + sq, dtype, f"row {b}", _one_part(dtype, B, sq, H))
+    for b in range(13):
+        if b != 2:
+            ref.append(slots[b], lens[b], _np(k[b]), _np(v[b]))
+    _same_state(c, ref)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("sq", [1, 5, 64])
 @pytest.mark.parametrize("span", [4, 14, 40, 90])
 def test_scales_of_any_size(cuda, dtype, sq, span):

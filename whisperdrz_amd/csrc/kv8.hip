@@ -15,7 +15,8 @@
 // the ring and its own new rows as they are. What it writes, ring rows of [len, len + sq) and the codes
 // of the block that they complete, nobody reads in the same launch: with sq <= 32 the positions
 // [c0, len + sq) are at most 63, so no new row shares a ring row with an old one that is still read,
-// and the append rides in the attention launch. Longer prompts append in a launch of their own behind it.
+// and the append rides in the attention launch. Longer prompts append in a launch of their own behind it; many of
+// them (kv8_prompt_kernel) write the codes, and the ring where no row reads it, beside their attention.
 //
 // One query: four lanes a key, dot products and sums on the VALU (kv8_row_kernel). More: a wavefront takes a
 // block of 32 keys and up to 16 queries a step on the matrix cores (kv8_attn_kernel):
@@ -175,20 +176,27 @@ __device__ __forceinline__ int64_t slot_head(const Kv8Cache& c, int64_t slot, in
 // blocks become codes and the rows of the last two blocks go to the ring. Ring rows of the first block's
 // old positions are read here too, so this block's workgroup also writes the later rows that take
 // their place (those of the later block of the same parity), after it has read them.
-template <typename T, typename Id>
-__global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Cache c, Kv8WriteArgs a, const Id* slots) {
-  __shared__ uint32_t red[2][4];
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int64_t slot = slots ? (int64_t)slots[b] : b;
-  const int start = a.starts ? a.starts[b] : a.start;
-  if (slot < 0 || slot >= c.n_slots || start < 0 || start > c.Lk - a.T) return;
-  if (slots) {
-    const SlotRows r = slot_rows(a.B, slot, start, [&](int i) { return (int64_t)slots[i]; },
-                                 [&](int i) { return a.starts ? a.starts[i] : start; });
-    if (r.conflict || r.src != b) return;
-  }
+// RINGS false: codes only.
+
+// Where row b is written: its slot and first position, or false.
+template <typename Id>
+__device__ __forceinline__ bool write_row(const Kv8Cache& c, const Kv8WriteArgs& a, const Id* slots, int b, int64_t& slot, int& start) {
+  slot = slots ? (int64_t)slots[b] : b;
+  start = a.starts ? a.starts[b] : a.start;
+  if (slot < 0 || slot >= c.n_slots || start < 0 || start > c.Lk - a.T) return false;
+  if (!slots) return true;
+  const int from = start;
+  const SlotRows r = slot_rows(a.B, slot, from, [&](int i) { return (int64_t)slots[i]; },
+                               [&](int i) { return a.starts ? a.starts[i] : from; });
+  return !r.conflict && r.src == b;
+}
+
+// The x-th block that row b touches.
+template <typename T, bool RINGS>
+__device__ __forceinline__ void write_block(const Kv8Cache& c, const Kv8WriteArgs& a, int64_t slot, int start, int b, int h, int x,
+                                            uint32_t (&red)[2][4]) {
   const int end = start + a.T, first = start / kBlk, last = (end - 1) / kBlk;
-  const int blk = first + (int)blockIdx.x;
+  const int blk = first + x;
   if (blk > last) return;
   const int tid = threadIdx.x, row = tid >> 3, ch = tid & 7;
   const int64_t sh = slot_head(c, slot, h);
@@ -209,7 +217,7 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Cache c, Kv8WriteArgs
     const int64_t code = (sh * c.n_blk + blk) * (kBlk * kHeadDim);
     quantize_block<T>(w[0], w[1], c.kc + code, c.vc + code, c.ks + sh * c.n_blk + blk, c.vs + sh * c.n_blk + blk, red);
   }
-  if (!c.kr) return;
+  if (!RINGS || !c.kr) return;
   const int keep = end / kBlk - 1;  // blocks from here on stand in the ring
   const bool shared = start % kBlk != 0;  // the first block has old rows in the ring
   if (blk >= keep && p >= start && p < end && (blk == first || !shared || (blk - first) % 2 != 0)) {
@@ -227,6 +235,47 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Cache c, Kv8WriteArgs
     }
   }
 }
+
+template <typename T, typename Id>
+__global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Cache c, Kv8WriteArgs a, const Id* slots) {
+  __shared__ uint32_t red[2][4];
+  int64_t slot;
+  int start;
+  if (write_row(c, a, slots, blockIdx.z, slot, start))
+    write_block<T, true>(c, a, slot, start, blockIdx.z, blockIdx.y, blockIdx.x, red);
+}
+
+// The ring rows of appends that start inside a block, whose codes kv8_prompt_kernel has written.
+__global__ __launch_bounds__(256) void kv8_ring_kernel(Kv8Cache c, Kv8WriteArgs a, const int32_t* slots) {
+  const int h = blockIdx.x, b = blockIdx.y;
+  if (a.starts[b] % kBlk == 0) return;
+  int64_t slot;
+  int start;
+  if (!write_row(c, a, slots, b, slot, start)) return;
+  const int end = start + a.T, ch = threadIdx.x & 7;
+  const int64_t ring = slot_head(c, slot, h) * (kRing * kRowBytes16) + ch * 16;
+  for (int p = max(start, (end / kBlk - 1) * kBlk) + (int)(threadIdx.x >> 3); p < end; p += 32) {
+    store16(c.kr + ring + (p % kRing) * kRowBytes16, load16(a.k + b * a.ks[0] + h * a.ks[2] + (int64_t)(p - start) * a.ks[1] + ch * 16));
+    store16(c.vr + ring + (p % kRing) * kRowBytes16, load16(a.v + b * a.vs[0] + h * a.vs[2] + (int64_t)(p - start) * a.vs[1] + ch * 16));
+  }
+}
+
+// The append of an attention launch's new rows as a write.
+__host__ __device__ inline Kv8WriteArgs append_args(const Kv8Args& a) {
+  Kv8WriteArgs w{};
+  w.k = a.kn;
+  w.v = a.vn;
+  for (int i = 0; i < 3; ++i) {
+    w.ks[i] = a.kns[i];
+    w.vs[i] = a.vns[i];
+  }
+  w.starts = a.seqlens;
+  w.B = a.B;
+  w.T = a.sq;
+  return w;
+}
+// Blocks that a row of T positions touches at most, wherever it starts.
+__host__ __device__ inline int touched_blocks(int T) { return (T + kBlk - 2) / kBlk + 1; }
 
 // ---- attention ----------------------------------------------------------------------------------
 
@@ -782,7 +831,9 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
 // sums come from the matrix cores too. Bound: issue, 18 matrix products of 16 cycles (28 with two-part
 // probabilities) and about 110 (145) VALU instructions a wavefront and stage, which add up: softmax and
 // matrix products of a SIMD's wavefronts hardly overlap (counters: VALU 61% and MFMA 27% of the time).
-// 16 prompts of 224 over 1500 positions 62 us bf16, 68 fp16; in blocks of 16 queries 93. 32 queries a
+// 16 prompts of 224 over 1500 positions 62 us bf16, 68 fp16; in blocks of 16 queries 93. Over themselves, with the
+// append's workgroups behind those of the attention, 26 us; with the append in a launch of its own 31 (it takes 10);
+// with each row's next to its attention's 31. 32 queries a
 // wavefront take 64 and more (640 workgroups on 256 CUs), stages of 32 keys 74 against 68.
 constexpr int kStageKeys = 2 * kBlk;
 
@@ -798,6 +849,19 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
 
   const int h = (int)(blockIdx.x % (unsigned)c.H);
   const int bq = (int)(blockIdx.x / (unsigned)c.H);
+  if (HAS_NEW && bq >= a.B * a.n_qblocks) {
+    // The append's workgroups. They write codes of blocks from len / 32 on, which nobody reads here. Ring
+    // rows are read only where len ends inside a block; those rows' are written by kv8_ring_kernel.
+    const int x = bq - a.B * a.n_qblocks, row = x % a.B;
+    const Kv8WriteArgs w = append_args(a);
+    int64_t to;
+    int start;
+    if (!write_row(c, w, a.bidx, row, to, start)) return;
+    uint32_t(&red)[2][4] = *reinterpret_cast<uint32_t(*)[2][4]>(sm_k);
+    if (start % kBlk == 0) write_block<T, true>(c, w, to, start, row, h, x / a.B, red);
+    else write_block<T, false>(c, w, to, start, row, h, x / a.B, red);
+    return;
+  }
   // the last queries of a causal prompt see the most keys: they start first
   const int b = bq / a.n_qblocks, t0 = (a.n_qblocks - 1 - bq % a.n_qblocks) * kPromptQueries;
   const int nq = min(kPromptQueries, a.sq - t0);
@@ -1044,7 +1108,7 @@ void launch_attn(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
 
 template <typename T>
 void launch_prompt(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
-  const dim3 grid((unsigned)((int64_t)a.B * a.n_qblocks * c.H)), block(256);
+  const dim3 grid((unsigned)((int64_t)a.B * (a.n_qblocks + (a.kn ? touched_blocks(a.sq) : 0)) * c.H)), block(256);
   if (a.kn) hipLaunchKernelGGL((kv8_prompt_kernel<T, true, true>), grid, block, 0, stream, c, a);
   else if (c.kr) hipLaunchKernelGGL((kv8_prompt_kernel<T, true, false>), grid, block, 0, stream, c, a);
   else hipLaunchKernelGGL((kv8_prompt_kernel<T, false, false>), grid, block, 0, stream, c, a);
@@ -1076,8 +1140,7 @@ void launch_attn_t(const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
 
 template <typename T, typename Id>
 void launch_write_t(const Kv8Cache& c, const Kv8WriteArgs& a, const Id* slots, hipStream_t stream) {
-  // a row of T positions touches at most this many blocks, wherever it starts
-  const int blocks = a.starts ? (a.T + kBlk - 2) / kBlk + 1 : (a.start + a.T - 1) / kBlk - a.start / kBlk + 1;
+  const int blocks = a.starts ? touched_blocks(a.T) : (a.start + a.T - 1) / kBlk - a.start / kBlk + 1;
   const dim3 grid((unsigned)blocks, (unsigned)c.H, (unsigned)a.B);
   hipLaunchKernelGGL((kv8_write_kernel<T, Id>), grid, dim3(256), 0, stream, c, a, slots);
 }
@@ -1100,8 +1163,8 @@ constexpr int64_t kSplitMinKeys = 512;
 // positions, 1 stream, 1 / 8 splits 23.3 / 9.6.
 // 64 queries a workgroup instead of 16 once blocks of 16 would be more than four workgroups a CU. Us, 16 / 64:
 // over 1500 positions 4 prompts of 224 (1120 blocks of 16) 28.6 / 32.7, 8 of 224 (2240) 48.5 / 42.1, 16 of 64
-// (1280) 37.8 / 33.7, 8 of 40 (480) 16.9 / 24.2; over themselves 4 of 224 19.8 / 16.8, 16 of 224 46.7 / 31.5,
-// 16 of 64 18.2 / 13.2. Up to 32 queries blocks of 16 append in the same launch (52 of 17: 68.8 / 74.3).
+// (1280) 37.8 / 33.7, 8 of 40 (480) 16.9 / 24.2; over themselves 4 of 224 19.8 / 13.8, 16 of 224 46.7 / 26.0,
+// 16 of 64 18.2 / 9.9. Up to 32 queries blocks of 16 append in the same launch (52 of 17: 68.8 / 74.3).
 constexpr int64_t kPromptWgs = 1024;
 void kv8_plan(int64_t B, int64_t sq, int64_t H, int64_t Lk, Kv8Args* a) {
   const int block = sq == 1 ? 1 : sq <= 8 ? 8 : sq <= kKv8FusedAppend || B * ((sq + 15) / 16) * H <= kPromptWgs ? 16 : kPromptQueries;
@@ -1127,22 +1190,16 @@ size_t kv8_workspace_bytes(int64_t B, int64_t sq, int64_t H, int64_t Lk) {
 }
 
 hipError_t launch_kv8_attn(int dtype, const Kv8Cache& c, const Kv8Args& a, hipStream_t stream) {
-  if ((int64_t)a.B * a.n_qblocks * c.H > 0x7fffffff) return hipErrorInvalidValue;
+  if ((int64_t)a.B * (a.n_qblocks + touched_blocks(a.sq)) * c.H > 0x7fffffff) return hipErrorInvalidValue;
   if (dtype == 2) launch_attn_t<Bf16>(c, a, stream);
   else launch_attn_t<F16>(c, a, stream);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !a.kn || a.append) return err;
-  Kv8WriteArgs w{};  // a long prompt's append, behind the launch that reads the ring
-  w.k = a.kn;
-  w.v = a.vn;
-  for (int i = 0; i < 3; ++i) {
-    w.ks[i] = a.kns[i];
-    w.vs[i] = a.vns[i];
-  }
-  w.starts = a.seqlens;
-  w.B = a.B;
-  w.T = a.sq;
-  return launch_kv8_write(dtype, c, w, a.bidx, nullptr, stream);
+  // a long prompt's append, or what is left of it, behind the launch that reads the ring
+  const Kv8WriteArgs w = append_args(a);
+  if (a.block != kPromptQueries) return launch_kv8_write(dtype, c, w, a.bidx, nullptr, stream);
+  hipLaunchKernelGGL(kv8_ring_kernel, dim3((unsigned)c.H, (unsigned)a.B), dim3(256), 0, stream, c, w, a.bidx);
+  return hipGetLastError();
 }
 
 hipError_t launch_kv8_write(int dtype, const Kv8Cache& c, const Kv8WriteArgs& a, const int32_t* slots32,

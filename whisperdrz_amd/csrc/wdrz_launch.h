@@ -74,7 +74,7 @@ struct Kv8Args {
   int* ws_count;
   int B, sq, n_qblocks, n_splits, split_len;
   int H;       // as the cache's
-  int block;   // queries a workgroup: 1, 8, 16, or 64 and 128 of a prompt
+  int block;   // queries a workgroup: 1, 8, 16, or 64 of a prompt
   int waves;   // wavefronts a workgroup
   int append;  // the attention launch writes the new rows
   int64_t qs[3], kns[3], vns[3], os[3];
