@@ -831,7 +831,8 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
 // sums come from the matrix cores too. Bound: issue, 18 matrix products of 16 cycles (28 with two-part
 // probabilities) and about 110 (145) VALU instructions a wavefront and stage, which add up: softmax and
 // matrix products of a SIMD's wavefronts hardly overlap (counters: VALU 61% and MFMA 27% of the time).
-// 16 prompts of 224 over 1500 positions 62 us bf16, 68 fp16; in blocks of 16 queries 93. Over themselves, with the
+// 16 prompts of 224 over 1500 positions 61 us bf16, 65 fp16 (63 and 68 with four blocks of 16 queries in every
+// workgroup but a prompt's last; 64 prompts 225 and 236); in blocks of 16 queries 93. Over themselves, with the
 // append's workgroups behind those of the attention, 26 us; with the append in a launch of its own 31 (it takes 10);
 // with each row's next to its attention's 31. 32 queries a
 // wavefront take 64 and more (640 workgroups on 256 CUs), stages of 32 keys 74 against 68.
@@ -863,11 +864,15 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
     return;
   }
   // the last queries of a causal prompt see the most keys: they start first
-  const int b = bq / a.n_qblocks, t0 = (a.n_qblocks - 1 - bq % a.n_qblocks) * kPromptQueries;
-  const int nq = min(kPromptQueries, a.sq - t0);
+  const int b = bq / a.n_qblocks, item = a.n_qblocks - 1 - bq % a.n_qblocks;
+  // a prompt's blocks of 16 queries, spread evenly over its workgroups: three or four each
+  const int n16 = (a.sq + 15) / 16, q0 = item * n16 / a.n_qblocks, q1 = (item + 1) * n16 / a.n_qblocks;
+  const int t0 = q0 * 16, nq = min(q1 * 16, a.sq) - t0;
   const int slot = a.bidx ? a.bidx[b] : b;
   const int len = a.seqlens ? a.seqlens[b] : c.Lk;
-  const int w0 = t0 + wave * 16;  // this wavefront's first query
+  // The wavefront without queries is another one from workgroup to workgroup of a CU, so that its SIMDs get alike.
+  const int wq = (wave + (int)(blockIdx.x >> 8)) & 3;
+  const int w0 = t0 + wq * 16;  // this wavefront's first query
   u32x4 qop[2];  // Q^T halves: query w0 + qi, dims 32 dh + 8 gq ..
   {
     const char* qrow = a.q + b * a.qs[0] + min(w0 + qi, a.sq - 1) * a.qs[1] + h * a.qs[2] + gq * 16;
@@ -880,7 +885,7 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
   const bool bad = slot < 0 || slot >= c.n_slots || len < 0 || len > c.Lk - (HAS_NEW ? a.sq : 0) || rows.conflict;
   const int k_end = bad ? 0 : HAS_NEW ? len + t0 + nq : len, k_last = k_end - 1;
   // the last key that any query of this wavefront sees
-  const int w_end = HAS_NEW ? min(k_end, len + w0 + 16) : k_end;
+  const int w_end = wq >= q1 - q0 ? 0 : HAS_NEW ? min(k_end, len + w0 + 16) : k_end;
   const int64_t sh = slot_head(c, bad ? 0 : slot, h);
   const uint8_t* codes = (tid < 128 ? c.kc : c.vc) + sh * c.n_blk * (kBlk * kHeadDim) + (tid & 3) * 16;
   const float* ks = c.ks + sh * c.n_blk;
@@ -1087,7 +1092,7 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
     }
   }
   const int t = w0 + qi;
-  if (t >= a.sq) return;
+  if (wq >= q1 - q0 || t >= a.sq) return;
   char* op = a.o + b * a.os[0] + t * a.os[1] + h * a.os[2] + gq * 8;
 #pragma unroll
   for (int db = 0; db < 4; ++db) {
