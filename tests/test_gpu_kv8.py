@@ -294,6 +294,36 @@ def test_many_prompts_append_to_named_slots(cuda, dtype, sq):
     _same_state(c, ref)
 
 
+def test_graph_of_many_prompts_that_append(cuda):
+    """Both launches of the append, replayed over changing lengths and rows: as the eager calls on a copy."""
+    from whisperdrz_amd import flash_attn_with_kvcache8
+
+    dtype, B, sq, H, L = torch.bfloat16, 18, 70, 20, 288
+    c, e = (_cache(cuda, dtype, B, L, H, True, 3) for _ in range(2))
+    g = _gen(cuda, 16)
+    q, k, v = (_randn(g, B, sq, H, 64, dtype=dtype) for _ in range(3))
+    lens = torch.zeros(B, dtype=torch.int32, device=cuda)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        flash_attn_with_kvcache8(q, c, k, v, cache_seqlens=lens)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = flash_attn_with_kvcache8(q, c, k, v, cache_seqlens=lens)
+    flash_attn_with_kvcache8(q, e, k, v, cache_seqlens=lens)  # the call before the capture
+    for step in range(4):
+        lens.copy_(torch.arange(B, device=cuda) * (32 if step % 2 else 13) % (L - sq + 1))
+        k.normal_(generator=g)
+        v.normal_(generator=g)
+        graph.replay()
+        want = flash_attn_with_kvcache8(q, e, k, v, cache_seqlens=lens)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        for x, y in zip(_bits(c), _bits(e)):
+            assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("sq", [1, 5, 64])
 @pytest.mark.parametrize("span", [4, 14, 40, 90])
