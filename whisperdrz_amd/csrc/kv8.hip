@@ -1167,8 +1167,8 @@ constexpr int64_t kSplitMinKeys = 512;
 // queries follow the same lines: cross over 1500, 1 stream 7.6 / 9.2, 8 10.1 / 12.3, 16 16.3 / 16.0; 6000
 // positions, 1 stream, 1 / 8 splits 23.3 / 9.6.
 // 64 queries a workgroup instead of 16 once blocks of 16 would be more than four workgroups a CU. Us, 16 / 64:
-// over 1500 positions 4 prompts of 224 (1120 blocks of 16) 28.6 / 32.7, 8 of 224 (2240) 48.5 / 42.1, 16 of 64
-// (1280) 37.8 / 33.7, 8 of 40 (480) 16.9 / 24.2; over themselves 4 of 224 19.8 / 13.8, 16 of 224 46.7 / 26.0,
+// over 1500 positions 4 prompts of 224 (1120 blocks of 16) 28.6 / 32.7, 8 of 224 (2240) 48.5 / 40.8, 16 of 64
+// (1280) 37.8 / 32.1, 8 of 40 (480) 16.9 / 24.2; over themselves 4 of 224 19.8 / 13.8, 16 of 224 46.7 / 26.0,
 // 16 of 64 18.2 / 9.9. Up to 32 queries blocks of 16 append in the same launch (52 of 17: 68.8 / 74.3).
 constexpr int64_t kPromptWgs = 1024;
 void kv8_plan(int64_t B, int64_t sq, int64_t H, int64_t Lk, Kv8Args* a) {
