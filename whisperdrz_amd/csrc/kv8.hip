@@ -31,8 +31,7 @@
 // with the launch). One query on the matrix cores instead took 59: eight exponentials and a pack for two
 // a key, the LDS round trip and 128 registers. Small calls: launch, the trip for the row's metadata, one
 // for its keys; 1 stream 6.2 us over 1500, append at 200 4.4 us.
-#include <algorithm>
-
+#include "kv8_plan.h"
 #include "kv_merge.h"
 #include "wdrz_common.h"
 #include "wdrz_launch.h"
@@ -40,8 +39,9 @@
 namespace wdrz {
 namespace {
 
-constexpr int kBlk = 32;                  // positions a scale covers
+constexpr int kBlk = kKv8Block;           // positions a scale covers
 constexpr int kRing = 64;                 // ring rows
+static_assert(kKv8MaxSplits <= kMaxMergeSplits, "kv_finish joins no more");
 constexpr int kRowBytes16 = kHeadDim * 2;
 constexpr int kVPitch = kHeadDim + 8;     // V tile row pitch (16-bit elements)
 constexpr float kTau = 8.0f;              // lazy-rescale threshold (log2 units)
@@ -383,8 +383,8 @@ __global__ __launch_bounds__(kWaves * 64) void kv8_row_kernel(Kv8Cache c, Kv8Arg
   const char* kn = HAS_NEW ? a.kn + rows.src * a.kns[0] + h * a.kns[2] : nullptr;
   const char* vn = HAS_NEW ? a.vn + rows.src * a.vns[0] + h * a.vns[2] : nullptr;
   // blocks of this split: codes [blk0, blk1), then, where the ring begins inside it, one of 16-bit rows
-  const int blk0 = k_begin / kBlk;
-  const int blk1 = RING ? min(len, k_end) / kBlk : (k_end + kBlk - 1) / kBlk;
+  const Kv8Blocks part = kv8_blocks(RING, len, k_begin, k_end);
+  const int blk0 = part.blk0, blk1 = part.blk1;
   const int tail0 = blk1 * kBlk;
   const int tails = RING && (blk1 - blk0) % kWaves == wave ? (k_end - tail0 + 15) / 16 : 0;  // 16-key steps, at most 2
   const int codes = max(0, (blk1 - blk0 - wave + kWaves - 1) / kWaves);
@@ -633,10 +633,9 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
   const float* vs = c.vs + sh * c.n_blk;
   const char* kn = HAS_NEW ? a.kn + rows.src * a.kns[0] + h * a.kns[2] : nullptr;
   const char* vn = HAS_NEW ? a.vn + rows.src * a.vns[0] + h * a.vns[2] : nullptr;
-  // blocks of this split: codes [blk0, blk1), then 16-bit rows, dealt on to the wavefronts in turn
-  const int blk0 = k_begin / kBlk;
-  const int blk1 = bad ? blk0 : RING ? min(len, k_end) / kBlk : (k_end + kBlk - 1) / kBlk;
-  const int blk2 = (k_end + kBlk - 1) / kBlk;
+  // blocks of this split: codes [blk0, blk1), then 16-bit rows [blk1, blk2), dealt on to the wavefronts in turn
+  const Kv8Blocks part = kv8_blocks(RING, len, k_begin, k_end);
+  const int blk0 = part.blk0, blk1 = part.blk1, blk2 = part.blk2;
 
   uint8_t* vt = sm_v[wave];
   float m = kNegBig, l = 0.f;
@@ -728,7 +727,7 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
     };
     const int64_t kstep = HAS_NEW ? a.kns[1] : 0, vstep = HAS_NEW ? a.vns[1] : 0;
     uint16_t* vt16 = reinterpret_cast<uint16_t*>(vt);
-    for (int tb = blk1 + (wave + kWaves - (blk1 - blk0) % kWaves) % kWaves; tb < blk2; tb += kWaves) {
+    for (int tb = kv8_first_rows(part, wave, kWaves); tb < blk2; tb += kWaves) {
       const int p0 = tb * kBlk;
       u32x4 kw[4], vw[4];
 #pragma unroll
@@ -838,7 +837,7 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
 // wavefront take 64 and more (640 workgroups on 256 CUs), stages of 32 keys 74 against 68.
 constexpr int kStageKeys = 2 * kBlk;
 
-constexpr int kPromptQueries = 64;
+constexpr int kPromptQueries = kKv8PromptQueries;
 
 template <typename T, bool RING, bool HAS_NEW>
 __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args a) {
@@ -893,7 +892,8 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
   const char* kn = HAS_NEW ? a.kn + rows.src * a.kns[0] + h * a.kns[2] : nullptr;
   const char* vn = HAS_NEW ? a.vn + rows.src * a.vns[0] + h * a.vns[2] : nullptr;
   const int64_t kstep = HAS_NEW ? a.kns[1] : 0, vstep = HAS_NEW ? a.vns[1] : 0;
-  const int blk1 = bad ? 0 : RING ? min(len, k_end) / kBlk : (k_end + kBlk - 1) / kBlk, blk2 = (k_end + kBlk - 1) / kBlk;
+  const Kv8Blocks part = kv8_blocks(RING, len, 0, k_end);
+  const int blk1 = part.blk1, blk2 = part.blk2;
 
   float m = kNegBig;
   f32x4 o[5];  // O^T blocks: dims 16 db + 4 gq + i, query qi; the last one the query's sum of probabilities
@@ -1151,42 +1151,6 @@ void launch_write_t(const Kv8Cache& c, const Kv8WriteArgs& a, const Id* slots, h
 }
 
 }  // namespace
-
-// One workgroup walks a row unless few long rows leave most of the chip idle: merging splits costs about
-// 2 us (publish, count, read back). One query, bf16, cold caches in a graph, us, unsplit / split:
-//   1 stream of 20 heads: 500 positions 4.6 / 6.0, 1000 5.3 / 6.3, 1500 6.4 / 6.9, 3000 11.8 / 7.6, 6000
-//   19.1 / 8.9, 20000 58.3 / 14.8; 2 streams: 1500 7.8 / 7.2, 3000 12.0 / 8.4; 4: 1500 8.1 / 8.2, 3000
-//   12.2 / 9.7, 6000 22.7 / 14.8; 6: 1500 8.4 / 8.7, 6000 24.0 / 19.7; 8: 1500 9.0 / 10.2.
-// More splits than fill the CUs once gain nothing (4 streams of 3000: 3 splits 9.7, 4 10.7).
-constexpr int64_t kCus = 256;
-constexpr int64_t kSplitMinLk = 2048;
-constexpr int64_t kSplitMinKeys = 512;
-// Eight wavefronts a workgroup while the launch has no more workgroups than CUs, else four. Us, eight /
-// four: cross over 1500, 1 stream 6.4 / 7.7, 8 9.0 / 11.2, 13 (260 workgroups) 14.6 / 13.0, 32 22.6 / 23.2;
-// self of 440, 4 streams 6.0 / 6.9, 52 of 447 14.8 / 12.9. Sixteen are slower from 8 streams on. Five
-// queries follow the same lines: cross over 1500, 1 stream 7.6 / 9.2, 8 10.1 / 12.3, 16 16.3 / 16.0; 6000
-// positions, 1 stream, 1 / 8 splits 23.3 / 9.6.
-// 64 queries a workgroup instead of 16 once blocks of 16 would be more than four workgroups a CU. Us, 16 / 64:
-// over 1500 positions 4 prompts of 224 (1120 blocks of 16) 28.6 / 32.7, 8 of 224 (2240) 48.5 / 40.8, 16 of 64
-// (1280) 37.8 / 32.1, 8 of 40 (480) 16.9 / 24.2; over themselves 4 of 224 19.8 / 13.8, 16 of 224 46.7 / 26.0,
-// 16 of 64 18.2 / 9.9. Up to 32 queries blocks of 16 append in the same launch (52 of 17: 68.8 / 74.3).
-constexpr int64_t kPromptWgs = 1024;
-void kv8_plan(int64_t B, int64_t sq, int64_t H, int64_t Lk, Kv8Args* a) {
-  const int block = sq == 1 ? 1 : sq <= 8 ? 8 : sq <= kKv8FusedAppend || B * ((sq + 15) / 16) * H <= kPromptWgs ? 16 : kPromptQueries;
-  a->block = block;
-  a->append = sq <= kKv8FusedAppend;
-  a->n_qblocks = (int)((sq + block - 1) / block);
-  a->n_splits = 1;
-  a->split_len = (int)((Lk + kBlk - 1) / kBlk * kBlk);
-  const int64_t units = B * a->n_qblocks * H;
-  if (block < kPromptQueries && units <= kCus / 2 && Lk >= kSplitMinLk) {
-    const int64_t want = std::min<int64_t>(std::min<int64_t>(kCus / units, Lk / kSplitMinKeys), kMaxMergeSplits);
-    const int64_t len = ((Lk + want - 1) / want + kBlk - 1) / kBlk * kBlk;
-    a->split_len = (int)len;
-    a->n_splits = (int)((Lk + len - 1) / len);
-  }
-  a->waves = units * a->n_splits <= kCus ? 8 : 4;
-}
 
 size_t kv8_workspace_bytes(int64_t B, int64_t sq, int64_t H, int64_t Lk) {
   Kv8Args a{};

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "../../include/wdrz_attn.h"
+#include "kv8_plan.h"
 #include "wdrz_launch.h"
 
 namespace {

@@ -88,7 +88,6 @@ struct Kv8WriteArgs {
   int B, T, start;
 };
 constexpr int kKv8FusedAppend = 32;  // new rows that the attention launch appends itself
-void kv8_plan(int64_t B, int64_t sq, int64_t H, int64_t Lk, Kv8Args* a);
 size_t kv8_workspace_bytes(int64_t B, int64_t sq, int64_t H, int64_t Lk);
 hipError_t launch_kv8_attn(int dtype, const Kv8Cache& c, const Kv8Args& a, hipStream_t stream);
 hipError_t launch_kv8_write(int dtype, const Kv8Cache& c, const Kv8WriteArgs& a, const int32_t* slots32,
