@@ -827,14 +827,13 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
 // 64 queries a workgroup, 16 a wavefront. Stages of up to 64 keys are widened to 16 bits once for the
 // four wavefronts, into one of two LDS buffers while the other is computed; no partial leaves a wavefront.
 // First the stages of codes, then those of 16-bit rows (the ring's and the new ones). The probabilities'
-// sums come from the matrix cores too. Bound: issue, 18 matrix products of 16 cycles (28 with two-part
-// probabilities) and about 110 (145) VALU instructions a wavefront and stage, which add up: softmax and
-// matrix products of a SIMD's wavefronts hardly overlap (counters: VALU 61% and MFMA 27% of the time).
-// 16 prompts of 224 over 1500 positions 61 us bf16, 65 fp16 (63 and 68 with four blocks of 16 queries in every
-// workgroup but a prompt's last; 64 prompts 225 and 236); in blocks of 16 queries 93. Over themselves, with the
+// sums come from the matrix cores too. Bound: issue, 28 matrix products of 16 cycles and about 145 VALU instructions a
+// wavefront and stage, which add up: softmax and matrix products of a SIMD's wavefronts hardly overlap.
+// 16 prompts of 224 over 1500 positions 67 us, 64 prompts 245; in blocks of 16 queries 93. Over themselves, with the
 // append's workgroups behind those of the attention, 26 us; with the append in a launch of its own 31 (it takes 10);
-// with each row's next to its attention's 31. 32 queries a
-// wavefront take 64 and more (640 workgroups on 256 CUs), stages of 32 keys 74 against 68.
+// with each row's next to its attention's 31. 32 queries a wavefront and stages of 32 keys were no faster.
+// Probabilities of bf16 prompts as one fp16 operand instead of two parts: 64 us, 64 prompts 220, but wrong where many
+// small ones count.
 constexpr int kStageKeys = 2 * kBlk;
 
 constexpr int kPromptQueries = kKv8PromptQueries;
@@ -938,18 +937,12 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
       for (int db = 0; db < 5; ++db) o[db] *= alpha;
     }
     constexpr uint32_t kOne = __is_same(E, Bf16) ? 0x3f803f80u : 0x3c003c00u;
-    constexpr bool ONE = __is_same(T, Bf16) && __is_same(E, F16);  // fp16 probabilities alone (see the codes' stages)
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) p[half][j] = fast_exp2(__builtin_fmaf(p[half][j], scale[half], -m));
       u32x4 ph, pl;
-      if (ONE) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ph[j] = Ops<E>::pack(p[half][2 * j], p[half][2 * j + 1]);
-      } else {
-        split_p<E>(p[half], ph, pl);
-      }
+      split_p<E>(p[half], ph, pl);
       const uint16_t* at = &sm_v[buf][(half * kBlk + 4 * gq + (qi >> 2)) * kVPitch + 4 * (qi & 3)];
 #pragma unroll
       for (int db = 0; db < 5; ++db) {
@@ -958,7 +951,7 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
           const u32x2 v0 = read_tr16(at + 16 * db), v1 = read_tr16(at + 16 * kVPitch + 16 * db);
           v = u32x4{v0[0], v0[1], v1[0], v1[1]};
         }
-        if (!ONE) o[db] = Ops<E>::mfma(v, pl, o[db]);
+        o[db] = Ops<E>::mfma(v, pl, o[db]);
         o[db] = Ops<E>::mfma(v, ph, o[db]);
       }
     }
@@ -986,16 +979,11 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
   };
 
   // ---- codes: threads 0..127 move K, the others V, a 16-byte piece (a quarter row) of each block ----
-  // For bf16 queries the probabilities are one fp16 operand: its rounding, 2^-11 at most, is an eighth of
-  // the result's own. The values, codes times a scale of any size, are held in fp16 as multiples of `ref`,
-  // the largest scale met so far (the sums are rescaled when it grows): exact while a scale is at least
-  // 2^-15 of it (fp16 ends at 2^-24, the codes at 2^-9). A stage with a smaller one takes bf16 values and
-  // two-part probabilities, as every stage of fp16 queries does.
+  // The values become bf16, which holds a code times a scale of any size; so do the two parts of a probability, whose
+  // small ones stay what they are (one fp16 operand would drop those under 2^-25: a million of them are 3% of a sum).
   if (blk1 > 0) {
-    constexpr bool ONE = __is_same(T, Bf16);
     u32x4 raw[2];
     float kscale[2], vscale[2];
-    float ref = 0.f, sum_ref = 0.f;  // of the buffer that is staged last, and of the sums
     auto fetch = [&](int blk) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -1005,15 +993,7 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
         vscale[i] = vs[x];
       }
     };
-    // x / y of two powers of two by their bits; 2^-126 where it is less.
-    auto ratio = [](float x, float y) __attribute__((always_inline)) {
-      const int r = (int)(__float_as_uint(x) - __float_as_uint(y)) + 0x3f800000;
-      return __uint_as_float((uint32_t)max(r, 0x00800000));
-    };
-    auto stage = [&](int buf) __attribute__((always_inline)) {  // returns whether the values are fp16
-      ref = ONE ? max2(ref, max2(vscale[0], vscale[1])) : 1.f;
-      const float v0 = ONE ? ratio(vscale[0], ref) : vscale[0], v1 = ONE ? ratio(vscale[1], ref) : vscale[1];
-      const bool one = ONE && __all(v0 >= 0x1p-15f && v1 >= 0x1p-15f);
+    auto stage = [&](int buf) __attribute__((always_inline)) {
       uint16_t* to = (tid < 128 ? sm_k : sm_v)[buf] + (tid >> 2 & 31) * kVPitch + (tid & 3) * 16;
       auto put = [&](auto etag, float s0, float s1) __attribute__((always_inline)) {
         typedef decltype(etag) E;
@@ -1024,31 +1004,17 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
         }
       };
       if (tid < 128) put(T{}, 1.f, 1.f);
-      else if (one) put(F16{}, v0, v1);
-      else put(Bf16{}, v0, v1);
-      return one;
+      else put(Bf16{}, vscale[0], vscale[1]);
     };
     fetch(0);
-    bool one = stage(0);
-    sum_ref = ref;
+    stage(0);
     __syncthreads();
     for (int blk = 0, buf = 0; blk < blk1; blk += 2, buf ^= 1) {
-      if (ref != sum_ref) {
-        const float f = ratio(sum_ref, ref);
-#pragma unroll
-        for (int db = 0; db < 4; ++db) o[db] *= f;
-        sum_ref = ref;
-      }
       const float scale[2] = {a.c * kscale[0], a.c * kscale[1]};
       fetch(blk + 2);
-      if (one) compute(buf, blk * kBlk, blk1 * kBlk, scale, false, F16{});
-      else compute(buf, blk * kBlk, blk1 * kBlk, scale, false, Bf16{});
-      one = stage(buf ^ 1);  // last read before the barrier that ended the stage before
+      compute(buf, blk * kBlk, blk1 * kBlk, scale, false, Bf16{});
+      stage(buf ^ 1);  // last read before the barrier that ended the stage before
       __syncthreads();
-    }
-    if (ONE) {
-#pragma unroll
-      for (int db = 0; db < 4; ++db) o[db] *= sum_ref;
     }
   }
   // ---- 16-bit rows: a 16-byte piece of K and of V a thread and block ----
