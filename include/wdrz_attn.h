@@ -443,7 +443,8 @@ int wdrz_median_filter(const float* x, int64_t x_stride, float* y, int64_t y_str
  * positions below 32 floor(length / 32) from the codes, the rest from the ring. A length may therefore
  * be set back to 32 below the furthest position written, or to any multiple of 32 (from where that count
  * starts anew), without another write. Without a ring every position is a code (a cache that is filled
- * at once). Scales are powers of two: the kernels read no more of them than the exponent.
+ * at once). Scales are powers of two: the kernels read no more of them than the exponent. A block whose codes
+ * and scales are 0, as in buffers that start as zeros, stands for zeros.
  * No counterpart in the reference, whose caches are 16-bit (FlashKVCache, src/whisperdrz/model.py:98-192).
  */
 typedef struct wdrz_kv8 {

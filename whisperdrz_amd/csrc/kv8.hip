@@ -647,10 +647,10 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
   auto softmax = [&](const f32x4 (&s)[2], float scale, int last, float (&p)[8]) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3];
-    if (__any(last < kBlk - 1)) {
+    if (__any(last < kBlk - 1)) {  // masked behind the scale, which may be 0 (a block nobody wrote): 0 times -inf is NaN
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if ((j >> 2) * 16 + 4 * gq + (j & 3) > last) p[j] = -INFINITY;
+      for (int j = 0; j < 8; ++j) p[j] = (j >> 2) * 16 + 4 * gq + (j & 3) > last ? -INFINITY : p[j] * scale;
+      scale = 1.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(p[j]));  // keep this rare path a branch
     }
@@ -901,10 +901,10 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
   auto row16 = [&](int p, const char* ring, const char* nw, int64_t step) __attribute__((always_inline)) {
     return HAS_NEW && p >= len ? nw + (int64_t)(p - len) * step : ring + sh * (kRing * kRowBytes16) + (p % kRing) * kRowBytes16;
   };
-  // One stage: rows of buffer `buf`, positions p0 .. p0 + 63 below `end`; scale[half] of the scores of each 32 of them,
+  // One stage: rows of buffer `buf`, positions p0 .. p0 + 63 below `end`; block_scale[half] of the scores of each 32 of them,
   // E the values' type. Both blocks go through each step together: one maximum, one branch, twice the
   // independent work.
-  auto compute = [&](int buf, int p0, int end, const float (&scale)[2], bool odd, auto etag) __attribute__((always_inline)) {
+  auto compute = [&](int buf, int p0, int end, const float (&block_scale)[2], bool odd, auto etag) __attribute__((always_inline)) {
     typedef decltype(etag) E;
     if (p0 >= w_end) return;  // no query of this wavefront sees the stage
     float p[2][8];
@@ -920,13 +920,15 @@ __global__ __launch_bounds__(256, 4) void kv8_prompt_kernel(Kv8Cache c, Kv8Args 
     }
     // the last key of the stage that this query sees
     const int lim = min(HAS_NEW ? min(k_last, len + w0 + qi) : k_last, end - 1) - p0;
-    if (p0 + kStageKeys > min(w_end - (HAS_NEW ? 16 : 0), end)) {
+    float scale[2] = {block_scale[0], block_scale[1]};
+    if (p0 + kStageKeys > min(w_end - (HAS_NEW ? 16 : 0), end)) {  // behind the scale, as in kv8_attn_kernel
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         float& x = p[j >> 3][j & 7];
-        if ((j >> 2) * 16 + 4 * gq + (j & 3) > lim) x = -INFINITY;
+        x = (j >> 2) * 16 + 4 * gq + (j & 3) > lim ? -INFINITY : x * scale[j >> 3];
         asm volatile("" : "+v"(x));  // keep this rare path a branch
       }
+      scale[0] = scale[1] = 1.f;
     }
     const float mb = group4_max(max2(max8(p[0]) * scale[0], max8(p[1]) * scale[1]));
     if (__any(mb > m + kTau)) {

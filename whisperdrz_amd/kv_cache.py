@@ -177,7 +177,7 @@ class FlashKVCache8:
     Buffers: ``k_codes`` / ``v_codes`` ``[batch_size, n_heads, blocks * 32, 64]`` (``float8_e4m3fn``),
     ``k_scales`` / ``v_scales`` ``[batch_size, n_heads, blocks]`` fp32, ``k_ring`` / ``v_ring``
     ``[batch_size, n_heads, 64, 64]`` of ``dtype``; ``storage`` places them in given (contiguous) tensors, which
-    the cache then keeps. Scales are powers of two.
+    the cache then keeps. Scales are powers of two. Blocks that nobody has written stand for zeros in buffers of zeros.
     Per slot and head 128 bytes a position and 16 KB of ring, against 256 bytes a position in 16 bits.
     """
 
