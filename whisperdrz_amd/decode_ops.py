@@ -185,19 +185,40 @@ def add_layernorm_partials_(x: torch.Tensor, partials: torch.Tensor, lin: nn.Lin
     return y.view(x.shape)
 
 
+def _check_linear4_sizes(lin: "QuantLinear4", packed: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor]) -> None:
+    """The kernels read all of a layer's buffers: they have to be as large as its features say."""
+    N, K = lin.out_features, lin.in_features
+    tiles = -(-N // 16)
+    if packed.shape != (tiles, -(-K // 128), 1024) or scales.shape != (tiles, K // lin.group, 16) \
+            or not (packed.is_contiguous() and scales.is_contiguous()):
+        raise ValueError(f"packed {tuple(packed.shape)} and scales {tuple(scales.shape)} must be contiguous "
+                         f"{(tiles, -(-K // 128), 1024)} and {(tiles, K // lin.group, 16)}")
+    if bias is not None and (bias.shape != (N,) or not bias.is_contiguous()):
+        raise ValueError(f"bias {tuple(bias.shape)} must be contiguous [{N}]")
+
+
 class QuantLinear4(nn.Module):
     """A Linear with 4-bit weights: ``weight[n, k] = codes[n, k] * scales[n, k // group]``, codes whole
     numbers -7..7 and scales of the activations' 16-bit type, packed once for :func:`linear4`.
 
     ``from_linear`` rounds a 16-bit Linear, ``from_codes`` takes codes and scales from elsewhere. ``group`` is
-    32, 64 or 128 and divides the inputs. Inference only: the weights are buffers without gradients."""
+    32, 64 or 128 and divides the inputs. Inference only: the weights are buffers without gradients, contiguous,
+    ``packed`` uint8 ``[ceil(N / 16), ceil(K / 128), 1024]``, ``scales`` ``[ceil(N / 16), K / group, 16]``, ``bias`` ``[N]``."""
 
     GROUPS = (32, 64, 128)
 
     def __init__(self, in_features: int, out_features: int, group: int, packed: torch.Tensor, scales: torch.Tensor,
                  bias: Optional[torch.Tensor]):
         super().__init__()
+        if group not in self.GROUPS or in_features <= 0 or out_features <= 0 or in_features % group:
+            raise NotImplementedError(f"group {group} must be one of {self.GROUPS} and divide the {in_features} inputs "
+                                      f"of {out_features} outputs")
+        if packed.dtype is not torch.uint8 or scales.dtype not in _LN16 or (bias is not None and bias.dtype != scales.dtype):
+            raise TypeError("packed must be uint8, scales and bias share a 16-bit dtype (bfloat16, float16)")
+        if scales.device != packed.device or (bias is not None and bias.device != packed.device):
+            raise ValueError("packed, scales and bias must be on one device")
         self.in_features, self.out_features, self.group = in_features, out_features, group
+        _check_linear4_sizes(self, packed, scales, bias)
         self.register_buffer("packed", packed)
         self.register_buffer("scales", scales)
         self.register_buffer("bias", bias)
@@ -277,6 +298,13 @@ def _linear4_operands(x: torch.Tensor, lin: QuantLinear4):
     if scales.dtype != dtype or scales.device != x.device or (
             bias is not None and (bias.dtype != dtype or bias.device != x.device)):
         raise TypeError("the Linear's scales and bias must have the activations' dtype and device")
+    # buffers can be replaced after the construction; their counts take 0.5 us a call, their shapes 0.7
+    tiles = (lin.out_features + 15) // 16
+    if packed.numel() != tiles * ((lin.in_features + 127) // 128) * 1024 or packed.dtype is not torch.uint8 \
+            or scales.numel() != tiles * 16 * (lin.in_features // lin.group) or not packed.is_contiguous() \
+            or not scales.is_contiguous() or (bias is not None and (bias.numel() != lin.out_features or not bias.is_contiguous())):
+        _check_linear4_sizes(lin, packed, scales, bias)
+        raise TypeError("the Linear's packed weights must be uint8")
     if x.dim() == 0 or x.shape[-1] != lin.in_features:
         raise ValueError(f"x must have {lin.in_features} features, got {tuple(x.shape)}")
     return x if x.dim() == 2 and x.stride(1) == 1 else _rows(x, "x"), packed, scales, bias
