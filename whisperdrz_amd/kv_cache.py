@@ -187,13 +187,9 @@ class FlashKVCache8:
     def __init__(self, batch_size: int, max_seq_length: int, n_heads: int, head_dim: int = 64, dtype=torch.bfloat16,
                  device=None, *, ring: bool = True, storage: Optional[dict[str, Tensor]] = None,
                  seq_lens: Optional[Tensor] = None):
-        if head_dim != 64:
-            raise NotImplementedError(f"head_dim {head_dim} is not supported (only 64)")
-        if dtype not in _FILL_DTYPES:
-            raise TypeError(f"dtype {dtype} is not supported (bfloat16, float16)")
+        layout = self.layout(batch_size, max_seq_length, n_heads, dtype, ring, head_dim)
         self.batch_size, self.max_seq_length = batch_size, max_seq_length
         self.n_heads, self.head_dim, self.dtype, self.has_ring = n_heads, head_dim, dtype, bool(ring)
-        layout = self.layout(batch_size, max_seq_length, n_heads, dtype, ring)
         if storage is None:
             storage = {n: torch.zeros(shape, dtype=torch.uint8, device=device).view(dt) if dt is torch.float8_e4m3fn
                        else torch.zeros(shape, dtype=dt, device=device) for n, (shape, dt) in layout.items()}
@@ -215,8 +211,12 @@ class FlashKVCache8:
         self.cross_attn_len = 0
 
     @classmethod
-    def layout(cls, batch_size: int, max_seq_length: int, n_heads: int, dtype, ring: bool) -> dict:
+    def layout(cls, batch_size: int, max_seq_length: int, n_heads: int, dtype, ring: bool, head_dim: int = 64) -> dict:
         """Shape and dtype of every buffer."""
+        if head_dim != 64:
+            raise NotImplementedError(f"head_dim {head_dim} is not supported (only 64)")
+        if dtype not in _FILL_DTYPES:
+            raise TypeError(f"dtype {dtype} is not supported (bfloat16, float16)")
         blocks = -(-max_seq_length // cls.BLOCK)
         res = {}
         for n in "kv":
@@ -307,7 +307,7 @@ def _cache_buffers(n_slots: int, n_heads: int, head_dim: int, seq_len: int, dtyp
                    ring: bool) -> dict[str, tuple[tuple[int, ...], torch.dtype]]:
     """Shape and dtype of every buffer of one cache, 16-bit (``dtype``'s, head-major) or 8-bit."""
     if bits == 8:
-        return FlashKVCache8.layout(n_slots, seq_len, n_heads, dtype, ring)
+        return FlashKVCache8.layout(n_slots, seq_len, n_heads, dtype, ring, head_dim)
     if bits != 16:
         raise ValueError(f"cache_bits {bits} is not 16 (dtype's) or 8")
     return {n: ((n_slots, n_heads, seq_len, head_dim), dtype) for n in ("k_storage", "v_storage")}
