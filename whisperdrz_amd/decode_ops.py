@@ -287,12 +287,39 @@ class QuantLinear4(nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, group={self.group}, bias={self.bias is not None}"
 
 
+class QuantLinear4Rows(QuantLinear4):
+    """``features`` output features of another layer from ``first`` on, whole tiles of 16: views of that layer's
+    buffers, taken at every use. It has none of its own, so ``to``, ``load_state_dict`` and copies leave the weights
+    in one place."""
+
+    def __init__(self, whole: QuantLinear4, first: int, features: int, bias: bool = True):
+        nn.Module.__init__(self)
+        if first % 16 or features % 16 or features <= 0 or not 0 <= first <= whole.out_features - features:
+            raise ValueError(f"features {first} .. {first + features - 1} are not whole tiles of the layer's {whole.out_features}")
+        self.in_features, self.out_features, self.group = whole.in_features, features, whole.group
+        self._whole, self._first, self._bias = (whole,), first, bias  # the tuple keeps it from being a submodule
+
+    @property
+    def packed(self) -> torch.Tensor:
+        return self._whole[0].packed[self._first // 16:(self._first + self.out_features) // 16]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._whole[0].scales[self._first // 16:(self._first + self.out_features) // 16]
+
+    @property
+    def bias(self) -> Optional[torch.Tensor]:
+        b = self._whole[0].bias
+        return b[self._first:self._first + self.out_features] if self._bias and b is not None else None
+
+
 def _linear4_operands(x: torch.Tensor, lin: QuantLinear4):
     """The checked rows ``[M, K]`` of ``x`` and the layer's packed weights, scales and bias."""
     dtype = x.dtype
     if dtype not in _LN16:
         raise TypeError(f"x: dtype {dtype} is not supported (bfloat16, float16)")
-    own = lin._buffers  # nn.Module's attribute lookup costs 0.15 us a name
+    # nn.Module's attribute lookup costs 0.15 us a name
+    own = lin._buffers or {"packed": lin.packed, "scales": lin.scales, "bias": lin.bias}
     packed, scales, bias = own["packed"], own["scales"], own["bias"]
     _check_cuda("x", x, packed.device)
     if scales.dtype != dtype or scales.device != x.device or (

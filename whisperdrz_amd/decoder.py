@@ -39,8 +39,9 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from .attention import flash_attn_with_kvcache, flash_attn_with_kvcache8, scaled_dot_product_attention
-from .decode_ops import (LN_LINEAR_MAX_K, LN_LINEAR_ROWS, QuantLinear4, add_layernorm_, add_layernorm_partials_, layer_norm,
-                         linear, linear4, linear4_partials, linear_gelu, linear_partials, ln_linear, step_begin, step_end_)
+from .decode_ops import (LN_LINEAR_MAX_K, LN_LINEAR_ROWS, QuantLinear4, QuantLinear4Rows, add_layernorm_,
+                         add_layernorm_partials_, layer_norm, linear, linear4, linear4_partials, linear_gelu,
+                         linear_partials, ln_linear, step_begin, step_end_)
 from .kv_cache import FlashKVCache, FlashKVCache8, KVSlotPool
 
 # Batch buckets of the captured decode step (reference transcriber.py:18).
@@ -179,16 +180,13 @@ class MultiHeadAttention(nn.Module):
                                  cache_batch_idx=batch_idx, softmax_scale=scale, causal=self.causal)
 
     def quantize_linears_(self, group: int) -> None:
-        """The projections of the activations in 4 bits: query (self: query, key and value, also as one
-        layer of whole feature tiles whose parts share its memory) and out. ``n_state`` a multiple of 16."""
+        """The projections of the activations in 4 bits: query (self: query, key and value, one layer ``qkv4``
+        whose rows the three are) and out. ``n_state`` a multiple of 16."""
         n = self.n_state
         if self.causal:
             w, b = self.qkv_weight()
             self.qkv4 = whole = QuantLinear4.from_weight(w, b, group)
-            part = lambda i, bias: QuantLinear4(n, n, group, whole.packed[i * n // 16:(i + 1) * n // 16],
-                                                whole.scales[i * n // 16:(i + 1) * n // 16],
-                                                whole.bias[i * n:(i + 1) * n] if bias else None)
-            self.query, self.key, self.value = part(0, True), part(1, False), part(2, True)
+            self.query, self.key, self.value = (QuantLinear4Rows(whole, i * n, n, bias=i != 1) for i in range(3))
             self._qkv_cache = None
         else:
             self.query = QuantLinear4.from_linear(self.query, group)
