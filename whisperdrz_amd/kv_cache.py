@@ -203,6 +203,7 @@ class FlashKVCache8:
         if not ring:
             self.k_ring = self.v_ring = None
         self.device = self.k_codes.device
+        self._held = tuple(storage[n] for n in layout)  # the kernels' pointers are these tensors', whatever the attributes become
         self.struct = _lib.Kv8(*(storage[n].data_ptr() if n in layout else None for n in
                                  ("k_codes", "v_codes", "k_scales", "v_scales", "k_ring", "v_ring")),
                                batch_size, n_heads, max_seq_length)
