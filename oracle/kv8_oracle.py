@@ -99,7 +99,8 @@ def bound(out, mag, big, n_keys: int, half_step: float, one_part: bool = False) 
     """How far a kernel may be from ``attend``: the result's own rounding (half a step of its type), and in
     units of sum p |v|: twice the error of a score (64 products and a few factors in fp32; it counts in
     the probability and in the sum), the probability's two 16-bit parts (2^-16) with its exp2 (2^-22),
-    and the fp32 sums over the keys. ``one_part``: the probabilities are one fp16 value each, p (1 + e) with
+    and the fp32 sums over the keys. ``one_part``, for a form that holds less than the kernels do: the
+    probabilities are one fp16 value each, p (1 + e) with
     |e| <= 2^-11, above and below the line alike: sum p e v - out sum p e over sum p, at most
     2^-11 (sum p |v| + |out|) <= 2^-10 sum p |v|; those under fp16's normal range, 2^-14 against a largest
     of at least 1, are off by 2^-25 instead, n_keys 2^-25 in all twice."""

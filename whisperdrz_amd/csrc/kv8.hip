@@ -828,12 +828,12 @@ __global__ __launch_bounds__(kWaves * 64, 4) void kv8_attn_kernel(Kv8Cache c, Kv
 // four wavefronts, into one of two LDS buffers while the other is computed; no partial leaves a wavefront.
 // First the stages of codes, then those of 16-bit rows (the ring's and the new ones). The probabilities'
 // sums come from the matrix cores too. Bound: issue, 28 matrix products of 16 cycles and about 145 VALU instructions a
-// wavefront and stage, which add up: softmax and matrix products of a SIMD's wavefronts hardly overlap.
-// 16 prompts of 224 over 1500 positions 67 us, 64 prompts 245; in blocks of 16 queries 93. Over themselves, with the
-// append's workgroups behind those of the attention, 26 us; with the append in a launch of its own 31 (it takes 10);
-// with each row's next to its attention's 31. 32 queries a wavefront and stages of 32 keys were no faster.
-// Probabilities of bf16 prompts as one fp16 operand instead of two parts: 64 us, 64 prompts 220, but wrong where many
-// small ones count.
+// wavefront and stage, which add up: softmax and matrix products of a SIMD's wavefronts hardly overlap (counters of 16
+// prompts of 224 over 1500 positions: VALU 60% of the time, MFMA 33%, both at once 11%). These take 67 us, 64 prompts
+// 245; in blocks of 16 queries 95. Over themselves, with the append's workgroups behind those of the attention, 26 us;
+// with the append in a launch of its own 31 (it takes 10), with each row's next to its attention's 31. 32 queries a
+// wavefront and stages of 32 keys were slower. Probabilities of bf16 prompts as one fp16 operand instead of two parts
+// took 64 us, 64 prompts 220, but are wrong where many small ones count.
 constexpr int kStageKeys = 2 * kBlk;
 
 constexpr int kPromptQueries = kKv8PromptQueries;

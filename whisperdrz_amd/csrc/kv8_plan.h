@@ -35,7 +35,10 @@ __host__ __device__ inline int kv8_first_rows(const Kv8Blocks& b, int wave, int 
 //   1 stream of 20 heads: 500 positions 4.6 / 6.0, 1000 5.3 / 6.3, 1500 6.4 / 6.9, 3000 11.8 / 7.6, 6000
 //   19.1 / 8.9, 20000 58.3 / 14.8; 2 streams: 1500 7.8 / 7.2, 3000 12.0 / 8.4; 4: 1500 8.1 / 8.2, 3000
 //   12.2 / 9.7, 6000 22.7 / 14.8; 6: 1500 8.4 / 8.7, 6000 24.0 / 19.7; 8: 1500 9.0 / 10.2.
-// More splits than fill the CUs once gain nothing (4 streams of 3000: 3 splits 9.7, 4 10.7).
+// More splits than fill the CUs once gain nothing (4 streams of 3000: 3 splits 9.7, 4 10.7). Nor do more queries
+// over 1500 positions, 1 / 2 / 3 / 4 splits: five queries of 4 streams 8.7 / 8.7 / 8.5 / 9.8, of 8 10.0 / 12.4 /
+// 11.3 / 12.1, of 16 15.1 / 17.0 / 17.0 / 18.2, of 52 39 / 43 / 44 / 46; 17 queries of 52 69 / 84 / 89 / 93. One
+// stream's five would gain 0.8 us (8.3 / 8.2 / 7.8 / 7.5).
 constexpr int64_t kKv8Cus = 256;
 constexpr int64_t kKv8SplitMinLk = 2048;
 constexpr int64_t kKv8SplitMinKeys = 512;
@@ -45,9 +48,9 @@ constexpr int64_t kKv8SplitMinKeys = 512;
 // queries follow the same lines: cross over 1500, 1 stream 7.6 / 9.2, 8 10.1 / 12.3, 16 16.3 / 16.0; 6000
 // positions, 1 stream, 1 / 8 splits 23.3 / 9.6.
 // 64 queries a workgroup instead of 16 once blocks of 16 would be more than four workgroups a CU. Us, 16 / 64:
-// over 1500 positions 4 prompts of 224 (1120 blocks of 16) 28.6 / 32.7, 8 of 224 (2240) 48.5 / 40.8, 16 of 64
-// (1280) 37.8 / 32.1, 8 of 40 (480) 16.9 / 24.2; over themselves 4 of 224 19.8 / 13.8, 16 of 224 46.7 / 26.0,
-// 16 of 64 18.2 / 9.9. Up to 32 queries blocks of 16 append in the same launch (52 of 17: 68.8 / 74.3).
+// over 1500 positions 4 prompts of 224 (1120 blocks of 16) 28.4 / 31.8, 8 of 224 (2240) 49.8 / 42.4, 16 of 64
+// (1280) 37.3 / 32.3, 8 of 40 (480) 16.5 / 23.6; over themselves 4 of 224 20.0 / 13.4, 16 of 224 46.7 / 27.0,
+// 16 of 64 17.9 / 9.6. Up to 32 queries blocks of 16 append in the same launch (52 of 17: 68.8 / 74.3).
 constexpr int64_t kKv8PromptWgs = 1024;
 inline void kv8_plan(int64_t B, int64_t sq, int64_t H, int64_t Lk, Kv8Args* a) {
   const int block = sq == 1 ? 1 : sq <= 8 ? 8 : sq <= kKv8FusedAppend || B * ((sq + 15) / 16) * H <= kKv8PromptWgs ? 16 : kKv8PromptQueries;
