@@ -514,6 +514,112 @@ int wdrz_linear4_partials(int dtype, const void* x, int64_t x_stride, const void
                           const void* scales_packed, float* partials, int64_t M, int64_t N, int64_t K,
                           int64_t group, int n_split, void* stream);
 
+/*
+ * Page tables of a paged key/value cache. A stream holds positions 0 .. seq_lens[s] - 1 in the pages
+ * tables[s][0 .. page_counts[s] - 1], position p in row p % page_size of page tables[s][p / page_size]; its
+ * slot is that page * page_size + p % page_size. The pages that no stream holds are free_pages[0 .. *n_free - 1].
+ * All device memory; page_size 16, 32, 64, 128 or 256; max_seq positions a stream at most, max_pages * page_size
+ * or less; n_streams up to 15360.
+ */
+typedef struct wdrz_page_tables {
+  int32_t* tables;      /* [n_streams, max_pages] */
+  int32_t* page_counts; /* [n_streams] */
+  int32_t* seq_lens;    /* [n_streams] */
+  int32_t* free_pages;  /* [n_pages] */
+  int32_t* n_free;      /* [1] */
+  int64_t n_streams, n_pages, page_size, max_pages, max_seq;
+} wdrz_page_tables;
+
+/*
+ * Gives B requests' new tokens their places, in place on the tables: request i adds new_lens[i] tokens
+ * (NULL: new_all each) to stream streams[i] (NULL: stream i), taking the pages that it needs from the end of
+ * free_pages, the first request first. Requests are served in order while pages last; one that needs more than
+ * are left gets nothing, and neither does one that names no stream or one that an earlier request named, a
+ * negative count, or more positions than max_seq: its stream stays as it was.
+ * cu_seqlens: [B + 1] sums of the new tokens. starts: [B] positions before them, -1: got nothing.
+ * slots, positions: int64 [total] of the packed tokens; -1 and 0 for those of a request that got nothing and
+ * behind the last request. total: at least the sum of the new tokens (sums are cut off at it).
+ */
+int wdrz_page_plan(const wdrz_page_tables* pages, const int32_t* new_lens, int64_t new_all,
+                   const int32_t* streams, int32_t* cu_seqlens, int32_t* starts, int64_t* slots,
+                   int64_t* positions, int64_t B, int64_t total, void* stream);
+
+/*
+ * Sets streams back to lens[i] positions (NULL: len_all each), their pages behind them free again (table entries
+ * -1). A request that names no stream or one that an earlier request named, or a length above the stream's, does
+ * nothing. After a plan of the same requests in the same order the stack is what it was before the plan.
+ */
+int wdrz_page_truncate(const wdrz_page_tables* pages, const int32_t* lens, int64_t len_all,
+                       const int32_t* streams, int64_t B, void* stream);
+
+/* One layer's pages, [n_pages, n_heads, page_size, head_dim] of a 16-bit dtype, head_dim 64 or 128. */
+typedef struct wdrz_kv_pages {
+  void* k_pages;
+  void* v_pages;
+  int64_t n_pages, n_heads, page_size, head_dim;
+} wdrz_kv_pages;
+
+/*
+ * Writes rows k_src, v_src [T, n_heads, head_dim] (strides of t, h; head_dim contiguous) to slots[t]. A slot
+ * outside the cache is left out. Of rows that name one slot any may stay. The counterpart of wdrz_kv_fill.
+ */
+int wdrz_page_write(int dtype, const wdrz_kv_pages* cache, const void* k_src, const int64_t* k_strides,
+                    const void* v_src, const int64_t* v_strides, const int64_t* slots, int64_t T, void* stream);
+
+/* Workspace (bytes) of wdrz_attn_kvpages: 256-byte aligned, zeroed once, kept per stream (calls leave its
+ * counters zero). max_seq as in the tables. */
+size_t wdrz_attn_kvpages_workspace_size(int64_t B, int64_t sq, int64_t H, int64_t n_heads, int64_t head_dim,
+                                        int64_t max_seq);
+
+/*
+ * Attention against a paged cache: the counterpart of wdrz_attn_kvcache.
+ *
+ * q, o: [B, sq, H, head_dim] of a 16-bit dtype, H a multiple of the cache's n_heads; query head h reads head
+ *   h / (H / n_heads). cache_batch_idx: int32 [B] row -> stream (NULL: row b is stream b).
+ * k_new, v_new [B, sq, n_heads, head_dim] given: written at positions cache_seqlens[b] + t, whose pages the table
+ *   has to name already (wdrz_page_plan); query t attends positions j <= cache_seqlens[b] + t. A row that
+ *   names the stream of another row gives NaN, and so does that one; neither is written.
+ * Both NULL: every query attends the first cache_seqlens[b] positions; none: zeros.
+ * A stream or length out of range gives NaN rows and writes nothing (a plan's starts of -1 do). A page out of
+ * range among a row's gives NaN; new rows are then written where their own page is in range.
+ * The pages' seq_lens and page_counts are not read.
+ */
+int wdrz_attn_kvpages(int dtype, const wdrz_kv_pages* cache, const wdrz_page_tables* pages, const void* q,
+                      const int64_t* q_strides, const void* k_new, const int64_t* kn_strides, const void* v_new,
+                      const int64_t* vn_strides, const int32_t* cache_seqlens, const int32_t* cache_batch_idx,
+                      void* o, const int64_t* o_strides, int64_t B, int64_t sq, int64_t H, float softmax_scale,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention of B packed sequences of different lengths: the counterpart of wdrz_attn_fwd without padding.
+ *
+ * q, o: [T, H, D], k, v: [Tk, Hk, D] of a 16-bit dtype, D 64 or 128, H a multiple of Hk (head h reads h / (H / Hk));
+ * strides of t, h; D contiguous. Sequence i is rows cu_q[i] .. cu_q[i + 1] - 1 of q and cu_k[i] .. cu_k[i + 1] - 1
+ * of k and v (cu_k NULL: cu_q), int32 [B + 1], ascending from 0 or above.
+ * causal: query t of a sequence attends its keys j <= t + (keys - queries), else all; none: zeros.
+ * Rows of o that no sequence holds are left as they are.
+ */
+int wdrz_attn_packed(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                     const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides,
+                     const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t T, int64_t Tk, int64_t H,
+                     int64_t Hk, int64_t D, float scale, int causal, void* stream);
+
+/* Workspace (bytes) of wdrz_token_logprobs: 256-byte aligned, zeroed once, kept per stream. */
+size_t wdrz_token_logprobs_workspace_size(int64_t rows, int64_t V, int64_t top);
+
+/*
+ * Log probabilities of tokens[rows] (int64) under logits [rows, V] (row stride l_stride, tokens contiguous), the
+ * entropy of each row's distribution (in nats) and its `top` (0 .. 32) likeliest tokens with their log
+ * probabilities, ties by the lower index. blocked: bool [rows, >= V] or NULL, tokens that count as -inf.
+ * A token out of range has NaN. Rows without a token above -inf: log probability -inf, entropy 0. NaN or +inf
+ * among a row's tokens: all NaN. Alternatives that do not exist have id -1 and -inf (NaN rows: NaN).
+ * V up to 2^20, rows up to 2^24.
+ */
+int wdrz_token_logprobs(int dtype, const void* logits, int64_t l_stride, const uint8_t* blocked, int64_t b_stride,
+                        const int64_t* tokens, float* logprobs, float* entropy, float* top_logprobs,
+                        int64_t* top_ids, int64_t rows, int64_t V, int64_t top, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,17 +10,21 @@ from .attention import (
     WorkspaceCache,
     flash_attn_with_kvcache,
     flash_attn_with_kvcache8,
+    flash_attn_with_kvpages,
     kvcache8_workspace_size,
     kvcache_workspace_size,
+    kvpages_workspace_size,
+    packed_attention,
     qkv_attention,
     scaled_dot_product_attention,
 )
 from .audio import LogMelSpectrogram, log_mel_spectrogram
-from .decode_ops import (QuantLinear4, add_layernorm_, add_layernorm_partials_, layer_norm, linear, linear4,
-                         linear4_partials, linear_gelu, linear_partials, ln_linear, masked_argmax)
+from .decode_ops import (QuantLinear4, TokenLogprobs, add_layernorm_, add_layernorm_partials_, layer_norm, linear, linear4,
+                         linear4_partials, linear_gelu, linear_partials, ln_linear, masked_argmax, token_logprobs)
 from .dtw import (compute_attention, dtw_attention_prep, dtw_prep, dtw_prep_batch, dtw_prep_workspace_size,
                   median_filter)
 from .kv_cache import FlashKVCache8
+from .paged import FlashKVPages, KVPagePool, PagePlan, PageTables
 
 from .debug import check_kvcache_metadata, force_torch, probe
 
@@ -34,6 +38,11 @@ __all__ = [
     "force_torch",
     "probe",
     "FlashKVCache8",
+    "FlashKVPages",
+    "KVPagePool",
+    "PagePlan",
+    "PageTables",
+    "TokenLogprobs",
     "LogMelSpectrogram",
     "QuantLinear4",
     "add_layernorm_",
@@ -46,6 +55,7 @@ __all__ = [
     "linear_partials",
     "ln_linear",
     "masked_argmax",
+    "token_logprobs",
     "log_mel_spectrogram",
     "compute_attention",
     "dtw_attention_prep",
@@ -56,8 +66,11 @@ __all__ = [
     "WorkspaceCache",
     "flash_attn_with_kvcache",
     "flash_attn_with_kvcache8",
+    "flash_attn_with_kvpages",
     "kvcache8_workspace_size",
     "kvcache_workspace_size",
+    "kvpages_workspace_size",
+    "packed_attention",
     "qkv_attention",
     "scaled_dot_product_attention",
 ]

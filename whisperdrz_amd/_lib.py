@@ -56,6 +56,14 @@ EXPORTED_SYMBOLS = (
     "wdrz_attn_kvcache8",
     "wdrz_linear4",
     "wdrz_linear4_partials",
+    "wdrz_page_plan",
+    "wdrz_page_truncate",
+    "wdrz_page_write",
+    "wdrz_attn_kvpages_workspace_size",
+    "wdrz_attn_kvpages",
+    "wdrz_attn_packed",
+    "wdrz_token_logprobs_workspace_size",
+    "wdrz_token_logprobs",
 )
 ABI_VERSION = 1
 
@@ -74,6 +82,19 @@ class Kv8(ctypes.Structure):
 
     _fields_ = [(n, _p) for n in ("k_codes", "v_codes", "k_scales", "v_scales", "k_ring", "v_ring")] + \
                [(n, _i64) for n in ("n_slots", "n_heads", "max_seq")]
+
+
+class PageTables(ctypes.Structure):
+    """``wdrz_page_tables``: the buffers and sizes of a paged cache's bookkeeping."""
+
+    _fields_ = [(n, _p) for n in ("tables", "page_counts", "seq_lens", "free_pages", "n_free")] + \
+               [(n, _i64) for n in ("n_streams", "n_pages", "page_size", "max_pages", "max_seq")]
+
+
+class KvPages(ctypes.Structure):
+    """``wdrz_kv_pages``: one layer's pages."""
+
+    _fields_ = [(n, _p) for n in ("k_pages", "v_pages")] + [(n, _i64) for n in ("n_pages", "n_heads", "page_size", "head_dim")]
 
 
 def _declare(lib: ctypes.CDLL) -> None:
@@ -209,6 +230,36 @@ def _declare(lib: ctypes.CDLL) -> None:
         ctypes.c_int, _p, _i64, _p, _p, _p,  # dtype, x, x stride, w, scales, partials
         _i64, _i64, _i64, _i64, ctypes.c_int, _p,  # M, N, K, group, n_split, stream
     ]
+    tablesp, kvpagesp = ctypes.POINTER(PageTables), ctypes.POINTER(KvPages)
+    lib.wdrz_page_plan.restype = ctypes.c_int
+    lib.wdrz_page_plan.argtypes = [
+        tablesp, _i32p, _i64, _i32p, _i32p, _i32p,  # pages, new_lens, new_all, streams, cu_seqlens, starts
+        _p, _p, _i64, _i64, _p,  # slots, positions, B, total, stream
+    ]
+    lib.wdrz_page_truncate.restype = ctypes.c_int
+    lib.wdrz_page_truncate.argtypes = [tablesp, _i32p, _i64, _i32p, _i64, _p]  # pages, lens, len_all, streams, B, stream
+    lib.wdrz_page_write.restype = ctypes.c_int
+    lib.wdrz_page_write.argtypes = [ctypes.c_int, kvpagesp, _p, _i64p, _p, _i64p, _p, _i64, _p]  # dtype, cache, k, v, slots, T, stream
+    lib.wdrz_attn_kvpages_workspace_size.restype = ctypes.c_size_t
+    lib.wdrz_attn_kvpages_workspace_size.argtypes = [_i64] * 6
+    lib.wdrz_attn_kvpages.restype = ctypes.c_int
+    lib.wdrz_attn_kvpages.argtypes = [
+        ctypes.c_int, kvpagesp, tablesp, _p, _i64p, _p, _i64p, _p, _i64p,  # dtype, cache, pages, q, k_new, v_new with strides
+        _i32p, _i32p, _p, _i64p,  # cache_seqlens, cache_batch_idx, out, strides
+        _i64, _i64, _i64, ctypes.c_float, _p, ctypes.c_size_t, _p,  # B, sq, H, softmax_scale, workspace, bytes, stream
+    ]
+    lib.wdrz_attn_packed.restype = ctypes.c_int
+    lib.wdrz_attn_packed.argtypes = [
+        ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _i32p, _i32p,  # dtype, q, k, v, out with strides, cu_q, cu_k
+        _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, ctypes.c_int, _p,  # B, T, Tk, H, Hk, D, scale, causal, stream
+    ]
+    lib.wdrz_token_logprobs_workspace_size.restype = ctypes.c_size_t
+    lib.wdrz_token_logprobs_workspace_size.argtypes = [_i64] * 3
+    lib.wdrz_token_logprobs.restype = ctypes.c_int
+    lib.wdrz_token_logprobs.argtypes = [
+        ctypes.c_int, _p, _i64, _p, _i64, _p, _p, _p, _p, _p,  # dtype, logits, stride, blocked, stride, tokens, outputs
+        _i64, _i64, _i64, _p, ctypes.c_size_t, _p,  # rows, V, top, workspace, bytes, stream
+    ]
 
 
 def load() -> ctypes.CDLL:
@@ -267,6 +318,12 @@ def last_error() -> str:
 def strides(s: tuple) -> ctypes.Array:
     """:func:`strides4` of a tuple, built once per value (the entry points only read it)."""
     return (ctypes.c_int64 * 4)(*s)
+
+
+@functools.lru_cache(maxsize=4096)
+def strides3(s: tuple) -> ctypes.Array:
+    """The strides of [T, H, D] rows, built once per value."""
+    return (ctypes.c_int64 * 3)(*s)
 
 
 def strides4(s) -> ctypes.Array:

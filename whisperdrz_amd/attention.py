@@ -31,8 +31,11 @@ __all__ = [
     "flash_attn_with_kvcache8",
     "scaled_dot_product_attention",
     "qkv_attention",
+    "flash_attn_with_kvpages",
+    "packed_attention",
     "kvcache_workspace_size",
     "kvcache8_workspace_size",
+    "kvpages_workspace_size",
     "WorkspaceCache",
 ]
 
@@ -357,6 +360,186 @@ def flash_attn_with_kvcache8(
     )
     if rc != _lib.WDRZ_OK:
         _raise(rc, "flash_attn_with_kvcache8")
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def kvpages_workspace_size(batch: int, sq: int, n_heads: int, n_kv_heads: int, head_dim: int, max_seq: int) -> int:
+    """Bytes of split-KV workspace :func:`flash_attn_with_kvpages` needs for these sizes."""
+    return int(_lib.load().wdrz_attn_kvpages_workspace_size(batch, sq, n_heads, n_kv_heads, head_dim, max_seq))
+
+
+# Workspaces whose counters stand at their start, apart from _WORKSPACES: calls of other shapes leave the counters
+# where they are, so nothing but they has to be zero after a call.
+_COUNTED_WORKSPACES = WorkspaceCache()
+
+
+def _counted_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """This stream's workspace; a captured call gets its own, cleared by every replay (another graph captured on
+    this stream may be replayed beside its graph)."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return _COUNTED_WORKSPACES.get(device, nbytes)
+
+
+def flash_attn_with_kvpages(
+    q: torch.Tensor,
+    cache,
+    k: Optional[torch.Tensor] = None,
+    v: Optional[torch.Tensor] = None,
+    cache_seqlens=None,
+    cache_batch_idx: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+    *,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """:func:`flash_attn_with_kvcache` against a paged cache (a ``FlashKVPages``), with grouped heads.
+
+    ``q`` ``[B, sq, H, D]`` in the cache's dtype, H a multiple of the cache's heads (query head h reads head
+    ``h // (H / n_heads)``); ``cache_seqlens`` ``[B]`` (a plan's ``starts``); ``cache_batch_idx`` ``[B]`` row -> stream
+    (identity if None). The streams' own ``seq_lens`` are not read.
+
+    With ``k`` / ``v`` ``[B, sq, n_heads, D]``: they are written at positions ``cache_seqlens[b] + t``, whose pages
+    ``PageTables.plan`` has given, and query ``t`` attends positions ``j <= cache_seqlens[b] + t``. Without them every
+    query attends the first ``cache_seqlens[b]`` positions; a row of none gives zeros.
+    A stream or length out of range (a start of -1 among them) gives NaN rows and writes nothing; so do rows that
+    append to one stream in one call. A page out of range gives NaN too (``WDRZ_DEBUG=1`` raises for all of these).
+
+    ``out`` is a preallocated output, ``workspace`` a caller-owned split-KV workspace (zero-filled before its first
+    use; :func:`kvpages_workspace_size`). Without it calls of one stream share a cached one, and a call that is
+    captured into a graph gets its own, cleared by every replay.
+    """
+    if not (isinstance(q, torch.Tensor) and q.is_cuda):
+        _check_cuda("q", q, q.device if isinstance(q, torch.Tensor) else None)
+    device, shape, dtype = q.device, q.shape, q.dtype
+    if cache.device != device:
+        raise RuntimeError(f"the cache is on {cache.device}, expected {device}")
+    if len(shape) != 4:
+        raise ValueError("q must be 4-D ([B, sq, H, D])")
+    B, sq, H, D = shape
+    heads = cache.n_heads
+    if H % heads or H == 0 or D != cache.head_dim:
+        raise ValueError(f"cache heads/head_dim {(heads, cache.head_dim)} do not match q {(H, D)}")
+    if dtype != cache.dtype:
+        raise TypeError(f"q must have the cache's dtype {cache.dtype}")
+    k_ptr = k_strides = v_ptr = v_strides = idx_ptr = ws_ptr = None
+    if k is not None or v is not None:
+        if k is None or v is None:
+            raise ValueError("k and v must be given together")
+        for name, t in (("k", k), ("v", v)):
+            if not isinstance(t, torch.Tensor) or t.device != device:
+                _check_cuda(name, t, device)
+            if t.shape != (B, sq, heads, D):
+                raise ValueError(f"{name} must have shape {(B, sq, heads, D)}")
+            if t.dtype is not dtype:
+                raise TypeError("k and v must have q's dtype")
+        k_ptr, k_strides, v_ptr, v_strides = k.data_ptr(), _lib.strides(k.stride()), v.data_ptr(), _lib.strides(v.stride())
+    if cache_seqlens is None:
+        raise ValueError("cache_seqlens is required")
+    cache_seqlens = _check_ids("cache_seqlens", cache_seqlens, B, device)
+    if cache_batch_idx is not None:
+        cache_batch_idx = _check_ids("cache_batch_idx", cache_batch_idx, B, device)
+        idx_ptr = cache_batch_idx.data_ptr()
+    if out is None:
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=device)
+    else:
+        _check_cuda("out", out, device)
+        if out.shape != shape or out.dtype != dtype:
+            raise ValueError("out must match q's shape and dtype")
+    if B == 0 or sq == 0:
+        return out
+    index = device.index
+    if index != _current_device():  # launches go to the current device
+        with torch.cuda.device(index):
+            return flash_attn_with_kvpages(q, cache, k, v, cache_seqlens, cache_batch_idx, softmax_scale, out=out,
+                                           workspace=workspace)
+    lib, ws_bytes = _lib.load(), 0
+    nbytes = kvpages_workspace_size(B, sq, H, heads, D, cache.max_seq_length)
+    if nbytes:
+        if workspace is None:
+            workspace = _counted_workspace(device, nbytes)
+        else:
+            _check_cuda("workspace", workspace, device)
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if ws_bytes < nbytes:
+            raise ValueError(f"workspace too small: need {nbytes} bytes")
+    rc = lib.wdrz_attn_kvpages(
+        _DTYPES16[dtype], cache.struct, cache.page_tables.struct, q.data_ptr(), _lib.strides(q.stride()), k_ptr, k_strides,
+        v_ptr, v_strides, cache_seqlens.data_ptr(), idx_ptr, out.data_ptr(), _lib.strides(out.stride()), B, sq, H,
+        D ** -0.5 if softmax_scale is None else softmax_scale, ws_ptr, ws_bytes, _raw_stream(index),
+    )
+    if rc != _lib.WDRZ_OK:
+        _raise(rc, "flash_attn_with_kvpages")
+    return out
+
+
+def packed_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    cu_seqlens_k: Optional[torch.Tensor] = None,
+    causal: bool = True,
+    scale: Optional[float] = None,
+    *,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of sequences of different lengths, packed without padding: ``q`` ``[T, H, D]``, ``k`` and ``v``
+    ``[Tk, Hk, D]`` in bf16 or fp16, D 64 or 128, H a multiple of Hk (query head h reads head ``h // (H / Hk)``); strided
+    views of a projection where the last dimension is contiguous.
+
+    Sequence i is rows ``cu_seqlens[i] .. cu_seqlens[i + 1] - 1`` of the queries (int32 ``[B + 1]``, ascending; a
+    plan's ``cu_seqlens``) and, with ``cu_seqlens_k``, rows of the keys of its own. ``causal``: query t sees the keys
+    ``j <= t + (keys - queries)`` of its sequence, the last query all of them; else every query sees all. A query that
+    sees none gives zeros. Rows that no sequence holds are left as they are in ``out`` (a new one is not filled there).
+    """
+    if not (isinstance(q, torch.Tensor) and q.is_cuda):
+        _check_cuda("q", q, q.device if isinstance(q, torch.Tensor) else None)
+    device, shape, dtype = q.device, q.shape, q.dtype
+    dt = _DTYPES16.get(dtype)
+    if dt is None:
+        raise TypeError(f"q: dtype {dtype} is not supported (bfloat16, float16)")
+    for name, t in (("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or t.device != device:
+            _check_cuda(name, t, device)
+        if t.dtype is not dtype:
+            raise TypeError("k and v must have q's dtype")
+    if len(shape) != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != shape[2]:
+        raise ValueError(f"q must be [T, H, D] and k, v [Tk, Hk, D], got {tuple(shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    T, H, D = shape
+    Tk, Hk = k.shape[0], k.shape[1]
+    if H == 0 or Hk == 0 or H % Hk:
+        raise ValueError(f"{H} query heads are not a multiple of {Hk}")
+    sums = []
+    for name, t in (("cu_seqlens", cu_seqlens), ("cu_seqlens_k", cu_seqlens_k)):
+        if t is None and name == "cu_seqlens_k":
+            if Tk != T:
+                raise ValueError(f"{Tk} keys for {T} queries need cu_seqlens_k")
+            sums.append(None)
+            continue
+        n = t.shape[0] if isinstance(t, torch.Tensor) and t.dim() == 1 else 0
+        if n == 0 or (sums and n != sums[0].shape[0]):
+            raise ValueError(f"{name} must be a tensor of whole numbers [B + 1]")
+        sums.append(_check_ids(name, t, n, device))
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device)
+    else:
+        _check_cuda("out", out, device)
+        if out.shape != shape or out.dtype != dtype:
+            raise ValueError("out must match q's shape and dtype")
+    index = device.index
+    if index != _current_device():  # launches go to the current device
+        with torch.cuda.device(index):
+            return packed_attention(q, k, v, sums[0], sums[1], causal, scale, out=out)
+    rc = _lib.load().wdrz_attn_packed(
+        dt, q.data_ptr(), _lib.strides3(q.stride()), k.data_ptr(), _lib.strides3(k.stride()), v.data_ptr(),
+        _lib.strides3(v.stride()), out.data_ptr(), _lib.strides3(out.stride()), sums[0].data_ptr(),
+        None if sums[1] is None else sums[1].data_ptr(), sums[0].shape[0] - 1, T, Tk, H, Hk, D,
+        D ** -0.5 if scale is None else scale, 1 if causal else 0, _raw_stream(index),
+    )
+    if rc != _lib.WDRZ_OK:
+        _raise(rc, "packed_attention")
     return out
 
 

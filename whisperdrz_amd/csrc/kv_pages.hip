@@ -1,0 +1,470 @@
+// kv_pages.hip — attention of new tokens over a paged key/value cache, with grouped heads.
+//
+// o[t, h] = sum_j p_j v_j / sum_j p_j, p_j = 2^(c q[t, h] k_j - m), c = scale log2(e), over the positions j that
+// query t sees: j <= n + t behind n cached positions where the call appends its rows, j < n where it only reads.
+// Position j of a stream is row j % P of page tables[stream][j / P]; pages are [head][P][D].
+//
+// A workgroup takes one key/value head of one batch row and up to 16 (query, head of the group) rows, which share
+// every key and value: one tile of the 16-row matrix instructions. A wavefront takes 32 positions at a time (two
+// tiles of 16, each inside one page, since pages hold a multiple of 16):
+//   S^T[key, row] = K Q^T     lane (li, g) = (lane % 16, lane / 16) loads 16 bytes of key 16 t + li, and gets the
+//                             scores of keys 16 t + 4 g + 0..3 for row li;
+//   O^T[dim, row] += V^T P^T  with the sum's index 8 g + 4 t + r standing for key 16 t + 4 g + r, the scores are the
+//                             operand as they lie, and V^T is made in registers: lane (li, g) loads D / 16
+//                             consecutive dims of its eight keys, whole rows by 16 lanes, and one v_perm_b32 pairs
+//                             two keys of a dim. Nothing goes through LDS before the wavefronts' sums.
+// Probabilities are two 16-bit operands (value and remainder, 2^-17 relative), since the matrix cores idle anyway.
+// A softmax reference is moved only when a score exceeds it by 2^8. The next block is requested before a block's
+// products. Bound: the bytes of keys and values, for short rows launch and the chain metadata -> table -> keys.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "wdrz_common.h"
+#include "wdrz_launch.h"
+
+namespace wdrz {
+namespace {
+
+constexpr int kRows = 16;           // (query, group head) rows a workgroup
+constexpr int kBlock = 32;          // positions a wavefront takes at a time
+constexpr int kPagesMaxSplits = 64;  // workgroups that a row's keys are cut into at most
+constexpr float kMove = 8.f;        // a reference is moved when a score is 2^8 above it
+
+template <typename T> struct Pg;
+template <> struct Pg<Bf16> {
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
+  static constexpr uint32_t kExp = 0x7f80u, kNan = 0x7fc07fc0u;
+};
+template <> struct Pg<F16> {
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
+  static __device__ __forceinline__ float lo(uint32_t w) { return f16_lo(w); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return f16_hi(w); }
+  static constexpr uint32_t kExp = 0x7c00u, kNan = 0x7e007e00u;
+};
+
+// Maximum and sum over the lanes li, li + 16, li + 32, li + 48 (every lane gets it).
+__device__ __forceinline__ float quarters_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+template <int D> struct VRow;  // D / 16 consecutive dims of a row
+template <> struct VRow<64> { typedef u32x2 type; };
+template <> struct VRow<128> { typedef u32x4 type; };
+
+template <typename T, int D, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void pages_attn_kernel(PagesArgs a) {
+  constexpr int KS = D / 32, NJ = D / 16, kThreads = 64 * kWaves, kRow = D * 2;
+  typedef typename VRow<D>::type vrow_t;
+  extern __shared__ __attribute__((aligned(16))) float sm_o[];  // [kWaves][rows of the launch][D]
+  __shared__ float sm_m[kWaves][kRows], sm_l[kWaves][kRows];
+  __shared__ float sm_pm[kPagesMaxSplits][kRows], sm_pl[kPagesMaxSplits][kRows];
+  __shared__ int sm_bad, sm_last;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int li = lane & 15, g = lane >> 4;
+  // row tiles of one (b, head) next to each other, on one XCD: they read the same keys
+  const int unit = a.n_rt > 1 ? remap_xcd((int)blockIdx.x, (int)gridDim.x) : (int)blockIdx.x;
+  const int rt = unit % a.n_rt, hk = unit / a.n_rt % a.Hk, b = unit / a.n_rt / a.Hk;
+  const int split = blockIdx.y;
+  const int r0 = rt * kRows, rows = min(kRows, a.sq * a.G - r0);
+  const int row_stride = min(kRows, a.sq * a.G);  // rows of a partial in LDS and the workspace
+
+  const bool has_new = a.kn != nullptr;
+  const int stream = a.streams ? a.streams[b] : b;
+  const int n = a.seqlens[b];
+  const int capacity = a.max_pages << a.shift;
+  bool bad = stream < 0 || stream >= a.n_streams || n < 0 || n > capacity - (has_new ? a.sq : 0);
+  if (has_new && a.streams) {  // a stream named twice: its rows would read what others write
+    bool twice = false;
+    for (int i = lane; i < a.B; i += 64) twice = twice || (i != b && a.streams[i] == stream);
+    bad = bad || __any(twice);
+  }
+  auto out_row = [&](int r) {  // r: row of the tile
+    const int t = (r0 + r) / a.G, h = hk * a.G + (r0 + r) % a.G;
+    return a.o + (int64_t)b * a.os[0] + (int64_t)t * a.os[1] + (int64_t)h * a.os[2];
+  };
+  if (bad) {
+    if (split == 0)
+      for (int i = tid; i < rows * (D / 8); i += kThreads)
+        store16(out_row(i / (D / 8)) + (i % (D / 8)) * 16, u32x4{Pg<T>::kNan, Pg<T>::kNan, Pg<T>::kNan, Pg<T>::kNan});
+    return;
+  }
+  const int32_t* table = a.tables + (int64_t)stream * a.max_pages;
+  const char* knew = has_new ? a.kn + (int64_t)b * a.kns[0] + (int64_t)hk * a.kns[2] : nullptr;
+  const char* vnew = has_new ? a.vn + (int64_t)b * a.vns[0] + (int64_t)hk * a.vns[2] : nullptr;
+  const int mask = (1 << a.shift) - 1;
+
+  // keys that some row of the tile sees, and this split's part of them
+  const int lim_hi = has_new ? n + (r0 + rows - 1) / a.G + 1 : n;
+  const int lim_lo = has_new ? n + r0 / a.G + 1 : n;
+  const int n_split_b = max(1, (lim_hi + a.chunk - 1) / a.chunk);
+  if (split >= n_split_b) return;
+  const int k0 = split * a.chunk, k1 = min(lim_hi, k0 + a.chunk);
+  if (tid == 0) sm_bad = 0;
+
+  // the new rows to their pages; every workgroup takes them from the call's own rows
+  if (has_new && rt == 0 && split == 0) {
+    for (int i = tid; i < a.sq * (D / 8); i += kThreads) {
+      const int t = i / (D / 8), p = i % (D / 8), pos = n + t;
+      const int page = table[pos >> a.shift];
+      if (page < 0 || page >= a.n_pages) continue;
+      const int64_t to = ((((int64_t)page * a.Hk + hk) << a.shift) + (pos & mask)) * kRow + p * 16;
+      store16(a.k_pages + to, load16(knew + (int64_t)t * a.kns[1] + p * 16));
+      store16(a.v_pages + to, load16(vnew + (int64_t)t * a.vns[1] + p * 16));
+    }
+  }
+
+  // queries: the B operand of S^T
+  u32x4 q[KS];
+  {
+    const int r = r0 + li, t = r / a.G, h = hk * a.G + r % a.G;
+    const char* p = a.q + (int64_t)b * a.qs[0] + (int64_t)t * a.qs[1] + (int64_t)h * a.qs[2] + g * 16;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] = li < rows ? load16(p + s * 64) : u32x4{0, 0, 0, 0};
+  }
+  const int lim = has_new ? n + min(r0 + li, r0 + rows - 1) / a.G + 1 : n;  // keys that row li sees
+
+  bool bad_page = false;
+  struct Block {
+    u32x4 k[2][KS];
+    vrow_t v[2][4];
+  };
+  // Pages of the two tiles of block kb (0 for one that is out of range or behind the keys).
+  auto pages_of = [&](int kb, int (&pg)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int pos = kb * kBlock + 16 * t;
+      pg[t] = pos < lim_hi ? table[pos >> a.shift] : 0;
+    }
+  };
+  auto load = [&](int kb, int (&pg)[2], Block& x) __attribute__((always_inline)) {
+    const int base = kb * kBlock;
+    const char* kp[2];
+    const char* vp[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      int page = __builtin_amdgcn_readfirstlane(pg[t]);
+      if (page < 0 || page >= a.n_pages) {
+        bad_page = true;
+        page = 0;
+      }
+      const int64_t at = ((((int64_t)page * a.Hk + hk) << a.shift) + ((base + 16 * t) & mask)) * kRow;
+      kp[t] = a.k_pages + at;
+      vp[t] = a.v_pages + at;
+    }
+    if (base + kBlock <= min(n, lim_hi)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x.k[t][s] = load16(kp[t] + li * kRow + g * 16 + s * 64);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x.v[t][r] = *reinterpret_cast<const vrow_t*>(vp[t] + (4 * g + r) * kRow + li * (D / 8));
+      return;
+    }
+    // cached rows, then the call's own, then none (zeros: what stands there does not count)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = base + 16 * t + li;
+      const char* p = key < n ? kp[t] + li * kRow : knew + (int64_t)(key - n) * a.kns[1];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) x.k[t][s] = key < lim_hi ? load16(p + g * 16 + s * 64) : u32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = base + 16 * t + 4 * g + r;
+        const char* p = key < n ? vp[t] + (4 * g + r) * kRow : vnew + (int64_t)(key - n) * a.vns[1];
+        x.v[t][r] = vrow_t{};
+        if (key < lim_hi) x.v[t][r] = *reinterpret_cast<const vrow_t*>(p + li * (D / 8));
+      }
+  };
+
+  f32x4 acc[NJ];  // [j][r]: row li, dim (D / 4) g + (D / 16) r + j
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, mu = 0.f, l = 0.f;  // reference, the same or 0 while there is none, this lane's sum
+
+  auto compute = [&](int kb, int (&pg)[2], Block& x) __attribute__((always_inline)) {
+    const int base = kb * kBlock;
+    float p[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; ++i) s = Pg<T>::mfma(x.k[t][i], q[i], s);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[t][r] = s[r] * a.c;
+    }
+    const bool mixed = base + kBlock > lim_lo;
+    if (mixed) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (base + 16 * t + 4 * g + r >= lim) p[t][r] = -INFINITY;
+    }
+    const float mx = quarters_max(fmaxf(fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[0][2], p[0][3])),
+                                        fmaxf(fmaxf(p[1][0], p[1][1]), fmaxf(p[1][2], p[1][3]))));
+    if (__any(mx > m + kMove)) {
+      const float to = fmaxf(m, mx);
+      const float f = m == -INFINITY ? 0.f : fast_exp2(m - to);
+      m = to;
+      mu = to == -INFINITY ? 0.f : to;
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] *= f;
+    }
+    u32x4 hi, lo;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float& p0 = p[t][2 * i];
+        float& p1 = p[t][2 * i + 1];
+        p0 = fast_exp2(p0 - mu);
+        p1 = fast_exp2(p1 - mu);
+        l += p0 + p1;
+        const uint32_t w = Pg<T>::pack(p0, p1);
+        hi[2 * t + i] = w;
+        lo[2 * t + i] = Pg<T>::pack(p0 - Pg<T>::lo(w), p1 - Pg<T>::hi(w));
+      }
+    if (mixed && has_new && a.sq > 1) {
+      // A row of the tile may not see all keys of the block: 0 times an infinity or NaN behind its mask would
+      // count in the products, so such blocks are summed key by key.
+      bool odd = false;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int w = 0; w < D / 32; ++w) {
+            const uint32_t e = x.v[t][r][w];
+            odd = odd || (e & Pg<T>::kExp) == Pg<T>::kExp || ((e >> 16) & Pg<T>::kExp) == Pg<T>::kExp;
+          }
+      if (__any(odd)) {
+#pragma unroll
+        for (int kk = 0; kk < kBlock; ++kk) {
+          const float pk = __shfl(p[kk >> 4][kk & 3], li + 16 * ((kk >> 2) & 3));
+          const int key = base + kk;
+          if (key >= lim) continue;
+          const int page = pg[kk >> 4];
+          const char* row = key < n ? a.v_pages + ((((int64_t)(page < 0 || page >= a.n_pages ? 0 : page) * a.Hk + hk) << a.shift) + (key & mask)) * kRow
+                                    : vnew + (int64_t)(key - n) * a.vns[1];
+          const uint16_t* v = reinterpret_cast<const uint16_t*>(row) + (D / 4) * g;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[j][r] = __builtin_fmaf(pk, Pg<T>::lo(v[NJ * r + j]), acc[j][r]);
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      u32x4 vt;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          vt[2 * t + i] = __builtin_amdgcn_perm(x.v[t][2 * i + 1][j / 2], x.v[t][2 * i][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+      acc[j] = Pg<T>::mfma(vt, hi, acc[j]);
+      acc[j] = Pg<T>::mfma(vt, lo, acc[j]);
+    }
+  };
+
+  // blocks of this wavefront: kb0, kb0 + kWaves, ..; the next one's loads and the one after's pages are in flight
+  const int kb_end = (k1 + kBlock - 1) / kBlock;
+  int kb = k0 / kBlock + wave;
+  if (kb < kb_end) {
+    Block cur, nxt;
+    int pg[2], pg1[2], pg2[2];
+    pages_of(kb, pg);
+    pages_of(kb + kWaves, pg1);
+    load(kb, pg, cur);
+    for (; kb < kb_end; kb += kWaves) {
+      pages_of(kb + 2 * kWaves, pg2);
+      if (kb + kWaves < kb_end) load(kb + kWaves, pg1, nxt);
+      compute(kb, pg, cur);
+      cur = nxt;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        pg[t] = pg1[t];
+        pg1[t] = pg2[t];
+      }
+    }
+  }
+  l = quarters_sum(l);
+
+  // ---- the wavefronts' sums ----
+  __syncthreads();  // sm_bad
+  if (bad_page && lane == 0) sm_bad = 1;
+  if (li < rows) {
+    float* o = sm_o + (wave * row_stride + li) * D + (D / 4) * g;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < NJ; j += 4)
+        *reinterpret_cast<f32x4*>(o + NJ * r + j) = f32x4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
+    if (g == 0) {
+      sm_m[wave][li] = m;
+      sm_l[wave][li] = l;
+    }
+  }
+  __syncthreads();
+  const bool nan = sm_bad != 0;
+  auto joined = [&](int r, int d, float& M, float& L) {
+    M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sm_m[w][r]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = fast_exp2(sm_m[w][r] - ref);
+      L = __builtin_fmaf(sm_l[w][r], f, L);
+      o += *reinterpret_cast<const f32x4*>(sm_o + (w * row_stride + r) * D + d) * f;
+    }
+    if (nan) L = __builtin_nanf("");
+    return o;
+  };
+  auto put = [&](int r, int d, f32x4 o, float L) {
+    const float f = L == 0.f ? 0.f : 1.f / L;  // a row that sees nothing is 0
+    *reinterpret_cast<u32x2*>(out_row(r) + d * 2) = u32x2{Pg<T>::pack(o[0] * f, o[1] * f), Pg<T>::pack(o[2] * f, o[3] * f)};
+  };
+  if (n_split_b == 1) {
+    for (int i = tid; i < rows * (D / 4); i += kThreads) {
+      float M, L;
+      const f32x4 o = joined(i / (D / 4), i % (D / 4) * 4, M, L);
+      put(i / (D / 4), i % (D / 4) * 4, o, L);
+    }
+    return;
+  }
+  // ---- several workgroups a row: each publishes its sums, the last to arrive joins them ----
+  // Agent-scope stores complete at the device's coherence point; every thread waits for its own (the counter may
+  // be seen by another XCD before a store that still travels), then one counts the arrival. No cache is flushed.
+  constexpr int kPart = D + 2;  // o[D], reference, sum
+  float* part = a.ws_part + (int64_t)unit * a.n_splits * row_stride * kPart;
+  for (int i = tid; i < rows * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    float M, L;
+    const f32x4 o = joined(r, d, M, L);
+    float* pp = part + (split * row_stride + r) * kPart;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) __hip_atomic_store(pp + d + e, o[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (d == 0) {
+      __hip_atomic_store(pp + D, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(pp + D + 1, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0);
+  asm volatile("" ::: "memory");
+  __syncthreads();
+  if (tid == 0) sm_last = __hip_atomic_fetch_add(a.ws_count + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n_split_b - 1;
+  __syncthreads();
+  if (!sm_last) return;
+  for (int i = tid; i < n_split_b * rows; i += kThreads) {
+    const int s = i / rows, r = i % rows;
+    const float* pp = part + (s * row_stride + r) * kPart + D;
+    sm_pm[s][r] = __hip_atomic_load(pp, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sm_pl[s][r] = __hip_atomic_load(pp + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  constexpr int kBatch = 8;
+  for (int i = tid; i < rows * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    float M = -INFINITY, L = 0.f;
+    for (int s = 0; s < n_split_b; ++s) M = fmaxf(M, sm_pm[s][r]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < n_split_b; s0 += kBatch) {
+      f32x4 x[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (s0 + u < n_split_b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[u][e] = __hip_atomic_load(part + ((s0 + u) * row_stride + r) * kPart + d + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (s0 + u < n_split_b) {
+          const float f = fast_exp2(sm_pm[s0 + u][r] - ref);
+          L = __builtin_fmaf(sm_pl[s0 + u][r], f, L);
+          o += x[u] * f;
+        }
+    }
+    put(r, d, o, L);
+  }
+  if (tid == 0) __hip_atomic_store(a.ws_count + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+}
+
+template <typename T, int D, int kWaves>
+void launch_w(const PagesArgs& a, hipStream_t stream) {
+  const size_t lds = (size_t)kWaves * std::min(kRows, a.sq * a.G) * D * 4;
+  hipLaunchKernelGGL((pages_attn_kernel<T, D, kWaves>), dim3((unsigned)(a.B * a.Hk * a.n_rt), (unsigned)a.n_splits), dim3(64 * kWaves), lds,
+                     stream, a);
+}
+template <typename T, int D>
+void launch_d(const PagesArgs& a, hipStream_t stream) {
+  if (a.waves == 8) launch_w<T, D, 8>(a, stream);
+  else launch_w<T, D, 4>(a, stream);
+}
+
+}  // namespace
+
+void pages_plan(int64_t B, int64_t sq, int64_t H, int64_t Hk, int64_t D, int64_t max_len, PagesArgs* a) {
+  a->G = (int)(H / Hk);
+  a->n_rt = (int)((sq * a->G + kRows - 1) / kRows);
+  const int64_t units = B * Hk * a->n_rt;
+  int64_t chunk = (max_len + kBlock - 1) / kBlock * kBlock;
+  if (max_len > 1024 && units <= kPagesCounters) {
+    const int64_t want = std::max<int64_t>(1, 1024 / units);
+    chunk = std::min<int64_t>((max_len + want - 1) / want, 4096);
+    chunk = std::max<int64_t>(std::max<int64_t>(chunk, 512), (max_len + kPagesMaxSplits - 1) / kPagesMaxSplits);
+    chunk = (chunk + kBlock - 1) / kBlock * kBlock;
+  }
+  a->chunk = (int)std::max<int64_t>(chunk, kBlock);
+  a->n_splits = (int)std::max<int64_t>(1, (max_len + a->chunk - 1) / a->chunk);
+  a->waves = units * a->n_splits <= 256 && D == 64 ? 8 : 4;
+}
+
+size_t pages_workspace_bytes(int64_t B, int64_t sq, int64_t H, int64_t Hk, int64_t D, int64_t max_len) {
+  PagesArgs a{};
+  pages_plan(B, sq, H, Hk, D, max_len, &a);
+  if (a.n_splits == 1) return 0;
+  return kPagesCounters * 4 + (size_t)B * Hk * a.n_rt * a.n_splits * std::min<int64_t>(kRows, sq * a.G) * (D + 2) * 4;
+}
+
+hipError_t launch_pages(int dtype, int D, const PagesArgs& a, hipStream_t stream) {
+  if (D == 64) {
+    if (dtype == 2) launch_d<Bf16, 64>(a, stream);
+    else launch_d<F16, 64>(a, stream);
+  } else {
+    if (dtype == 2) launch_d<Bf16, 128>(a, stream);
+    else launch_d<F16, 128>(a, stream);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace wdrz

@@ -1,0 +1,268 @@
+// page_tables.hip — the bookkeeping of a paged key/value cache, on the GPU: which pages a request's new tokens
+// go to, and the writes of their keys and values.
+//
+// A stream s holds `lens[s]` positions in `counts[s]` pages, tables[s][0 .. counts[s] - 1] in order; the pages
+// that nobody holds are the first n_free entries of a stack. Request i adds m_i tokens to stream s_i. With P
+// positions a page it needs
+//     need_i = max(0, ceil((lens + m_i) / P) - counts),   off_i = need_0 + .. + need_(i-1)
+// more pages, and gets the stack's entries n_free - 1 - off_i, n_free - 2 - off_i, ..; token t of it stands at
+// position lens + t, slot tables[s][position / P] * P + position % P. Requests are served in their order while
+// pages last: one whose off_i + need_i is above n_free gets nothing, and nor does one that names no stream, a
+// stream that an earlier one named, or a length that the table cannot hold.
+//
+// Bound: launch and a chain of four dependent trips to memory (stream -> its length -> the stack -> the table).
+// One workgroup does the scan, since every request's pages depend on all before it.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "wdrz_common.h"
+#include "wdrz_launch.h"
+
+namespace wdrz {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / 64;
+
+// Exclusive sums of two values over the workgroup's threads, and the totals. `sm` is free to use afterwards.
+// The first are capped at `cap` (sums of 2^30 and more would leave 32 bits).
+__device__ __forceinline__ void scan2(int& a, int& b, int cap, int& total_a, int& total_b, int64_t (&sm_a)[kPlanWaves],
+                                      int (&sm_b)[kPlanWaves]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t sa = a;
+  int sb = b;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t ua = __shfl_up(sa, o);
+    const int ub = __shfl_up(sb, o);
+    if (lane >= o) {
+      sa += ua;
+      sb += ub;
+    }
+  }
+  if (lane == 63) {
+    sm_a[wave] = sa;
+    sm_b[wave] = sb;
+  }
+  __syncthreads();
+  int64_t base_a = 0, sum_a = 0;
+  int base_b = 0;
+  total_b = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    base_a += w < wave ? sm_a[w] : 0;
+    base_b += w < wave ? sm_b[w] : 0;
+    sum_a += sm_a[w];
+    total_b += sm_b[w];
+  }
+  __syncthreads();
+  a = (int)min(base_a + sa - a, (int64_t)cap);
+  total_a = (int)min(sum_a, (int64_t)cap);
+  b = base_b + sb - b;
+}
+
+constexpr int kPageBatch = 8;  // entries of a request moved together: one trip to memory for each batch
+constexpr int kMostPages = 1 << 30;  // sums of needed pages are held at it
+
+// The first request that names each stream, in claims[n_streams] (LDS); the others count as naming none.
+__device__ __forceinline__ void claim_streams(const PageArgs& a, int* claims) {
+  for (int s = threadIdx.x; s < a.n_streams; s += kPlanThreads) claims[s] = 0x7fffffff;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.B; i += kPlanThreads) {
+    const int s = a.streams[i];
+    if (s >= 0 && s < a.n_streams) atomicMin(claims + s, i);
+  }
+  __syncthreads();
+}
+
+// Request i's stream with its length and pages; false where it names none (or not first, or the state is not one).
+__device__ __forceinline__ bool request(const PageArgs& a, const int* claims, int i, int& s, int& len, int& count) {
+  s = a.streams ? a.streams[i] : i;
+  if (s < 0 || s >= a.n_streams) return false;
+  len = a.lens[s];
+  count = a.counts[s];
+  if (a.streams && claims[s] != i) return false;
+  return len >= 0 && len <= a.max_len && count >= 0 && count <= a.max_pages;
+}
+
+// Slots and positions of the call's tokens from the finished tables. cu: the B + 1 sums (LDS where they fit).
+__device__ __forceinline__ void emit_tokens(const PageArgs& a, const int* cu, int t) {
+  int64_t slot = -1, pos = 0;
+  if (t < cu[a.B]) {
+    int lo = 0, hi = a.B;  // the last request that begins at t or before
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cu[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    const int start = a.starts[lo];
+    if (start >= 0) {
+      pos = (int64_t)start + t - cu[lo];
+      const int s = a.streams ? a.streams[lo] : lo;
+      const int page = a.tables[(int64_t)s * a.max_pages + (pos >> a.shift)];
+      slot = ((int64_t)page << a.shift) + (pos & ((1 << a.shift) - 1));
+    }
+  }
+  a.slots[t] = slot;
+  a.positions[t] = pos;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PageArgs a) {
+  extern __shared__ int sm_dyn[];
+  __shared__ int64_t sm_a[kPlanWaves];
+  __shared__ int sm_b[kPlanWaves], sm_taken;
+  int* const claims = sm_dyn;
+  const int tid = threadIdx.x;
+  if (tid == 0) sm_taken = 0;
+  const int top = min(max(*a.n_free, 0), a.n_pages);
+  if (a.streams) claim_streams(a, claims);
+  else __syncthreads();
+  int base_new = 0, base_need = 0, taken = 0;
+  for (int i0 = 0; i0 < a.B; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int s = 0, len = 0, count = 0, m = 0, need = 0;
+    bool ok = false;
+    if (i < a.B) {
+      m = a.new_lens ? a.new_lens[i] : a.new_all;
+      ok = request(a, claims, i, s, len, count) && m >= 0 && m <= a.max_len - len;
+      if (ok) need = max(0, ((len + m + (1 << a.shift) - 1) >> a.shift) - count);
+    }
+    int cu = min(max(m, 0), a.total), off = need, all_new, all_need;
+    scan2(cu, off, a.total, all_new, all_need, sm_a, sm_b);
+    cu = min(cu + base_new, a.total);
+    off += base_need;
+    base_new = min(base_new + all_new, a.total);
+    base_need = min(base_need + all_need, kMostPages);
+    if (i < a.B) {
+      ok = ok && (need == 0 || off + need <= top);
+      a.cu[i] = cu;
+      a.starts[i] = ok ? len : -1;
+      if (ok) {
+        int32_t* row = a.tables + (int64_t)s * a.max_pages + count;
+        for (int j = 0; j < need; j += kPageBatch) {
+          int32_t page[kPageBatch];
+#pragma unroll
+          for (int u = 0; u < kPageBatch; ++u)
+            if (j + u < need) page[u] = a.free_pages[top - 1 - off - j - u];
+#pragma unroll
+          for (int u = 0; u < kPageBatch; ++u)
+            if (j + u < need) row[j + u] = page[u];
+        }
+        if (need) {
+          a.counts[s] = count + need;
+          taken = off + need;  // ascending over a thread's requests
+        }
+        a.lens[s] = len + m;
+      }
+    }
+  }
+  if (taken) atomicMax(&sm_taken, taken);
+  if (tid == 0) a.cu[a.B] = base_new;
+  __syncthreads();  // this workgroup's writes are visible to it
+  if (tid == 0 && sm_taken) *a.n_free = top - sm_taken;
+  if (a.emit)
+    for (int t = tid; t < a.total; t += kPlanThreads) emit_tokens(a, a.cu, t);
+}
+
+__global__ __launch_bounds__(256) void page_slots_kernel(PageArgs a) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t < a.total) emit_tokens(a, a.cu, t);
+}
+
+// Streams set back to lens_new: the pages behind go back to the stack, in the order that gives the stack of
+// before where the plan took them in one call of the same requests.
+__global__ __launch_bounds__(kPlanThreads) void page_truncate_kernel(PageArgs a) {
+  extern __shared__ int sm_dyn[];
+  __shared__ int64_t sm_a[kPlanWaves];
+  __shared__ int sm_b[kPlanWaves];
+  int* const claims = sm_dyn;
+  const int tid = threadIdx.x;
+  const int top = min(max(*a.n_free, 0), a.n_pages);
+  if (a.streams) claim_streams(a, claims);
+  else __syncthreads();
+  auto gone_of = [&](int i, int& s, int& keep) {
+    int len, count;
+    if (i >= a.B || !request(a, claims, i, s, len, count)) return -1;
+    const int n = a.new_lens ? a.new_lens[i] : a.new_all;
+    if (n < 0 || n > len) return -1;
+    keep = (n + (1 << a.shift) - 1) >> a.shift;
+    return max(0, count - keep);
+  };
+  int total = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int base = 0;
+    for (int i0 = 0; i0 < a.B; i0 += kPlanThreads) {
+      int s = 0, keep = 0;
+      const int gone = gone_of(i0 + tid, s, keep);
+      int unused = 0, off = max(gone, 0), none, all;
+      scan2(unused, off, 0, none, all, sm_a, sm_b);
+      off += base;
+      base = min(base + all, kMostPages);
+      if (pass == 1 && gone >= 0) {
+        int32_t* row = a.tables + (int64_t)s * a.max_pages + keep;
+        for (int j = 0; j < gone; j += kPageBatch) {
+          int32_t page[kPageBatch];
+#pragma unroll
+          for (int u = 0; u < kPageBatch; ++u)
+            if (j + u < gone) page[u] = row[j + u];
+#pragma unroll
+          for (int u = 0; u < kPageBatch; ++u) {
+            if (j + u >= gone) continue;
+            const int at = top + total - 1 - off - j - u;
+            if (at >= 0 && at < a.n_pages) a.free_pages[at] = page[u];  // counts that are not the state's own stay in bounds
+            row[j + u] = -1;
+          }
+        }
+        a.lens[s] = a.new_lens ? a.new_lens[i0 + tid] : a.new_all;
+        if (gone) a.counts[s] = keep;
+      }
+    }
+    total = base;
+  }
+  if (tid == 0) *a.n_free = min(top + total, a.n_pages);
+}
+
+// ---- writes: row t's keys and values to slot slots[t] of every head's page ------------------------------
+// A thread moves 16 bytes of a key and of a value; rows whose slot lies outside the cache are left out.
+__global__ __launch_bounds__(256) void page_write_kernel(PageWriteArgs a) {
+  const int pieces = a.D / 8;
+  const int64_t n = (int64_t)a.T * a.Hk * pieces;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (idx >= n) return;
+  const int p = (int)(idx % pieces);
+  const int64_t row = idx / pieces;
+  const int h = (int)(row % a.Hk);
+  const int64_t t = row / a.Hk;
+  const int64_t slot = a.slots[t];
+  if (slot < 0 || slot >= ((int64_t)a.n_pages << a.shift)) return;
+  const int64_t page = slot >> a.shift, in = slot & ((1 << a.shift) - 1);
+  const int64_t to = (((page * a.Hk + h) << a.shift) + in) * a.D * 2 + p * 16;
+  const u32x4 kv = load16(a.k + t * a.ks[0] + h * a.ks[1] + p * 16), vv = load16(a.v + t * a.vs[0] + h * a.vs[1] + p * 16);
+  store16(a.k_pages + to, kv);
+  store16(a.v_pages + to, vv);
+}
+
+}  // namespace
+
+hipError_t launch_page_plan(PageArgs a, hipStream_t stream) {
+  const size_t lds = a.streams ? (size_t)a.n_streams * 4 : 0;
+  a.emit = a.total <= kPlanThreads;
+  hipLaunchKernelGGL(page_plan_kernel, dim3(1), dim3(kPlanThreads), lds, stream, a);
+  if (!a.emit) hipLaunchKernelGGL(page_slots_kernel, dim3((unsigned)((a.total + 255) / 256)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_page_truncate(const PageArgs& a, hipStream_t stream) {
+  const size_t lds = a.streams ? (size_t)a.n_streams * 4 : 0;
+  hipLaunchKernelGGL(page_truncate_kernel, dim3(1), dim3(kPlanThreads), lds, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_page_write(const PageWriteArgs& a, hipStream_t stream) {
+  const int64_t n = (int64_t)a.T * a.Hk * (a.D / 8);
+  if (n == 0) return hipSuccess;
+  hipLaunchKernelGGL(page_write_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace wdrz

@@ -6,6 +6,7 @@
 // during hipGraph stream capture.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -176,6 +177,60 @@ int debug_check_kv8_metadata(const int32_t* seqlens, const int32_t* bidx, bool h
                   hb[i], hs[f], hs[i]);
     f = (int32_t)i;
   }
+  return WDRZ_OK;
+}
+
+// A call on the paged cache: streams, lengths and the pages that hold them; appending rows name a stream once.
+int debug_check_pages_metadata(const wdrz_page_tables* p, const int32_t* seqlens, const int32_t* streams, bool has_new,
+                               int64_t B, int64_t sq) {
+  std::vector<int32_t> hs(B), hb(B), tables((size_t)p->n_streams * p->max_pages), first(p->n_streams, -1);
+  for (int64_t i = 0; i < B; ++i) hb[i] = (int32_t)i;
+  if ((streams && hipMemcpy(hb.data(), streams, B * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess) ||
+      hipMemcpy(hs.data(), seqlens, B * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess ||
+      hipMemcpy(tables.data(), p->tables, tables.size() * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess)
+    return fail(WDRZ_ELAUNCH, "debug check: reading the rows' streams, lengths and tables failed");
+  for (int64_t i = 0; i < B; ++i) {
+    if (hb[i] < 0 || hb[i] >= p->n_streams)
+      return fail(WDRZ_EINVAL, "debug check: row %lld names stream %d outside [0, %lld)", (long long)i, hb[i],
+                  (long long)p->n_streams);
+    const int64_t end = hs[i] + (has_new ? sq : 0);
+    if (hs[i] < 0 || end > p->max_pages * p->page_size)
+      return fail(WDRZ_EINVAL, "debug check: row %lld covers [%d, %lld) outside [0, %lld)", (long long)i, hs[i],
+                  (long long)end, (long long)(p->max_pages * p->page_size));
+    if (has_new && first[hb[i]] >= 0)
+      return fail(WDRZ_EINVAL, "debug check: rows %d and %lld append to stream %d", first[hb[i]], (long long)i, hb[i]);
+    first[hb[i]] = (int32_t)i;
+    for (int64_t j = 0; j * p->page_size < end; ++j) {
+      const int32_t page = tables[(size_t)hb[i] * p->max_pages + j];
+      if (page < 0 || page >= p->n_pages)
+        return fail(WDRZ_EINVAL, "debug check: row %lld of stream %d: page %lld of its table is %d, outside [0, %lld)",
+                    (long long)i, hb[i], (long long)j, page, (long long)p->n_pages);
+    }
+  }
+  return WDRZ_OK;
+}
+
+// Slots of a write: inside the cache or negative, each named once.
+int debug_check_slots(const int64_t* slots, int64_t T, int64_t n) {
+  std::vector<int64_t> h(T);
+  if (hipMemcpy(h.data(), slots, T * sizeof(int64_t), hipMemcpyDeviceToHost) != hipSuccess)
+    return fail(WDRZ_ELAUNCH, "debug check: reading the slots failed");
+  std::sort(h.begin(), h.end());
+  for (int64_t i = 0; i < T; ++i) {
+    if (h[i] >= n) return fail(WDRZ_EINVAL, "debug check: slot %lld outside [0, %lld)", (long long)h[i], (long long)n);
+    if (i > 0 && h[i] >= 0 && h[i] == h[i - 1]) return fail(WDRZ_EINVAL, "debug check: slot %lld is named twice", (long long)h[i]);
+  }
+  return WDRZ_OK;
+}
+
+// Sums of packed lengths: ascending, inside the rows.
+int debug_check_sums(const char* name, const int32_t* cu, int64_t B, int64_t T) {
+  std::vector<int32_t> h(B + 1);
+  if (hipMemcpy(h.data(), cu, h.size() * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess)
+    return fail(WDRZ_ELAUNCH, "debug check: reading %s failed", name);
+  for (int64_t i = 0; i <= B; ++i)
+    if (h[i] < (i ? h[i - 1] : 0) || h[i] > T)
+      return fail(WDRZ_EINVAL, "debug check: %s[%lld] = %d is not ascending in [0, %lld]", name, (long long)i, h[i], (long long)T);
   return WDRZ_OK;
 }
 #endif
@@ -1032,6 +1087,292 @@ int wdrz_linear4_partials(int dtype, const void* x, int64_t x_stride, const void
   a.part = partials;
   a.n_split = n_split;
   hipError_t err = wdrz::launch_linear4(dtype, a, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  return WDRZ_OK;
+}
+
+// ---- the paged cache, packed sequences and token log probabilities ----
+
+static int log2_page(int64_t page_size) {
+  for (int s = 4; s <= 8; ++s)
+    if (page_size == (int64_t)1 << s) return s;
+  return -1;
+}
+
+static int page_tables(const wdrz_page_tables* p, wdrz::PageArgs* a) {
+  if (!p) return fail(WDRZ_EINVAL, "pages is NULL");
+  if (!p->tables || !p->page_counts || !p->seq_lens || !p->free_pages || !p->n_free)
+    return fail(WDRZ_EINVAL, "a buffer of the page tables is NULL");
+  a->shift = log2_page(p->page_size);
+  if (a->shift < 0) return fail(WDRZ_EUNSUPPORTED, "page_size %lld is not 16, 32, 64, 128 or 256", (long long)p->page_size);
+  if (p->n_streams <= 0 || p->n_pages <= 0 || p->max_pages <= 0 || p->max_seq <= 0 || p->max_seq > p->max_pages * p->page_size)
+    return fail(WDRZ_EINVAL, "bad page table sizes n_streams=%lld n_pages=%lld max_pages=%lld max_seq=%lld",
+                (long long)p->n_streams, (long long)p->n_pages, (long long)p->max_pages, (long long)p->max_seq);
+  if (p->n_streams > 15360 || p->n_pages > (1 << 26) || p->max_pages > (1 << 20) || p->max_seq > (1 << 24))
+    return fail(WDRZ_EUNSUPPORTED, "sizes too large (15360 streams, 2^26 pages, 2^24 positions a stream at most)");
+  a->tables = p->tables;
+  a->counts = p->page_counts;
+  a->lens = p->seq_lens;
+  a->free_pages = p->free_pages;
+  a->n_free = p->n_free;
+  a->n_streams = (int)p->n_streams;
+  a->n_pages = (int)p->n_pages;
+  a->max_pages = (int)p->max_pages;
+  a->max_len = (int)p->max_seq;
+  return WDRZ_OK;
+}
+
+static int page_requests(const wdrz_page_tables* p, const int32_t* lens, int64_t all, const int32_t* streams, int64_t B,
+                         wdrz::PageArgs* a) {
+  int rc = page_tables(p, a);
+  if (rc) return rc;
+  if (B < 0) return fail(WDRZ_EINVAL, "bad sizes B=%lld", (long long)B);
+  if (B > 65535) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (!lens && (all < 0 || all > a->max_len)) return fail(WDRZ_EINVAL, "length %lld outside [0, %d]", (long long)all, a->max_len);
+  if (!streams && B > a->n_streams) return fail(WDRZ_EINVAL, "%lld requests exceed the %d streams", (long long)B, a->n_streams);
+  a->new_lens = lens;
+  a->new_all = lens ? 0 : (int)all;
+  a->streams = streams;
+  a->B = (int)B;
+  return WDRZ_OK;
+}
+
+int wdrz_page_plan(const wdrz_page_tables* pages, const int32_t* new_lens, int64_t new_all, const int32_t* streams,
+                   int32_t* cu_seqlens, int32_t* starts, int64_t* slots, int64_t* positions, int64_t B, int64_t total,
+                   void* stream) {
+  g_last_error.clear();
+  wdrz::PageArgs a{};
+  int rc = page_requests(pages, new_lens, new_all, streams, B, &a);
+  if (rc) return rc;
+  if (total < 0) return fail(WDRZ_EINVAL, "bad sizes total=%lld", (long long)total);
+  if (total > (1 << 28)) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (!cu_seqlens || (B > 0 && !starts) || (total > 0 && (!slots || !positions)))
+    return fail(WDRZ_EINVAL, "cu_seqlens, starts, slots or positions is NULL");
+  a.cu = cu_seqlens;
+  a.starts = starts;
+  a.slots = slots;
+  a.positions = positions;
+  a.total = (int)total;
+  hipError_t err = wdrz::launch_page_plan(a, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  return WDRZ_OK;
+}
+
+int wdrz_page_truncate(const wdrz_page_tables* pages, const int32_t* lens, int64_t len_all, const int32_t* streams,
+                       int64_t B, void* stream) {
+  g_last_error.clear();
+  wdrz::PageArgs a{};
+  int rc = page_requests(pages, lens, len_all, streams, B, &a);
+  if (rc) return rc;
+  if (B == 0) return WDRZ_OK;
+  hipError_t err = wdrz::launch_page_truncate(a, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  return WDRZ_OK;
+}
+
+static int kv_pages(int dtype, const wdrz_kv_pages* c, int* shift) {
+  int rc;
+  if ((rc = check_dtype16(dtype))) return rc;
+  if (!c) return fail(WDRZ_EINVAL, "cache is NULL");
+  if ((*shift = log2_page(c->page_size)) < 0)
+    return fail(WDRZ_EUNSUPPORTED, "page_size %lld is not 16, 32, 64, 128 or 256", (long long)c->page_size);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(WDRZ_EUNSUPPORTED, "head_dim %lld is not supported (64, 128)", (long long)c->head_dim);
+  if (c->n_pages <= 0 || c->n_heads <= 0)
+    return fail(WDRZ_EINVAL, "bad cache sizes n_pages=%lld n_heads=%lld", (long long)c->n_pages, (long long)c->n_heads);
+  if (c->n_pages > (1 << 26) || c->n_heads > 65535) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if ((rc = check_ptr("k_pages", c->k_pages)) || (rc = check_ptr("v_pages", c->v_pages))) return rc;
+  return WDRZ_OK;
+}
+
+// [T, H, D] rows of a 16-bit type: pointer and the strides of t, h, in bytes.
+static int rows16_packed(const char* name, const void* p, const int64_t* s, int64_t* bytes) {
+  int rc = check_ptr(name, p);
+  if (rc) return rc;
+  if (!s) return fail(WDRZ_EINVAL, "%s: strides pointer is NULL", name);
+  if (s[2] != 1) return fail(WDRZ_EINVAL, "%s: head_dim stride must be 1 (got %lld)", name, (long long)s[2]);
+  for (int i = 0; i < 2; ++i) {
+    if (s[i] % 8) return fail(WDRZ_EINVAL, "%s: stride[%d]=%lld elements is not 16-byte aligned", name, i, (long long)s[i]);
+    bytes[i] = s[i] * 2;
+  }
+  return WDRZ_OK;
+}
+
+int wdrz_page_write(int dtype, const wdrz_kv_pages* cache, const void* k_src, const int64_t* k_strides, const void* v_src,
+                    const int64_t* v_strides, const int64_t* slots, int64_t T, void* stream) {
+  g_last_error.clear();
+  wdrz::PageWriteArgs a{};
+  int rc = kv_pages(dtype, cache, &a.shift);
+  if (rc) return rc;
+  if (T < 0) return fail(WDRZ_EINVAL, "bad sizes T=%lld", (long long)T);
+  if (T > (1 << 28) || T * cache->n_heads * (cache->head_dim / 8) > ((int64_t)1 << 38)) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (T == 0) return WDRZ_OK;
+  if (!slots) return fail(WDRZ_EINVAL, "slots is NULL");
+  if ((rc = rows16_packed("k", k_src, k_strides, a.ks)) || (rc = rows16_packed("v", v_src, v_strides, a.vs))) return rc;
+#ifdef WDRZ_DEBUG_CHECKS
+  if ((rc = debug_check_slots(slots, T, cache->n_pages * cache->page_size))) return rc;
+#endif
+  a.k = static_cast<const char*>(k_src);
+  a.v = static_cast<const char*>(v_src);
+  a.k_pages = static_cast<char*>(cache->k_pages);
+  a.v_pages = static_cast<char*>(cache->v_pages);
+  a.slots = slots;
+  a.T = (int)T;
+  a.Hk = (int)cache->n_heads;
+  a.D = (int)cache->head_dim;
+  a.n_pages = (int)cache->n_pages;
+  hipError_t err = wdrz::launch_page_write(a, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  return WDRZ_OK;
+}
+
+size_t wdrz_attn_kvpages_workspace_size(int64_t B, int64_t sq, int64_t H, int64_t n_heads, int64_t head_dim, int64_t max_seq) {
+  if (B <= 0 || sq <= 0 || H <= 0 || n_heads <= 0 || H % n_heads || head_dim <= 0 || max_seq <= 0) return 0;
+  return wdrz::pages_workspace_bytes(B, sq, H, n_heads, head_dim, max_seq);
+}
+
+int wdrz_attn_kvpages(int dtype, const wdrz_kv_pages* cache, const wdrz_page_tables* pages, const void* q,
+                      const int64_t* q_strides, const void* k_new, const int64_t* kn_strides, const void* v_new,
+                      const int64_t* vn_strides, const int32_t* cache_seqlens, const int32_t* cache_batch_idx, void* o,
+                      const int64_t* o_strides, int64_t B, int64_t sq, int64_t H, float softmax_scale, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  wdrz::PagesArgs a{};
+  wdrz::PageArgs t{};
+  int rc;
+  if ((rc = kv_pages(dtype, cache, &a.shift)) || (rc = page_tables(pages, &t))) return rc;
+  if (pages->page_size != cache->page_size || pages->n_pages != cache->n_pages)
+    return fail(WDRZ_EINVAL, "the tables are of %lld pages of %lld, the cache has %lld of %lld", (long long)pages->n_pages,
+                (long long)pages->page_size, (long long)cache->n_pages, (long long)cache->page_size);
+  if (B < 0 || sq <= 0 || H <= 0) return fail(WDRZ_EINVAL, "bad sizes B=%lld sq=%lld H=%lld", (long long)B, (long long)sq, (long long)H);
+  if (H % cache->n_heads) return fail(WDRZ_EINVAL, "%lld query heads are not a multiple of the cache's %lld", (long long)H, (long long)cache->n_heads);
+  if (B > 65535 || sq > 65536 || H > 65535) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (!(softmax_scale > 0.f) || softmax_scale > 3.0e38f) return fail(WDRZ_EINVAL, "softmax_scale must be a positive finite number");
+  const bool has_new = k_new || v_new;
+  if (has_new && (!k_new || !v_new)) return fail(WDRZ_EINVAL, "k and v must be given together");
+  if (!cache_seqlens) return fail(WDRZ_EINVAL, "cache_seqlens is NULL");
+  if (!cache_batch_idx && B > pages->n_streams)
+    return fail(WDRZ_EINVAL, "%lld rows exceed the %lld streams", (long long)B, (long long)pages->n_streams);
+  if (B == 0) return WDRZ_OK;
+  if ((rc = rows16("q", q, q_strides, a.qs)) || (rc = rows16("out", o, o_strides, a.os))) return rc;
+  if (has_new && ((rc = rows16("k", k_new, kn_strides, a.kns)) || (rc = rows16("v", v_new, vn_strides, a.vns)))) return rc;
+#ifdef WDRZ_DEBUG_CHECKS
+  if ((rc = debug_check_pages_metadata(pages, cache_seqlens, cache_batch_idx, has_new, B, sq))) return rc;
+#endif
+  a.q = static_cast<const char*>(q);
+  a.k_pages = static_cast<char*>(cache->k_pages);
+  a.v_pages = static_cast<char*>(cache->v_pages);
+  a.kn = static_cast<const char*>(k_new);
+  a.vn = static_cast<const char*>(v_new);
+  a.tables = pages->tables;
+  a.seqlens = cache_seqlens;
+  a.streams = cache_batch_idx;
+  a.o = static_cast<char*>(o);
+  a.c = softmax_scale * 1.4426950408889634f;
+  a.B = (int)B;
+  a.sq = (int)sq;
+  a.H = (int)H;
+  a.Hk = (int)cache->n_heads;
+  a.n_streams = (int)pages->n_streams;
+  a.n_pages = (int)pages->n_pages;
+  a.max_pages = (int)pages->max_pages;
+  wdrz::pages_plan(B, sq, H, a.Hk, cache->head_dim, pages->max_seq, &a);
+  if (B * a.Hk * a.n_rt > 0x7fffffff) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  const size_t need = wdrz::pages_workspace_bytes(B, sq, H, a.Hk, cache->head_dim, pages->max_seq);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return fail(WDRZ_EWORKSPACE, "workspace of %zu bytes required (got %zu)", need, workspace ? workspace_bytes : 0);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return fail(WDRZ_EINVAL, "workspace is not 256-byte aligned");
+    a.ws_count = static_cast<int*>(workspace);
+    a.ws_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + wdrz::kPagesCounters * 4);
+  }
+  hipError_t err = wdrz::launch_pages(dtype, (int)cache->head_dim, a, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  return WDRZ_OK;
+}
+
+int wdrz_attn_packed(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                     const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides, const int32_t* cu_q,
+                     const int32_t* cu_k, int64_t B, int64_t T, int64_t Tk, int64_t H, int64_t Hk, int64_t D, float scale,
+                     int causal, void* stream) {
+  g_last_error.clear();
+  int rc;
+  if ((rc = check_dtype16(dtype))) return rc;
+  if (D != 64 && D != 128) return fail(WDRZ_EUNSUPPORTED, "head_dim %lld is not supported (64, 128)", (long long)D);
+  if (B < 0 || T < 0 || Tk < 0 || H <= 0 || Hk <= 0)
+    return fail(WDRZ_EINVAL, "bad sizes B=%lld T=%lld Tk=%lld H=%lld Hk=%lld", (long long)B, (long long)T, (long long)Tk,
+                (long long)H, (long long)Hk);
+  if (H % Hk) return fail(WDRZ_EINVAL, "%lld query heads are not a multiple of %lld", (long long)H, (long long)Hk);
+  if (B > 65535 || T > (1 << 24) || Tk > (1 << 24) || H > 65535) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (!(scale > 0.f) || scale > 3.0e38f) return fail(WDRZ_EINVAL, "scale must be a positive finite number");
+  if (!cu_q) return fail(WDRZ_EINVAL, "cu_seqlens is NULL");
+  if (!cu_k && Tk != T) return fail(WDRZ_EINVAL, "%lld keys for %lld queries need sums of their own", (long long)Tk, (long long)T);
+  if (B == 0 || T == 0) return WDRZ_OK;
+  wdrz::PackedArgs a{};
+  if ((rc = rows16_packed("q", q, q_strides, a.qs)) || (rc = rows16_packed("out", o, o_strides, a.os))) return rc;
+  if (Tk > 0 && ((rc = rows16_packed("k", k, k_strides, a.ks)) || (rc = rows16_packed("v", v, v_strides, a.vs)))) return rc;
+  if ((T / 128 + B) * H > 0x7fffffff) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+#ifdef WDRZ_DEBUG_CHECKS
+  if ((rc = debug_check_sums("cu_seqlens", cu_q, B, T)) || (cu_k && (rc = debug_check_sums("cu_seqlens_k", cu_k, B, Tk)))) return rc;
+#endif
+  a.q = static_cast<const char*>(q);
+  a.k = static_cast<const char*>(k);
+  a.v = static_cast<const char*>(v);
+  a.o = static_cast<char*>(o);
+  a.cu_q = cu_q;
+  a.cu_k = cu_k ? cu_k : cu_q;
+  a.c = scale * 1.4426950408889634f;
+  a.B = (int)B;
+  a.T = (int)T;
+  a.Tk = (int)Tk;
+  a.H = (int)H;
+  a.Hk = (int)Hk;
+  a.causal = causal ? 1 : 0;
+  hipError_t err = wdrz::launch_packed(dtype, (int)D, a, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
+  return WDRZ_OK;
+}
+
+size_t wdrz_token_logprobs_workspace_size(int64_t rows, int64_t V, int64_t top) {
+  if (rows <= 0 || V <= 0 || top < 0) return 0;
+  return wdrz::logprobs_workspace_bytes(rows, V, top);
+}
+
+int wdrz_token_logprobs(int dtype, const void* logits, int64_t l_stride, const uint8_t* blocked, int64_t b_stride,
+                        const int64_t* tokens, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
+                        int64_t rows, int64_t V, int64_t top, void* workspace, size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  const int eb = elem_bytes(dtype);
+  if (!eb) return fail(WDRZ_EINVAL, "dtype %d is not one of WDRZ_F32/F16/BF16", dtype);
+  if (rows < 0 || V <= 0) return fail(WDRZ_EINVAL, "bad sizes rows=%lld V=%lld", (long long)rows, (long long)V);
+  if (top < 0 || top > 32) return fail(WDRZ_EUNSUPPORTED, "top=%lld is not 0 .. 32", (long long)top);
+  if (rows > (1 << 24) || V > (1 << 20)) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (l_stride < 0 || (blocked && b_stride < 0)) return fail(WDRZ_EINVAL, "negative row strides");
+  if (rows == 0) return WDRZ_OK;
+  if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_logprobs || !top_ids)))
+    return fail(WDRZ_EINVAL, "logits, tokens or an output is NULL");
+  if (reinterpret_cast<uintptr_t>(logits) % eb) return fail(WDRZ_EINVAL, "logits is not aligned to its elements");
+  wdrz::LogprobArgs a{};
+  const size_t need = wdrz::logprobs_workspace_bytes(rows, V, top);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return fail(WDRZ_EWORKSPACE, "workspace of %zu bytes required (got %zu)", need, workspace ? workspace_bytes : 0);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return fail(WDRZ_EINVAL, "workspace is not 256-byte aligned");
+    a.ws = workspace;
+  }
+  a.logits = logits;
+  a.l_stride = l_stride;
+  a.blocked = blocked;
+  a.m_stride = b_stride;
+  a.tokens = tokens;
+  a.logprob = logprobs;
+  a.entropy = entropy;
+  a.top_logprob = top_logprobs;
+  a.top_id = top_ids;
+  a.rows = (int)rows;
+  a.V = (int)V;
+  a.top = (int)top;
+  hipError_t err = wdrz::launch_token_logprobs(dtype, a, reinterpret_cast<hipStream_t>(stream));
   if (err != hipSuccess) return fail(WDRZ_ELAUNCH, "kernel launch failed: %s", hipGetErrorString(err));
   return WDRZ_OK;
 }

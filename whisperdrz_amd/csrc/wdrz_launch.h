@@ -269,6 +269,94 @@ struct LogMelArgs {
 size_t logmel_workspace_bytes(int64_t B, int64_t n_mels);
 hipError_t launch_logmel(LogMelArgs a, void* ws, hipStream_t stream);
 
+// Page tables of a paged cache (page_tables.hip). shift: log2 of a page's positions.
+struct PageArgs {
+  int32_t* tables;  // [n_streams][max_pages]
+  int32_t* counts;  // [n_streams] pages held
+  int32_t* lens;    // [n_streams] positions held
+  int32_t* free_pages;  // [n_pages], the first *n_free are the stack
+  int32_t* n_free;
+  const int32_t* new_lens;  // [B], or null: new_all for every request (plan: added tokens; truncate: lengths)
+  const int32_t* streams;   // [B], or null: request i is stream i
+  int32_t* cu;         // plan: [B + 1] sums of the added tokens
+  int32_t* starts;     // plan: [B] positions before them, -1 where nothing was given
+  int64_t* slots;      // plan: [total]
+  int64_t* positions;  // plan: [total]
+  int new_all, B, n_streams, n_pages, max_pages, max_len, shift, total;
+  int emit;       // plan: the tokens in the same launch (set by the launcher)
+};
+hipError_t launch_page_plan(PageArgs a, hipStream_t stream);
+hipError_t launch_page_truncate(const PageArgs& a, hipStream_t stream);
+
+// pages[slots[t] >> shift][h][slots[t] % 2^shift][:] = src[t][h][:] of keys and values, 16-bit; strides in bytes.
+struct PageWriteArgs {
+  const char* k;
+  const char* v;
+  int64_t ks[2], vs[2];  // t, h
+  char* k_pages;
+  char* v_pages;
+  const int64_t* slots;
+  int T, Hk, D, n_pages, shift;
+};
+hipError_t launch_page_write(const PageWriteArgs& a, hipStream_t stream);
+
+// Attention of new tokens over pages (kv_pages.hip). Strides in bytes.
+constexpr int kPagesCounters = 4096;  // arrival counters at the start of its workspace
+struct PagesArgs {
+  const char* q;
+  char* k_pages;  // [n_pages][Hk][2^shift][D]
+  char* v_pages;
+  const char* kn;  // [B, sq, Hk, D] appended rows, or null
+  const char* vn;
+  const int32_t* tables;   // [n_streams][max_pages]
+  const int32_t* seqlens;  // [B]
+  const int32_t* streams;  // [B], or null: row b is stream b
+  char* o;
+  int64_t qs[3], kns[3], vns[3], os[3];  // b, t, h
+  float c;  // softmax scale * log2(e)
+  int B, sq, H, Hk, G, n_streams, n_pages, max_pages, shift;
+  int n_rt;             // row tiles of 16 (query, group head) rows a kv head
+  int n_splits, chunk;  // key splits at most, keys of one
+  int waves;
+  int* ws_count;
+  float* ws_part;
+};
+void pages_plan(int64_t B, int64_t sq, int64_t H, int64_t Hk, int64_t D, int64_t max_len, PagesArgs* a);
+size_t pages_workspace_bytes(int64_t B, int64_t sq, int64_t H, int64_t Hk, int64_t D, int64_t max_len);
+hipError_t launch_pages(int dtype, int D, const PagesArgs& a, hipStream_t stream);
+
+// Attention of packed sequences (packed.hip). Strides in bytes.
+struct PackedArgs {
+  const char* q;  // [T, H, D]
+  const char* k;  // [Tk, Hk, D]
+  const char* v;
+  char* o;
+  int64_t qs[2], ks[2], vs[2], os[2];  // t, h
+  const int32_t* cu_q;  // [B + 1]
+  const int32_t* cu_k;  // [B + 1] (cu_q where the keys are the queries' own)
+  float c;              // softmax scale * log2(e)
+  int B, T, Tk, H, Hk, causal;
+};
+hipError_t launch_packed(int dtype, int D, const PackedArgs& a, hipStream_t stream);
+
+// Log probabilities of tokens (token_logprobs.hip).
+struct LogprobArgs {
+  const void* logits;
+  int64_t l_stride;
+  const uint8_t* blocked;  // bool [rows, V] or nullptr
+  int64_t m_stride;
+  const int64_t* tokens;  // [rows] or nullptr
+  float* logprob;         // [rows] or nullptr with tokens
+  float* entropy;         // [rows]
+  float* top_logprob;     // [rows, top]
+  int64_t* top_id;
+  int rows, V, top;
+  int splits;  // workgroups a row (set by the launcher)
+  void* ws;
+};
+size_t logprobs_workspace_bytes(int64_t rows, int64_t V, int64_t top);
+hipError_t launch_token_logprobs(int dtype, LogprobArgs a, hipStream_t stream);
+
 size_t dtw_workspace_bytes(int64_t B, int64_t H, int64_t T, int64_t A);
 // The prep with the scores computed from the heads' Q / K inside both passes (A <= 1536).
 constexpr int kDtwQkMaxA = 1536;

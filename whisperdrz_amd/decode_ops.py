@@ -7,6 +7,7 @@
   one to four rows of a small step.
 * :func:`masked_argmax` — ``decode_batch``'s greedy sampling tail (``decoding.py:1729-1761``):
   additive -65504 mask, repetition penalty, argmax, one launch instead of six.
+* :func:`token_logprobs` — log probabilities of given tokens, entropy and top alternatives of each row, one pass.
 * :func:`linear_gelu` — the MLP's ``Linear(n_state, 4 n_state)`` + ``GELU`` (``model.py:388-391``,
   applied at ``model.py:434``): GEMM, bias, rounding and exact GELU in one launch.
 * :func:`linear4` — the same with 4-bit weights and group scales (:class:`QuantLinear4`).
@@ -15,15 +16,16 @@ There is no fallback: CPU tensors, fp32 LayerNorm inputs and a missing library r
 """
 from __future__ import annotations
 
-from typing import Optional
+import functools
+from typing import NamedTuple, Optional
 
 import torch
 import torch.nn as nn
 
 from . import _lib
-from .attention import (_check_cuda, _current_device, _dtype_code, _raise, _raw_stream, _stream_handle)
+from .attention import (_check_cuda, _counted_workspace, _current_device, _dtype_code, _raise, _raw_stream, _stream_handle)
 
-__all__ = ["QuantLinear4", "add_layernorm_", "layer_norm", "linear4", "linear4_partials", "linear_gelu", "ln_linear",
+__all__ = ["QuantLinear4", "TokenLogprobs", "token_logprobs", "add_layernorm_", "layer_norm", "linear4", "linear4_partials", "linear_gelu", "ln_linear",
            "masked_argmax"]
 
 _LN16 = {torch.bfloat16: _lib.WDRZ_BF16, torch.float16: _lib.WDRZ_F16}
@@ -96,6 +98,71 @@ def masked_argmax(logits: torch.Tensor, blocked: Optional[torch.Tensor] = None,
     if rc != _lib.WDRZ_OK:
         _raise(rc, "masked_argmax")
     return out
+
+
+class TokenLogprobs(NamedTuple):
+    """``logprobs`` and ``entropy`` fp32 ``[...]``, ``top_logprobs`` fp32 and ``top_ids`` int64 ``[..., top]``."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor
+    top_ids: torch.Tensor
+
+
+@functools.lru_cache(maxsize=1024)
+def _logprobs_workspace_size(rows: int, V: int, top: int) -> int:
+    return int(_lib.load().wdrz_token_logprobs_workspace_size(rows, V, top))
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
+                   blocked: Optional[torch.Tensor] = None) -> TokenLogprobs:
+    """What ``logits`` ``[..., V]`` say about ``tokens`` ``[...]`` (int64): ``log_softmax(logits)`` at each token, the
+    distribution's entropy in nats, and the ``top`` (0 .. 32) likeliest tokens, of equal ones the lower index first.
+    bf16, fp16 or fp32 logits of up to 2^20 tokens; sums and results in fp32 or more. Inference only.
+
+    ``blocked`` (bool ``[rows, >= V]``, as :func:`masked_argmax` takes it) are tokens that cannot be chosen: they count
+    as -inf. A token out of range has NaN. A row that has nothing left has log probabilities of -inf, entropy 0
+    and no alternatives; one with NaN or +inf among its tokens is NaN. Alternatives that do not exist have id -1.
+    """
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda):
+        _check_cuda("logits", logits, logits.device if isinstance(logits, torch.Tensor) else None)
+    device = logits.device
+    dt = _dtype_code(logits, "logits")
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError("logits must be [..., V] with tokens")
+    _check_cuda("tokens", tokens, device)
+    shape, V = logits.shape[:-1], logits.shape[-1]
+    if tokens.shape != shape or tokens.dtype is not torch.int64:
+        raise ValueError(f"tokens must be int64 {tuple(shape)}, got {tokens.dtype} {tuple(tokens.shape)}")
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if x.stride(1) != 1 and V > 1 or x.stride(0) < 0:
+        x = x.contiguous()
+    rows = x.shape[0]
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    mask, m_stride = None, 0
+    if blocked is not None:
+        _check_cuda("blocked", blocked, device)
+        if blocked.dtype is not torch.bool or blocked.dim() != 2 or blocked.shape[0] != rows or blocked.shape[1] < V \
+                or blocked.stride(1) != 1:
+            raise ValueError(f"blocked must be a bool [{rows}, >= {V}] tensor with contiguous rows")
+        mask, m_stride = blocked.data_ptr(), blocked.stride(0)
+    index = device.index
+    if index != _current_device():  # launches go to the current device
+        with torch.cuda.device(index):
+            return token_logprobs(logits, tokens, top, blocked)
+    values = torch.empty(2, *shape, dtype=torch.float32, device=device)
+    top_logprobs = torch.empty(*shape, max(top, 0), dtype=torch.float32, device=device)
+    top_ids = torch.empty(*shape, max(top, 0), dtype=torch.int64, device=device)
+    lib, nbytes = _lib.load(), _logprobs_workspace_size(rows, V, max(top, 0))
+    workspace = _counted_workspace(device, nbytes) if nbytes else None
+    rc = lib.wdrz_token_logprobs(
+        dt, x.data_ptr(), x.stride(0), mask, m_stride, tokens.data_ptr(), values.data_ptr(), values.data_ptr() + 4 * rows,
+        top_logprobs.data_ptr(), top_ids.data_ptr(), rows, V, top, None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else workspace.numel(), _raw_stream(index))
+    if rc != _lib.WDRZ_OK:
+        _raise(rc, "token_logprobs")
+    return TokenLogprobs(values[0], values[1], top_logprobs, top_ids)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], gelu: bool = False) -> torch.Tensor:
