@@ -26,24 +26,33 @@ namespace {
 
 constexpr int kTile = 64;           // keys a stage
 constexpr int kSub = 32;            // keys a step
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
 constexpr float kSumLimit = 1024.f;
+
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+// A buffer resource over [base, base + bytes): loads past the end return zero.
+__device__ __forceinline__ i32x4 rsrc(const void* base, uint32_t bytes) {
+  const uint64_t p = (uint64_t)(uintptr_t)base;
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)p);
+  r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32) & 0xffff);  // stride 0
+  r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
+  r[3] = 0x00020000;  // 32-bit data format
+  return r;
+}
 
 template <typename T> struct Pk;
 template <> struct Pk<Bf16> {
   typedef bf16x8 op_t;
   static __device__ __forceinline__ f32x16 mfma(op_t a, op_t b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
-  static __device__ __forceinline__ float one(uint16_t w) { return bf16_lo(w); }
-  static constexpr uint32_t kExp = 0x7f80u;
+  static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u;
 };
 template <> struct Pk<F16> {
   typedef f16x8 op_t;
   static __device__ __forceinline__ f32x16 mfma(op_t a, op_t b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
-  static __device__ __forceinline__ float one(uint16_t w) { return f16_lo(w); }
-  static constexpr uint32_t kExp = 0x7c00u;
+  static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
 };
 
 // max of x over the two 32-lane halves of the wavefront (every lane gets the result)
@@ -103,119 +112,150 @@ __device__ __forceinline__ bool find_item(const PackedArgs& a, int rows, int idx
   return false;
 }
 
-template <typename T, int D, int QB>
-__global__ __launch_bounds__(kThreads, 2) void packed_attn_kernel(PackedArgs a) {
+// 16 bytes a lane from memory to LDS, lane l to byte `to` + 16 l, without passing through registers; zeros where the
+// offset lies behind the resource. The compiler does not know of it: waits are written out below.
+__device__ __forceinline__ void load_lds(i32x4 from, uint32_t offset, uint32_t to) {
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(to) : "memory");
+#else
+  (void)from, (void)offset, (void)to;
+#endif
+}
+template <int N> __device__ __forceinline__ void landed_barrier() {  // all but the last N loads, of every wavefront
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+#endif
+}
+
+template <typename T, int D, int NW, int NBUF>
+__global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedArgs a) {
   typedef typename Pk<T>::op_t op_t;
   typedef uint16_t e_t;
-  constexpr int kBM = 32 * QB * kWaves, kPitch = D + 8, KS = D / 16, DB = D / 32;
-  constexpr int kPieces = kTile * D / 8 / kThreads;  // 16-byte pieces a thread and tile
-  __shared__ __attribute__((aligned(16))) e_t sK[2][kTile * kPitch];
-  __shared__ __attribute__((aligned(16))) e_t sV[2][kTile * kPitch];
+  constexpr int KS = D / 16, DB = D / 32, kRow = D * 2, kPiece = kRow / 16, kHalf = kTile * kRow, kBuf = 2 * kHalf;
+  constexpr int kLoads = kHalf / 1024 / NW;  // a wavefront's loads of a tile's keys (and of its values)
+  __shared__ __attribute__((aligned(1024))) char smem[NBUF * kBuf];  // tiles: keys, then values
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
-  // heads fastest, the heads of different groups side by side: with a multiple of eight groups a group's heads run
-  // on one XCD and share its L2
-  const int hid = (int)blockIdx.x % a.H, idx = (int)blockIdx.x / a.H;
-  const int hk = hid % a.Hk, h = hk * (a.H / a.Hk) + hid / a.Hk;
+  // groups fastest: with a multiple of eight key/value heads a head's workgroups run on one XCD and share its L2
+  const int sub = (int)blockIdx.x % (a.H / a.nh), idx = (int)blockIdx.x / (a.H / a.nh);
+  const int hk = sub % a.Hk, nqb = NW / a.nh;  // query blocks a head
   Item it;
-  if (!find_item(a, kBM, idx, it)) return;
-
-  const int q_wg = it.block * kBM, q_wave = q_wg + wave * 32 * QB;
+  if (!find_item(a, 32 * nqb, idx, it)) return;
+  // wavefronts w and w + 4 share a SIMD: under the mask the later blocks of one half meet the earlier ones of the other
+  const int qbi = wave < 4 || NW == 4 ? wave / a.nh : nqb - 1 - (wave - 4) / a.nh;
+  const int h = hk * (a.H / a.Hk) + sub / a.Hk * a.nh + wave % a.nh;
+  const int q_wg = it.block * 32 * nqb, q_wave = q_wg + qbi * 32;
   const int shift = a.causal ? it.nk - it.nq : 0;  // query t sees the keys up to t + shift
-  const int k_lim = a.causal ? max(0, min(it.nk, min(q_wg + kBM, it.nq) + shift)) : it.nk;
+  const int k_lim = a.causal ? max(0, min(it.nk, min(q_wg + 32 * nqb, it.nq) + shift)) : it.nk;
   const int n_tiles = (k_lim + kTile - 1) / kTile;
-  const int w_lim = a.causal ? max(0, min(k_lim, q_wave + 32 * QB + shift)) : it.nk;  // keys of this wavefront
+  const int w_lim = q_wave >= it.nq ? 0 : a.causal ? max(0, min(k_lim, q_wave + 32 + shift)) : it.nk;  // keys of this wavefront
   const int n_sub = (w_lim + kSub - 1) / kSub;
+  const int lim = a.causal ? min(it.nk, q_wave + l32 + shift + 1) : it.nk;        // keys that this lane's query sees
+  const int lim_lo = a.causal ? min(it.nk, q_wave + shift + 1) : it.nk;           // keys that every query sees
 
   const char* Q = a.q + (int64_t)it.q0 * a.qs[0] + (int64_t)h * a.qs[1];
   const char* K = a.k + (int64_t)it.k0 * a.ks[0] + (int64_t)hk * a.ks[1];
   const char* V = a.v + (int64_t)it.k0 * a.vs[0] + (int64_t)hk * a.vs[1];
 
-  op_t q[QB][KS];
+  // Tiles lie in LDS as rows of kPiece 16-byte pieces, piece p of row r at place p ^ swizzle(r): the 16 rows of a K
+  // operand's piece and the 4 rows x 64 bytes of a V^T operand's lie in different banks.
+  auto swizzle = [](int r) { return D == 64 ? ((r >> 1 & 1) << 2) | (r >> 2 & 3) : ((r & 3) << 2) | (r >> 2 & 3); };
+  uint32_t k_from[kLoads], v_from[kLoads];
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const int t = min(q_wave + qb * 32 + l32, it.nq - 1);
-#pragma unroll
-    for (int s = 0; s < KS; ++s) q[qb][s] = __builtin_bit_cast(op_t, load16(Q + (int64_t)t * a.qs[0] + s * 32 + hl * 16));
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = (i * NW + wave) * (1024 / kRow) + lane / kPiece, p = (lane % kPiece) ^ swizzle(r);
+    k_from[i] = (uint32_t)(r * (int)a.ks[0] + p * 16);  // 64 rows fit 31 bits (checked by the caller)
+    v_from[i] = (uint32_t)(r * (int)a.vs[0] + p * 16);
   }
-
-  u32x4 rk[kPieces], rv[kPieces];
-  auto fetch = [&](int tile) __attribute__((always_inline)) {
+  const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
+  auto issue = [&](int t) __attribute__((always_inline)) {
+    const int rows = min(it.nk - t * kTile, kTile);  // rows behind the sequence come as zeros: another's, which must not count
+    const i32x4 kr = rsrc(K + (int64_t)t * kTile * a.ks[0], rows > 0 ? (uint32_t)((rows - 1) * (int)a.ks[0] + kRow) : 0u);
+    const i32x4 vr = rsrc(V + (int64_t)t * kTile * a.vs[0], rows > 0 ? (uint32_t)((rows - 1) * (int)a.vs[0] + kRow) : 0u);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(t % NBUF) * kBuf + wave * 1024);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int piece = tid + i * kThreads, row = piece / (D / 8), p = piece % (D / 8), key = tile * kTile + row;
-      rk[i] = rv[i] = u32x4{0, 0, 0, 0};  // behind the sequence: another's rows, which must not count
-      if (key < it.nk) {
-        rk[i] = load16(K + (int64_t)key * a.ks[0] + p * 16);
-        rv[i] = load16(V + (int64_t)key * a.vs[0] + p * 16);
-      }
-    }
-  };
-  auto stage = [&](int buf) __attribute__((always_inline)) {
+    for (int i = 0; i < kLoads; ++i) load_lds(kr, k_from[i], to + i * NW * 1024);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int piece = tid + i * kThreads, row = piece / (D / 8), p = piece % (D / 8);
-      *reinterpret_cast<u32x4*>(&sK[buf][row * kPitch + p * 8]) = rk[i];
-      *reinterpret_cast<u32x4*>(&sV[buf][row * kPitch + p * 8]) = rv[i];
-    }
+    for (int i = 0; i < kLoads; ++i) load_lds(vr, v_from[i], to + kHalf + i * NW * 1024);
   };
 
-  // K operand: key row 8 i + 4 j + e of a step stands at row 16 (i / 2) + 8 j + 4 (i % 2) + e, so that score x of a
-  // lane is key 16 (x / 8) + 8 hl + x % 8
-  const int k_off = (16 * (l32 >> 4) + 8 * ((l32 >> 2) & 1) + 4 * ((l32 >> 3) & 1) + (l32 & 3)) * kPitch + hl * 8;
-  const int g16 = lane >> 4, j16 = lane & 15;
-  const int v_off = (8 * (g16 >> 1) + (j16 >> 2)) * kPitch + 16 * (g16 & 1) + 4 * (j16 & 3);
+  f32x16 acc[DB];  // O^T: query l32, dim 32 db + 8 (x / 4) + 4 hl + x % 4
+  float m = 0.f, l = 0.f;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) acc[db][x] = 0.f;
 
-  f32x16 acc[DB][QB];  // O^T: query l32 of block qb, dim 32 db + 8 (x / 4) + 4 hl + x % 4
-  float m[QB], l[QB];
+  if (n_tiles > 0) {
+    issue(0);
+    u32x4 q[KS];
+    {
+      const char* row = Q + (int64_t)min(q_wave + l32, it.nq - 1) * a.qs[0] + hl * 16;
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    m[qb] = l[qb] = 0.f;
+      for (int s = 0; s < KS; ++s) q[s] = load16(row + s * 32);
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int x = 0; x < 16; ++x) acc[db][qb][x] = 0.f;
-  }
-
-  auto step = [&](int s, int buf) __attribute__((always_inline)) {
-    const int base = s * kSub;
-    const e_t* kb = &sK[buf][(s & 1) * kSub * kPitch + k_off];
-    const e_t* vb = &sV[buf][(s & 1) * kSub * kPitch + v_off];
-    const bool edge = base + kSub > (a.causal ? min(it.nk, q_wave + shift + 1) : it.nk);
-    f32x16 sc[QB];
-#pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      const op_t k = __builtin_bit_cast(op_t, *reinterpret_cast<const u32x4*>(kb + i * 16));
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) sc[qb] = Pk<T>::mfma(k, q[qb][i], i == 0 ? f32x16{} : sc[qb]);
+      for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[s]));  // here, not behind the next tiles
     }
-    if (edge) {
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        const int lim = a.causal ? min(it.nk, q_wave + qb * 32 + l32 + shift + 1) : it.nk;
+    for (int t = 1; t < NBUF - 1; ++t) issue(t);
+    landed_barrier<2 * kLoads * (NBUF - 2)>();
+
+    // K operand: key row 8 i + 4 j + e of a step stands at row 16 (i / 2) + 8 j + 4 (i % 2) + e, so that score x of a
+    // lane is key 16 (x / 8) + 8 hl + x % 8. Piece 2 s + hl of it: the place of piece hl, ^ 2 s.
+    const int k_row = 16 * (l32 >> 4) + 8 * (l32 >> 2 & 1) + 4 * (l32 >> 3 & 1) + (l32 & 3);
+    const uint32_t k_at = k_row * kRow + ((hl ^ swizzle(k_row)) << 4);
+    // V^T operand: rows 8 hl + j / 4 (j = lane % 16) and those 4 further, dims 16 (lane / 16 % 2) + 4 (j % 4) of a block
+    const int j16 = lane & 15, v_row = 8 * hl + (j16 >> 2);
+    const uint32_t v_at = v_row * kRow + (((2 * (lane >> 4 & 1) + (j16 >> 1 & 1)) ^ swizzle(v_row)) << 4) + (j16 & 1) * 8;
+    op_t k[KS], v[2][DB];
+    auto read_k = [&](int s) __attribute__((always_inline)) {
+      const uint32_t at = k_at + ((s >> 1) % NBUF) * kBuf + (s & 1) * kSub * kRow;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) k[i] = __builtin_bit_cast(op_t, *reinterpret_cast<const u32x4*>(smem + (at ^ (i << 5))));
+    };
+    auto read_v = [&](int s) __attribute__((always_inline)) {
+      const uint32_t at = v_at + ((s >> 1) % NBUF) * kBuf + kHalf + (s & 1) * kSub * kRow;
+#pragma unroll
+      for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const u32x2 lo = read_tr(reinterpret_cast<const e_t*>(smem + (at ^ (db << 6)) + ch * 16 * kRow));
+          const u32x2 hi = read_tr(reinterpret_cast<const e_t*>(smem + (at ^ (db << 6) ^ 16) + (ch * 16 + 4) * kRow));
+          v[ch][db] = __builtin_bit_cast(op_t, u32x4{lo[0], lo[1], hi[0], hi[1]});
+        }
+    };
+    auto scores = [&](f32x16& sc) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i) sc = Pk<T>::mfma(k[i], __builtin_bit_cast(op_t, q[i]), i == 0 ? f32x16{} : sc);
+    };
+    // One step: the next step's scores and this one's V^T operands are under way while the softmax runs.
+    auto step = [&](int s, f32x16& sc, f32x16& next) __attribute__((always_inline)) {
+      const int base = s * kSub;
+      const bool edge = base + kSub > lim_lo;
+      read_v(s);
+      if (s + 1 < n_sub) scores(next);
+      __builtin_amdgcn_sched_barrier(0);
+      if (edge) {
 #pragma unroll
         for (int x = 0; x < 16; ++x)
-          if (base + 16 * (x >> 3) + 8 * hl + (x & 7) >= lim) sc[qb][x] = -INFINITY;
+          if (base + 16 * (x >> 3) + 8 * hl + (x & 7) >= lim) sc[x] = -INFINITY;
       }
-    }
-    op_t p[QB][2];
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
+      op_t p[2];
       float st;
       auto exps = [&]() __attribute__((always_inline)) {
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        float part[4];
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
           u32x4 w;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p0 = fast_exp2(__builtin_fmaf(sc[qb][8 * ch + 2 * e], a.c, -m[qb]));
-            const float p1 = fast_exp2(__builtin_fmaf(sc[qb][8 * ch + 2 * e + 1], a.c, -m[qb]));
+            const float p0 = fast_exp2(__builtin_fmaf(sc[8 * ch + 2 * e], a.c, -m));
+            const float p1 = fast_exp2(__builtin_fmaf(sc[8 * ch + 2 * e + 1], a.c, -m));
             w[e] = Pk<T>::pack(p0, p1);
-            part[e] += p0 + p1;
+            part[e] = ch == 0 ? p0 + p1 : part[e] + p0 + p1;
           }
-          p[qb][ch] = __builtin_bit_cast(op_t, w);
+          p[ch] = __builtin_bit_cast(op_t, w);
         }
         st = (part[0] + part[1]) + (part[2] + part[3]);
       };
@@ -224,127 +264,150 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attn_kernel(PackedArgs a) 
         asm volatile("" ::: "memory");  // rare: stays a branch
         float mx = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[qb][x]);
+        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[x]);
         mx = halves_max(mx) * a.c;
-        const float to = s == 0 ? (mx == -INFINITY ? 0.f : mx) : fmaxf(m[qb], mx);
-        const float f = fast_exp2(m[qb] - to);
-        m[qb] = to;
+        const float to = s == 0 ? (mx == -INFINITY ? 0.f : mx) : fmaxf(m, mx);
+        const float f = fast_exp2(m - to);
+        m = to;
         if (s != 0) {
-          l[qb] *= f;
+          l *= f;
 #pragma unroll
           for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int x = 0; x < 16; ++x) acc[db][qb][x] *= f;
+            for (int x = 0; x < 16; ++x) acc[db][x] *= f;
         }
         exps();
       }
-      l[qb] += st;
-    }
-    op_t v[2][DB];
-#pragma unroll
-    for (int ch = 0; ch < 2; ++ch)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const e_t* at = vb + ch * 16 * kPitch + db * 32;
-        const u32x2 lo = read_tr(at), hi = read_tr(at + 4 * kPitch);
-        v[ch][db] = __builtin_bit_cast(op_t, u32x4{lo[0], lo[1], hi[0], hi[1]});
-      }
-    if (edge && a.causal) {
-      // Some query of the block sees some key of it and not others: 0 times an infinity or NaN behind the mask
-      // would count in the products, so such keys are added one by one.
+      l += st;
+      __builtin_amdgcn_sched_barrier(0);
+      // Where some query sees some key of the step and not others, 0 times an infinity or NaN behind the mask would
+      // count in the products: such values are taken out of V, and given to the queries that see them.
       bool odd = false;
+      if (edge) {
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t w = __builtin_bit_cast(u32x4, v[ch][db])[e];
+              odd = odd || (w & Pk<T>::kExp) == Pk<T>::kExp || ((w >> 16) & Pk<T>::kExp) == Pk<T>::kExp;
+            }
+        if (__any(odd)) {
+          op_t sees[2];
+#pragma unroll
+          for (int ch = 0; ch < 2; ++ch) {
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = base + 16 * ch + 8 * hl + 2 * e;
+              w[e] = Pk<T>::pack(key < lim ? 1.f : 0.f, key + 1 < lim ? 1.f : 0.f);
+            }
+            sees[ch] = __builtin_bit_cast(op_t, w);
+          }
+          // the values of one kind (inf, -inf, NaN) as ones
+          auto ones = [&](op_t x, int kind) __attribute__((always_inline)) {
+            u32x4 w = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t r = 0;
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const uint32_t u = w[e] >> (16 * half) & 0xffffu;
+                const bool is = kind == 2 ? (u & 0x7fffu) > Pk<T>::kExp : u == (Pk<T>::kExp | (kind ? 0x8000u : 0u));
+                r |= is ? Pk<T>::kOne << (16 * half) : 0u;
+              }
+              w[e] = r;
+            }
+            return __builtin_bit_cast(op_t, w);
+          };
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+#pragma unroll 1
+            for (int kind = 0; kind < 3; ++kind) {
+              f32x16 n = Pk<T>::mfma(ones(v[0][db], kind), sees[0], f32x16{});
+              n = Pk<T>::mfma(ones(v[1][db], kind), sees[1], n);
+              const float value = kind == 2 ? __builtin_nanf("") : kind ? -INFINITY : INFINITY;
+#pragma unroll
+              for (int x = 0; x < 16; ++x) acc[db][x] += n[x] > 0.f ? value : 0.f;
+            }
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+              u32x4 w = __builtin_bit_cast(u32x4, v[ch][db]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((w[e] & Pk<T>::kExp) == Pk<T>::kExp) w[e] &= 0xffff0000u;
+                if ((w[e] >> 16 & Pk<T>::kExp) == Pk<T>::kExp) w[e] &= 0xffffu;
+              }
+              v[ch][db] = __builtin_bit_cast(op_t, w);
+            }
+          }
+        }
+      }
+      read_k(s + 2);
 #pragma unroll
       for (int ch = 0; ch < 2; ++ch)
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t w = __builtin_bit_cast(u32x4, v[ch][db])[e];
-            odd = odd || (w & Pk<T>::kExp) == Pk<T>::kExp || ((w >> 16) & Pk<T>::kExp) == Pk<T>::kExp;
-          }
-      if (__any(odd)) {
-        const e_t* rows = &sV[buf][(s & 1) * kSub * kPitch];
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-          const int lim = min(it.nk, q_wave + qb * 32 + l32 + shift + 1);
-#pragma unroll 1
-          for (int kk = 0; kk < kSub; ++kk) {
-            // key 16 ch + 8 half + e: element e of operand ch in the lane of that half
-            const u32x4 w0 = __builtin_bit_cast(u32x4, p[qb][0]), w1 = __builtin_bit_cast(u32x4, p[qb][1]);
-            const int e = (kk & 7) >> 1;
-            uint32_t w = kk & 16 ? (e & 2 ? (e & 1 ? w1[3] : w1[2]) : (e & 1 ? w1[1] : w1[0]))
-                                 : (e & 2 ? (e & 1 ? w0[3] : w0[2]) : (e & 1 ? w0[1] : w0[0]));
-            w = __shfl(w, l32 + 32 * ((kk >> 3) & 1));
-            const float pk = Pk<T>::one((uint16_t)(kk & 1 ? w >> 16 : w & 0xffffu));
-            if (base + kk >= lim) continue;
-#pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-              for (int x = 0; x < 16; ++x)
-                acc[db][qb][x] = __builtin_fmaf(pk, Pk<T>::one(rows[kk * kPitch + 32 * db + 8 * (x >> 2) + 4 * hl + (x & 3)]), acc[db][qb][x]);
-          }
-        }
-        return;
-      }
-    }
-#pragma unroll
-    for (int ch = 0; ch < 2; ++ch)
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) acc[db][qb] = Pk<T>::mfma(v[ch][db], p[qb][ch], acc[db][qb]);
-  };
+        for (int db = 0; db < DB; ++db) acc[db] = Pk<T>::mfma(v[ch][db], p[ch], acc[db]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
 
-  if (n_tiles > 0) {
-    fetch(0);
-    stage(0);
-    __syncthreads();
+    f32x16 s0, s1;
+    read_k(0);
+    scores(s0);
+    read_k(1);
     for (int t = 0; t < n_tiles; ++t) {
-      const int buf = t & 1;
-      if (t + 1 < n_tiles) fetch(t + 1);
-      if (2 * t < n_sub) step(2 * t, buf);
-      if (2 * t + 1 < n_sub) step(2 * t + 1, buf);
-      if (t + 1 < n_tiles) {
-        stage(buf ^ 1);  // its last readers passed the barrier of the tile before
-        __syncthreads();
-      }
+      // tile t + 1, whose keys the steps of this tile read, is there; nobody reads tile t - 1 any more
+      landed_barrier<2 * kLoads * (NBUF - 3)>();
+      issue(t + NBUF - 1);
+      if (2 * t < n_sub) step(2 * t, s0, s1);
+      if (2 * t + 1 < n_sub) step(2 * t + 1, s1, s0);
     }
   }
 
+  // O^T through LDS, so that memory sees whole rows: the wavefront's 32 rows in its own part
+  landed_barrier<0>();
+  const float sum = l + __shfl_xor(l, 32);
+  const float f = sum == 0.f ? 0.f : 1.f / sum;  // a query that sees no key is 0
+  char* mine = smem + wave * 32 * kRow;
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const float sum = l[qb] + __shfl_xor(l[qb], 32);
-    const float f = sum == 0.f ? 0.f : 1.f / sum;  // a query that sees no key is 0
-    const int t = q_wave + qb * 32 + l32;
-    if (t >= it.nq) continue;
-    char* o = a.o + (int64_t)(it.q0 + t) * a.os[0] + (int64_t)h * a.os[1];
+  for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int i = 0; i < 4; ++i) {
+      const f32x16& r = acc[db];
+      const int at = l32 * kRow + (((4 * db + i) ^ swizzle(l32)) << 4) + hl * 8;
+      *reinterpret_cast<u32x2*>(mine + at) = u32x2{Pk<T>::pack(r[4 * i] * f, r[4 * i + 1] * f), Pk<T>::pack(r[4 * i + 2] * f, r[4 * i + 3] * f)};
+    }
+  __builtin_amdgcn_wave_barrier();
+  char* o = a.o + (int64_t)(it.q0 + q_wave) * a.os[0] + (int64_t)h * a.os[1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x16& r = acc[db][qb];
-        *reinterpret_cast<u32x2*>(o + (32 * db + 8 * i + 4 * hl) * 2) =
-            u32x2{Pk<T>::pack(r[4 * i] * f, r[4 * i + 1] * f), Pk<T>::pack(r[4 * i + 2] * f, r[4 * i + 3] * f)};
-      }
+  for (int i = 0; i < 32 * kPiece / 64; ++i) {
+    const int r = i * (64 / kPiece) + lane / kPiece, p = lane % kPiece;
+    const u32x4 w = *reinterpret_cast<const u32x4*>(mine + r * kRow + ((p ^ swizzle(r)) << 4));
+    if (q_wave + r < it.nq) store16(o + (int64_t)r * a.os[0] + p * 16, w);
   }
 }
 
-template <typename T, int D, int QB>
-void launch_q(const PackedArgs& a, hipStream_t stream) {
-  constexpr int kBM = 32 * QB * kWaves;
-  const int64_t blocks = a.T / kBM + std::min(a.B, a.T);  // at most: every sequence's last block is part full
-  hipLaunchKernelGGL((packed_attn_kernel<T, D, QB>), dim3((unsigned)(blocks * a.H)), dim3(kThreads), 0, stream, a);
+template <typename T, int D, int NW, int NBUF>
+void launch_q(PackedArgs a, hipStream_t stream) {
+  // heads of a group share a workgroup's keys: as many as divide the group and the wavefronts
+  const int group = a.H / a.Hk;
+  a.nh = 1;
+  while (a.nh < NW && group % (2 * a.nh) == 0) a.nh *= 2;
+  const int rows = 32 * NW / a.nh;
+  const int64_t blocks = a.T / rows + std::min(a.B, a.T);  // at most: every sequence's last block is part full
+  hipLaunchKernelGGL((packed_attn_kernel<T, D, NW, NBUF>), dim3((unsigned)(blocks * (a.H / a.nh))), dim3(64 * NW), 0, stream, a);
 }
 
 }  // namespace
 
 hipError_t launch_packed(int dtype, int D, const PackedArgs& a, hipStream_t stream) {
   if (D == 64) {
-    if (dtype == 2) launch_q<Bf16, 64, 2>(a, stream);
-    else launch_q<F16, 64, 2>(a, stream);
+    if (dtype == 2) launch_q<Bf16, 64, 4, 4>(a, stream);
+    else launch_q<F16, 64, 4, 4>(a, stream);
   } else {
-    if (dtype == 2) launch_q<Bf16, 128, 1>(a, stream);
-    else launch_q<F16, 128, 1>(a, stream);
+    if (dtype == 2) launch_q<Bf16, 128, 8, 4>(a, stream);
+    else launch_q<F16, 128, 8, 4>(a, stream);
   }
   return hipGetLastError();
 }

@@ -336,6 +336,7 @@ struct PackedArgs {
   const int32_t* cu_k;  // [B + 1] (cu_q where the keys are the queries' own)
   float c;              // softmax scale * log2(e)
   int B, T, Tk, H, Hk, causal;
+  int nh;  // heads of a group that share a workgroup (set by the launcher)
 };
 hipError_t launch_packed(int dtype, int D, const PackedArgs& a, hipStream_t stream);
 
