@@ -95,14 +95,13 @@ __device__ __forceinline__ bool find_item(const PackedArgs& a, int rows, int idx
       const int u = __shfl_up(sum, o);
       if (lane >= o) sum += u;
     }
-    const int total = __shfl(sum, 63);
+    const int total = __builtin_amdgcn_readlane(sum, 63);
     if (idx < total) {
       const uint64_t here = __ballot(idx < sum);
-      const int src = __ffsll((unsigned long long)here) - 1;
-      const int s = __builtin_amdgcn_readfirstlane(a.B - 1 - i0 - src);
-      it.q0 = __builtin_amdgcn_readfirstlane(__shfl(c0, src));
-      it.nq = __builtin_amdgcn_readfirstlane(__shfl(c1, src)) - it.q0;
-      it.block = __builtin_amdgcn_readfirstlane(__shfl(sum, src) - 1 - idx);
+      const int src = __ffsll((unsigned long long)here) - 1, s = a.B - 1 - i0 - src;
+      it.q0 = __builtin_amdgcn_readlane(c0, src);
+      it.nq = __builtin_amdgcn_readlane(c1, src) - it.q0;
+      it.block = __builtin_amdgcn_readlane(sum, src) - 1 - idx;
       it.k0 = min(max(a.cu_k[s], 0), a.Tk);
       it.nk = min(max(a.cu_k[s + 1], it.k0), a.Tk) - it.k0;
       return true;
@@ -127,8 +126,9 @@ template <int N> __device__ __forceinline__ void landed_barrier() {  // all but 
 #endif
 }
 
-template <typename T, int D, int NW, int NBUF>
-__global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedArgs a) {
+// AHEAD: the next step's scores run under this step's softmax; else the other wavefronts of the SIMD (SIMD_WAVES) fill it.
+template <typename T, int D, int NW, int NBUF, bool AHEAD, int SIMD_WAVES>
+__global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(PackedArgs a) {
   typedef typename Pk<T>::op_t op_t;
   typedef uint16_t e_t;
   constexpr int KS = D / 16, DB = D / 32, kRow = D * 2, kPiece = kRow / 16, kHalf = kTile * kRow, kBuf = 2 * kHalf;
@@ -137,14 +137,15 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedArgs a) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
-  // groups fastest: with a multiple of eight key/value heads a head's workgroups run on one XCD and share its L2
-  const int sub = (int)blockIdx.x % (a.H / a.nh), idx = (int)blockIdx.x / (a.H / a.nh);
-  const int hk = sub % a.Hk, nqb = NW / a.nh;  // query blocks a head
+  // blocks fastest, neighbours on one XCD: those of a sequence read the same keys of a head
+  const int unit = remap_xcd((int)blockIdx.x, (int)gridDim.x), n_idx = (int)gridDim.x / (a.H / a.nh);
+  const int sub = unit / n_idx, idx = unit % n_idx, per_group = a.H / a.Hk / a.nh;
+  const int hk = sub / per_group, nqb = NW / a.nh;  // query blocks a head
   Item it;
   if (!find_item(a, 32 * nqb, idx, it)) return;
   // wavefronts w and w + 4 share a SIMD: under the mask the later blocks of one half meet the earlier ones of the other
   const int qbi = wave < 4 || NW == 4 ? wave / a.nh : nqb - 1 - (wave - 4) / a.nh;
-  const int h = hk * (a.H / a.Hk) + sub / a.Hk * a.nh + wave % a.nh;
+  const int h = sub * a.nh + wave % a.nh;
   const int q_wg = it.block * 32 * nqb, q_wave = q_wg + qbi * 32;
   const int shift = a.causal ? it.nk - it.nq : 0;  // query t sees the keys up to t + shift
   const int k_lim = a.causal ? max(0, min(it.nk, min(q_wg + 32 * nqb, it.nq) + shift)) : it.nk;
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedArgs a) {
     }
 #pragma unroll
     for (int t = 1; t < NBUF - 1; ++t) issue(t);
-    landed_barrier<2 * kLoads * (NBUF - 2)>();
+    if (AHEAD) landed_barrier<2 * kLoads * (NBUF - 2)>();
 
     // K operand: key row 8 i + 4 j + e of a step stands at row 16 (i / 2) + 8 j + 4 (i % 2) + e, so that score x of a
     // lane is key 16 (x / 8) + 8 hl + x % 8. Piece 2 s + hl of it: the place of piece hl, ^ 2 s.
@@ -233,13 +234,19 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedArgs a) {
     auto step = [&](int s, f32x16& sc, f32x16& next) __attribute__((always_inline)) {
       const int base = s * kSub;
       const bool edge = base + kSub > lim_lo;
-      read_v(s);
-      if (s + 1 < n_sub) scores(next);
+      if (AHEAD) {
+        read_v(s);
+        if (s + 1 < n_sub) scores(next);
+      } else {
+        read_k(s);
+        scores(sc);
+      }
       __builtin_amdgcn_sched_barrier(0);
       if (edge) {
+        const int sees = lim - base - 8 * hl;
 #pragma unroll
         for (int x = 0; x < 16; ++x)
-          if (base + 16 * (x >> 3) + 8 * hl + (x & 7) >= lim) sc[x] = -INFINITY;
+          if (16 * (x >> 3) + (x & 7) >= sees) sc[x] = -INFINITY;
       }
       op_t p[2];
       float st;
@@ -279,6 +286,7 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedArgs a) {
         exps();
       }
       l += st;
+      if (!AHEAD) read_v(s);
       __builtin_amdgcn_sched_barrier(0);
       // Where some query sees some key of the step and not others, 0 times an infinity or NaN behind the mask would
       // count in the products: such values are taken out of V, and given to the queries that see them.
@@ -344,7 +352,7 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedArgs a) {
           }
         }
       }
-      read_k(s + 2);
+      if (AHEAD) read_k(s + 2);
 #pragma unroll
       for (int ch = 0; ch < 2; ++ch)
 #pragma unroll
@@ -353,15 +361,20 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedArgs a) {
     };
 
     f32x16 s0, s1;
-    read_k(0);
-    scores(s0);
-    read_k(1);
+    if (AHEAD) {
+      read_k(0);
+      scores(s0);
+      read_k(1);
+    }
     for (int t = 0; t < n_tiles; ++t) {
-      // tile t + 1, whose keys the steps of this tile read, is there; nobody reads tile t - 1 any more
-      landed_barrier<2 * kLoads * (NBUF - 3)>();
+      // the last tile that this one's steps read (AHEAD: the next one's keys) is there; nobody reads tile t - 1 any more
+      landed_barrier<2 * kLoads * (NBUF - (AHEAD ? 3 : 2))>();
       issue(t + NBUF - 1);
       if (2 * t < n_sub) step(2 * t, s0, s1);
-      if (2 * t + 1 < n_sub) step(2 * t + 1, s1, s0);
+      if (2 * t + 1 < n_sub) {
+        if (AHEAD) step(2 * t + 1, s1, s0);
+        else step(2 * t + 1, s0, s1);
+      }
     }
   }
 
@@ -388,7 +401,7 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedArgs a) {
   }
 }
 
-template <typename T, int D, int NW, int NBUF>
+template <typename T, int D, int NW, int NBUF, bool AHEAD, int SIMD_WAVES>
 void launch_q(PackedArgs a, hipStream_t stream) {
   // heads of a group share a workgroup's keys: as many as divide the group and the wavefronts
   const int group = a.H / a.Hk;
@@ -396,18 +409,18 @@ void launch_q(PackedArgs a, hipStream_t stream) {
   while (a.nh < NW && group % (2 * a.nh) == 0) a.nh *= 2;
   const int rows = 32 * NW / a.nh;
   const int64_t blocks = a.T / rows + std::min(a.B, a.T);  // at most: every sequence's last block is part full
-  hipLaunchKernelGGL((packed_attn_kernel<T, D, NW, NBUF>), dim3((unsigned)(blocks * (a.H / a.nh))), dim3(64 * NW), 0, stream, a);
+  hipLaunchKernelGGL((packed_attn_kernel<T, D, NW, NBUF, AHEAD, SIMD_WAVES>), dim3((unsigned)(blocks * (a.H / a.nh))), dim3(64 * NW), 0, stream, a);
 }
 
 }  // namespace
 
 hipError_t launch_packed(int dtype, int D, const PackedArgs& a, hipStream_t stream) {
   if (D == 64) {
-    if (dtype == 2) launch_q<Bf16, 64, 4, 4>(a, stream);
-    else launch_q<F16, 64, 4, 4>(a, stream);
+    if (dtype == 2) launch_q<Bf16, 64, 4, 3, false, 3>(a, stream);
+    else launch_q<F16, 64, 4, 3, false, 3>(a, stream);
   } else {
-    if (dtype == 2) launch_q<Bf16, 128, 8, 4>(a, stream);
-    else launch_q<F16, 128, 8, 4>(a, stream);
+    if (dtype == 2) launch_q<Bf16, 128, 8, 4, true, 2>(a, stream);
+    else launch_q<F16, 128, 8, 4, true, 2>(a, stream);
   }
   return hipGetLastError();
 }
