@@ -290,17 +290,16 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
       __builtin_amdgcn_sched_barrier(0);
       // Where some query sees some key of the step and not others, 0 times an infinity or NaN behind the mask would
       // count in the products: such values are taken out of V, and given to the queries that see them.
-      bool odd = false;
       if (edge) {
+        f32x16 zero = {};  // 0 times each value: 0, or NaN where there is such a one
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch)
 #pragma unroll
-          for (int db = 0; db < DB; ++db)
+          for (int db = 0; db < DB; ++db) zero = Pk<T>::mfma(v[ch][db], op_t{}, zero);
+        float any = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t w = __builtin_bit_cast(u32x4, v[ch][db])[e];
-              odd = odd || (w & Pk<T>::kExp) == Pk<T>::kExp || ((w >> 16) & Pk<T>::kExp) == Pk<T>::kExp;
-            }
+        for (int x = 0; x < 16; ++x) any += zero[x];
+        const bool odd = any != any;
         if (__any(odd)) {
           op_t sees[2];
 #pragma unroll
