@@ -369,17 +369,21 @@ def kvpages_workspace_size(batch: int, sq: int, n_heads: int, n_kv_heads: int, h
     return int(_lib.load().wdrz_attn_kvpages_workspace_size(batch, sq, n_heads, n_kv_heads, head_dim, max_seq))
 
 
-# Workspaces whose counters stand at their start, apart from _WORKSPACES: calls of other shapes leave the counters
-# where they are, so nothing but they has to be zero after a call.
-_COUNTED_WORKSPACES = WorkspaceCache()
+# Workspaces by (device, stream) whose counters stand at their start, apart from _WORKSPACES: calls of other shapes leave
+# the counters where they are, so nothing but they has to be zero after a call.
+_COUNTED_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 
 
 def _counted_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """This stream's workspace; a captured call gets its own, cleared by every replay (another graph captured on
-    this stream may be replayed beside its graph)."""
+    """The current stream's workspace of ``device``, the current device; a captured call gets its own, cleared by every
+    replay (another graph captured on this stream may be replayed beside its graph)."""
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return _COUNTED_WORKSPACES.get(device, nbytes)
+    key = (device.index, _raw_stream(device.index))
+    buf = _COUNTED_WORKSPACES.get(key)
+    if buf is None or buf.numel() < nbytes:
+        buf = _COUNTED_WORKSPACES[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+    return buf
 
 
 def flash_attn_with_kvpages(

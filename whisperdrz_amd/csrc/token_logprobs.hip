@@ -4,17 +4,18 @@
 //   d_i = x_i - M,  Z = sum e^d_i,  log p_i = d_i - ln Z,  H = -sum p_i log p_i = ln Z - sum e^d_i d_i / Z
 //
 // In the sums the term of the largest token, e^0, stands apart: Z = 1 + r, ln Z = log1p(r), so a row with one likely
-// token keeps the digits of its small ln Z. Blocked tokens count as -inf. A row in which nothing is left has log probabilities of -inf, entropy 0 and no
-// alternatives (ids -1); NaN or +inf among its tokens makes all of the row NaN. e^d is taken as 2^(d log2 e) of the
-// difference, so the terms that count are exact to 2^-22; sums are fp32 in a thread (up to 64 terms of one
-// reference) and fp64 across threads.
+// token keeps the digits of its small ln Z. Blocked tokens count as -inf. A row in which nothing is left has log
+// probabilities of -inf, entropy 0 and no alternatives (ids -1); NaN or +inf among its tokens makes all of the row
+// NaN. e^d is taken as 2^(d log2 e) of the difference, so the terms that count are exact to 2^-22; sums are fp32 in a
+// wavefront and fp64 above it.
 //
 // Alternatives are ordered by logit, equal ones by index: keys of 64 bits, (order of the fp32 bits, ~index), are all
-// different. A thread keeps its largest key while it sums. The k-th largest T of the threads' keys bounds the
-// k-th largest of all from below, and only the at most k threads whose key is T or above own a key that can be
-// among the first k: their tokens alone are read again.
+// different. A thread keeps its largest key while it sums. The k-th largest of the keys of 16 or 64 groups of threads
+// bounds the k-th largest of all from below. A workgroup of one load a thread lists its tokens that are no smaller, a
+// few more than k; one of more loads lists such threads, and reads the tokens of the k first again, which alone can own
+// a key among the first k. Where a list grows beyond a wavefront it is ranked in full.
 //
-// Bound: the bytes of the logits; for few rows launch, a trip to memory, and the counting of keys.
+// Bound: the bytes of the logits; for few rows launch, two trips to memory and a handful of barriers.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -29,14 +30,13 @@ namespace {
 
 constexpr int kVec = 8;         // tokens a load
 constexpr int kBatch = 4;       // loads in flight a thread
-constexpr int kThreads = 1024;
+constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 32;
-constexpr int kPerSplit = 65536;  // tokens a workgroup takes at most
-constexpr int kMaxSplits = 16;
-constexpr int kOwned = kPerSplit / kThreads;  // tokens a thread takes at most
+constexpr int kMaxSplits = 32;
+constexpr int kList = kThreads * kVec + kVec + kMaxTop;  // tokens listed at most, with those of the round before
 constexpr float kFar = -200.f;    // e^-200 is 0 in fp32, and so are the terms of all logits further down
-constexpr int kCounters = 4096;   // rows of a launch that is split: their counters stand before the partials
+constexpr int kCounters = 4096;   // of rows that are split (1024 at most), before their partials
 
 // Order of fp32 values as unsigned numbers, above 0 for what can be chosen (-inf cannot).
 __device__ __forceinline__ uint32_t order(float x) {
@@ -50,26 +50,48 @@ __device__ __forceinline__ uint64_t key_of(float x, int i) {
   return o ? (uint64_t)o << 32 | (uint32_t)~i : 0;
 }
 
-// The tokens of a part of the row: the largest, m (-inf: none), the sum r of the others' e^(x - m) and the sum w of
-// e^(x - m) (x - m). r is NaN where a token is NaN or +inf.
-struct Sum {
-  double r, w;
-  float m;
-};
-__device__ __forceinline__ void join(Sum& a, float m, double r, double w) {
-  if (m == -INFINITY || a.m == -INFINITY) {
-    const bool other = a.m == -INFINITY;
-    a.r += r;  // one is 0, or NaN
-    a.w = other ? w : a.w;
-    a.m = other ? m : a.m;
-    return;
+// Maximum of different keys over the wavefront's first N lanes (N a power of two); every one of them gets it.
+template <int N> __device__ __forceinline__ uint64_t key_max(uint64_t k) {
+#pragma unroll
+  for (int o = N / 2; o >= 1; o >>= 1) {
+    const uint64_t other = __shfl_xor(k, o);
+    k = other > k ? other : k;
   }
-  const bool up = m > a.m;  // the smaller side's largest token joins the others
-  const double d = up ? (double)a.m - m : (double)m - a.m, f = (double)expf((float)d);
-  const double less_r = 1. + (up ? a.r : r), less_w = up ? a.w : w;
-  a.r = (up ? r : a.r) + less_r * f;
-  a.w = (up ? w : a.w) + (less_w + d * less_r) * f;
-  a.m = up ? m : a.m;
+  return k;
+}
+// The rank of this lane's key among the wavefront's first n (0: the largest).
+__device__ __forceinline__ int key_rank(uint64_t k, int n) {
+  int rank = 0;
+  for (int i = 0; i < n; ++i) {
+    const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), i) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)k, i);
+    rank += other > k;
+  }
+  return rank;
+}
+// The nth largest of the wavefront's first n keys, whose ranks are given; 1, below every key, where there are fewer.
+__device__ __forceinline__ uint64_t nth_key(uint64_t k, int rank, int n, int nth) {
+  const uint64_t lanes = __ballot((int)(threadIdx.x & 63) < n && rank == nth - 1 && k != 0);
+  if (!lanes) return 1;
+  const int src = __ffsll((unsigned long long)lanes) - 1;
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), src) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)k, src);
+}
+__device__ __forceinline__ float key_value(uint64_t k) { return k ? unorder((uint32_t)(k >> 32)) : -INFINITY; }
+
+// The tokens of a part of the row: the largest key, the sum r of the others' e^(x - m) and the sum w of e^(x - m)
+// (x - m), m the largest logit. Sums over the wavefront's first N lanes, every part with a largest key of its own.
+template <int N, typename F> __device__ __forceinline__ void join(uint64_t key, F& r, F& w, uint64_t& top_key) {
+  top_key = key_max<N>(key);
+  const float m = key_value(key), to = key_value(top_key);
+  const float d = m == -INFINITY ? kFar : fmaxf(m - to, kFar);
+  const F f = key == 0 ? F(0) : F(expf(d)), others = key == top_key ? r : r + F(1);
+  w = (w + F(d) * others) * f;
+  r = key == 0 ? r : others * f;  // r without a key: 0, or NaN
+#pragma unroll
+  for (int o = N / 2; o >= 1; o >>= 1) {
+    r += __shfl_xor(r, o);
+    w += __shfl_xor(w, o);
+  }
 }
 
 // The k largest of n different keys (0: none), sorted, to out[0 .. k - 1] (0 behind the last). Every thread of the
@@ -86,20 +108,36 @@ __device__ __forceinline__ void largest(const uint64_t* keys, int n, int k, uint
   __syncthreads();
 }
 
+// The same for the first wavefront alone where they fit it; it may read `out` afterwards, the others behind a barrier.
+__device__ __forceinline__ void sort_top(const uint64_t* keys, int n, int k, uint64_t* out) {
+  if (n > 64) {
+    largest(keys, n, k, out);
+    return;
+  }
+  if (threadIdx.x >= 64) return;
+  const int lane = threadIdx.x;
+  const uint64_t mine = lane < n ? keys[lane] : 0;
+  const int rank = key_rank(mine, n);
+  if (lane < k) out[lane] = 0;
+  __builtin_amdgcn_wave_barrier();
+  if (mine && rank < k) out[rank] = mine;
+  __builtin_amdgcn_wave_barrier();
+}
+
+static_assert(2 * kMaxSplits * kMaxTop <= kList, "the splits' keys and those of them that count");
 struct Partial {  // one split's sums and keys, in the workspace
   double r, w;
-  uint64_t m;  // fp32 bits
+  uint64_t top;
   uint64_t key[kMaxTop];
 };
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a) {
   constexpr int EB = ElemBytes<T>::value, kWords = kVec * EB / 4;
-  __shared__ uint64_t sm_keys[kMaxTop * (kOwned + kVec)];  // candidates
-  __shared__ uint64_t sm_wave[kWaves * kMaxTop], sm_top[kMaxTop];
+  __shared__ uint64_t sm_keys[kList];
+  __shared__ uint64_t sm_list[kWaves * kMaxTop], sm_top[kMaxTop], sm_group[64], sm_wave[kWaves];
   __shared__ double sm_r[kWaves], sm_w[kWaves];
-  __shared__ float sm_m[kWaves];
-  __shared__ int sm_owner[kMaxTop], sm_n, sm_owners, sm_last;
+  __shared__ int sm_n, sm_listed, sm_last;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x, split = blockIdx.y, top = a.top;
   const char* lr = static_cast<const char*>(a.logits) + (int64_t)row * a.l_stride * EB;
@@ -109,18 +147,17 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
   const int c_begin = (int)((int64_t)n_vec * split / a.splits), c_end = (int)((int64_t)n_vec * (split + 1) / a.splits);
   const int tail = split == a.splits - 1 ? a.V - n_vec * kVec : 0;
 
-  float m = -INFINITY, far = -3.402823466e38f, r = 0.f, w = 0.f;
-  int at = 0;  // the largest token's index
+  float m = -INFINITY, ref = 0.f, r = 0.f, w = 0.f;  // the largest logit, the same or 0 while there is none
+  int at = 0;  // its index
   auto take = [&](float (&x)[kVec], int i0) __attribute__((always_inline)) {
     float mx = x[0];
 #pragma unroll
     for (int e = 1; e < kVec; ++e) mx = fmaxf(mx, x[e]);
     if (mx > m) {
       const float d = fmaxf(m - mx, kFar), f = fast_exp2(d * kLog2e);
-      w = m == -INFINITY ? w : (w + d * (1.f + r)) * f;
+      w = m == -INFINITY ? w : (w + d * kLog2e * (1.f + r)) * f;
       r = m == -INFINITY ? r : (1.f + r) * f;
-      m = mx;
-      far = mx + kFar;
+      m = ref = mx;
       int first = 0;
 #pragma unroll
       for (int e = kVec - 1; e >= 0; --e)
@@ -130,13 +167,15 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
         if (e == first) x[e] = -INFINITY;  // its term stands apart
       at = i0 + first;
     }
+    float p[kVec], u = 0.f;  // a load's sums first: a thread's grow by one term a load
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
-      const float d = x[e] < far ? kFar : x[e] - m;
-      const float p = fast_exp2(d * kLog2e);
-      r += p;
-      w = __builtin_fmaf(p, d, w);
+      const float t = (x[e] - ref) * kLog2e;
+      p[e] = fast_exp2(t);
+      u = __builtin_fmaf(p[e], fmaxf(t, kFar), u);  // in units of ln 2; 0 times the far ones is 0
     }
+    r += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    w += u;
   };
   // token e of a load of tokens i0 .. i0 + 7
   auto widen = [&](const uint32_t* raw, const u32x2& mask, float (&x)[kVec]) __attribute__((always_inline)) {
@@ -146,9 +185,9 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
       if (mask[e >> 2] >> (8 * (e & 3)) & 0xffu) x[e] = -INFINITY;
     }
   };
+  uint32_t raw[kBatch][kWords];
+  u32x2 mask[kBatch];
   for (int c0 = c_begin + tid; c0 < c_end; c0 += kBatch * kThreads) {
-    uint32_t raw[kBatch][kWords];
-    u32x2 mask[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const int c = c0 + u * kThreads;
@@ -178,77 +217,127 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
     tail_token(x, n_vec * kVec + tid);
     take(x, n_vec * kVec + tid);
   }
-  const bool bad = !(r < INFINITY) || !(m < INFINITY);  // NaN among the tokens, or +inf
+  if (!(m < INFINITY)) r = __builtin_nanf("");  // +inf among the tokens
 
-  // ---- sums over the workgroup ----
-  Sum s{(double)r, (double)w, m};
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) join(s, __shfl_xor(s.m, o), __shfl_xor(s.r, o), __shfl_xor(s.w, o));
-  if (__any(bad)) s.r = __builtin_nan("");
-  if (lane == 0) {
-    sm_r[wave] = s.r;
-    sm_w[wave] = s.w;
-    sm_m[wave] = s.m;
+  // ---- sums over the wavefront, then the workgroup (in the first wavefront) ----
+  const uint64_t mine = key_of(m, at);
+  const int groups = top <= 8 ? 16 : 64, lanes = kThreads / groups;  // of threads, for the bound of the alternatives
+  if (tid == 0) sm_n = sm_listed = 0;
+  {
+    uint64_t k = mine, wave_key;
+    for (int o = 1; o < lanes; o <<= 1) {
+      const uint64_t other = __shfl_xor(k, o);
+      k = other > k ? other : k;
+    }
+    if (tid % lanes == 0) sm_group[tid / lanes] = k;
+    float wr = r, ww = w * 0.69314718055994531f;
+    join<64>(mine, wr, ww, wave_key);
+    if (lane == 0) {
+      sm_wave[wave] = wave_key;
+      sm_r[wave] = wr;
+      sm_w[wave] = ww;
+    }
   }
-  if (tid == 0) sm_n = sm_owners = 0;
+  __syncthreads();
+  double sr = 0., sw = 0.;
+  uint64_t best = 0;
+  if (wave == 0) {
+    if (lane < kWaves) {
+      sr = sm_r[lane];
+      sw = sm_w[lane];
+    }
+    join<kWaves>(lane < kWaves ? sm_wave[lane] : 0, sr, sw, best);
+  }
 
   // ---- alternatives ----
   if (top) {
-    const uint64_t mine = key_of(m, at);
-    int rank = 0;  // among the wavefront's keys
-    for (int i = 0; i < 64; ++i) rank += __shfl(mine, i) > mine;
-    if (lane < top) sm_wave[wave * top + lane] = 0;
-    __builtin_amdgcn_wave_barrier();
-    if (mine && rank < top) sm_wave[wave * top + rank] = mine;
-    __syncthreads();
-    largest(sm_wave, kWaves * top, top, sm_top);
-    const uint64_t least = max(sm_top[top - 1], (uint64_t)1);
-    if (mine >= least) sm_owner[atomicAdd(&sm_owners, 1)] = tid;  // at most `top` of them
-    __syncthreads();
-    const int per = (c_end - c_begin + kThreads - 1) / kThreads + 1;  // an owner's loads, and its tail token
-    for (int i = tid; i < sm_owners * per; i += kThreads) {
-      const int t = sm_owner[i / per], j = i % per, c = c_begin + t + j * kThreads;
-      float x[kVec];
-      int i0;
-      if (j == per - 1) {
-        if (t >= tail) continue;
-        i0 = n_vec * kVec + t;
-        tail_token(x, i0);
-      } else {
-        if (c >= c_end) continue;
-        uint32_t raw[kWords];
-        u32x2 mask = {0, 0};
-        __builtin_memcpy(raw, lr + (int64_t)c * kVec * EB, sizeof(raw));
-        if (bm) __builtin_memcpy(&mask, bm + (int64_t)c * kVec, 8);
-        widen(raw, mask, x);
-        i0 = c * kVec;
-      }
+    auto list = [&](const float (&x)[kVec], int first, uint64_t least) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        const uint64_t key = key_of(x[e], i0 + e);
+        const uint64_t key = key_of(x[e], first + e);
         if (key >= least) sm_keys[atomicAdd(&sm_n, 1)] = key;
       }
+    };
+    const uint64_t gk = sm_group[lane & (groups - 1)];
+    uint64_t least = nth_key(gk, key_rank(gk, groups), groups, top);
+    if (c_end - c_begin <= kThreads) {  // every token is still here
+      float x[kVec];
+      if (c_begin + tid < c_end) {
+        widen(raw[0], mask[0], x);
+        list(x, (c_begin + tid) * kVec, least);
+      }
+      if (tid < tail) {
+        tail_token(x, n_vec * kVec + tid);
+        list(x, n_vec * kVec + tid, least);
+      }
+      __syncthreads();
+    } else {
+      if (mine >= least) {
+        const int i = atomicAdd(&sm_listed, 1);
+        if (i < 64) sm_list[i] = mine;
+      }
+      __syncthreads();
+      const int listed = sm_listed;
+      if (listed > 64) {
+        __syncthreads();
+        const int rank = key_rank(mine, 64);
+        if (lane < top) sm_list[wave * top + lane] = 0;
+        __builtin_amdgcn_wave_barrier();
+        if (mine && rank < top) sm_list[wave * top + rank] = mine;
+        __syncthreads();
+        largest(sm_list, kWaves * top, top, sm_top);
+      }
+      const int n = listed > 64 ? top : listed;  // different keys, some of them 0
+      const uint64_t k = lane < n ? (listed > 64 ? sm_top[lane] : sm_list[lane]) : 0;
+      least = nth_key(k, key_rank(k, n), n, top);
+      const uint64_t own = __ballot(k != 0 && k >= least);  // lanes whose key's thread is read again: `top` at most
+      // thread t's loads are c_begin + t, + kThreads, .., and the tail token n_vec * kVec + t
+      const int owners = __popcll(own), per = (c_end - c_begin + kThreads - 1) / kThreads + 1;
+      for (int i0 = 0; i0 < owners * per; i0 += kThreads) {
+        const int i = i0 + tid, j = i % per;
+        int src = 0;
+        uint64_t left = own;
+        for (int o = min(i / per, owners - 1); o > 0; --o) left &= left - 1;
+        src = __ffsll((unsigned long long)left) - 1;
+        const int index = (int)~(uint32_t)__shfl(k, src);  // of its largest token
+        const int t = index >= n_vec * kVec ? index - n_vec * kVec : (index / kVec - c_begin) % kThreads, c = c_begin + t + j * kThreads;
+        float x[kVec];
+        if (i < owners * per && j == per - 1 && t < tail) {
+          tail_token(x, n_vec * kVec + t);
+          list(x, n_vec * kVec + t, least);
+        } else if (i < owners * per && j < per - 1 && c < c_end) {
+          uint32_t again[kWords];
+          u32x2 m8 = {0, 0};
+          __builtin_memcpy(again, lr + (int64_t)c * kVec * EB, sizeof(again));
+          if (bm) __builtin_memcpy(&m8, bm + (int64_t)c * kVec, 8);
+          widen(again, m8, x);
+          list(x, c * kVec, least);
+        }
+        __syncthreads();
+        if (i0 + kThreads < owners * per) {  // room for the next round: the first `top` so far
+          largest(sm_keys, sm_n, top, sm_top);
+          if (tid < top) sm_keys[tid] = sm_top[tid];
+          if (tid == 0) sm_n = top;
+          __syncthreads();
+        }
+      }
+      if (owners == 0) __syncthreads();
     }
-    __syncthreads();
-    largest(sm_keys, sm_n, top, sm_top);
-  } else {
-    __syncthreads();
-  }
-  if (wave == 0) {  // every lane the same
-    s = Sum{sm_r[0], sm_w[0], sm_m[0]};
-    for (int i = 1; i < kWaves; ++i) join(s, sm_m[i], sm_r[i], sm_w[i]);
+    sort_top(sm_keys, sm_n, top, sm_top);
   }
 
   if (a.splits > 1) {
     // every split publishes its sums and keys at the device's coherence point; the last to arrive joins them
     Partial* const parts = reinterpret_cast<Partial*>(static_cast<char*>(a.ws) + kCounters * 4) + (int64_t)row * a.splits;
     int* const count = static_cast<int*>(a.ws) + row;
-    if (tid == 0) {
-      __hip_atomic_store(&parts[split].r, s.r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(&parts[split].w, s.w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(&parts[split].m, (uint64_t)__float_as_uint(s.m), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (wave == 0) {
+      if (lane == 0) {
+        __hip_atomic_store(&parts[split].r, sr, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&parts[split].w, sw, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&parts[split].top, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      if (lane < top) __hip_atomic_store(&parts[split].key[lane], sm_top[lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    if (tid < top) __hip_atomic_store(&parts[split].key[tid], sm_top[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0);
     asm volatile("" ::: "memory");
@@ -258,53 +347,64 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
     if (!sm_last) return;
     if (tid == 0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
     if (wave == 0) {
-      s = Sum{0., 0., -INFINITY};
+      uint64_t key = 0;
+      sr = sw = 0.;
       if (lane < a.splits) {
-        s.r = __hip_atomic_load(&parts[lane].r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s.w = __hip_atomic_load(&parts[lane].w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s.m = __uint_as_float((uint32_t)__hip_atomic_load(&parts[lane].m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        sr = __hip_atomic_load(&parts[lane].r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sw = __hip_atomic_load(&parts[lane].w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        key = __hip_atomic_load(&parts[lane].top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
-      const bool nan = __any(!(s.r < INFINITY));
-#pragma unroll
-      for (int o = kMaxSplits / 2; o >= 1; o >>= 1) join(s, __shfl_xor(s.m, o), __shfl_xor(s.r, o), __shfl_xor(s.w, o));
-      s = Sum{__shfl(s.r, 0), __shfl(s.w, 0), __shfl(s.m, 0)};  // for the lanes behind the splits too
-      if (nan) s.r = __builtin_nan("");
+      join<kMaxSplits>(key, sr, sw, best);
     }
     if (top) {
-      for (int i = tid; i < a.splits * top; i += kThreads)
+      const int n = a.splits * top;
+      for (int i = tid; i < n; i += kThreads)
         sm_keys[i] = __hip_atomic_load(&parts[i / top].key[i % top], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (tid == 0) sm_n = 0;
       __syncthreads();
-      largest(sm_keys, a.splits * top, top, sm_top);
+      if (n <= 64) {
+        sort_top(sm_keys, n, top, sm_top);
+      } else {
+        // the splits' keys are sorted: the first few of each bound the `top`-th of all
+        const int first = a.splits * ((top + a.splits - 1) / a.splits);  // 64 at most
+        const uint64_t k = lane < first ? sm_keys[lane % a.splits * top + lane / a.splits] : 0;
+        const uint64_t least = nth_key(k, key_rank(k, first), first, top);
+        for (int i = tid; i < n; i += kThreads)
+          if (sm_keys[i] >= least) sm_keys[kMaxSplits * kMaxTop + atomicAdd(&sm_n, 1)] = sm_keys[i];
+        __syncthreads();
+        sort_top(sm_keys + kMaxSplits * kMaxTop, sm_n, top, sm_top);
+      }
     }
   }
   // ---- results, by the first wavefront ----
   if (wave != 0) return;
-  const bool nan = !(s.r < INFINITY), none = !nan && s.m == -INFINITY;
+  sr = __shfl(sr, 0);
+  best = __shfl(best, 0);
+  const float m_row = key_value(best);
+  const bool nan = !(sr < INFINITY), none = !nan && best == 0;
   const float fnan = __builtin_nanf("");
-  const double lz = nan || none ? 0. : log1p(s.r);
+  const double lz = nan || none ? 0. : log1p(sr);
   if (lane == 0) {
-    a.entropy[row] = nan ? fnan : none ? 0.f : (float)(lz - s.w / (1. + s.r));
+    a.entropy[row] = nan ? fnan : none ? 0.f : (float)(lz - sw / (1. + sr));
     const int64_t t = a.tokens[row];
     float lp = fnan;  // a token out of range
     if (!nan && t >= 0 && t < a.V) {
       const float x = bm && bm[t] ? -INFINITY : Elem<T>::load1(lr, (int)t);
-      lp = none || x == -INFINITY ? -INFINITY : (float)((double)x - s.m - lz);
+      lp = none || x == -INFINITY ? -INFINITY : (float)((double)x - m_row - lz);
     }
     a.logprob[row] = lp;
   }
   if (lane < top) {
     const uint64_t key = sm_top[lane];
     a.top_id[(int64_t)row * top + lane] = nan || !key ? -1 : (int64_t)(uint32_t)~(uint32_t)key;
-    a.top_logprob[(int64_t)row * top + lane] =
-        nan ? fnan : !key ? -INFINITY : (float)((double)unorder((uint32_t)(key >> 32)) - s.m - lz);
+    a.top_logprob[(int64_t)row * top + lane] = nan ? fnan : !key ? -INFINITY : (float)((double)key_value(key) - m_row - lz);
   }
 }
 
+// Workgroups a row.
 int plan_splits(int64_t rows, int64_t V) {
-  const int64_t least = (V + kPerSplit - 1) / kPerSplit;
-  int64_t want = 1;
-  if (rows <= 64) want = std::min<int64_t>(V / (kVec * kThreads), 512 / rows);
-  return (int)std::min<int64_t>(std::max<int64_t>(std::max<int64_t>(want, 1), least), kMaxSplits);
+  const int64_t one = (V / kVec + kThreads - 1) / kThreads;  // of one load a thread
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(one, 1024 / rows), kMaxSplits));
 }
 
 }  // namespace
@@ -312,30 +412,15 @@ int plan_splits(int64_t rows, int64_t V) {
 size_t logprobs_workspace_bytes(int64_t rows, int64_t V, int64_t top) {
   (void)top;
   const int s = plan_splits(rows, V);
-  return s == 1 ? 0 : kCounters * 4 + (size_t)std::min<int64_t>(rows, kCounters) * s * sizeof(Partial);
+  return s == 1 ? 0 : kCounters * 4 + (size_t)rows * s * sizeof(Partial);
 }
 
 hipError_t launch_token_logprobs(int dtype, LogprobArgs a, hipStream_t stream) {
-  const int64_t rows = a.rows, most = plan_splits(rows, a.V) > 1 ? kCounters : rows;
-  const int eb = dtype == 0 ? 4 : 2;
-  a.splits = plan_splits(rows, a.V);
-  for (int64_t r0 = 0; r0 < rows; r0 += most) {
-    LogprobArgs b = a;
-    b.rows = (int)std::min(most, rows - r0);
-    b.logits = static_cast<const char*>(a.logits) + r0 * a.l_stride * eb;
-    if (a.blocked) b.blocked = a.blocked + r0 * a.m_stride;
-    b.tokens = a.tokens + r0;
-    b.logprob = a.logprob + r0;
-    b.entropy = a.entropy + r0;
-    if (a.top) {
-      b.top_logprob = a.top_logprob + r0 * a.top;
-      b.top_id = a.top_id + r0 * a.top;
-    }
-    const dim3 grid((unsigned)b.rows, (unsigned)b.splits);
-    if (dtype == 2) hipLaunchKernelGGL((token_logprobs_kernel<Bf16>), grid, dim3(kThreads), 0, stream, b);
-    else if (dtype == 1) hipLaunchKernelGGL((token_logprobs_kernel<F16>), grid, dim3(kThreads), 0, stream, b);
-    else hipLaunchKernelGGL((token_logprobs_kernel<F32>), grid, dim3(kThreads), 0, stream, b);
-  }
+  a.splits = plan_splits(a.rows, a.V);
+  const dim3 grid((unsigned)a.rows, (unsigned)a.splits);
+  if (dtype == 2) hipLaunchKernelGGL((token_logprobs_kernel<Bf16>), grid, dim3(kThreads), 0, stream, a);
+  else if (dtype == 1) hipLaunchKernelGGL((token_logprobs_kernel<F16>), grid, dim3(kThreads), 0, stream, a);
+  else hipLaunchKernelGGL((token_logprobs_kernel<F32>), grid, dim3(kThreads), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -151,18 +151,19 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     if index != _current_device():  # launches go to the current device
         with torch.cuda.device(index):
             return token_logprobs(logits, tokens, top, blocked)
-    values = torch.empty(2, *shape, dtype=torch.float32, device=device)
+    logprobs = torch.empty(*shape, dtype=torch.float32, device=device) if shape else torch.empty((), dtype=torch.float32, device=device)
+    entropy = torch.empty_like(logprobs)
     top_logprobs = torch.empty(*shape, max(top, 0), dtype=torch.float32, device=device)
     top_ids = torch.empty(*shape, max(top, 0), dtype=torch.int64, device=device)
     lib, nbytes = _lib.load(), _logprobs_workspace_size(rows, V, max(top, 0))
     workspace = _counted_workspace(device, nbytes) if nbytes else None
     rc = lib.wdrz_token_logprobs(
-        dt, x.data_ptr(), x.stride(0), mask, m_stride, tokens.data_ptr(), values.data_ptr(), values.data_ptr() + 4 * rows,
+        dt, x.data_ptr(), x.stride(0), mask, m_stride, tokens.data_ptr(), logprobs.data_ptr(), entropy.data_ptr(),
         top_logprobs.data_ptr(), top_ids.data_ptr(), rows, V, top, None if workspace is None else workspace.data_ptr(),
         0 if workspace is None else workspace.numel(), _raw_stream(index))
     if rc != _lib.WDRZ_OK:
         _raise(rc, "token_logprobs")
-    return TokenLogprobs(values[0], values[1], top_logprobs, top_ids)
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], gelu: bool = False) -> torch.Tensor:
