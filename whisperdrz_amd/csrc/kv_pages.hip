@@ -41,7 +41,7 @@ template <> struct Pg<Bf16> {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
   static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
   static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
-  static constexpr uint32_t kExp = 0x7f80u, kNan = 0x7fc07fc0u;
+  static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u, kNan = 0x7fc07fc0u;
 };
 template <> struct Pg<F16> {
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -50,7 +50,7 @@ template <> struct Pg<F16> {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
   static __device__ __forceinline__ float lo(uint32_t w) { return f16_lo(w); }
   static __device__ __forceinline__ float hi(uint32_t w) { return f16_hi(w); }
-  static constexpr uint32_t kExp = 0x7c00u, kNan = 0x7e007e00u;
+  static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u, kNan = 0x7e007e00u;
 };
 
 // Maximum and sum over the lanes li, li + 16, li + 32, li + 48 (every lane gets it).
@@ -68,7 +68,7 @@ template <> struct VRow<64> { typedef u32x2 type; };
 template <> struct VRow<128> { typedef u32x4 type; };
 
 template <typename T, int D, int kWaves>
-__global__ __launch_bounds__(64 * kWaves) void pages_attn_kernel(PagesArgs a) {
+__global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void pages_attn_kernel(PagesArgs a) {
   constexpr int KS = D / 32, NJ = D / 16, kThreads = 64 * kWaves, kRow = D * 2;
   typedef typename VRow<D>::type vrow_t;
   extern __shared__ __attribute__((aligned(16))) float sm_o[];  // [kWaves][rows of the launch][D]
@@ -145,57 +145,72 @@ __global__ __launch_bounds__(64 * kWaves) void pages_attn_kernel(PagesArgs a) {
     u32x4 k[2][KS];
     vrow_t v[2][4];
   };
-  // Pages of the two tiles of block kb (0 for one that is out of range or behind the keys).
-  auto pages_of = [&](int kb, int (&pg)[2]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int pos = kb * kBlock + 16 * t;
-      pg[t] = pos < lim_hi ? table[pos >> a.shift] : 0;
+  // Blocks of this wavefront: kb0, kb0 + kWaves, ..; the first n_whole hold cached rows alone, which every row of the tile
+  // sees. Lane l holds the page of tile l % 2 of the (l / 2)-th of them from a multiple of 32 on (0 for one behind the
+  // keys): the loads of keys wait for no table entry.
+  const int kb_end = (k1 + kBlock - 1) / kBlock, kb0 = k0 / kBlock + wave;
+  const int n_blocks = kb0 < kb_end ? (kb_end - kb0 + kWaves - 1) / kWaves : 0;
+  const int whole_end = min(n, k1) / kBlock, n_whole = kb0 < whole_end ? (whole_end - kb0 + kWaves - 1) / kWaves : 0;
+  int ids = 0, ids_at = -1;
+  auto places = [&](int i, const char* (&kp)[2], const char* (&vp)[2]) __attribute__((always_inline)) {
+    if (i >> 5 != ids_at) {
+      ids_at = i >> 5;
+      const int pos = (kb0 + (ids_at * 32 + (lane >> 1)) * kWaves) * kBlock + 16 * (lane & 1);
+      ids = pos < min(lim_hi, kb_end * kBlock) ? table[pos >> a.shift] : 0;
     }
-  };
-  auto load = [&](int kb, int (&pg)[2], Block& x) __attribute__((always_inline)) {
-    const int base = kb * kBlock;
-    const char* kp[2];
-    const char* vp[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      int page = __builtin_amdgcn_readfirstlane(pg[t]);
+      int page = __builtin_amdgcn_readlane(ids, (i & 31) * 2 + t);
       if (page < 0 || page >= a.n_pages) {
         bad_page = true;
         page = 0;
       }
-      const int64_t at = ((((int64_t)page * a.Hk + hk) << a.shift) + ((base + 16 * t) & mask)) * kRow;
+      const int64_t at = ((((int64_t)page * a.Hk + hk) << a.shift) + (((kb0 + i * kWaves) * kBlock + 16 * t) & mask)) * kRow;
       kp[t] = a.k_pages + at;
       vp[t] = a.v_pages + at;
     }
-    if (base + kBlock <= min(n, lim_hi)) {
+  };
+  const uint32_t k_off = li * kRow + g * 16, v_off = 4 * g * kRow + li * (D / 8);
+  Block x;
+  const char* vp[2];  // of the block of the last load_keys
+  // Cached rows; behind them the call's own, then none (zeros: what stands there does not count).
+  auto load_keys = [&](int i) __attribute__((always_inline)) {
+    const char* kp[2];
+    places(i, kp, vp);
+    if (i < n_whole) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) x.k[t][s] = load16(kp[t] + li * kRow + g * 16 + s * 64);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x.v[t][r] = *reinterpret_cast<const vrow_t*>(vp[t] + (4 * g + r) * kRow + li * (D / 8));
+        for (int s = 0; s < KS; ++s) x.k[t][s] = load16(kp[t] + k_off + s * 64);
       return;
     }
-    // cached rows, then the call's own, then none (zeros: what stands there does not count)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int key = base + 16 * t + li;
-      const char* p = key < n ? kp[t] + li * kRow : knew + (int64_t)(key - n) * a.kns[1];
+      const int key = (kb0 + i * kWaves) * kBlock + 16 * t + li;
+      const char* p = (key < n ? kp[t] + li * kRow : knew + (int64_t)(key - n) * a.kns[1]) + g * 16;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x.k[t][s] = key < lim_hi ? load16(p + g * 16 + s * 64) : u32x4{0, 0, 0, 0};
+      for (int s = 0; s < KS; ++s) x.k[t][s] = u32x4{0, 0, 0, 0};
+      if (key < lim_hi)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x.k[t][s] = load16(p + s * 64);
+    }
+  };
+  auto load_values = [&](int i) __attribute__((always_inline)) {  // behind load_keys(i)
+    if (i < n_whole) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x.v[t][r] = *reinterpret_cast<const vrow_t*>(vp[t] + v_off + r * kRow);
+      return;
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int key = base + 16 * t + 4 * g + r;
-        const char* p = key < n ? vp[t] + (4 * g + r) * kRow : vnew + (int64_t)(key - n) * a.vns[1];
+        const int key = (kb0 + i * kWaves) * kBlock + 16 * t + 4 * g + r;
+        const char* p = (key < n ? vp[t] + (4 * g + r) * kRow : vnew + (int64_t)(key - n) * a.vns[1]) + li * (D / 8);
         x.v[t][r] = vrow_t{};
-        if (key < lim_hi) x.v[t][r] = *reinterpret_cast<const vrow_t*>(p + li * (D / 8));
+        if (key < lim_hi) x.v[t][r] = *reinterpret_cast<const vrow_t*>(p);
       }
   };
 
@@ -203,26 +218,31 @@ __global__ __launch_bounds__(64 * kWaves) void pages_attn_kernel(PagesArgs a) {
 #pragma unroll
   for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, mu = 0.f, l = 0.f;  // reference, the same or 0 while there is none, this lane's sum
+  auto values = [&](int j, uint32_t low, uint32_t high) __attribute__((always_inline)) {  // dims j, j + NJ, .. of V^T
+    u32x4 vt;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        vt[2 * t + i] = __builtin_amdgcn_perm(x.v[t][2 * i + 1][j / 2], x.v[t][2 * i][j / 2], j & 1 ? high : low);
+    return vt;
+  };
+  constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;  // the low, the high halves of two words
 
-  auto compute = [&](int kb, int (&pg)[2], Block& x) __attribute__((always_inline)) {
-    const int base = kb * kBlock;
+  // The keys of the next block are requested when this one's have been used, its values when this one's have been.
+  auto compute = [&](int i) __attribute__((always_inline)) {
+    const bool mixed = (kb0 + i * kWaves + 1) * kBlock > lim_lo;  // some rows do not see some keys of the block
+    const int sees = lim - (kb0 + i * kWaves) * kBlock - 4 * g;   // key 16 t + r of this lane's: where below
     float p[2][4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < KS; ++i) s = Pg<T>::mfma(x.k[t][i], q[i], s);
+      for (int e = 0; e < KS; ++e) s = Pg<T>::mfma(x.k[t][e], q[e], s);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) p[t][r] = s[r] * a.c;
+      for (int r = 0; r < 4; ++r) p[t][r] = 16 * t + r >= sees ? -INFINITY : s[r] * a.c;
     }
-    const bool mixed = base + kBlock > lim_lo;
-    if (mixed) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (base + 16 * t + 4 * g + r >= lim) p[t][r] = -INFINITY;
-    }
+    if (i + 1 < n_blocks) load_keys(i + 1);
     const float mx = quarters_max(fmaxf(fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[0][2], p[0][3])),
                                         fmaxf(fmaxf(p[1][0], p[1][1]), fmaxf(p[1][2], p[1][3]))));
     if (__any(mx > m + kMove)) {
@@ -238,81 +258,77 @@ __global__ __launch_bounds__(64 * kWaves) void pages_attn_kernel(PagesArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float& p0 = p[t][2 * i];
-        float& p1 = p[t][2 * i + 1];
-        p0 = fast_exp2(p0 - mu);
-        p1 = fast_exp2(p1 - mu);
+      for (int e = 0; e < 2; ++e) {
+        const float p0 = fast_exp2(p[t][2 * e] - mu), p1 = fast_exp2(p[t][2 * e + 1] - mu);
         l += p0 + p1;
         const uint32_t w = Pg<T>::pack(p0, p1);
-        hi[2 * t + i] = w;
-        lo[2 * t + i] = Pg<T>::pack(p0 - Pg<T>::lo(w), p1 - Pg<T>::hi(w));
+        hi[2 * t + e] = w;
+        lo[2 * t + e] = Pg<T>::pack(p0 - Pg<T>::lo(w), p1 - Pg<T>::hi(w));
       }
+    bool odd = false;
     if (mixed && has_new && a.sq > 1) {
-      // A row of the tile may not see all keys of the block: 0 times an infinity or NaN behind its mask would
-      // count in the products, so such blocks are summed key by key.
-      bool odd = false;
+      // 0 times an infinity or NaN that a row does not see would count in the products: such values are taken out
+      // of V, and given to the rows that see them. 0 times each value first: 0, or NaN where there is such a one.
+      uint32_t low = kLow, high = kHigh;
+      asm("" : "+s"(low), "+s"(high));  // made anew below: kept from here they would take the loop's registers
+      f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) zero = Pg<T>::mfma(values(j, low, high), u32x4{0, 0, 0, 0}, zero);
+      const float any = (zero[0] + zero[1]) + (zero[2] + zero[3]);
+      odd = __any(any != any);
+    }
+    if (odd) {
+      u32x4 seen;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int e = 0; e < 2; ++e) seen[2 * t + e] = Pg<T>::pack(16 * t + 2 * e < sees ? 1.f : 0.f, 16 * t + 2 * e + 1 < sees ? 1.f : 0.f);
 #pragma unroll
-          for (int w = 0; w < D / 32; ++w) {
-            const uint32_t e = x.v[t][r][w];
-            odd = odd || (e & Pg<T>::kExp) == Pg<T>::kExp || ((e >> 16) & Pg<T>::kExp) == Pg<T>::kExp;
+      for (int j = 0; j < NJ; ++j) {
+        u32x4 vt = values(j, kLow, kHigh);
+#pragma unroll 1
+        for (int kind = 0; kind < 3; ++kind) {  // inf, -inf, NaN, as ones
+          u32x4 ones;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t u = vt[e] >> (16 * half) & 0xffffu;
+              const bool is = kind == 2 ? (u & 0x7fffu) > Pg<T>::kExp : u == (Pg<T>::kExp | (kind ? 0x8000u : 0u));
+              w |= is ? Pg<T>::kOne << (16 * half) : 0u;
+            }
+            ones[e] = w;
           }
-      if (__any(odd)) {
+          const f32x4 count = Pg<T>::mfma(ones, seen, f32x4{0.f, 0.f, 0.f, 0.f});
+          const float value = kind == 2 ? __builtin_nanf("") : kind ? -INFINITY : INFINITY;
 #pragma unroll
-        for (int kk = 0; kk < kBlock; ++kk) {
-          const float pk = __shfl(p[kk >> 4][kk & 3], li + 16 * ((kk >> 2) & 3));
-          const int key = base + kk;
-          if (key >= lim) continue;
-          const int page = pg[kk >> 4];
-          const char* row = key < n ? a.v_pages + ((((int64_t)(page < 0 || page >= a.n_pages ? 0 : page) * a.Hk + hk) << a.shift) + (key & mask)) * kRow
-                                    : vnew + (int64_t)(key - n) * a.vns[1];
-          const uint16_t* v = reinterpret_cast<const uint16_t*>(row) + (D / 4) * g;
-#pragma unroll
-          for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[j][r] = __builtin_fmaf(pk, Pg<T>::lo(v[NJ * r + j]), acc[j][r]);
+          for (int r = 0; r < 4; ++r) acc[j][r] += count[r] > 0.f ? value : 0.f;
         }
-        return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((vt[e] & Pg<T>::kExp) == Pg<T>::kExp) vt[e] &= 0xffff0000u;
+          if ((vt[e] >> 16 & Pg<T>::kExp) == Pg<T>::kExp) vt[e] &= 0xffffu;
+        }
+        acc[j] = Pg<T>::mfma(vt, hi, acc[j]);
+        acc[j] = Pg<T>::mfma(vt, lo, acc[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const u32x4 vt = values(j, kLow, kHigh);
+        acc[j] = Pg<T>::mfma(vt, hi, acc[j]);
+        acc[j] = Pg<T>::mfma(vt, lo, acc[j]);
       }
     }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      u32x4 vt;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          vt[2 * t + i] = __builtin_amdgcn_perm(x.v[t][2 * i + 1][j / 2], x.v[t][2 * i][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
-      acc[j] = Pg<T>::mfma(vt, hi, acc[j]);
-      acc[j] = Pg<T>::mfma(vt, lo, acc[j]);
-    }
+    if (i + 1 < n_blocks) load_values(i + 1);
   };
 
-  // blocks of this wavefront: kb0, kb0 + kWaves, ..; the next one's loads and the one after's pages are in flight
-  const int kb_end = (k1 + kBlock - 1) / kBlock;
-  int kb = k0 / kBlock + wave;
-  if (kb < kb_end) {
-    Block cur, nxt;
-    int pg[2], pg1[2], pg2[2];
-    pages_of(kb, pg);
-    pages_of(kb + kWaves, pg1);
-    load(kb, pg, cur);
-    for (; kb < kb_end; kb += kWaves) {
-      pages_of(kb + 2 * kWaves, pg2);
-      if (kb + kWaves < kb_end) load(kb + kWaves, pg1, nxt);
-      compute(kb, pg, cur);
-      cur = nxt;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        pg[t] = pg1[t];
-        pg1[t] = pg2[t];
-      }
-    }
+  if (n_blocks) {
+    load_keys(0);
+    load_values(0);
   }
+  for (int i = 0; i < n_blocks; ++i) compute(i);
   l = quarters_sum(l);
 
   // ---- the wavefronts' sums ----
