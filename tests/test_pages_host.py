@@ -106,7 +106,7 @@ def test_the_workspace_covers_the_plan(lib):
             for L in (1, 448, 1024, 1025, 4096, 32768, 1 << 20):
                 n = lib.wdrz_attn_kvpages_workspace_size(B, sq, H, Hk, D, L)
                 assert n == 0 or n > 16384 and n % 4 == 0
-                assert L > 1024 or n == 0
+                assert L > 512 or n == 0  # such rows are not split
                 last = max(last, n)
             assert last < 1 << 31
     assert lib.wdrz_attn_kvpages_workspace_size(0, 1, 4, 4, 64, 100) == 0

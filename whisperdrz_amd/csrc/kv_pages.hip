@@ -113,9 +113,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void pages_attn_kerne
   // keys that some row of the tile sees, and this split's part of them
   const int lim_hi = has_new ? n + (r0 + rows - 1) / a.G + 1 : n;
   const int lim_lo = has_new ? n + r0 / a.G + 1 : n;
-  const int n_split_b = max(1, (lim_hi + a.chunk - 1) / a.chunk);
+  const int parts = a.n_splits == 1 ? 1 : min(a.n_splits, max(1, (lim_hi + a.min_chunk - 1) / a.min_chunk));
+  const int chunk = ((lim_hi + parts - 1) / parts + kBlock - 1) / kBlock * kBlock;  // whole blocks: there may be fewer parts
+  const int n_split_b = max(1, (lim_hi + chunk - 1) / max(chunk, 1));
   if (split >= n_split_b) return;
-  const int k0 = split * a.chunk, k1 = min(lim_hi, k0 + a.chunk);
+  const int k0 = split * chunk, k1 = min(lim_hi, k0 + chunk);
   if (tid == 0) sm_bad = 0;
 
   // the new rows to their pages; every workgroup takes them from the call's own rows
@@ -443,26 +445,38 @@ void launch_w(const PagesArgs& a, hipStream_t stream) {
 }
 template <typename T, int D>
 void launch_d(const PagesArgs& a, hipStream_t stream) {
-  if (a.waves == 8) launch_w<T, D, 8>(a, stream);
+  if constexpr (D == 64)
+    if (a.waves == 8) return launch_w<T, D, 8>(a, stream);
+  if (a.waves == 2) launch_w<T, D, 2>(a, stream);
   else launch_w<T, D, 4>(a, stream);
 }
 
 }  // namespace
 
+// How many workgroups a row's keys are cut into (n_splits at most, each of min_chunk keys or more, even parts of the
+// row's own length) and the wavefronts of one. Joining costs about 2 us; a workgroup walks 1000 keys in 5 us. So rows are
+// cut until there is one workgroup a CU, and further only to hold the time of a long row among short ones. One token, bf16,
+// cold caches in a graph, us, unsplit / parts of 1024, 512, 256 keys:
+//   20 heads of 64: 1 stream of 447 positions 8.7 / - / - / 8.9 (two parts), 1000 12.8 / - / 11.2 / 9.4, 2000 20.8 / 15.1 /
+//   11.5 / 10.2; 8 of 4000 48.8 / 38.3 / 38.1 / 41.5 (two parts 37.9); 32 of 4000 124 / 121 / 124 / 131;
+//   32/8 heads of 128: 1 of 32000 390 / 34.3 / 39.7 / -; 4 of 32000 412 / 102 / 112 / - (eight parts 95); 16 of 2000 34.3 /
+//   29.9 / 29.7 / 33.3; 32 of 2000 49.8 / 52.5 / 55.2 / 61.0.
+// Wavefronts, us of 2 / 4 / 8: 160 workgroups 12.8 / 10.3 / 9.5, 260 12.3 / 11.1 / 13.6, 520 14.6 / 14.5 / 20.2, 800 17.6 /
+// 20.7 / 27.1, 1280 31.2 / 34.2 / 43.0.
+constexpr int64_t kCus = 256;
 void pages_plan(int64_t B, int64_t sq, int64_t H, int64_t Hk, int64_t D, int64_t max_len, PagesArgs* a) {
   a->G = (int)(H / Hk);
   a->n_rt = (int)((sq * a->G + kRows - 1) / kRows);
   const int64_t units = B * Hk * a->n_rt;
-  int64_t chunk = (max_len + kBlock - 1) / kBlock * kBlock;
-  if (max_len > 1024 && units <= kPagesCounters) {
-    const int64_t want = std::max<int64_t>(1, 1024 / units);
-    chunk = std::min<int64_t>((max_len + want - 1) / want, 4096);
-    chunk = std::max<int64_t>(std::max<int64_t>(chunk, 512), (max_len + kPagesMaxSplits - 1) / kPagesMaxSplits);
-    chunk = (chunk + kBlock - 1) / kBlock * kBlock;
+  int64_t least = max_len, splits = 1;
+  if (units <= kPagesCounters && max_len > 512) {
+    least = units >= kCus ? std::max<int64_t>(4096, (max_len + kPagesMaxSplits - 1) / kPagesMaxSplits) : 256;
+    splits = (max_len + least - 1) / least;
+    if (units < kCus) splits = std::min<int64_t>(std::min<int64_t>(splits, (kCus + units - 1) / units), kPagesMaxSplits / 2);
   }
-  a->chunk = (int)std::max<int64_t>(chunk, kBlock);
-  a->n_splits = (int)std::max<int64_t>(1, (max_len + a->chunk - 1) / a->chunk);
-  a->waves = units * a->n_splits <= 256 && D == 64 ? 8 : 4;
+  a->n_splits = (int)splits;
+  a->min_chunk = (int)least;
+  a->waves = units * splits <= 160 && D == 64 ? 8 : units * splits < 768 ? 4 : 2;
 }
 
 size_t pages_workspace_bytes(int64_t B, int64_t sq, int64_t H, int64_t Hk, int64_t D, int64_t max_len) {

@@ -21,13 +21,14 @@
 namespace wdrz {
 namespace {
 
+constexpr int kSmallThreads = 256;  // threads of the workgroup, for up to as many requests and tokens; else
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanWaves = kPlanThreads / 64;
+constexpr int kLdsSums = 2048;  // requests whose sums the tokens' workgroups keep in LDS
 
 // Exclusive sums of two values over the workgroup's threads, and the totals. `sm` is free to use afterwards.
 // The first are capped at `cap` (sums of 2^30 and more would leave 32 bits).
-__device__ __forceinline__ void scan2(int& a, int& b, int cap, int& total_a, int& total_b, int64_t (&sm_a)[kPlanWaves],
-                                      int (&sm_b)[kPlanWaves]) {
+template <int kW>
+__device__ __forceinline__ void scan2(int& a, int& b, int cap, int& total_a, int& total_b, int64_t (&sm_a)[kW], int (&sm_b)[kW]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int64_t sa = a;
   int sb = b;
@@ -49,7 +50,7 @@ __device__ __forceinline__ void scan2(int& a, int& b, int cap, int& total_a, int
   int base_b = 0;
   total_b = 0;
 #pragma unroll
-  for (int w = 0; w < kPlanWaves; ++w) {
+  for (int w = 0; w < kW; ++w) {
     base_a += w < wave ? sm_a[w] : 0;
     base_b += w < wave ? sm_b[w] : 0;
     sum_a += sm_a[w];
@@ -66,9 +67,9 @@ constexpr int kMostPages = 1 << 30;  // sums of needed pages are held at it
 
 // The first request that names each stream, in claims[n_streams] (LDS); the others count as naming none.
 __device__ __forceinline__ void claim_streams(const PageArgs& a, int* claims) {
-  for (int s = threadIdx.x; s < a.n_streams; s += kPlanThreads) claims[s] = 0x7fffffff;
+  for (int s = threadIdx.x; s < a.n_streams; s += blockDim.x) claims[s] = 0x7fffffff;
   __syncthreads();
-  for (int i = threadIdx.x; i < a.B; i += kPlanThreads) {
+  for (int i = threadIdx.x; i < a.B; i += blockDim.x) {
     const int s = a.streams[i];
     if (s >= 0 && s < a.n_streams) atomicMin(claims + s, i);
   }
@@ -85,8 +86,8 @@ __device__ __forceinline__ bool request(const PageArgs& a, const int* claims, in
   return len >= 0 && len <= a.max_len && count >= 0 && count <= a.max_pages;
 }
 
-// Slots and positions of the call's tokens from the finished tables. cu: the B + 1 sums (LDS where they fit).
-__device__ __forceinline__ void emit_tokens(const PageArgs& a, const int* cu, int t) {
+// Slot and position of token t from the finished tables. cu: the B + 1 sums, starts: the positions before them.
+__device__ __forceinline__ void emit_token(const PageArgs& a, const int* cu, const int* starts, int t) {
   int64_t slot = -1, pos = 0;
   if (t < cu[a.B]) {
     int lo = 0, hi = a.B;  // the last request that begins at t or before
@@ -95,7 +96,7 @@ __device__ __forceinline__ void emit_tokens(const PageArgs& a, const int* cu, in
       if (cu[mid] <= t) lo = mid;
       else hi = mid;
     }
-    const int start = a.starts[lo];
+    const int start = starts[lo];
     if (start >= 0) {
       pos = (int64_t)start + t - cu[lo];
       const int s = a.streams ? a.streams[lo] : lo;
@@ -107,10 +108,11 @@ __device__ __forceinline__ void emit_tokens(const PageArgs& a, const int* cu, in
   a.positions[t] = pos;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PageArgs a) {
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void page_plan_kernel(PageArgs a) {
   extern __shared__ int sm_dyn[];
-  __shared__ int64_t sm_a[kPlanWaves];
-  __shared__ int sm_b[kPlanWaves], sm_taken;
+  __shared__ int64_t sm_a[kThreads / 64];
+  __shared__ int sm_b[kThreads / 64], sm_taken, sm_cu[kThreads + 1], sm_starts[kThreads];
   int* const claims = sm_dyn;
   const int tid = threadIdx.x;
   if (tid == 0) sm_taken = 0;
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PageArgs a) {
   if (a.streams) claim_streams(a, claims);
   else __syncthreads();
   int base_new = 0, base_need = 0, taken = 0;
-  for (int i0 = 0; i0 < a.B; i0 += kPlanThreads) {
+  for (int i0 = 0; i0 < a.B; i0 += kThreads) {
     const int i = i0 + tid;
     int s = 0, len = 0, count = 0, m = 0, need = 0;
     bool ok = false;
@@ -135,8 +137,8 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PageArgs a) {
     base_need = min(base_need + all_need, kMostPages);
     if (i < a.B) {
       ok = ok && (need == 0 || off + need <= top);
-      a.cu[i] = cu;
-      a.starts[i] = ok ? len : -1;
+      a.cu[i] = sm_cu[tid] = cu;
+      a.starts[i] = sm_starts[tid] = ok ? len : -1;
       if (ok) {
         int32_t* row = a.tables + (int64_t)s * a.max_pages + count;
         for (int j = 0; j < need; j += kPageBatch) {
@@ -157,24 +159,42 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PageArgs a) {
     }
   }
   if (taken) atomicMax(&sm_taken, taken);
-  if (tid == 0) a.cu[a.B] = base_new;
+  if (tid == 0) {
+    a.cu[a.B] = base_new;
+    if (a.B <= kThreads) sm_cu[a.B] = base_new;
+  }
   __syncthreads();  // this workgroup's writes are visible to it
   if (tid == 0 && sm_taken) *a.n_free = top - sm_taken;
   if (a.emit)
-    for (int t = tid; t < a.total; t += kPlanThreads) emit_tokens(a, a.cu, t);
+    for (int t = tid; t < a.total; t += kThreads) {
+      if (a.B <= kThreads) emit_token(a, sm_cu, sm_starts, t);
+      else emit_token(a, a.cu, a.starts, t);
+    }
 }
 
 __global__ __launch_bounds__(256) void page_slots_kernel(PageArgs a) {
+  __shared__ int sm_cu[kLdsSums + 1], sm_starts[kLdsSums];
   const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t < a.total) emit_tokens(a, a.cu, t);
+  if (a.B > kLdsSums) {
+    if (t < a.total) emit_token(a, a.cu, a.starts, t);
+    return;
+  }
+  for (int i = threadIdx.x; i < a.B; i += 256) {
+    sm_cu[i] = a.cu[i];
+    sm_starts[i] = a.starts[i];
+  }
+  if (threadIdx.x == 0) sm_cu[a.B] = a.cu[a.B];
+  __syncthreads();
+  if (t < a.total) emit_token(a, sm_cu, sm_starts, t);
 }
 
 // Streams set back to lens_new: the pages behind go back to the stack, in the order that gives the stack of
 // before where the plan took them in one call of the same requests.
-__global__ __launch_bounds__(kPlanThreads) void page_truncate_kernel(PageArgs a) {
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void page_truncate_kernel(PageArgs a) {
   extern __shared__ int sm_dyn[];
-  __shared__ int64_t sm_a[kPlanWaves];
-  __shared__ int sm_b[kPlanWaves];
+  __shared__ int64_t sm_a[kThreads / 64];
+  __shared__ int sm_b[kThreads / 64];
   int* const claims = sm_dyn;
   const int tid = threadIdx.x;
   const int top = min(max(*a.n_free, 0), a.n_pages);
@@ -189,15 +209,17 @@ __global__ __launch_bounds__(kPlanThreads) void page_truncate_kernel(PageArgs a)
     return max(0, count - keep);
   };
   int total = 0;
-  for (int pass = 0; pass < 2; ++pass) {
+  // the sum of all first, where one round of the scan does not hold them
+  for (int pass = a.B <= kThreads ? 1 : 0; pass < 2; ++pass) {
     int base = 0;
-    for (int i0 = 0; i0 < a.B; i0 += kPlanThreads) {
+    for (int i0 = 0; i0 < a.B; i0 += kThreads) {
       int s = 0, keep = 0;
       const int gone = gone_of(i0 + tid, s, keep);
       int unused = 0, off = max(gone, 0), none, all;
       scan2(unused, off, 0, none, all, sm_a, sm_b);
       off += base;
       base = min(base + all, kMostPages);
+      if (a.B <= kThreads) total = base;
       if (pass == 1 && gone >= 0) {
         int32_t* row = a.tables + (int64_t)s * a.max_pages + keep;
         for (int j = 0; j < gone; j += kPageBatch) {
@@ -247,14 +269,19 @@ __global__ __launch_bounds__(256) void page_write_kernel(PageWriteArgs a) {
 hipError_t launch_page_plan(PageArgs a, hipStream_t stream) {
   const size_t lds = a.streams ? (size_t)a.n_streams * 4 : 0;
   a.emit = a.total <= kPlanThreads;
-  hipLaunchKernelGGL(page_plan_kernel, dim3(1), dim3(kPlanThreads), lds, stream, a);
-  if (!a.emit) hipLaunchKernelGGL(page_slots_kernel, dim3((unsigned)((a.total + 255) / 256)), dim3(256), 0, stream, a);
+  if (a.B <= kSmallThreads && a.total <= kSmallThreads) {
+    hipLaunchKernelGGL((page_plan_kernel<kSmallThreads>), dim3(1), dim3(kSmallThreads), lds, stream, a);
+  } else {
+    hipLaunchKernelGGL((page_plan_kernel<kPlanThreads>), dim3(1), dim3(kPlanThreads), lds, stream, a);
+    if (!a.emit) hipLaunchKernelGGL(page_slots_kernel, dim3((unsigned)((a.total + 255) / 256)), dim3(256), 0, stream, a);
+  }
   return hipGetLastError();
 }
 
 hipError_t launch_page_truncate(const PageArgs& a, hipStream_t stream) {
   const size_t lds = a.streams ? (size_t)a.n_streams * 4 : 0;
-  hipLaunchKernelGGL(page_truncate_kernel, dim3(1), dim3(kPlanThreads), lds, stream, a);
+  if (a.B <= kSmallThreads) hipLaunchKernelGGL((page_truncate_kernel<kSmallThreads>), dim3(1), dim3(kSmallThreads), lds, stream, a);
+  else hipLaunchKernelGGL((page_truncate_kernel<kPlanThreads>), dim3(1), dim3(kPlanThreads), lds, stream, a);
   return hipGetLastError();
 }
 

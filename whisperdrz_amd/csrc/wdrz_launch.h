@@ -316,7 +316,7 @@ struct PagesArgs {
   float c;  // softmax scale * log2(e)
   int B, sq, H, Hk, G, n_streams, n_pages, max_pages, shift;
   int n_rt;             // row tiles of 16 (query, group head) rows a kv head
-  int n_splits, chunk;  // key splits at most, keys of one
+  int n_splits, min_chunk;  // parts that a row's keys are cut into at most, keys of one at least
   int waves;
   int* ws_count;
   float* ws_part;

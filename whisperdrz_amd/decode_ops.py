@@ -151,10 +151,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     if index != _current_device():  # launches go to the current device
         with torch.cuda.device(index):
             return token_logprobs(logits, tokens, top, blocked)
-    logprobs = torch.empty(*shape, dtype=torch.float32, device=device) if shape else torch.empty((), dtype=torch.float32, device=device)
+    logprobs = torch.empty(shape, dtype=torch.float32, device=device)
     entropy = torch.empty_like(logprobs)
-    top_logprobs = torch.empty(*shape, max(top, 0), dtype=torch.float32, device=device)
-    top_ids = torch.empty(*shape, max(top, 0), dtype=torch.int64, device=device)
+    top_logprobs = logprobs.new_empty(*shape, max(top, 0))
+    top_ids = tokens.new_empty(*shape, max(top, 0))
     lib, nbytes = _lib.load(), _logprobs_workspace_size(rows, V, max(top, 0))
     workspace = _counted_workspace(device, nbytes) if nbytes else None
     rc = lib.wdrz_token_logprobs(

@@ -80,6 +80,10 @@ class PageTables:
 
     def _requests(self, name: str, lens, streams: Optional[Tensor], B: Optional[int]):
         """The checked int32 ``lens`` (a tensor, or one number for all) and ``streams`` of a call, and its size."""
+        if (type(lens) is Tensor and type(streams) is Tensor and lens.dtype is streams.dtype is torch.int32 and lens.dim() == 1
+                and lens.shape == streams.shape and lens.is_contiguous() and streams.is_contiguous()
+                and lens.device == streams.device == self.device):
+            return lens, streams, lens.shape[0]
         if streams is not None:
             if not isinstance(streams, Tensor) or streams.dim() != 1:
                 raise ValueError("streams must be a tensor of whole numbers [B]")
@@ -116,12 +120,12 @@ class PageTables:
         if index != _current_device():  # launches go to the current device
             with torch.cuda.device(index):
                 return self.plan(lens, total, streams)
-        # four allocations: 4.7 us on the host, two with a view each 9.6
-        cu_seqlens = torch.empty(B + 1, dtype=torch.int32, device=self.device)
-        starts = torch.empty(B, dtype=torch.int32, device=self.device)
+        # four allocations: 4.5 us on the host, two with a view each 9.6
+        each = isinstance(lens, int)
+        cu_seqlens = self.n_free.new_empty(B + 1)
+        starts = self.n_free.new_empty(B) if each else torch.empty_like(lens)
         slots = torch.empty(total, dtype=torch.int64, device=self.device)
         positions = torch.empty_like(slots)
-        each = isinstance(lens, int)
         rc = _lib.load().wdrz_page_plan(
             self.struct, None if each else lens.data_ptr(), lens if each else 0, None if streams is None else streams.data_ptr(),
             cu_seqlens.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), B, total, _raw_stream(index))
