@@ -519,7 +519,7 @@ int wdrz_linear4_partials(int dtype, const void* x, int64_t x_stride, const void
  * tables[s][0 .. page_counts[s] - 1], position p in row p % page_size of page tables[s][p / page_size]; its
  * slot is that page * page_size + p % page_size. The pages that no stream holds are free_pages[0 .. *n_free - 1].
  * All device memory; page_size 16, 32, 64, 128 or 256; max_seq positions a stream at most, max_pages * page_size
- * or less; n_streams up to 15360.
+ * or less; n_streams up to 12288.
  */
 typedef struct wdrz_page_tables {
   int32_t* tables;      /* [n_streams, max_pages] */

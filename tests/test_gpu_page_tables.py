@@ -94,6 +94,20 @@ def test_large_numbers_stay_whole(cuda):
     assert plan.cu_seqlens.tolist() == [0, 10, 10, 10, 10] and plan.starts.tolist() == [-1, -1, 0, -1] and int(t.n_free) == 4
 
 
+def test_as_many_streams_as_there_may_be(cuda):
+    n = w.PageTables.MAX_STREAMS
+    t = w.PageTables(n, 3 * n, 16, 64, device=cuda)
+    order = torch.randperm(n, device=cuda).to(torch.int32)
+    new = (torch.arange(n, device=cuda) % 40).to(torch.int32)
+    plan = t.plan(new, int(new.sum()), order)
+    assert torch.equal(plan.starts, torch.zeros_like(new)) and torch.equal(t.seq_lens[order.long()], new)
+    held = (new + 15) // 16
+    assert torch.equal(t.page_counts[order.long()], held) and int(t.n_free) == 3 * n - int(held.sum())
+    assert plan.slots.unique().numel() == plan.slots.numel() and bool((plan.slots >= 0).all())
+    t.truncate(0, order)
+    assert torch.equal(t.free_pages, torch.arange(3 * n - 1, -1, -1, dtype=torch.int32, device=cuda))
+
+
 def test_ids_of_other_types_and_strides(cuda):
     t, ref = w.PageTables(8, 30, 16, 64, device=cuda), Tables(8, 30, 16, 64)
     streams = torch.tensor([5, 0, 3, 0, 1, 0], device=cuda)[::2]

@@ -43,7 +43,7 @@ BAD_TABLES = [
     (dict(tables=None), INVALID, "NULL"), (dict(n_free=None), INVALID, "NULL"), (dict(page_size=24), UNSUPPORTED, "page_size"),
     (dict(page_size=8), UNSUPPORTED, "page_size"), (dict(page_size=512), UNSUPPORTED, "page_size"),
     (dict(n_streams=0), INVALID, "sizes"), (dict(n_pages=0), INVALID, "sizes"), (dict(max_seq=449), INVALID, "sizes"),
-    (dict(n_streams=15361), UNSUPPORTED, "too large"), (dict(n_pages=(1 << 26) + 1), UNSUPPORTED, "too large"),
+    (dict(n_streams=12289), UNSUPPORTED, "too large"), (dict(n_pages=(1 << 26) + 1), UNSUPPORTED, "too large"),
 ]
 
 
@@ -149,7 +149,7 @@ def test_nothing_to_do_is_no_error(lib):
     assert lib.wdrz_token_logprobs(2, None, 0, None, 0, None, None, None, None, None, 0, 10, 0, None, 0, None) == 0
 
 
-@pytest.mark.parametrize("kw,err", [(dict(page_size=24), NotImplementedError), (dict(n_streams=0), ValueError), (dict(n_streams=15361), ValueError),
+@pytest.mark.parametrize("kw,err", [(dict(page_size=24), NotImplementedError), (dict(n_streams=0), ValueError), (dict(n_streams=12289), ValueError),
                                     (dict(n_pages=0), ValueError), (dict(max_seq_length=0), ValueError)])
 def test_page_tables_are_refused(kw, err):
     with pytest.raises(err):

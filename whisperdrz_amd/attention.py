@@ -446,7 +446,7 @@ def flash_attn_with_kvpages(
         cache_batch_idx = _check_ids("cache_batch_idx", cache_batch_idx, B, device)
         idx_ptr = cache_batch_idx.data_ptr()
     if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(B, sq, H, D, dtype=dtype, device=device)
     else:
         _check_cuda("out", out, device)
         if out.shape != shape or out.dtype != dtype:
@@ -527,7 +527,7 @@ def packed_attention(
             raise ValueError(f"{name} must be a tensor of whole numbers [B + 1]")
         sums.append(_check_ids(name, t, n, device))
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty(T, H, D, dtype=dtype, device=device)
     else:
         _check_cuda("out", out, device)
         if out.shape != shape or out.dtype != dtype:

@@ -1108,8 +1108,8 @@ static int page_tables(const wdrz_page_tables* p, wdrz::PageArgs* a) {
   if (p->n_streams <= 0 || p->n_pages <= 0 || p->max_pages <= 0 || p->max_seq <= 0 || p->max_seq > p->max_pages * p->page_size)
     return fail(WDRZ_EINVAL, "bad page table sizes n_streams=%lld n_pages=%lld max_pages=%lld max_seq=%lld",
                 (long long)p->n_streams, (long long)p->n_pages, (long long)p->max_pages, (long long)p->max_seq);
-  if (p->n_streams > 15360 || p->n_pages > (1 << 26) || p->max_pages > (1 << 20) || p->max_seq > (1 << 24))
-    return fail(WDRZ_EUNSUPPORTED, "sizes too large (15360 streams, 2^26 pages, 2^24 positions a stream at most)");
+  if (p->n_streams > 12288 || p->n_pages > (1 << 26) || p->max_pages > (1 << 20) || p->max_seq > (1 << 24))
+    return fail(WDRZ_EUNSUPPORTED, "sizes too large (12288 streams, 2^26 pages, 2^24 positions a stream at most)");
   a->tables = p->tables;
   a->counts = p->page_counts;
   a->lens = p->seq_lens;

@@ -151,7 +151,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     if index != _current_device():  # launches go to the current device
         with torch.cuda.device(index):
             return token_logprobs(logits, tokens, top, blocked)
-    logprobs = torch.empty(shape, dtype=torch.float32, device=device)
+    logprobs = torch.empty(*(shape or ((),)), dtype=torch.float32, device=device)
     entropy = torch.empty_like(logprobs)
     top_logprobs = logprobs.new_empty(*shape, max(top, 0))
     top_ids = tokens.new_empty(*shape, max(top, 0))

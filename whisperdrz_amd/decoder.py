@@ -21,6 +21,8 @@ cached attention, so the HIP kernels can be exercised exactly as WhisperDRZ driv
   GPU activations.
 * 8-bit caches (``KVSlotPool(cache_bits=8)``) and 4-bit Linears (``TextDecoderStack.quantize_linears_``) run on
   their own kernels in the same step.
+* paged self caches (``KVPagePool``): ``forward_flash`` plans a step's tokens once for all layers and attends over
+  pages; ``TextDecoderStack.prefill_packed`` runs prompts of different lengths next to each other, without padding.
 * ``BucketedDecodeGraphs`` — one captured decode step per batch bucket, replayed with static
   token / position / slot buffers (reference ``transcriber.py:18-173``); on ROCm
   ``torch.cuda.CUDAGraph`` is a hipGraph.
@@ -38,11 +40,13 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
-from .attention import flash_attn_with_kvcache, flash_attn_with_kvcache8, scaled_dot_product_attention
+from .attention import (flash_attn_with_kvcache, flash_attn_with_kvcache8, flash_attn_with_kvpages, packed_attention,
+                        scaled_dot_product_attention)
 from .decode_ops import (LN_LINEAR_MAX_K, LN_LINEAR_ROWS, QuantLinear4, QuantLinear4Rows, add_layernorm_,
                          add_layernorm_partials_, layer_norm, linear, linear4, linear4_partials, linear_gelu,
                          linear_partials, ln_linear, step_begin, step_end_)
 from .kv_cache import FlashKVCache, FlashKVCache8, KVSlotPool
+from .paged import FlashKVPages, KVPagePool, PagePlan
 
 # Batch buckets of the captured decode step (reference transcriber.py:18).
 GRAPH_BUCKETS = [1, 2, 4, 8, 16, 32, 42, 52, 54]
@@ -67,6 +71,33 @@ def _out_add_layernorm(x: Tensor, o: Tensor, out: nn.Linear, ln: nn.LayerNorm) -
     elif out.in_features % 256 == 0 and out.out_features <= 1536 and out.bias is not None:
         return add_layernorm_partials_(x, linear_partials(o, out, 2), out, ln)
     return add_layernorm_(x, out(o), ln)
+
+
+class PackedSelf:
+    """One layer's pages as a packed prompt's self-attention takes them: the rows are written to the plan's slots and
+    attended where they are."""
+
+    def __init__(self, cache: FlashKVPages, plan: PagePlan):
+        self.cache, self.plan = cache, plan
+
+    def attend(self, q: Tensor, k: Tensor, v: Tensor, scale: float) -> Tensor:
+        self.cache.write(k, v, self.plan.slots)
+        return packed_attention(q, k, v, self.plan.cu_seqlens, causal=True, scale=scale)
+
+
+class PackedCross:
+    """One layer's cross-attention of a packed prompt: the encoder output's keys and values, projected when they are
+    needed, go to the streams' slots and are attended where they are."""
+
+    def __init__(self, attn: "MultiHeadAttention", xa: Tensor, cache: FlashKVCache, slots: Tensor, plan: PagePlan, cu_audio: Tensor):
+        self.attn, self.xa, self.cache, self.slots, self.plan, self.cu_audio = attn, xa, cache, slots, plan, cu_audio
+
+    def attend(self, q: Tensor, k: None, v: None, scale: float) -> Tensor:
+        H, d = q.shape[1:]
+        kv = F.linear(self.xa, *self.attn.kv_weight()).view(*self.xa.shape[:2], 2, H, d)
+        self.cache.set_cross_attention(kv[:, :, 0], kv[:, :, 1], self.slots)
+        kv = kv.view(-1, 2, H, d)
+        return packed_attention(q, kv[:, 0], kv[:, 1], self.plan.cu_seqlens, self.cu_audio, causal=False, scale=scale)
 
 
 def lengths_matrix(self_kv: list[FlashKVCache]) -> Optional[Tensor]:
@@ -170,6 +201,10 @@ class MultiHeadAttention(nn.Module):
         """The cached attention of ``[B, sq, H, d]`` rows, appending ``k`` / ``v`` (self) or not (cross), on
         the cache's own kernels."""
         scale = (self.n_state // self.n_head) ** -0.5
+        if isinstance(kv_cache, (PackedSelf, PackedCross)):  # one batch row of packed tokens
+            return kv_cache.attend(q[0], None if k is None else k[0], None if v is None else v[0], scale)[None]
+        if isinstance(kv_cache, FlashKVPages):
+            return flash_attn_with_kvpages(q, kv_cache, k, v, cache_seqlens=seqlens, cache_batch_idx=batch_idx, softmax_scale=scale)
         if isinstance(kv_cache, FlashKVCache8):
             return flash_attn_with_kvcache8(q, kv_cache, k, v, cache_seqlens=seqlens, cache_batch_idx=batch_idx,
                                             softmax_scale=scale)
@@ -285,6 +320,8 @@ class TextDecoderStack(nn.Module):
         B, seq_len = tokens.shape
         if positions.dim() == 1:
             positions = positions.unsqueeze(1).expand(B, seq_len)
+        if self_kv and isinstance(self_kv[0], FlashKVPages):
+            return self._forward_pages(tokens, self_kv, cross_kv, positions, slot_indices)
         lens = lengths_matrix(self_kv)
         if lens is not None and self._fused_prologue(tokens, positions, slot_indices, lens):
             x, h, batch_idx, seqlens = step_begin(tokens, positions, self.token_embedding.weight,
@@ -320,6 +357,31 @@ class TextDecoderStack(nn.Module):
                 else:
                     s_kv.seq_lens[:B] += seq_len
         return self._logits(h)
+
+    def _needs_16bit_gpu(self, what: str) -> None:
+        w = self.token_embedding.weight
+        if not (self.fused_small_ops and w.is_cuda and w.dtype in (torch.bfloat16, torch.float16)):
+            raise NotImplementedError(f"{what} need 16-bit weights on the GPU and the fused small operations")
+
+    def _forward_pages(self, tokens: Tensor, self_kv: list[FlashKVPages], cross_kv: list[FlashKVCache], positions: Tensor,
+                       slot_indices: Optional[Tensor]) -> Tensor:
+        """``forward_flash`` on paged self caches: the tokens get their places in one launch for all layers, which also adds
+        them to the streams' lengths. A row whose stream is none (-1: a padded row) or gets no pages has NaN logits and
+        changes nothing."""
+        self._needs_16bit_gpu("paged caches")
+        tables = self_kv[0].page_tables
+        B, seq_len = tokens.shape
+        lens = tables.seq_lens.view(1, -1)
+        if self._fused_prologue(tokens, positions, slot_indices, lens):
+            x, h, streams, _ = step_begin(tokens, positions, self.token_embedding.weight, self.positional_embedding,
+                                          self.blocks[0].attn_ln, slot_indices, lens)
+        else:
+            x = (self.token_embedding(tokens) + self.positional_embedding[positions]).contiguous()
+            h, streams = layer_norm(x, self.blocks[0].attn_ln), None if slot_indices is None else slot_indices.to(torch.int32)
+        if streams is None:
+            streams = torch.arange(B, dtype=torch.int32, device=x.device)
+        plan = tables.plan(seq_len, B * seq_len, streams)
+        return self._logits(self._fused_blocks(x, h, self_kv, cross_kv, streams, [plan.starts] * len(self.blocks)))
 
     def _fused_prologue(self, tokens: Tensor, positions: Tensor, slot_indices: Optional[Tensor], lens: Tensor) -> bool:
         """Whether ``step_begin`` / ``step_end_`` take this step: 16-bit, 16-byte aligned tables of up
@@ -411,16 +473,40 @@ class TextDecoderStack(nn.Module):
         return self.forward_flash(tokens, self_kv, cross_kv, positions, slot_indices)
 
 
+    def prefill_packed(self, tokens: Tensor, new_lens: Tensor, xa: Tensor, pool: KVPagePool, slot_indices: Tensor) -> tuple[Tensor, PagePlan]:
+        """:meth:`prefill_flash` for prompts of different lengths into a :class:`KVPagePool`: ``tokens`` ``[T]`` are the
+        prompts one behind the other, ``new_lens`` int ``[B]`` their lengths, ``xa`` ``[B, audio, n_state]`` the encoder
+        output, ``slot_indices`` ``[B]`` the streams, which start anew. Returns the logits ``[T, n_vocab]`` of every token
+        (``token_logprobs(logits, next_tokens)`` scores whole texts) and the plan: a prompt that found no pages has
+        ``plan.starts`` -1 and logits, but no cache."""
+        self._needs_16bit_gpu("packed prompts")
+        B, audio = xa.shape[:2]
+        if tokens.dim() != 1 or tuple(new_lens.shape) != (B,) or tuple(slot_indices.shape) != (B,):
+            raise ValueError(f"tokens must be [T], new_lens and slot_indices [{B}], got {tuple(tokens.shape)}, {tuple(new_lens.shape)}, "
+                             f"{tuple(slot_indices.shape)}")
+        streams = slot_indices.to(torch.int32)
+        pool.tables.truncate(0, streams)
+        plan = pool.tables.plan(new_lens, tokens.shape[0], streams)
+        x = (self.token_embedding(tokens) + self.positional_embedding[plan.positions])[None].contiguous()
+        cu_audio = torch.arange(0, B * audio + 1, audio, dtype=torch.int32, device=xa.device)
+        self_kv = [PackedSelf(c, plan) for c in pool.self_kv]
+        cross_kv = [PackedCross(b.cross_attn, xa, c, slot_indices, plan, cu_audio) for b, c in zip(self.blocks, pool.cross_kv, strict=True)]
+        h = self._fused_blocks(x, layer_norm(x, self.blocks[0].attn_ln), self_kv, cross_kv, None, [None] * len(self.blocks))
+        return self._logits(h[0]), plan
+
+
 class BucketedDecodeGraphs:
     """Captured single-token decode steps per batch bucket (reference transcriber.py:31-173).
 
     Padded rows of a bucket keep the slot ids they were captured or last called with, as in the
     reference, so callers that pad must make those slots harmless (the reference's own
-    behaviour: padded rows append into, and bump the lengths of, those slots).
+    behaviour: padded rows append into, and bump the lengths of, those slots). With a ``KVPagePool`` padded rows
+    name no stream (-1) and change nothing, nor does the capture.
     """
 
-    def __init__(self, decoder: TextDecoderStack, pool: KVSlotPool, n_vocab: int, buckets: Optional[list[int]] = None):
+    def __init__(self, decoder: TextDecoderStack, pool: KVSlotPool | KVPagePool, n_vocab: int, buckets: Optional[list[int]] = None):
         self.decoder, self.pool, self.n_vocab = decoder, pool, n_vocab
+        self.paged = isinstance(pool, KVPagePool)
         self.buckets = list(buckets if buckets is not None else GRAPH_BUCKETS)
         self.graphs: dict[int, torch.cuda.CUDAGraph] = {}
         self.static: dict[int, dict[str, Tensor]] = {}
@@ -433,11 +519,12 @@ class BucketedDecodeGraphs:
                                           slot_indices=st["slots"])
 
     def capture(self, bucket: int) -> None:
-        dev = self.pool.arena.device
+        dev = self.pool.device
+        slots = torch.arange(bucket, dtype=torch.long, device=dev)
         self.static[bucket] = {
             "tokens": torch.zeros(bucket, 1, dtype=torch.long, device=dev),
             "positions": torch.zeros(bucket, dtype=torch.long, device=dev),
-            "slots": torch.arange(bucket, dtype=torch.long, device=dev),
+            "slots": slots.fill_(-1) if self.paged else slots,
         }
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
@@ -460,6 +547,8 @@ class BucketedDecodeGraphs:
         self.hits[bucket] += 1
         st = self.static[bucket]
         # one launch where the inputs are int64 on this device, else a copy each
+        if self.paged and B < bucket:
+            st["slots"][B:].fill_(-1)
         torch._foreach_copy_([st["tokens"][:B], st["positions"][:B], st["slots"][:B]], [tokens, positions, slot_indices])
         self.graphs[bucket].replay()
         return st["logits"][:B]

@@ -384,6 +384,10 @@ class KVSlotPool:
             self.self_kv.append(cache(self_len, True, self.self_seq_lens[l]))
             self.cross_kv.append(cache(cross_len, False, None))
 
+    @property
+    def device(self) -> torch.device:
+        return self.arena.device
+
     @staticmethod
     def arena_bytes(n_slots: int, n_layers: int, n_heads: int, head_dim: int, self_len: int, cross_len: int,
                     dtype: torch.dtype, cache_bits: int = 16) -> int:

@@ -44,7 +44,7 @@ class PageTables:
     """
 
     PAGE_SIZES = (16, 32, 64, 128, 256)
-    MAX_STREAMS = 15360
+    MAX_STREAMS = 12288
 
     def __init__(self, n_streams: int, n_pages: int, page_size: int = 16, max_seq_length: int = 448, device=None, *,
                  storage: Optional[dict[str, Tensor]] = None):
