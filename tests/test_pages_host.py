@@ -205,3 +205,14 @@ def test_a_pool_and_its_bytes():
     held = sum(t.numel() * 2 for c in pool.self_kv for t in (c.k_pages, c.v_pages))
     assert held == 12 * w.KVPagePool.page_bytes(2, 4, 64, 32, torch.bfloat16)
     assert w.KVPagePool.page_bytes(32, 20, 64, 16, torch.bfloat16) == 2621440
+
+
+def test_launches_of_too_many_threads_are_refused(lib):
+    """2^32 threads and more along the grid's first axis: refused before the launch, not by it."""
+    q4 = strides(1 << 20, 1 << 20, 64, 1)
+    assert lib.wdrz_page_write(2, pages(n_heads=65535), FAKE, R3, FAKE, R3, FAKE, 1 << 14, None) == UNSUPPORTED
+    assert lib.wdrz_attn_packed(2, FAKE, R3, FAKE, R3, FAKE, R3, FAKE, R3, FAKE, FAKE, 1, 1 << 24, 8, 128, 128, 64, 0.125, 1, None) == UNSUPPORTED
+    assert lib.wdrz_attn_packed(2, FAKE, R3, FAKE, R3, FAKE, R3, FAKE, R3, FAKE, FAKE, 65535, 65535, 8, 131, 131, 128, 0.125, 1, None) == UNSUPPORTED
+    assert lib.wdrz_attn_kvpages(2, pages(n_heads=1024), tables(), FAKE, q4, None, None, None, None, FAKE, FAKE, FAKE, q4, 65535, 16, 1024, 0.125, None, 0, None) == UNSUPPORTED
+    assert lib.wdrz_token_logprobs(0, FAKE, 10, None, 0, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 24, 10, 0, None, 0, None) == UNSUPPORTED
+    assert b"too large" in lib.wdrz_last_error()

@@ -372,13 +372,16 @@ def kvpages_workspace_size(batch: int, sq: int, n_heads: int, n_kv_heads: int, h
 # Workspaces by (device, stream) whose counters stand at their start, apart from _WORKSPACES: calls of other shapes leave
 # the counters where they are, so nothing but they has to be zero after a call.
 _COUNTED_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
+_COUNTER_BYTES = 4096 * 4
 
 
 def _counted_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """The current stream's workspace of ``device``, the current device; a captured call gets its own, cleared by every
-    replay (another graph captured on this stream may be replayed beside its graph)."""
+    """The current stream's workspace of ``device``, the current device; a captured call gets its own, its counters cleared by
+    every replay (another graph captured on this stream may be replayed beside its graph)."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buf[:_COUNTER_BYTES].zero_()
+        return buf
     key = (device.index, _raw_stream(device.index))
     buf = _COUNTED_WORKSPACES.get(key)
     if buf is None or buf.numel() < nbytes:

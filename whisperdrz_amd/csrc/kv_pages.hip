@@ -31,7 +31,9 @@ namespace {
 constexpr int kRows = 16;           // (query, group head) rows a workgroup
 constexpr int kBlock = 32;          // positions a wavefront takes at a time
 constexpr int kPagesMaxSplits = 64;  // workgroups that a row's keys are cut into at most
-constexpr float kMove = 8.f;        // a reference is moved when a score is 2^8 above it
+// A row's reference lies 2^7 below its largest probability, so that the two fp16 operands hold small ones too (2^-32 of
+// the largest), and is moved where one exceeds it by 2^15: none leaves fp16.
+constexpr float kBelow = 7.f, kMove = 15.f;
 
 template <typename T> struct Pg;
 template <> struct Pg<Bf16> {
@@ -248,7 +250,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void pages_attn_kerne
     const float mx = quarters_max(fmaxf(fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[0][2], p[0][3])),
                                         fmaxf(fmaxf(p[1][0], p[1][1]), fmaxf(p[1][2], p[1][3]))));
     if (__any(mx > m + kMove)) {
-      const float to = fmaxf(m, mx);
+      const float to = fmaxf(m, mx - kBelow);
       const float f = m == -INFINITY ? 0.f : fast_exp2(m - to);
       m = to;
       mu = to == -INFINITY ? 0.f : to;

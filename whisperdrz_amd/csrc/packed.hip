@@ -26,7 +26,9 @@ namespace {
 
 constexpr int kTile = 64;           // keys a stage
 constexpr int kSub = 32;            // keys a step
-constexpr float kSumLimit = 1024.f;
+// A query's reference lies 2^8 below its largest probability, so that fp16 operands hold those down to 2^-22 of it with
+// all digits, and is moved where a lane's 16 sum to more than 2^15: none leaves fp16.
+constexpr float kBelow = 8.f, kSumLimit = 32768.f;
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
@@ -273,7 +275,7 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
 #pragma unroll
         for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[x]);
         mx = halves_max(mx) * a.c;
-        const float to = s == 0 ? (mx == -INFINITY ? 0.f : mx) : fmaxf(m, mx);
+        const float to = s == 0 ? (mx == -INFINITY ? 0.f : mx - kBelow) : fmaxf(m, mx - kBelow);
         const float f = fast_exp2(m - to);
         m = to;
         if (s != 0) {
@@ -400,26 +402,36 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
   }
 }
 
+constexpr int kWaves64 = 4, kWaves128 = 8;  // wavefronts a workgroup, by the head's dims
+
+// Heads of a group share a workgroup's keys: as many as divide the group and the wavefronts.
+int heads_together(int64_t group, int waves) {
+  int nh = 1;
+  while (nh < waves && group % (2 * nh) == 0) nh *= 2;
+  return nh;
+}
+
 template <typename T, int D, int NW, int NBUF, bool AHEAD, int SIMD_WAVES>
 void launch_q(PackedArgs a, hipStream_t stream) {
-  // heads of a group share a workgroup's keys: as many as divide the group and the wavefronts
-  const int group = a.H / a.Hk;
-  a.nh = 1;
-  while (a.nh < NW && group % (2 * a.nh) == 0) a.nh *= 2;
-  const int rows = 32 * NW / a.nh;
-  const int64_t blocks = a.T / rows + std::min(a.B, a.T);  // at most: every sequence's last block is part full
-  hipLaunchKernelGGL((packed_attn_kernel<T, D, NW, NBUF, AHEAD, SIMD_WAVES>), dim3((unsigned)(blocks * (a.H / a.nh))), dim3(64 * NW), 0, stream, a);
+  a.nh = heads_together(a.H / a.Hk, NW);
+  hipLaunchKernelGGL((packed_attn_kernel<T, D, NW, NBUF, AHEAD, SIMD_WAVES>), dim3((unsigned)packed_blocks(a.T, a.B, a.H, a.Hk, D)),
+                     dim3(64 * NW), 0, stream, a);
 }
 
 }  // namespace
 
+int64_t packed_blocks(int64_t T, int64_t B, int64_t H, int64_t Hk, int64_t D) {
+  const int waves = D == 64 ? kWaves64 : kWaves128, nh = heads_together(H / Hk, waves);
+  return (T / (32 * waves / nh) + std::min(B, T)) * (H / nh);  // at most: every sequence's last block is part full
+}
+
 hipError_t launch_packed(int dtype, int D, const PackedArgs& a, hipStream_t stream) {
   if (D == 64) {
-    if (dtype == 2) launch_q<Bf16, 64, 4, 3, false, 3>(a, stream);
-    else launch_q<F16, 64, 4, 3, false, 3>(a, stream);
+    if (dtype == 2) launch_q<Bf16, 64, kWaves64, 3, false, 3>(a, stream);
+    else launch_q<F16, 64, kWaves64, 3, false, 3>(a, stream);
   } else {
-    if (dtype == 2) launch_q<Bf16, 128, 8, 4, true, 2>(a, stream);
-    else launch_q<F16, 128, 8, 4, true, 2>(a, stream);
+    if (dtype == 2) launch_q<Bf16, 128, kWaves128, 4, true, 2>(a, stream);
+    else launch_q<F16, 128, kWaves128, 4, true, 2>(a, stream);
   }
   return hipGetLastError();
 }

@@ -63,7 +63,7 @@ __device__ __forceinline__ void scan2(int& a, int& b, int cap, int& total_a, int
 }
 
 constexpr int kPageBatch = 8;  // entries of a request moved together: one trip to memory for each batch
-constexpr int kMostPages = 1 << 30;  // sums of needed pages are held at it
+constexpr int kMostPages = 1 << 29;  // sums of pages are held at it: with a round's 1024 x 2^20 behind they stay in 31 bits
 
 // The first request that names each stream, in claims[n_streams] (LDS); the others count as naming none.
 __device__ __forceinline__ void claim_streams(const PageArgs& a, int* claims) {

@@ -1093,6 +1093,9 @@ int wdrz_linear4_partials(int dtype, const void* x, int64_t x_stride, const void
 
 // ---- the paged cache, packed sequences and token log probabilities ----
 
+// A launch holds fewer than 2^32 threads along its first axis.
+static bool grid_too_large(int64_t blocks, int64_t threads) { return blocks > 0x7fffffff || blocks * threads > 0xffffffffll; }
+
 static int log2_page(int64_t page_size) {
   for (int s = 4; s <= 8; ++s)
     if (page_size == (int64_t)1 << s) return s;
@@ -1205,7 +1208,7 @@ int wdrz_page_write(int dtype, const wdrz_kv_pages* cache, const void* k_src, co
   int rc = kv_pages(dtype, cache, &a.shift);
   if (rc) return rc;
   if (T < 0) return fail(WDRZ_EINVAL, "bad sizes T=%lld", (long long)T);
-  if (T > (1 << 28) || T * cache->n_heads * (cache->head_dim / 8) > ((int64_t)1 << 38)) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (T > (1 << 28) || grid_too_large((T * cache->n_heads * (cache->head_dim / 8) + 255) / 256, 256)) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
   if (T == 0) return WDRZ_OK;
   if (!slots) return fail(WDRZ_EINVAL, "slots is NULL");
   if ((rc = rows16_packed("k", k_src, k_strides, a.ks)) || (rc = rows16_packed("v", v_src, v_strides, a.vs))) return rc;
@@ -1277,7 +1280,7 @@ int wdrz_attn_kvpages(int dtype, const wdrz_kv_pages* cache, const wdrz_page_tab
   a.n_pages = (int)pages->n_pages;
   a.max_pages = (int)pages->max_pages;
   wdrz::pages_plan(B, sq, H, a.Hk, cache->head_dim, pages->max_seq, &a);
-  if (B * a.Hk * a.n_rt > 0x7fffffff) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (grid_too_large(B * a.Hk * a.n_rt, 64 * a.waves)) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
   const size_t need = wdrz::pages_workspace_bytes(B, sq, H, a.Hk, cache->head_dim, pages->max_seq);
   if (need > 0) {
     if (!workspace || workspace_bytes < need)
@@ -1312,7 +1315,7 @@ int wdrz_attn_packed(int dtype, const void* q, const int64_t* q_strides, const v
   if ((rc = rows16_packed("q", q, q_strides, a.qs)) || (rc = rows16_packed("out", o, o_strides, a.os))) return rc;
   if (Tk > 0 && ((rc = rows16_packed("k", k, k_strides, a.ks)) || (rc = rows16_packed("v", v, v_strides, a.vs)))) return rc;
   // 64 rows of keys are addressed by 31-bit offsets
-  if ((T / 32 + B) * H > 0x7fffffff || (Tk > 0 && (a.ks[0] >= (1 << 25) || a.vs[0] >= (1 << 25) || a.ks[0] < 0 || a.vs[0] < 0)))
+  if (grid_too_large(wdrz::packed_blocks(T, B, H, Hk, D), D == 64 ? 256 : 512) || (Tk > 0 && (a.ks[0] >= (1 << 25) || a.vs[0] >= (1 << 25) || a.ks[0] < 0 || a.vs[0] < 0)))
     return fail(WDRZ_EUNSUPPORTED, "sizes or strides too large");
 #ifdef WDRZ_DEBUG_CHECKS
   if ((rc = debug_check_sums("cu_seqlens", cu_q, B, T)) || (cu_k && (rc = debug_check_sums("cu_seqlens_k", cu_k, B, Tk)))) return rc;
@@ -1348,7 +1351,7 @@ int wdrz_token_logprobs(int dtype, const void* logits, int64_t l_stride, const u
   if (!eb) return fail(WDRZ_EINVAL, "dtype %d is not one of WDRZ_F32/F16/BF16", dtype);
   if (rows < 0 || V <= 0) return fail(WDRZ_EINVAL, "bad sizes rows=%lld V=%lld", (long long)rows, (long long)V);
   if (top < 0 || top > 32) return fail(WDRZ_EUNSUPPORTED, "top=%lld is not 0 .. 32", (long long)top);
-  if (rows > (1 << 24) || V > (1 << 20)) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
+  if (grid_too_large(rows, 256) || V > (1 << 20)) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
   if (l_stride < 0 || (blocked && b_stride < 0)) return fail(WDRZ_EINVAL, "negative row strides");
   if (rows == 0) return WDRZ_OK;
   if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_logprobs || !top_ids)))

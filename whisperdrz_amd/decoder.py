@@ -484,6 +484,8 @@ class TextDecoderStack(nn.Module):
         if tokens.dim() != 1 or tuple(new_lens.shape) != (B,) or tuple(slot_indices.shape) != (B,):
             raise ValueError(f"tokens must be [T], new_lens and slot_indices [{B}], got {tuple(tokens.shape)}, {tuple(new_lens.shape)}, "
                              f"{tuple(slot_indices.shape)}")
+        if pool.self_len > self.positional_embedding.shape[0]:
+            raise ValueError(f"the pool's streams hold {pool.self_len} positions, the decoder has {self.positional_embedding.shape[0]}")
         streams = slot_indices.to(torch.int32)
         pool.tables.truncate(0, streams)
         plan = pool.tables.plan(new_lens, tokens.shape[0], streams)

@@ -184,7 +184,6 @@ class FlashKVPages:
         self.device = tables.device
         self._held = (storage["k_pages"], storage["v_pages"])
         self.struct = _lib.KvPages(self.k_pages.data_ptr(), self.v_pages.data_ptr(), tables.n_pages, n_heads, tables.page_size, head_dim)
-        self.done, self.cross_attn_len = False, 0
 
     @property
     def seq_lens(self) -> Tensor:
