@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import whisperdrz_amd as w
-from oracle.paged_oracle import attention, logprobs
+from oracle.paged_oracle import Tables, attention, logprobs
 from whisperdrz_amd.decoder import TextDecoderStack
 
 pytestmark = pytest.mark.gpu
@@ -157,3 +157,23 @@ def test_captured_workspaces_are_cleared_by_replays(cuda):
             assert torch.equal(a, b), i
     want = logprobs(logits.cpu(), tokens.cpu(), 3)
     assert torch.equal(outs[4].cpu(), want[3])
+
+
+@pytest.mark.parametrize("lens", [[33000, 0, 17, 33000], [40] * 300 + [9000] + [3] * 1500, [5000] * 20])
+def test_requests_of_many_pages(cuda, lens):
+    """Long and short requests in one call, taken and given back in part and whole, with a request in between that finds no
+    pages; equal to the restatement that moves a page at a time."""
+    n, most = len(lens), max(lens)
+    pages = sum(-(-x // 16) for x in lens) - 2
+    t, ref = w.PageTables(n, pages, 16, most, device=cuda), Tables(n, pages, 16, most)
+    order = torch.randperm(n, generator=torch.Generator().manual_seed(n)).tolist()
+    streams = ids(cuda, order)
+    for new, back in ((lens, [x // 3 for x in lens]), ([x - x // 3 for x in lens], [0] * n)):
+        got, want = t.plan(ids(cuda, new), sum(new), streams), ref.plan(order, new, sum(new))
+        for a, b in zip(got, want):
+            assert a.tolist() == list(b)
+        t.truncate(ids(cuda, back), streams)
+        ref.truncate(order, back)
+        assert t.free_pages[: int(t.n_free)].tolist() == ref.free and t.seq_lens.tolist() == ref.lens
+        for row, held in zip(t.tables.tolist(), ref.rows):
+            assert row[: len(held)] == held and set(row[len(held):]) <= {-1}
