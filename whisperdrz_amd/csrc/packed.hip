@@ -4,15 +4,28 @@
 // Its query t sees all its keys, or under the causal mask those at t + (keys - queries) and before; a query that
 // sees none gives zeros. Query head h reads key/value head h / (H / Hk).
 //
-// A workgroup takes 128 QB queries of one head, a wavefront 32 QB of them (QB blocks of 32), over tiles of 64 keys
-// that pass through registers into one of two LDS buffers while the other is computed. As in the encoder's
-// attention the products are transposed, S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 matrix instructions, with
-// the keys' rows permuted so that the scores of a lane are already the operand of the second product, and V^T is
-// read from row-major V by transposing LDS reads.
+// A wavefront takes 32 queries of one head; a workgroup of 4 (64 dims) or 8 (128 dims) holds as many heads of a group as
+// divide both, which read the same keys, and blocks of 32 queries beside each other. Tiles of 64 keys and values go
+// from memory to one of 3 or 4 LDS buffers past the registers, the next ones while one is computed; a tile's rows are
+// swizzled so that neither operand's reads meet in a bank. As in the encoder's attention the products are transposed,
+// S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 matrix instructions, with the keys' rows permuted so that the scores of
+// a lane are already the operand of the second product, and V^T is read from row-major V by transposing LDS reads. Work
+// items, the longest first, are found from the sums by every workgroup: the host does not know them.
 //
-// Softmax: p = 2^(c s - m) in fp32 with a reference m per query, taken from the first 32 keys and moved only
-// where a lane's 16 probabilities sum to more than 2^10 (some exceeds 2^6): no maximum is taken otherwise. Every
-// query that sees any key sees the first, so the first keys give a reference.
+// Softmax: p = 2^(c s - m) in fp32 with a reference m per query, taken from the first 32 keys and moved only where a
+// lane's 16 probabilities sum to more than 2^15: no maximum is taken otherwise. Every query that sees any key sees
+// the first, so the first keys give a reference. Sums are of the fp32 probabilities. The products take them in the
+// operands' type, one rounding of half a step (2^-8 or 2^-11 of each; the attention over pages, whose matrix cores
+// idle, takes two operands): a second product would cost a third of the matrix instructions.
+//
+// Bound: at 128 dims the matrix cores, at 64 the exponentials and what is around them (4 matrix instructions to 16
+// exponentials a lane, twice as many at 128). 2 x 8192 tokens of 32/8 heads of 128, causal: 680 .. 715 us, 1.0 PFLOP/s of the
+// 1.39 that a library product of 8192^3 reaches; 16 prompts over 1500 keys of 20 heads of 64: 41 us, 390 TFLOP/s.
+// Measured, us, at 64 dims (long batch with its write / cross) and 128:
+//   4 wavefronts, 3 buffers, 3 a SIMD     110 / 41.6    the form taken: other wavefronts of the SIMD fill the softmax's time
+//     4 buffers, next scores ahead, 2     127 / 47.8      2 buffers, 4 a SIMD 112 / 41.9; 3 buffers, ahead, 3 a SIMD 114 / 42.2
+//   8 wavefronts, 4 buffers, ahead, 2     154 / 51.7      685 at 128, the form taken (registers allow 2 a SIMD)
+//     3 buffers, not ahead                691 at 128      4 wavefronts 1169
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -11,7 +11,9 @@
 // stream that an earlier one named, or a length that the table cannot hold.
 //
 // Bound: launch and a chain of four dependent trips to memory (stream -> its length -> the stack -> the table).
-// One workgroup does the scan, since every request's pages depend on all before it.
+// One workgroup does the scan, since every request's pages depend on all before it. Plan and truncation of 8 streams 3.5 and
+// 2.5 us on the GPU (13 us a pair of calls: the host's side), of 1000 prompts 12.3 (and 4.6 for 168000 tokens' slots) and 8.3:
+// one CU's scattered reads and writes of lengths and tables; a scan over several workgroups would add a trip for each.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -281,7 +283,8 @@ __global__ __launch_bounds__(kThreads) void page_truncate_kernel(PageArgs a) {
 }
 
 // ---- writes: row t's keys and values to slot slots[t] of every head's page ------------------------------
-// A thread moves 16 bytes of a key and of a value; rows whose slot lies outside the cache are left out.
+// A thread moves 16 bytes of a key and of a value; rows whose slot lies outside the cache are left out. Bound: bytes, read and
+// written once: 39 us for 21500 rows of 20 heads of 64, 5.6 TB/s, as fast as a large copy.
 __global__ __launch_bounds__(256) void page_write_kernel(PageWriteArgs a) {
   const int pieces = a.D / 8;
   const int64_t n = (int64_t)a.T * a.Hk * pieces;

@@ -475,7 +475,7 @@ class TextDecoderStack(nn.Module):
 
     def prefill_packed(self, tokens: Tensor, new_lens: Tensor, xa: Tensor, pool: KVPagePool, slot_indices: Tensor) -> tuple[Tensor, PagePlan]:
         """:meth:`prefill_flash` for prompts of different lengths into a :class:`KVPagePool`: ``tokens`` ``[T]`` are the
-        prompts one behind the other, ``new_lens`` int ``[B]`` their lengths, ``xa`` ``[B, audio, n_state]`` the encoder
+        prompts one behind the other, ``new_lens`` int ``[B]`` their lengths (T in all), ``xa`` ``[B, audio, n_state]`` the encoder
         output, ``slot_indices`` ``[B]`` the streams, which start anew. Returns the logits ``[T, n_vocab]`` of every token
         (``token_logprobs(logits, next_tokens)`` scores whole texts) and the plan: a prompt that found no pages has
         ``plan.starts`` -1 and logits, but no cache."""
