@@ -151,3 +151,32 @@ def test_captured_calls_follow_their_sums(cuda):
         out.zero_()
         g.replay()
         assert torch.equal(out, w.packed_attention(q, k, v, cu, out=torch.zeros_like(q)))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("H,Hk", [(1, 1), (4, 4), (6, 3), (8, 1)])
+def test_few_queries_over_many_keys(cuda, causal, H, Hk):
+    """Two wavefronts share a query block: sequences of which one half of a tile's keys is empty, that begin or end inside a tile, and
+    queries that see no key at all."""
+    check(cuda, BF16, [1, 40, 3, 70, 0, 33], H, Hk, 64, causal, klens=[20, 700, 0, 33, 900, 1100])
+    check(cuda, FP16, [5], H, Hk, 64, causal, klens=[289])
+
+
+def test_few_queries_of_many_sequences(cuda):
+    check(cuda, BF16, [1] * 40 + [0, 2] * 15, 1, 1, 64, False, klens=[300, 250] * 35)
+
+
+@pytest.mark.parametrize("odd", [float("nan"), float("inf")])
+def test_what_nobody_sees_does_not_count_in_halves(cuda, odd):
+    """As above with one sequence long enough for two wavefronts: either may hold the value, in its first step or later."""
+    for at in (0, 31, 32, 63, 64, 250, 300):
+        g = torch.Generator().manual_seed(at)
+        q, k, v = (torch.randn(310, 2, 64, generator=g).to(BF16) for _ in range(3))
+        k[at], v[at] = odd, odd
+        got = w.packed_attention(q.to(cuda), k.to(cuda), v.to(cuda), sums([305]).to(cuda)).cpu()
+        pick = [t for t in (0, 1, 15, 16, 31, 32, 60, 249, 299) if t < at]
+        if pick:
+            clean = pick[-1] + 1
+            want, big = attention(q[pick], k[:clean], v[:clean], [t + 1 for t in pick], 64**-0.5)
+            assert_rows(got[pick], want, big, float(v[:clean].float().abs().max()), BF16, 64)
+        assert got[at:305].isnan().all()

@@ -5,7 +5,8 @@
 // sees none gives zeros. Query head h reads key/value head h / (H / Hk).
 //
 // A wavefront takes 32 queries of one head; a workgroup of 4 (64 dims) or 8 (128 dims) holds as many heads of a group as
-// divide both, which read the same keys, and blocks of 32 queries beside each other. Tiles of 64 keys and values go
+// divide both, which read the same keys, and blocks of 32 queries beside each other; where blocks are few two wavefronts
+// share one, each with half of every tile's keys, and join at the end. Tiles of 64 keys and values go
 // from memory to one of 3 or 4 LDS buffers past the registers, the next ones while one is computed; a tile's rows are
 // swizzled so that neither operand's reads meet in a bank. As in the encoder's attention the products are transposed,
 // S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 matrix instructions, with the keys' rows permuted so that the scores of
@@ -89,41 +90,69 @@ __device__ __forceinline__ u32x2 read_tr(const uint16_t* p) {
 #endif
 }
 
-// Sequence and query block of the work item `idx`, blocks of a sequence counted from its end (under the mask the
-// last needs the most keys), sequences from the last; false where there is none. Every lane of a wavefront calls it.
+// Work items: the query blocks of the sequences, counted from a sequence's end (under the mask the last needs the most
+// keys), sequences from the last. Every lane of a wavefront calls these.
 struct Item {
   int q0, nq, k0, nk, block;
 };
-__device__ __forceinline__ bool find_item(const PackedArgs& a, int rows, int idx, Item& it) {
-  const int lane = threadIdx.x & 63;
-  for (int i0 = 0; i0 < a.B; i0 += 64) {
-    const int i = a.B - 1 - i0 - lane;
-    int c0 = 0, c1 = 0;
-    if (i >= 0) {
-      c0 = min(max(a.cu_q[i], 0), a.T);  // sums that are not ascending or in range stay in bounds
-      c1 = min(max(a.cu_q[i + 1], c0), a.T);
-    }
-    const int n = (c1 - c0 + rows - 1) / rows;
-    int sum = n;
+// 64 sequences from B - 1 - i0 down, one a lane: its rows and the items up to it.
+struct Chunk {
+  int c0, c1, sum, total;
+};
+__device__ __forceinline__ Chunk scan_items(const PackedArgs& a, int rows, int i0) {
+  const int lane = threadIdx.x & 63, i = a.B - 1 - i0 - lane;
+  Chunk c = {0, 0, 0, 0};
+  if (i >= 0) {
+    c.c0 = min(max(a.cu_q[i], 0), a.T);  // sums that are not ascending or in range stay in bounds
+    c.c1 = min(max(a.cu_q[i + 1], c.c0), a.T);
+  }
+  c.sum = (c.c1 - c.c0 + rows - 1) / rows;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(sum, o);
-      if (lane >= o) sum += u;
-    }
-    const int total = __builtin_amdgcn_readlane(sum, 63);
-    if (idx < total) {
-      const uint64_t here = __ballot(idx < sum);
-      const int src = __ffsll((unsigned long long)here) - 1, s = a.B - 1 - i0 - src;
-      it.q0 = __builtin_amdgcn_readlane(c0, src);
-      it.nq = __builtin_amdgcn_readlane(c1, src) - it.q0;
-      it.block = __builtin_amdgcn_readlane(sum, src) - 1 - idx;
-      it.k0 = min(max(a.cu_k[s], 0), a.Tk);
-      it.nk = min(max(a.cu_k[s + 1], it.k0), a.Tk) - it.k0;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(c.sum, o);
+    if (lane >= o) c.sum += u;
+  }
+  c.total = __builtin_amdgcn_readlane(c.sum, 63);
+  return c;
+}
+// The item `idx` of the chunk's `total`.
+__device__ __forceinline__ Item pick_item(const PackedArgs& a, const Chunk& c, int i0, int idx) {
+  const int src = __ffsll((unsigned long long)__ballot(idx < c.sum)) - 1, s = a.B - 1 - i0 - src;
+  Item it;
+  it.q0 = __builtin_amdgcn_readlane(c.c0, src);
+  it.nq = __builtin_amdgcn_readlane(c.c1, src) - it.q0;
+  it.block = __builtin_amdgcn_readlane(c.sum, src) - 1 - idx;
+  it.k0 = min(max(a.cu_k[s], 0), a.Tk);
+  it.nk = min(max(a.cu_k[s + 1], it.k0), a.Tk) - it.k0;
+  return it;
+}
+// This workgroup's item, and its group of heads in `sub`; false where it has none. Items of a group of heads are next to
+// each other, on one XCD: those of a sequence read the same keys. The host launches as many workgroups as there may be
+// items; where one chunk holds all sequences their number is known, the first workgroups take them and the CUs get
+// equally many (64 prompts with their writes 109.5 us with the others in between, 108.4 so).
+__device__ __forceinline__ bool find_item(const PackedArgs& a, int rows, int& sub, Item& it) {
+  const int n_wg = (int)gridDim.x, groups = a.H / a.nh;
+  Chunk c = scan_items(a, rows, 0);
+  if (a.B <= 64) {
+    const int n = (int)min((int64_t)c.total * groups, (int64_t)n_wg);
+    if ((int)blockIdx.x >= n) return false;
+    const int unit = remap_xcd((int)blockIdx.x, n);
+    sub = unit / c.total;
+    it = pick_item(a, c, 0, unit % c.total);
+    return sub < groups;
+  }
+  const int unit = remap_xcd((int)blockIdx.x, n_wg), n_idx = n_wg / groups;
+  sub = unit / n_idx;
+  int idx = unit % n_idx;
+  for (int i0 = 0;;) {
+    if (idx < c.total) {
+      it = pick_item(a, c, i0, idx);
       return true;
     }
-    idx -= total;
+    idx -= c.total;
+    if ((i0 += 64) >= a.B) return false;
+    c = scan_items(a, rows, i0);
   }
-  return false;
 }
 
 // 16 bytes a lane from memory to LDS, lane l to byte `to` + 16 l, without passing through registers; zeros where the
@@ -142,7 +171,8 @@ template <int N> __device__ __forceinline__ void landed_barrier() {  // all but 
 }
 
 // AHEAD: the next step's scores run under this step's softmax; else the other wavefronts of the SIMD (SIMD_WAVES) fill it.
-template <typename T, int D, int NW, int NBUF, bool AHEAD, int SIMD_WAVES>
+// HALVES 2: two wavefronts share a query block, each takes one half of every tile's keys.
+template <typename T, int D, int NW, int NBUF, bool AHEAD, int SIMD_WAVES, int HALVES>
 __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(PackedArgs a) {
   typedef typename Pk<T>::op_t op_t;
   typedef uint16_t e_t;
@@ -152,15 +182,15 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
-  // blocks fastest, neighbours on one XCD: those of a sequence read the same keys of a head
-  const int unit = remap_xcd((int)blockIdx.x, (int)gridDim.x), n_idx = (int)gridDim.x / (a.H / a.nh);
-  const int sub = unit / n_idx, idx = unit % n_idx, per_group = a.H / a.Hk / a.nh;
-  const int hk = sub / per_group, nqb = NW / a.nh;  // query blocks a head
+  const int nqb = NW / HALVES / a.nh;  // query blocks a head
+  int sub;
   Item it;
-  if (!find_item(a, 32 * nqb, idx, it)) return;
+  if (!find_item(a, 32 * nqb, sub, it)) return;
+  const int hk = sub / (a.H / a.Hk / a.nh);
   // wavefronts w and w + 4 share a SIMD: under the mask the later blocks of one half meet the earlier ones of the other
-  const int qbi = wave < 4 || NW == 4 ? wave / a.nh : nqb - 1 - (wave - 4) / a.nh;
-  const int h = sub * a.nh + wave % a.nh;
+  const int slot = wave % (NW / HALVES), half = wave / (NW / HALVES);
+  const int qbi = slot < 4 || NW == 4 ? slot / a.nh : nqb - 1 - (slot - 4) / a.nh;
+  const int h = sub * a.nh + slot % a.nh;
   const int q_wg = it.block * 32 * nqb, q_wave = q_wg + qbi * 32;
   const int shift = a.causal ? it.nk - it.nq : 0;  // query t sees the keys up to t + shift
   const int k_lim = a.causal ? max(0, min(it.nk, min(q_wg + 32 * nqb, it.nq) + shift)) : it.nk;
@@ -281,17 +311,18 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
         }
         st = (part[0] + part[1]) + (part[2] + part[3]);
       };
-      if (s != 0) exps();
-      if (s == 0 || __any(!(st <= kSumLimit))) {
+      const bool first = s == half;
+      if (!first) exps();
+      if (first || __any(!(st <= kSumLimit))) {
         asm volatile("" ::: "memory");  // rare: stays a branch
         float mx = -INFINITY;
 #pragma unroll
         for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[x]);
         mx = halves_max(mx) * a.c;
-        const float to = s == 0 ? (mx == -INFINITY ? 0.f : mx - kBelow) : fmaxf(m, mx - kBelow);
+        const float to = first ? (mx == -INFINITY ? 0.f : mx - kBelow) : fmaxf(m, mx - kBelow);
         const float f = fast_exp2(m - to);
         m = to;
-        if (s != 0) {
+        if (!first) {
           l *= f;
 #pragma unroll
           for (int db = 0; db < DB; ++db)
@@ -384,6 +415,10 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
       // the last tile that this one's steps read (AHEAD: the next one's keys) is there; nobody reads tile t - 1 any more
       landed_barrier<2 * kLoads * (NBUF - (AHEAD ? 3 : 2))>();
       issue(t + NBUF - 1);
+      if (HALVES == 2) {
+        if (2 * t + half < n_sub) step(2 * t + half, s0, s1);
+        continue;
+      }
       if (2 * t < n_sub) step(2 * t, s0, s1);
       if (2 * t + 1 < n_sub) {
         if (AHEAD) step(2 * t + 1, s1, s0);
@@ -394,9 +429,31 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
 
   // O^T through LDS, so that memory sees whole rows: the wavefront's 32 rows in its own part
   landed_barrier<0>();
-  const float sum = l + __shfl_xor(l, 32);
+  float sum = l + __shfl_xor(l, 32);
+  constexpr int kPart = HALVES == 1 ? 32 * kRow : (DB * 16 + 2) * 64 * 4;  // a query block's part of the LDS
+  if (HALVES == 2) {  // the second half's sums to the first's wavefront
+    float* part = reinterpret_cast<float*>(smem + slot * kPart) + lane;
+    if (half) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) part[(db * 16 + x) * 64] = acc[db][x];
+      part[DB * 16 * 64] = m;
+      part[(DB * 16 + 1) * 64] = sum;
+    }
+    __syncthreads();
+    if (half) return;
+    const float m1 = part[DB * 16 * 64], sum1 = part[(DB * 16 + 1) * 64];
+    const float M = sum == 0.f ? m1 : sum1 == 0.f ? m : fmaxf(m, m1);  // a half that sees nothing has no reference
+    const float f0 = sum == 0.f ? 0.f : fast_exp2(m - M), f1 = sum1 == 0.f ? 0.f : fast_exp2(m1 - M);
+    sum = sum * f0 + sum1 * f1;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) acc[db][x] = acc[db][x] * f0 + part[(db * 16 + x) * 64] * f1;
+  }
   const float f = sum == 0.f ? 0.f : 1.f / sum;  // a query that sees no key is 0
-  char* mine = smem + wave * 32 * kRow;
+  char* mine = smem + slot * kPart;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -415,37 +472,48 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
   }
 }
 
+// A query block's chain of steps takes 530 ns for 32 keys however few there are: with up to 1.5 blocks a SIMD, and keys enough
+// to make up for the join, two wavefronts take half of it each. 20 heads of 64 over 1500 keys, us, one / two wavefronts, by
+// prompts of 128 tokens: 1 26.7 / 18.4, 8 29.4 / 25.7, 16 37.1 / 32.5, 24 41.3 / 44.9, 64 118.6 / 135.7; 8 over 150 keys 7.8 / 8.2.
+constexpr int64_t kFewBlocks = 1536;
 constexpr int kWaves64 = 4, kWaves128 = 8;  // wavefronts a workgroup, by the head's dims
 
-// Heads of a group share a workgroup's keys: as many as divide the group and the wavefronts.
-int heads_together(int64_t group, int waves) {
-  int nh = 1;
-  while (nh < waves && group % (2 * nh) == 0) nh *= 2;
-  return nh;
+// How a call is cut: wavefronts to a query block, heads of a group in a workgroup (as many as divide the group and the
+// workgroup's query blocks), workgroups.
+struct Cut {
+  int halves, nh, rows;
+  int64_t blocks;
+};
+Cut cut_of(int64_t T, int64_t Tk, int64_t B, int64_t H, int64_t Hk, int64_t D) {
+  Cut c;
+  c.halves = D == 64 && T / 32 * H <= kFewBlocks && Tk >= 256 * B ? 2 : 1;
+  const int slots = (D == 64 ? kWaves64 : kWaves128) / c.halves;
+  c.nh = 1;
+  while (c.nh < slots && H / Hk % (2 * c.nh) == 0) c.nh *= 2;
+  c.rows = 32 * slots / c.nh;
+  c.blocks = (T / c.rows + std::min(B, T)) * (H / c.nh);  // at most: every sequence's last block is part full
+  return c;
 }
 
-template <typename T, int D, int NW, int NBUF, bool AHEAD, int SIMD_WAVES>
-void launch_q(PackedArgs a, hipStream_t stream) {
-  a.nh = heads_together(a.H / a.Hk, NW);
-  hipLaunchKernelGGL((packed_attn_kernel<T, D, NW, NBUF, AHEAD, SIMD_WAVES>), dim3((unsigned)packed_blocks(a.T, a.B, a.H, a.Hk, D)),
-                     dim3(64 * NW), 0, stream, a);
+template <typename T, int D, int NW, int NBUF, bool AHEAD, int SIMD_WAVES, int HALVES>
+void launch_q(PackedArgs a, const Cut& c, hipStream_t stream) {
+  a.nh = c.nh;
+  hipLaunchKernelGGL((packed_attn_kernel<T, D, NW, NBUF, AHEAD, SIMD_WAVES, HALVES>), dim3((unsigned)c.blocks), dim3(64 * NW), 0, stream, a);
+}
+template <typename T> void launch_t(int D, const PackedArgs& a, hipStream_t stream) {
+  const Cut c = cut_of(a.T, a.Tk, a.B, a.H, a.Hk, D);
+  if (D == 128) launch_q<T, 128, kWaves128, 4, true, 2, 1>(a, c, stream);
+  else if (c.halves == 2) launch_q<T, 64, kWaves64, 3, false, 3, 2>(a, c, stream);
+  else launch_q<T, 64, kWaves64, 3, false, 3, 1>(a, c, stream);
 }
 
 }  // namespace
 
-int64_t packed_blocks(int64_t T, int64_t B, int64_t H, int64_t Hk, int64_t D) {
-  const int waves = D == 64 ? kWaves64 : kWaves128, nh = heads_together(H / Hk, waves);
-  return (T / (32 * waves / nh) + std::min(B, T)) * (H / nh);  // at most: every sequence's last block is part full
-}
+int64_t packed_blocks(int64_t T, int64_t Tk, int64_t B, int64_t H, int64_t Hk, int64_t D) { return cut_of(T, Tk, B, H, Hk, D).blocks; }
 
 hipError_t launch_packed(int dtype, int D, const PackedArgs& a, hipStream_t stream) {
-  if (D == 64) {
-    if (dtype == 2) launch_q<Bf16, 64, kWaves64, 3, false, 3>(a, stream);
-    else launch_q<F16, 64, kWaves64, 3, false, 3>(a, stream);
-  } else {
-    if (dtype == 2) launch_q<Bf16, 128, kWaves128, 4, true, 2>(a, stream);
-    else launch_q<F16, 128, kWaves128, 4, true, 2>(a, stream);
-  }
+  if (dtype == 2) launch_t<Bf16>(D, a, stream);
+  else launch_t<F16>(D, a, stream);
   return hipGetLastError();
 }
 

@@ -1315,7 +1315,7 @@ int wdrz_attn_packed(int dtype, const void* q, const int64_t* q_strides, const v
   if ((rc = rows16_packed("q", q, q_strides, a.qs)) || (rc = rows16_packed("out", o, o_strides, a.os))) return rc;
   if (Tk > 0 && ((rc = rows16_packed("k", k, k_strides, a.ks)) || (rc = rows16_packed("v", v, v_strides, a.vs)))) return rc;
   // 64 rows of keys are addressed by 31-bit offsets
-  if (grid_too_large(wdrz::packed_blocks(T, B, H, Hk, D), D == 64 ? 256 : 512) || (Tk > 0 && (a.ks[0] >= (1 << 25) || a.vs[0] >= (1 << 25) || a.ks[0] < 0 || a.vs[0] < 0)))
+  if (grid_too_large(wdrz::packed_blocks(T, Tk, B, H, Hk, D), D == 64 ? 256 : 512) || (Tk > 0 && (a.ks[0] >= (1 << 25) || a.vs[0] >= (1 << 25) || a.ks[0] < 0 || a.vs[0] < 0)))
     return fail(WDRZ_EUNSUPPORTED, "sizes or strides too large");
 #ifdef WDRZ_DEBUG_CHECKS
   if ((rc = debug_check_sums("cu_seqlens", cu_q, B, T)) || (cu_k && (rc = debug_check_sums("cu_seqlens_k", cu_k, B, Tk)))) return rc;

@@ -338,7 +338,7 @@ struct PackedArgs {
   int B, T, Tk, H, Hk, causal;
   int nh;  // heads of a group that share a workgroup (set by the launcher)
 };
-int64_t packed_blocks(int64_t T, int64_t B, int64_t H, int64_t Hk, int64_t D);  // workgroups of a launch
+int64_t packed_blocks(int64_t T, int64_t Tk, int64_t B, int64_t H, int64_t Hk, int64_t D);  // workgroups of a launch
 hipError_t launch_packed(int dtype, int D, const PackedArgs& a, hipStream_t stream);
 
 // Log probabilities of tokens (token_logprobs.hip).
