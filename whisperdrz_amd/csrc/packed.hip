@@ -6,21 +6,20 @@
 //
 // A wavefront takes 32 queries of one head; a workgroup of 4 (64 dims) or 8 (128 dims) holds as many heads of a group as
 // divide both, which read the same keys, and blocks of 32 queries beside each other; where blocks are few two wavefronts
-// share one, each with half of every tile's keys, and join at the end. Tiles of 64 keys and values go
-// from memory to one of 3 or 4 LDS buffers past the registers, the next ones while one is computed; a tile's rows are
-// swizzled so that neither operand's reads meet in a bank. As in the encoder's attention the products are transposed,
+// share one, each with half of every tile's keys, and join at the end. Tiles of 64 keys and values go from memory to
+// one of 3 or 4 LDS buffers past the registers, the next ones while one is computed; a tile's rows are swizzled so that neither operand's reads meet in a bank. As in the encoder's attention the products are transposed,
 // S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 matrix instructions, with the keys' rows permuted so that the scores of
 // a lane are already the operand of the second product, and V^T is read from row-major V by transposing LDS reads. Work
 // items, the longest first, are found from the sums by every workgroup: the host does not know them.
 //
 // Softmax: p = 2^(c s - m) in fp32 with a reference m per query, taken from the first 32 keys and moved only where a
-// lane's 16 probabilities sum to more than 2^15: no maximum is taken otherwise. Every query that sees any key sees
-// the first, so the first keys give a reference. Sums are of the fp32 probabilities. The products take them in the
+// lane's 16 probabilities sum to more than 2^15: no maximum is taken otherwise. Every query that sees any key (of a
+// half) sees the first, so the first keys give a reference. Sums are of the fp32 probabilities. The products take them in the
 // operands' type, one rounding of half a step (2^-8 or 2^-11 of each; the attention over pages, whose matrix cores
-// idle, takes two operands): a second product would cost a third of the matrix instructions.
+// idle, takes two operands): a second product would be half as many matrix instructions again.
 //
-// Bound: at 128 dims the matrix cores, at 64 the exponentials and what is around them (4 matrix instructions to 16
-// exponentials a lane, twice as many at 128). 2 x 8192 tokens of 32/8 heads of 128, causal: 680 .. 715 us, 1.0 PFLOP/s of the
+// Bound: at 128 dims the matrix cores, at 64 the exponentials and what is around them (8 matrix instructions to 16
+// exponentials a lane and step, twice as many at 128), with few blocks the chain of a step. 2 x 8192 tokens of 32/8 heads of 128, causal: 680 .. 715 us, 1.0 PFLOP/s of the
 // 1.39 that a library product of 8192^3 reaches; 16 prompts over 1500 keys of 20 heads of 64: 41 us, 390 TFLOP/s.
 // Measured, us, at 64 dims (long batch with its write / cross) and 128:
 //   4 wavefronts, 3 buffers, 3 a SIMD     110 / 41.6    the form taken: other wavefronts of the SIMD fill the softmax's time
