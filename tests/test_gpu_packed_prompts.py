@@ -1,0 +1,59 @@
+"""TextDecoderStack.prefill_packed where a prompt is not served: what it returns, and what it leaves as it was.
+
+The restatement is the same decoder on slot caches, prompt by prompt; the bound is the decoder tests' own for 16-bit
+activations, 2e-2 of the largest logit."""
+import pytest
+import torch
+
+from whisperdrz_amd import KVPagePool
+from whisperdrz_amd.decoder import TextDecoderStack
+from whisperdrz_amd.kv_cache import KVSlotPool
+
+pytestmark = pytest.mark.gpu
+
+N_VOCAB, N_CTX, N_STATE, N_HEAD, N_LAYER, AUDIO = 300, 80, 128, 2, 2, 50
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def stack(cuda):
+    torch.manual_seed(5)
+    stack = TextDecoderStack(N_VOCAB, N_CTX, N_STATE, N_HEAD, N_LAYER).requires_grad_(False)
+    stack.positional_embedding.mul_(50.0)  # as large as the tokens': a wrong position is seen
+    return stack.to(cuda, BF16).eval()
+
+
+def pool(cuda, n_pages=60, streams=6):
+    return KVPagePool(N_LAYER, streams, n_pages, N_HEAD, 64, N_CTX, AUDIO, BF16, cuda)
+
+
+def prompts(cuda, lens, seed=0):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    return (torch.randint(0, N_VOCAB, (sum(lens),), generator=g, device=cuda), torch.tensor(lens, device=cuda),
+            torch.randn(len(lens), AUDIO, N_STATE, generator=g, device=cuda).to(BF16))
+
+
+def alone(cuda, stack, tokens, xa):
+    """The logits of one prompt by itself."""
+    slots = KVSlotPool(N_LAYER, 1, N_HEAD, 64, self_len=N_CTX, cross_len=AUDIO, dtype=BF16, device=cuda)
+    return stack.prefill_flash(tokens[None], xa[None], slots.self_kv, slots.cross_kv, torch.zeros(1, dtype=torch.long, device=cuda))[0]
+
+
+def close(a, b):
+    a, b = a.float(), b.float()
+    return bool(torch.isfinite(a).all()) and (a - b).abs().max().item() <= 2e-2 * max(b.abs().max().item(), 1.0)
+
+
+@pytest.mark.parametrize("lens,named,n_pages,served", [
+    ([16, 33, 17, 5], [0, 1, 2, 3], 4, [0, 0, -1, -1]),  # pages run out
+    ([20, 9, 30, 40], [3, 3, -1, 6], 60, [0, -1, -1, -1]),  # named twice, no stream
+    ([70, 81, 100, 3], [0, 1, 2, 4], 60, [0, -1, -1, 0])])  # longer than the decoder
+def test_logits_of_prompts_that_are_not_served(cuda, stack, lens, named, n_pages, served):
+    """A prompt without a cache has the logits that it has by itself; positions that the decoder does not have are NaN."""
+    pages = pool(cuda, n_pages)
+    tokens, new, xa = prompts(cuda, lens)
+    logits, plan = stack.prefill_packed(tokens, new, xa, pages, torch.tensor(named, device=cuda))
+    assert plan.starts.tolist() == served
+    for i, (got, t) in enumerate(zip(logits.split(lens), tokens.split(lens))):
+        assert close(got[:N_CTX], alone(cuda, stack, t[:N_CTX], xa[i])), i
+        assert got[N_CTX:].isnan().all()

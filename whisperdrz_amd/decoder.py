@@ -477,8 +477,9 @@ class TextDecoderStack(nn.Module):
         """:meth:`prefill_flash` for prompts of different lengths into a :class:`KVPagePool`: ``tokens`` ``[T]`` are the
         prompts one behind the other, ``new_lens`` int ``[B]`` their lengths (T in all), ``xa`` ``[B, audio, n_state]`` the encoder
         output, ``slot_indices`` ``[B]`` the streams, which start anew. Returns the logits ``[T, n_vocab]`` of every token
-        (``token_logprobs(logits, next_tokens)`` scores whole texts) and the plan: a prompt that found no pages has
-        ``plan.starts`` -1 and logits, but no cache."""
+        (``token_logprobs(logits, next_tokens)`` scores whole texts) and the plan: a prompt that is not served (see
+        ``PageTables.plan``) has ``plan.starts`` -1 and no cache, but the logits that it has by itself; those of positions that
+        the decoder does not have are NaN."""
         self._needs_16bit_gpu("packed prompts")
         B, audio = xa.shape[:2]
         if tokens.dim() != 1 or tuple(new_lens.shape) != (B,) or tuple(slot_indices.shape) != (B,):
@@ -489,7 +490,12 @@ class TextDecoderStack(nn.Module):
         streams = slot_indices.to(torch.int32)
         pool.tables.truncate(0, streams)
         plan = pool.tables.plan(new_lens, tokens.shape[0], streams)
-        x = (self.token_embedding(tokens) + self.positional_embedding[plan.positions])[None].contiguous()
+        # positions from the sums, not the plan's, which are 0 for a prompt that is not served
+        cu, t = plan.cu_seqlens.long(), torch.arange(tokens.shape[0], device=plan.slots.device)
+        positions = t - cu[torch.bucketize(t, cu[1:], right=True)]
+        none = positions >= self.positional_embedding.shape[0]
+        x = self.token_embedding(tokens) + self.positional_embedding[positions.masked_fill(none, 0)]
+        x = x.masked_fill(none[:, None], float("nan"))[None]
         cu_audio = torch.arange(0, B * audio + 1, audio, dtype=torch.int32, device=xa.device)
         self_kv = [PackedSelf(c, plan) for c in pool.self_kv]
         cross_kv = [PackedCross(b.cross_attn, xa, c, slot_indices, plan, cu_audio) for b, c in zip(self.blocks, pool.cross_kv, strict=True)]
