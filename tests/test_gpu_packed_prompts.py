@@ -57,3 +57,19 @@ def test_logits_of_prompts_that_are_not_served(cuda, stack, lens, named, n_pages
     for i, (got, t) in enumerate(zip(logits.split(lens), tokens.split(lens))):
         assert close(got[:N_CTX], alone(cuda, stack, t[:N_CTX], xa[i])), i
         assert got[N_CTX:].isnan().all()
+
+
+def test_cross_caches_of_prompts_that_are_not_served(cuda, stack):
+    """The windows of prompts without pages, and of a stream's second prompt, go to no slot."""
+    pages = pool(cuda, 4)
+    for c in pages.cross_kv:
+        c.k_cache.fill_(3.0), c.v_cache.fill_(3.0)
+    lens, named = [16, 33, 17, 2, 5], [4, 0, 2, 4, 0]
+    tokens, new, xa = prompts(cuda, lens, 1)
+    logits, plan = stack.prefill_packed(tokens, new, xa, pages, torch.tensor(named, device=cuda))
+    assert plan.starts.tolist() == [0, 0, -1, -1, -1]
+    for block, c in zip(stack.blocks, pages.cross_kv):
+        kv = torch.nn.functional.linear(xa, *block.cross_attn.kv_weight()).view(len(lens), AUDIO, 2, N_HEAD, 64)
+        for s in range(6):
+            want = kv[named.index(s)] if s in (0, 4) else torch.full_like(kv[0], 3.0)
+            assert torch.equal(c.k_cache[s], want[:, 0]) and torch.equal(c.v_cache[s], want[:, 1]), s

@@ -87,7 +87,7 @@ class PackedSelf:
 
 class PackedCross:
     """One layer's cross-attention of a packed prompt: the encoder output's keys and values, projected when they are
-    needed, go to the streams' slots and are attended where they are."""
+    needed, go to the streams' ``slots`` (-1: to none) and are attended where they are."""
 
     def __init__(self, attn: "MultiHeadAttention", xa: Tensor, cache: FlashKVCache, slots: Tensor, plan: PagePlan, cu_audio: Tensor):
         self.attn, self.xa, self.cache, self.slots, self.plan, self.cu_audio = attn, xa, cache, slots, plan, cu_audio
@@ -498,7 +498,8 @@ class TextDecoderStack(nn.Module):
         x = x.masked_fill(none[:, None], float("nan"))[None]
         cu_audio = torch.arange(0, B * audio + 1, audio, dtype=torch.int32, device=xa.device)
         self_kv = [PackedSelf(c, plan) for c in pool.self_kv]
-        cross_kv = [PackedCross(b.cross_attn, xa, c, slot_indices, plan, cu_audio) for b, c in zip(self.blocks, pool.cross_kv, strict=True)]
+        slots = slot_indices.long().masked_fill(plan.starts < 0, -1)  # -1: to no slot
+        cross_kv = [PackedCross(b.cross_attn, xa, c, slots, plan, cu_audio) for b, c in zip(self.blocks, pool.cross_kv, strict=True)]
         h = self._fused_blocks(x, layer_norm(x, self.blocks[0].attn_ln), self_kv, cross_kv, None, [None] * len(self.blocks))
         return self._logits(h[0]), plan
 
