@@ -73,3 +73,32 @@ def test_cross_caches_of_prompts_that_are_not_served(cuda, stack):
         for s in range(6):
             want = kv[named.index(s)] if s in (0, 4) else torch.full_like(kv[0], 3.0)
             assert torch.equal(c.k_cache[s], want[:, 0]) and torch.equal(c.v_cache[s], want[:, 1]), s
+
+
+def state(pages):
+    t = pages.tables
+    caches = [x for c in pages.self_kv for x in (c.k_pages, c.v_pages)] + [x for c in pages.cross_kv for x in (c.k_cache, c.v_cache)]
+    return [x.clone() for x in (t.tables, t.page_counts, t.seq_lens, t.free_pages, t.n_free, *caches)]
+
+
+def test_calls_that_are_refused_change_nothing(cuda, stack):
+    """Windows that are not the cross caches' length (steps attend all of a slot's rows), and inputs of other types, devices and
+    shapes: refused before a stream is emptied or a page is taken."""
+    pages = pool(cuda)
+    tokens, new, xa = prompts(cuda, [20, 9], 2)
+    at = torch.tensor([1, 4], device=cuda)
+    stack.prefill_packed(tokens, new, xa, pages, at)
+    other = TextDecoderStack(N_VOCAB, N_CTX, N_STATE, N_HEAD, N_LAYER + 1).to(cuda, BF16)
+    wide = TextDecoderStack(N_VOCAB, N_CTX, 2 * N_STATE, 2 * N_HEAD, N_LAYER).to(cuda, BF16)
+    before = state(pages)
+    for s, args, err in ((stack, (tokens, new, xa[:, :-1], pages, at), ValueError), (stack, (tokens, new, torch.cat([xa, xa], 1), pages, at), ValueError),
+                         (stack, (tokens, new, xa.float(), pages, at), TypeError), (stack, (tokens, new, xa[..., :64], pages, at), ValueError),
+                         (stack, (tokens, new, xa.cpu(), pages, at), RuntimeError), (stack, (tokens, new.cpu(), xa, pages, at), RuntimeError),
+                         (stack, (tokens, new.float(), xa, pages, at), TypeError), (stack, (tokens.float(), new, xa, pages, at), TypeError),
+                         (stack, (tokens, new, xa, pages, at.float()), TypeError), (stack, (tokens.cpu(), new, xa, pages, at), RuntimeError),
+                         (stack, (tokens, new, xa, KVPagePool(N_LAYER, 6, 60, N_HEAD, 64, N_CTX, AUDIO, torch.float16, cuda), at), TypeError),
+                         (other, (tokens, new, xa, pages, at), ValueError),
+                         (wide, (tokens, new, torch.cat([xa, xa], 2), pages, at), ValueError)):
+        with pytest.raises(err):
+            s.prefill_packed(*args)
+        assert all(torch.equal(a, b) for a, b in zip(before, state(pages)))

@@ -40,8 +40,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
-from .attention import (flash_attn_with_kvcache, flash_attn_with_kvcache8, flash_attn_with_kvpages, packed_attention,
-                        scaled_dot_product_attention)
+from .attention import (_check_cuda, _check_ids, flash_attn_with_kvcache, flash_attn_with_kvcache8, flash_attn_with_kvpages,
+                        packed_attention, scaled_dot_product_attention)
 from .decode_ops import (LN_LINEAR_MAX_K, LN_LINEAR_ROWS, QuantLinear4, QuantLinear4Rows, add_layernorm_,
                          add_layernorm_partials_, layer_norm, linear, linear4, linear4_partials, linear_gelu,
                          linear_partials, ln_linear, step_begin, step_end_)
@@ -363,6 +363,18 @@ class TextDecoderStack(nn.Module):
         if not (self.fused_small_ops and w.is_cuda and w.dtype in (torch.bfloat16, torch.float16)):
             raise NotImplementedError(f"{what} need 16-bit weights on the GPU and the fused small operations")
 
+    def _check_pages(self, self_kv: list[FlashKVPages], cross_kv: list[FlashKVCache]) -> None:
+        """Whether the caches are this decoder's, before a plan changes their tables."""
+        if not self_kv or not len(self_kv) == len(cross_kv) == len(self.blocks) or len({id(c.page_tables) for c in self_kv}) > 1:
+            raise ValueError(f"{len(self.blocks)} layers need as many caches, in the pages of one table")
+        for H, d, dtype, device in {(c.n_heads, c.head_dim, c.dtype, c.device) for c in (*self_kv, *cross_kv)}:
+            if (H, d) != (self.n_head, self.n_state // self.n_head):
+                raise ValueError(f"cache heads/head_dim {(H, d)} do not match the decoder's {(self.n_head, self.n_state // self.n_head)}")
+            if dtype != self.token_embedding.weight.dtype:
+                raise TypeError(f"the caches must have the decoder's dtype {self.token_embedding.weight.dtype}, got {dtype}")
+            if device != self.token_embedding.weight.device:
+                raise RuntimeError(f"a cache is on {device}, expected {self.token_embedding.weight.device}")
+
     def _forward_pages(self, tokens: Tensor, self_kv: list[FlashKVPages], cross_kv: list[FlashKVCache], positions: Tensor,
                        slot_indices: Optional[Tensor]) -> Tensor:
         """``forward_flash`` on paged self caches: the tokens get their places in one launch for all layers, which also adds
@@ -475,8 +487,8 @@ class TextDecoderStack(nn.Module):
 
     def prefill_packed(self, tokens: Tensor, new_lens: Tensor, xa: Tensor, pool: KVPagePool, slot_indices: Tensor) -> tuple[Tensor, PagePlan]:
         """:meth:`prefill_flash` for prompts of different lengths into a :class:`KVPagePool`: ``tokens`` ``[T]`` are the
-        prompts one behind the other, ``new_lens`` int ``[B]`` their lengths (T in all), ``xa`` ``[B, audio, n_state]`` the encoder
-        output, ``slot_indices`` ``[B]`` the streams, which start anew. Returns the logits ``[T, n_vocab]`` of every token
+        prompts one behind the other, ``new_lens`` int ``[B]`` their lengths (T in all), ``xa`` ``[B, pool.cross_len, n_state]`` the
+        encoder output, ``slot_indices`` ``[B]`` the streams, which start anew. Returns the logits ``[T, n_vocab]`` of every token
         (``token_logprobs(logits, next_tokens)`` scores whole texts) and the plan: a prompt that is not served (see
         ``PageTables.plan``) has ``plan.starts`` -1 and no cache, but the logits that it has by itself; those of positions that
         the decoder does not have are NaN."""
@@ -487,7 +499,15 @@ class TextDecoderStack(nn.Module):
                              f"{tuple(slot_indices.shape)}")
         if pool.self_len > self.positional_embedding.shape[0]:
             raise ValueError(f"the pool's streams hold {pool.self_len} positions, the decoder has {self.positional_embedding.shape[0]}")
-        streams = slot_indices.to(torch.int32)
+        if tuple(xa.shape) != (B, pool.cross_len, self.n_state):  # steps attend all rows of a slot
+            raise ValueError(f"xa must be [{B}, {pool.cross_len}, {self.n_state}], got {tuple(xa.shape)}")
+        self._check_pages(pool.self_kv, pool.cross_kv)
+        _check_cuda("xa", xa, pool.device)
+        _check_cuda("tokens", tokens, pool.device)
+        if xa.dtype != pool.dtype or tokens.dtype not in (torch.int64, torch.int32):
+            raise TypeError(f"xa must be {pool.dtype} and tokens whole numbers, got {xa.dtype} and {tokens.dtype}")
+        new_lens = _check_ids("new_lens", new_lens, B, pool.device)
+        streams = _check_ids("slot_indices", slot_indices, B, pool.device)
         pool.tables.truncate(0, streams)
         plan = pool.tables.plan(new_lens, tokens.shape[0], streams)
         # positions from the sums, not the plan's, which are 0 for a prompt that is not served
