@@ -102,3 +102,23 @@ def test_calls_that_are_refused_change_nothing(cuda, stack):
         with pytest.raises(err):
             s.prefill_packed(*args)
         assert all(torch.equal(a, b) for a, b in zip(before, state(pages)))
+
+
+@pytest.mark.parametrize("lens,told,served", [
+    ([16, 9, 12], [16, 9, 14], [0, 0, -1]), ([16, 9, 12], [16, 9 + 2**31 - 40, 12], [0, -1, -1]), ([16, 9, 12], [16, 9, 3], [0, 0, 0]),
+    ([16, 9, 12], [16, -1, 12], [0, -1, 0])])
+def test_lengths_that_do_not_match_the_tokens(cuda, stack, lens, told, served):
+    """A prompt whose tokens are not all there takes nothing, nor do those behind it; tokens of no prompt have NaN."""
+    pages = pool(cuda)
+    tokens, _, xa = prompts(cuda, lens, 3)
+    at = torch.tensor([2, 5, 0], device=cuda)
+    logits, plan = stack.prefill_packed(tokens, torch.tensor(told, device=cuda), xa, pages, at)
+    assert plan.starts.tolist() == served
+    held = [n if s == 0 else 0 for n, s in zip(told, served)]
+    assert pages.tables.seq_lens[at].tolist() == held and 60 - int(pages.tables.n_free) == sum(-(-n // 16) for n in held)
+    a = 0
+    for i, n in enumerate(held):
+        if n:
+            assert close(logits[a : a + n], alone(cuda, stack, tokens[a : a + n], xa[i]))
+        a += n
+    assert logits[a:].isnan().all() and (plan.slots[a:] == -1).all()

@@ -491,7 +491,8 @@ class TextDecoderStack(nn.Module):
         encoder output, ``slot_indices`` ``[B]`` the streams, which start anew. Returns the logits ``[T, n_vocab]`` of every token
         (``token_logprobs(logits, next_tokens)`` scores whole texts) and the plan: a prompt that is not served (see
         ``PageTables.plan``) has ``plan.starts`` -1 and no cache, but the logits that it has by itself; those of positions that
-        the decoder does not have are NaN."""
+        the decoder does not have are NaN. So are those of tokens behind the last prompt; a prompt of which tokens are missing is not
+        served, and nor are those behind it."""
         self._needs_16bit_gpu("packed prompts")
         B, audio = xa.shape[:2]
         if tokens.dim() != 1 or tuple(new_lens.shape) != (B,) or tuple(slot_indices.shape) != (B,):
@@ -508,12 +509,15 @@ class TextDecoderStack(nn.Module):
             raise TypeError(f"xa must be {pool.dtype} and tokens whole numbers, got {xa.dtype} and {tokens.dtype}")
         new_lens = _check_ids("new_lens", new_lens, B, pool.device)
         streams = _check_ids("slot_indices", slot_indices, B, pool.device)
+        # a prompt of which tokens are missing counts as -1: it has none, and nor do those behind it
+        new_lens = new_lens.masked_fill(new_lens.clamp(min=0).cumsum(0) > tokens.shape[0], -1)
         pool.tables.truncate(0, streams)
         plan = pool.tables.plan(new_lens, tokens.shape[0], streams)
         # positions from the sums, not the plan's, which are 0 for a prompt that is not served
         cu, t = plan.cu_seqlens.long(), torch.arange(tokens.shape[0], device=plan.slots.device)
-        positions = t - cu[torch.bucketize(t, cu[1:], right=True)]
-        none = positions >= self.positional_embedding.shape[0]
+        prompt = torch.bucketize(t, cu[1:], right=True)
+        positions = t - cu[prompt]
+        none = (prompt == B) | (positions >= self.positional_embedding.shape[0])
         x = self.token_embedding(tokens) + self.positional_embedding[positions.masked_fill(none, 0)]
         x = x.masked_fill(none[:, None], float("nan"))[None]
         cu_audio = torch.arange(0, B * audio + 1, audio, dtype=torch.int32, device=xa.device)
