@@ -122,3 +122,25 @@ def test_lengths_that_do_not_match_the_tokens(cuda, stack, lens, told, served):
             assert close(logits[a : a + n], alone(cuda, stack, tokens[a : a + n], xa[i]))
         a += n
     assert logits[a:].isnan().all() and (plan.slots[a:] == -1).all()
+
+
+def test_steps_that_are_refused_change_nothing(cuda, stack):
+    """A step on caches that do not fit the decoder, or with streams that do not fit its rows, takes no place for its tokens."""
+    pages = pool(cuda)
+    tokens, new, xa = prompts(cuda, [20, 9], 4)
+    at = torch.tensor([1, 4], device=cuda)
+    stack.prefill_packed(tokens, new, xa, pages, at)
+    before = state(pages)
+    wide = TextDecoderStack(N_VOCAB, N_CTX, 2 * N_STATE, 2 * N_HEAD, N_LAYER).to(cuda, BF16)
+    half = TextDecoderStack(N_VOCAB, N_CTX, N_STATE, N_HEAD, N_LAYER).to(cuda, torch.float16)
+    two, pos = torch.zeros(2, 1, dtype=torch.long, device=cuda), torch.tensor([20, 9], device=cuda)
+    elsewhere = pool(cuda)
+    mixed = KVPagePool(N_LAYER, 6, 60, N_HEAD, 64, N_CTX, AUDIO, torch.float16, cuda)
+    for s, args, err in ((stack, (two, pages.self_kv[:1], pages.cross_kv, pos, at), ValueError), (stack, (two, pages.self_kv, pages.cross_kv[:1], pos, at), ValueError),
+                         (stack, (two, [pages.self_kv[0], elsewhere.self_kv[1]], pages.cross_kv, pos, at), ValueError),
+                         (stack, (two, pages.self_kv, mixed.cross_kv, pos, at), TypeError), (wide, (two, pages.self_kv, pages.cross_kv, pos, at), ValueError),
+                         (half, (two, pages.self_kv, pages.cross_kv, pos, at), TypeError), (stack, (two, pages.self_kv, pages.cross_kv, pos, at[:1]), ValueError),
+                         (stack, (two, pages.self_kv, pages.cross_kv, pos, torch.tensor([1, 4, 0], device=cuda)), ValueError)):
+        with pytest.raises(err):
+            s.forward_flash(*args)
+        assert all(torch.equal(a, b) for a, b in zip(before, state(pages)))

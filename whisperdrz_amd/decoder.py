@@ -381,15 +381,19 @@ class TextDecoderStack(nn.Module):
         them to the streams' lengths. A row whose stream is none (-1: a padded row) or gets no pages has NaN logits and
         changes nothing."""
         self._needs_16bit_gpu("paged caches")
+        self._check_pages(self_kv, cross_kv)
         tables = self_kv[0].page_tables
         B, seq_len = tokens.shape
+        if slot_indices is not None and tuple(slot_indices.shape) != (B,):
+            raise ValueError(f"slot_indices must be [{B}], got {tuple(slot_indices.shape)}")
         lens = tables.seq_lens.view(1, -1)
         if self._fused_prologue(tokens, positions, slot_indices, lens):
             x, h, streams, _ = step_begin(tokens, positions, self.token_embedding.weight, self.positional_embedding,
                                           self.blocks[0].attn_ln, slot_indices, lens)
         else:
             x = (self.token_embedding(tokens) + self.positional_embedding[positions]).contiguous()
-            h, streams = layer_norm(x, self.blocks[0].attn_ln), None if slot_indices is None else slot_indices.to(torch.int32)
+            h = layer_norm(x, self.blocks[0].attn_ln)
+            streams = None if slot_indices is None else _check_ids("slot_indices", slot_indices, B, x.device)
         if streams is None:
             streams = torch.arange(B, dtype=torch.int32, device=x.device)
         plan = tables.plan(seq_len, B * seq_len, streams)
