@@ -220,13 +220,15 @@ class FlashKVPages:
 class KVPagePool:
     """All layers' caches with the self-attention's in pages: the counterpart of ``KVSlotPool`` for streams of
     different lengths. ``tables`` is one :class:`PageTables` for all layers (a page holds its positions of every layer),
-    ``self_kv[l]`` a :class:`FlashKVPages`, ``cross_kv[l]`` a ``FlashKVCache`` of ``n_streams`` slots.
+    ``self_kv[l]`` a :class:`FlashKVPages`, ``cross_kv[l]`` a ``FlashKVCache`` of ``n_streams`` slots. Heads of 64.
 
     A step plans its tokens once for all layers (``TextDecoderStack.forward_flash`` does it); ``release`` ends streams.
     """
 
     def __init__(self, n_layers: int, n_streams: int, n_pages: int, n_heads: int = 20, head_dim: int = 64, self_len: int = 448,
                  cross_len: int = 1500, dtype: torch.dtype = torch.bfloat16, device=None, page_size: int = 16):
+        if head_dim != 64:  # FlashKVPages take 128, flash_attn_with_kvcache over the cross caches does not
+            raise NotImplementedError(f"head_dim {head_dim} is not supported (64)")
         self.n_layers, self.n_slots, self.n_pages = n_layers, n_streams, n_pages
         self.n_heads, self.head_dim, self.self_len, self.cross_len, self.dtype = n_heads, head_dim, self_len, cross_len, dtype
         self.tables = PageTables(n_streams, n_pages, page_size, self_len, device)
