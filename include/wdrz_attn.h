@@ -533,9 +533,10 @@ typedef struct wdrz_page_tables {
 /*
  * Gives B requests' new tokens their places, in place on the tables: request i adds new_lens[i] tokens
  * (NULL: new_all each) to stream streams[i] (NULL: stream i), taking the pages that it needs from the end of
- * free_pages, the first request first. Requests are served in order while pages last; one that needs more than
- * are left gets nothing, and neither does one that names no stream or one that an earlier request named, a
- * negative count, or more positions than max_seq: its stream stays as it was.
+ * free_pages, the first request first. Requests are served in order while pages last: behind the first that needs
+ * more than are left, none that needs pages gets any, whether or not its own would be there. A request that gets
+ * nothing leaves its stream as it was, and so does one that names no stream or one that an earlier request named,
+ * a negative count, or more positions than max_seq.
  * cu_seqlens: [B + 1] sums of the new tokens. starts: [B] positions before them, -1: got nothing.
  * slots, positions: int64 [total] of the packed tokens; -1 and 0 for those of a request that got nothing and
  * behind the last request. total: at least the sum of the new tokens (sums are cut off at it).

@@ -107,7 +107,8 @@ class PageTables:
         packed tokens, ``sum(new_lens)`` or more; it may be left out where ``new_lens`` is an int.
 
         A request that cannot be served whole changes nothing and has ``starts`` -1: no stream or one that an earlier
-        request named, more than ``max_seq_length`` positions, a negative count, or more pages than are left then.
+        request named, more than ``max_seq_length`` positions, a negative count, or too few pages. Nobody overtakes: behind the
+        first request that finds too few pages, all that need any have to wait, also where what is left would do.
         """
         lens, streams, B = self._requests("new_lens", new_lens, streams, None)
         if total is None:
