@@ -539,7 +539,7 @@ typedef struct wdrz_page_tables {
  * a negative count, or more positions than max_seq.
  * cu_seqlens: [B + 1] sums of the new tokens. starts: [B] positions before them, -1: got nothing.
  * slots, positions: int64 [total] of the packed tokens; -1 and 0 for those of a request that got nothing and
- * behind the last request. total: at least the sum of the new tokens (sums are cut off at it).
+ * behind the last request. total: at least the sum of the new tokens (sums are cut off at it, lengths are not).
  */
 int wdrz_page_plan(const wdrz_page_tables* pages, const int32_t* new_lens, int64_t new_all,
                    const int32_t* streams, int32_t* cu_seqlens, int32_t* starts, int64_t* slots,

@@ -210,6 +210,17 @@ int debug_check_pages_metadata(const wdrz_page_tables* p, const int32_t* seqlens
   return WDRZ_OK;
 }
 
+// A plan's counts: what the requests add has a place each.
+int debug_check_counts(const int32_t* new_lens, int64_t new_all, int64_t B, int64_t total) {
+  std::vector<int32_t> h(B, (int32_t)new_all);
+  if (new_lens && B && hipMemcpy(h.data(), new_lens, B * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess)
+    return fail(WDRZ_ELAUNCH, "debug check: reading the requests' counts failed");
+  int64_t sum = 0;
+  for (int32_t m : h) sum += std::max(m, 0);
+  if (sum > total) return fail(WDRZ_EINVAL, "debug check: the requests add %lld tokens, total is %lld", (long long)sum, (long long)total);
+  return WDRZ_OK;
+}
+
 // Slots of a write: inside the cache or negative, each named once.
 int debug_check_slots(const int64_t* slots, int64_t T, int64_t n) {
   std::vector<int64_t> h(T);
@@ -1151,6 +1162,9 @@ int wdrz_page_plan(const wdrz_page_tables* pages, const int32_t* new_lens, int64
   if (total > (1 << 28)) return fail(WDRZ_EUNSUPPORTED, "sizes too large");
   if (!cu_seqlens || (B > 0 && !starts) || (total > 0 && (!slots || !positions)))
     return fail(WDRZ_EINVAL, "cu_seqlens, starts, slots or positions is NULL");
+#ifdef WDRZ_DEBUG_CHECKS
+  if ((rc = debug_check_counts(new_lens, new_all, B, total))) return rc;
+#endif
   a.cu = cu_seqlens;
   a.starts = starts;
   a.slots = slots;

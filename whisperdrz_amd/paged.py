@@ -104,7 +104,8 @@ class PageTables:
     def plan(self, new_lens: Union[Tensor, int], total: Optional[int] = None, streams: Optional[Tensor] = None) -> PagePlan:
         """Gives request i's ``new_lens[i]`` tokens (one int: each as many) their places behind stream ``streams[i]``
         (``None``: stream i), in the order of the requests, and adds them to ``seq_lens``. ``total`` is the number of
-        packed tokens, ``sum(new_lens)`` or more; it may be left out where ``new_lens`` is an int.
+        packed tokens, ``sum(new_lens)`` or more (the sum stands on the device, and only ``WDRZ_DEBUG=1`` reads it: with less the
+        tokens behind have no slots, while their streams count them); it may be left out where ``new_lens`` is an int.
 
         A request that cannot be served whole changes nothing and has ``starts`` -1: no stream or one that an earlier
         request named, more than ``max_seq_length`` positions, a negative count, or too few pages. Nobody overtakes: behind the
@@ -115,6 +116,8 @@ class PageTables:
             if not isinstance(lens, int):
                 raise ValueError("total is required where new_lens is a tensor")
             total = B * lens
+        if total < 0 or (isinstance(lens, int) and total < B * lens):
+            raise ValueError(f"total {total} is less than the {B} requests' tokens")
         index = self.device.index
         if not self.tables.is_cuda:
             _check_cuda("the page tables", self.tables, self.device)
