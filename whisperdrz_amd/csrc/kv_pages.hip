@@ -33,6 +33,7 @@ namespace {
 
 constexpr int kRows = 16;           // (query, group head) rows a workgroup
 constexpr int kBlock = 32;          // positions a wavefront takes at a time
+constexpr int kLeast = 16;          // positions of the smallest page
 constexpr int kPagesMaxSplits = 64;  // workgroups that a row's keys are cut into at most
 // A row's reference lies 2^7 below its largest probability, so that the two fp16 operands hold small ones too (2^-32 of
 // the largest), and is moved where one exceeds it by 2^15: none leaves fp16.
@@ -371,7 +372,41 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void pages_attn_kerne
     if (nan) L = __builtin_nanf("");
     return o;
   };
-  auto put = [&](int r, int d, f32x4 o, float L) {
+  // An infinite value times a probability's two parts, of which the second may be 0 or of the other sign, has become NaN: dims
+  // d .. d + 3 of row r from the values that it sees, each of which has weight. NaN of the scores is in the row's sum as well.
+  auto infinite = [&](int r, int d, f32x4 o) __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");  // rare: stays a branch
+    const int seen = has_new ? n + (r0 + r) / a.G + 1 : n;
+    uint32_t kinds = 0;  // bits 8 e and on of dim d + e: inf, -inf, NaN
+#pragma unroll 1
+    for (int key0 = 0; key0 < seen; key0 += kLeast) {  // inside one page
+      const char* vp = a.v_pages + ((((int64_t)table[key0 >> a.shift] * a.Hk + hk) << a.shift) + (key0 & mask)) * kRow + d * 2;
+      u32x2 x[kLeast];
+#pragma unroll
+      for (int i = 0; i < kLeast; ++i) {
+        x[i] = u32x2{0, 0};
+        if (key0 + i < seen)
+          x[i] = *reinterpret_cast<const u32x2*>(key0 + i < n ? vp + i * kRow : vnew + (int64_t)(key0 + i - n) * a.vns[1] + d * 2);
+      }
+#pragma unroll
+      for (int i = 0; i < kLeast; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t u = x[i][e / 2] >> (16 * (e & 1)) & 0xffffu;
+          if ((u & Pg<T>::kExp) == Pg<T>::kExp) kinds |= ((u & 0x7fffu) > Pg<T>::kExp ? 4u : u >> 15 ? 2u : 1u) << (8 * e);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t is = kinds >> (8 * e) & 7u;
+      if (is == 1u) o[e] = INFINITY;
+      if (is == 2u) o[e] = -INFINITY;
+    }
+    return o;
+  };
+  auto put = [&](int r, int d, f32x4 o, float L) __attribute__((always_inline)) {
+    const float any = (o[0] + o[1]) + (o[2] + o[3]);
+    if (any != any && L == L) o = infinite(r, d, o);
     const float f = L == 0.f ? 0.f : 1.f / L;  // a row that sees nothing is 0
     *reinterpret_cast<u32x2*>(out_row(r) + d * 2) = u32x2{Pg<T>::pack(o[0] * f, o[1] * f), Pg<T>::pack(o[2] * f, o[3] * f)};
   };
