@@ -12,9 +12,8 @@
 // a lane are already the operand of the second product, and V^T is read from row-major V by transposing LDS reads. Work
 // items, the longest first, are found from the sums by every workgroup: the host does not know them.
 //
-// Softmax: p = 2^(c s - m) in fp32 with a reference m per query, taken from the first 32 keys and moved only where a
-// lane's 16 probabilities sum to more than 2^15: no maximum is taken otherwise. Every query that sees any key (of a
-// half) sees the first, so the first keys give a reference. Sums are of the fp32 probabilities. The products take them in the
+// Softmax: p = 2^(c s - m) in fp32 with a reference m per query, taken from the first 32 keys of which one has weight (a score
+// above -inf) and moved only where a lane's 16 probabilities sum to more than 2^15: no maximum is taken otherwise. Sums are of the fp32 probabilities. The products take them in the
 // operands' type, one rounding of half a step (2^-8 or 2^-11 of each; the attention over pages, whose matrix cores
 // idle, takes two operands): a second product would be half as many matrix instructions again.
 //
@@ -226,7 +225,7 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
   };
 
   f32x16 acc[DB];  // O^T: query l32, dim 32 db + 8 (x / 4) + 4 hl + x % 4
-  float m = 0.f, l = 0.f;
+  float m = -INFINITY, l = 0.f;  // reference (-inf: no key had weight yet), this lane's sum
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -294,15 +293,15 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
       }
       op_t p[2];
       float st;
-      auto exps = [&]() __attribute__((always_inline)) {
+      auto exps = [&](float ref) __attribute__((always_inline)) {
         float part[4];
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
           u32x4 w;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p0 = fast_exp2(__builtin_fmaf(sc[8 * ch + 2 * e], a.c, -m));
-            const float p1 = fast_exp2(__builtin_fmaf(sc[8 * ch + 2 * e + 1], a.c, -m));
+            const float p0 = fast_exp2(__builtin_fmaf(sc[8 * ch + 2 * e], a.c, -ref));
+            const float p1 = fast_exp2(__builtin_fmaf(sc[8 * ch + 2 * e + 1], a.c, -ref));
             w[e] = Pk<T>::pack(p0, p1);
             part[e] = ch == 0 ? p0 + p1 : part[e] + p0 + p1;
           }
@@ -311,24 +310,24 @@ __global__ __launch_bounds__(64 * NW, SIMD_WAVES) void packed_attn_kernel(Packed
         st = (part[0] + part[1]) + (part[2] + part[3]);
       };
       const bool first = s == half;
-      if (!first) exps();
-      if (first || __any(!(st <= kSumLimit))) {
+      if (!first) exps(m);
+      if (first || __any(!(st <= kSumLimit))) {  // without a reference st is infinite or NaN
         asm volatile("" ::: "memory");  // rare: stays a branch
         float mx = -INFINITY;
 #pragma unroll
         for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[x]);
         mx = halves_max(mx) * a.c;
-        const float to = first ? (mx == -INFINITY ? 0.f : mx - kBelow) : fmaxf(m, mx - kBelow);
-        const float f = fast_exp2(m - to);
-        m = to;
+        const float to = fmaxf(m, mx - kBelow);
         if (!first) {
+          const float f = to == m ? 1.f : fast_exp2(m - to);
           l *= f;
 #pragma unroll
           for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int x = 0; x < 16; ++x) acc[db][x] *= f;
         }
-        exps();
+        m = to;
+        exps(m == -INFINITY ? 0.f : m);
       }
       l += st;
       if (!AHEAD) read_v(s);
