@@ -157,7 +157,7 @@ __device__ __forceinline__ bool find_item(const PackedArgs& a, int rows, int& su
 // offset lies behind the resource. The compiler does not know of it: waits are written out below.
 __device__ __forceinline__ void load_lds(i32x4 from, uint32_t offset, uint32_t to) {
 #if __HIP_DEVICE_COMPILE__
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(to) : "m0", "memory");
 #else
   (void)from, (void)offset, (void)to;
 #endif
