@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -180,15 +181,23 @@ int debug_check_kv8_metadata(const int32_t* seqlens, const int32_t* bidx, bool h
   return WDRZ_OK;
 }
 
+// A check that wants more host memory than there is says so; no exception leaves a C entry.
+template <typename F> int with_memory(F check) {
+  try {
+    return check();
+  } catch (const std::bad_alloc&) {
+    return fail(WDRZ_ELAUNCH, "debug check: out of host memory");
+  }
+}
+
 // A call on the paged cache: streams, lengths and the pages that hold them; appending rows name a stream once.
 int debug_check_pages_metadata(const wdrz_page_tables* p, const int32_t* seqlens, const int32_t* streams, bool has_new,
                                int64_t B, int64_t sq) {
-  std::vector<int32_t> hs(B), hb(B), tables((size_t)p->n_streams * p->max_pages), first(p->n_streams, -1);
+  std::vector<int32_t> hs(B), hb(B), table, first(p->n_streams, -1);
   for (int64_t i = 0; i < B; ++i) hb[i] = (int32_t)i;
   if ((streams && hipMemcpy(hb.data(), streams, B * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess) ||
-      hipMemcpy(hs.data(), seqlens, B * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess ||
-      hipMemcpy(tables.data(), p->tables, tables.size() * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess)
-    return fail(WDRZ_ELAUNCH, "debug check: reading the rows' streams, lengths and tables failed");
+      hipMemcpy(hs.data(), seqlens, B * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess)
+    return fail(WDRZ_ELAUNCH, "debug check: reading the rows' streams and lengths failed");
   for (int64_t i = 0; i < B; ++i) {
     if (hb[i] < 0 || hb[i] >= p->n_streams)
       return fail(WDRZ_EINVAL, "debug check: row %lld names stream %d outside [0, %lld)", (long long)i, hb[i],
@@ -200,12 +209,13 @@ int debug_check_pages_metadata(const wdrz_page_tables* p, const int32_t* seqlens
     if (has_new && first[hb[i]] >= 0)
       return fail(WDRZ_EINVAL, "debug check: rows %d and %lld append to stream %d", first[hb[i]], (long long)i, hb[i]);
     first[hb[i]] = (int32_t)i;
-    for (int64_t j = 0; j * p->page_size < end; ++j) {
-      const int32_t page = tables[(size_t)hb[i] * p->max_pages + j];
-      if (page < 0 || page >= p->n_pages)
+    table.resize((end + p->page_size - 1) / p->page_size);
+    if (!table.empty() && hipMemcpy(table.data(), p->tables + hb[i] * p->max_pages, table.size() * sizeof(int32_t), hipMemcpyDeviceToHost) != hipSuccess)
+      return fail(WDRZ_ELAUNCH, "debug check: reading the table of stream %d failed", hb[i]);
+    for (size_t j = 0; j < table.size(); ++j)
+      if (table[j] < 0 || table[j] >= p->n_pages)
         return fail(WDRZ_EINVAL, "debug check: row %lld of stream %d: page %lld of its table is %d, outside [0, %lld)",
-                    (long long)i, hb[i], (long long)j, page, (long long)p->n_pages);
-    }
+                    (long long)i, hb[i], (long long)j, table[j], (long long)p->n_pages);
   }
   return WDRZ_OK;
 }
@@ -1163,7 +1173,7 @@ int wdrz_page_plan(const wdrz_page_tables* pages, const int32_t* new_lens, int64
   if (!cu_seqlens || (B > 0 && !starts) || (total > 0 && (!slots || !positions)))
     return fail(WDRZ_EINVAL, "cu_seqlens, starts, slots or positions is NULL");
 #ifdef WDRZ_DEBUG_CHECKS
-  if ((rc = debug_check_counts(new_lens, new_all, B, total))) return rc;
+  if ((rc = with_memory([&] { return debug_check_counts(new_lens, new_all, B, total); }))) return rc;
 #endif
   a.cu = cu_seqlens;
   a.starts = starts;
@@ -1227,7 +1237,7 @@ int wdrz_page_write(int dtype, const wdrz_kv_pages* cache, const void* k_src, co
   if (!slots) return fail(WDRZ_EINVAL, "slots is NULL");
   if ((rc = rows16_packed("k", k_src, k_strides, a.ks)) || (rc = rows16_packed("v", v_src, v_strides, a.vs))) return rc;
 #ifdef WDRZ_DEBUG_CHECKS
-  if ((rc = debug_check_slots(slots, T, cache->n_pages * cache->page_size))) return rc;
+  if ((rc = with_memory([&] { return debug_check_slots(slots, T, cache->n_pages * cache->page_size); }))) return rc;
 #endif
   a.k = static_cast<const char*>(k_src);
   a.v = static_cast<const char*>(v_src);
@@ -1274,7 +1284,7 @@ int wdrz_attn_kvpages(int dtype, const wdrz_kv_pages* cache, const wdrz_page_tab
   if ((rc = rows16("q", q, q_strides, a.qs)) || (rc = rows16("out", o, o_strides, a.os))) return rc;
   if (has_new && ((rc = rows16("k", k_new, kn_strides, a.kns)) || (rc = rows16("v", v_new, vn_strides, a.vns)))) return rc;
 #ifdef WDRZ_DEBUG_CHECKS
-  if ((rc = debug_check_pages_metadata(pages, cache_seqlens, cache_batch_idx, has_new, B, sq))) return rc;
+  if ((rc = with_memory([&] { return debug_check_pages_metadata(pages, cache_seqlens, cache_batch_idx, has_new, B, sq); }))) return rc;
 #endif
   a.q = static_cast<const char*>(q);
   a.k_pages = static_cast<char*>(cache->k_pages);
@@ -1332,7 +1342,11 @@ int wdrz_attn_packed(int dtype, const void* q, const int64_t* q_strides, const v
   if (grid_too_large(wdrz::packed_blocks(T, Tk, B, H, Hk, D), D == 64 ? 256 : 512) || (Tk > 0 && (a.ks[0] >= (1 << 25) || a.vs[0] >= (1 << 25) || a.ks[0] < 0 || a.vs[0] < 0)))
     return fail(WDRZ_EUNSUPPORTED, "sizes or strides too large");
 #ifdef WDRZ_DEBUG_CHECKS
-  if ((rc = debug_check_sums("cu_seqlens", cu_q, B, T)) || (cu_k && (rc = debug_check_sums("cu_seqlens_k", cu_k, B, Tk)))) return rc;
+  if ((rc = with_memory([&] {
+         const int bad = debug_check_sums("cu_seqlens", cu_q, B, T);
+         return bad || !cu_k ? bad : debug_check_sums("cu_seqlens_k", cu_k, B, Tk);
+       })))
+    return rc;
 #endif
   a.q = static_cast<const char*>(q);
   a.k = static_cast<const char*>(k);
