@@ -144,3 +144,23 @@ def test_steps_that_are_refused_change_nothing(cuda, stack):
         with pytest.raises(err):
             s.forward_flash(*args)
         assert all(torch.equal(a, b) for a, b in zip(before, state(pages)))
+
+
+@pytest.mark.parametrize("lens,n", [([0, 5, 0], 5), ([0, 0], 0), ([], 0), ([], 3)])
+def test_prompts_without_tokens(cuda, stack, lens, n):
+    """Their windows are kept, so that a first step gives what it gives after a prompt into slots; without streams nothing is."""
+    pages = pool(cuda)
+    tokens, new, xa = prompts(cuda, lens or [n], 6)
+    if not lens:
+        new, xa = new[:0], xa[:0]
+    at = torch.tensor([5, 2, 3][: len(lens)], dtype=torch.long, device=cuda)
+    logits, plan = stack.prefill_packed(tokens, new, xa, pages, at)
+    assert logits.shape == (n, N_VOCAB) and plan.starts.tolist() == [0] * len(lens)
+    assert bool(logits.isfinite().all()) if lens else bool(logits.isnan().all())
+    step = torch.randint(0, N_VOCAB, (len(lens), 1), device=cuda)
+    got = stack.forward_flash(step, pages.self_kv, pages.cross_kv, new, at)
+    assert got.shape == (len(lens), 1, N_VOCAB)
+    a = 0
+    for i, m in enumerate(lens):
+        assert close(got[i], alone(cuda, stack, torch.cat([tokens[a : a + m], step[i]]), xa[i])[-1:])
+        a += m

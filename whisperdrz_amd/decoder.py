@@ -92,11 +92,14 @@ class PackedCross:
     def __init__(self, attn: "MultiHeadAttention", xa: Tensor, cache: FlashKVCache, slots: Tensor, plan: PagePlan, cu_audio: Tensor):
         self.attn, self.xa, self.cache, self.slots, self.plan, self.cu_audio = attn, xa, cache, slots, plan, cu_audio
 
-    def attend(self, q: Tensor, k: None, v: None, scale: float) -> Tensor:
-        H, d = q.shape[1:]
-        kv = F.linear(self.xa, *self.attn.kv_weight()).view(*self.xa.shape[:2], 2, H, d)
+    def write(self) -> Tensor:
+        """Fills the slots; the rows ``[B * audio, 2, H, d]`` of keys and values."""
+        kv = F.linear(self.xa, *self.attn.kv_weight()).view(*self.xa.shape[:2], 2, self.cache.n_heads, self.cache.head_dim)
         self.cache.set_cross_attention(kv[:, :, 0], kv[:, :, 1], self.slots)
-        kv = kv.view(-1, 2, H, d)
+        return kv.flatten(0, 1)
+
+    def attend(self, q: Tensor, k: None, v: None, scale: float) -> Tensor:
+        kv = self.write()
         return packed_attention(q, kv[:, 0], kv[:, 1], self.plan.cu_seqlens, self.cu_audio, causal=False, scale=scale)
 
 
@@ -386,6 +389,8 @@ class TextDecoderStack(nn.Module):
         B, seq_len = tokens.shape
         if slot_indices is not None and tuple(slot_indices.shape) != (B,):
             raise ValueError(f"slot_indices must be [{B}], got {tuple(slot_indices.shape)}")
+        if tokens.numel() == 0:
+            return self.token_embedding.weight.new_empty(B, seq_len, self.token_embedding.num_embeddings)
         lens = tables.seq_lens.view(1, -1)
         if self._fused_prologue(tokens, positions, slot_indices, lens):
             x, h, streams, _ = step_begin(tokens, positions, self.token_embedding.weight, self.positional_embedding,
@@ -524,10 +529,14 @@ class TextDecoderStack(nn.Module):
         none = (prompt == B) | (positions >= self.positional_embedding.shape[0])
         x = self.token_embedding(tokens) + self.positional_embedding[positions.masked_fill(none, 0)]
         x = x.masked_fill(none[:, None], float("nan"))[None]
-        cu_audio = torch.arange(0, B * audio + 1, audio, dtype=torch.int32, device=xa.device)
+        cu_audio = audio * torch.arange(B + 1, dtype=torch.int32, device=xa.device)
         self_kv = [PackedSelf(c, plan) for c in pool.self_kv]
         slots = slot_indices.long().masked_fill(plan.starts < 0, -1)  # -1: to no slot
         cross_kv = [PackedCross(b.cross_attn, xa, c, slots, plan, cu_audio) for b, c in zip(self.blocks, pool.cross_kv, strict=True)]
+        if B == 0 or tokens.shape[0] == 0:  # no prompts, or windows alone
+            for c in cross_kv if B else ():
+                c.write()
+            return self.token_embedding.weight.new_full((tokens.shape[0], self.token_embedding.num_embeddings), float("nan")), plan
         h = self._fused_blocks(x, layer_norm(x, self.blocks[0].attn_ln), self_kv, cross_kv, None, [None] * len(self.blocks))
         return self._logits(h[0]), plan
 
