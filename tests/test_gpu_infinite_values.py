@@ -51,3 +51,23 @@ def test_infinite_values_that_are_seen(cuda, dtype, heads, group, dim, sq, appen
         vmax = float(V.float()[V.isfinite()].abs().max())
         tol = torch.finfo(dtype).eps / 2 * want.abs() + (2 * d + 2.0**-16) * vmax + 1e-7
         assert bool(((got[b].double() - want).abs() <= tol)[fine].all())
+
+
+@pytest.mark.parametrize("sq,max_len", [(1, 200), (1, 3000), (4, 200)])
+def test_infinite_values_of_the_call_itself(cuda, sq, max_len):
+    """An infinite value among the appended rows: its own query and those behind it have it, those before it do not."""
+    n, dim = max_len - sq, 64
+    g = torch.Generator().manual_seed(sq)
+    t = w.PageTables(1, -(-max_len // 16), 16, max_len, device=cuda)
+    cache = w.FlashKVPages(t, 2, dim, torch.bfloat16)
+    k, v = (torch.randn(n, 2, dim, generator=g).bfloat16() for _ in range(2))
+    cache.write(k.to(cuda), v.to(cuda), t.plan(n).slots)
+    q, kn, vn = (torch.randn(1, sq, 2, dim, generator=g).bfloat16() for _ in range(3))
+    vn[0, sq // 2, 0, 7], vn[0, sq - 1, 1, 0] = -INF, INF
+    start = t.plan(sq).starts
+    got = w.flash_attn_with_kvpages(q.to(cuda), cache, kn.to(cuda), vn.to(cuda), cache_seqlens=start).cpu()[0].double()
+    want, big = attention(q[0], torch.cat([k, kn[0]]), torch.cat([v, vn[0]]), [n + i + 1 for i in range(sq)], dim**-0.5)
+    fine = want.isfinite()
+    assert int((~fine).sum()) == sq - sq // 2 + 1 and torch.equal(got[~fine], want[~fine])
+    tol = 2.0**-8 * want.abs() + (2 * (dim + 4) * 2.0**-24 * dim**-0.5 * big + 2.0**-16) * float(v.float().abs().max() + 4) + 1e-7
+    assert bool(((got - want).abs() <= tol)[fine].all())
