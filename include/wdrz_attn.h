@@ -614,7 +614,7 @@ size_t wdrz_token_logprobs_workspace_size(int64_t rows, int64_t V, int64_t top);
  * probabilities, ties by the lower index. blocked: bool [rows, >= V] or NULL, tokens that count as -inf.
  * A token out of range has NaN. Rows without a token above -inf: log probability -inf, entropy 0. NaN or +inf
  * among a row's tokens: all NaN. Alternatives that do not exist have id -1 and -inf (NaN rows: NaN).
- * V up to 2^20, rows up to 2^24.
+ * V up to 2^20, rows below 2^24.
  */
 int wdrz_token_logprobs(int dtype, const void* logits, int64_t l_stride, const uint8_t* blocked, int64_t b_stride,
                         const int64_t* tokens, float* logprobs, float* entropy, float* top_logprobs,

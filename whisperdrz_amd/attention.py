@@ -500,7 +500,8 @@ def packed_attention(
     plan's ``cu_seqlens``) and, with ``cu_seqlens_k``, rows of the keys of its own. ``causal``: query t sees the keys
     ``j <= t + (keys - queries)`` of its sequence, the last query all of them; else every query sees all. A query that
     sees none gives zeros. Rows that no sequence holds are left as they are in ``out`` (a new one is not filled there).
-    Inference only.
+    Scores, softmax and sums are fp32; a probability is rounded once to q's type before it weighs a value (half a step, 2^-8 or 2^-11
+    of it), where :func:`flash_attn_with_kvpages` keeps what the rounding leaves. Inference only.
     """
     if not (isinstance(q, torch.Tensor) and q.is_cuda):
         _check_cuda("q", q, q.device if isinstance(q, torch.Tensor) else None)

@@ -17,8 +17,8 @@
 // A softmax reference is moved only when a score exceeds it by 2^15. The next block's keys are requested when this one's
 // have been used, its values when this one's have been: one block of registers, and loads under way at all times.
 // Bound: the bytes of keys and values, for short rows launch and the chain metadata -> table -> keys. One token, bf16,
-// in a graph: 52 streams of up to 448 positions, 20 heads of 64, 19.7 us (4.6 TB/s; a large copy reaches 5.2); 4 x 32768,
-// 32/8 heads of 128, 83 us (4.8 TB/s); one stream of 200 8 us, of which the launch and its host side are most.
+// in a graph: 52 streams of 224 to 448 positions, 20 heads of 64, 20 us (4.5 TB/s; a large copy reaches 5.2); 4 of 16384 to
+// 32768, 32/8 heads of 128, 83 us (4.8 TB/s); one stream of 200 8 us, of which the launch and its host side are most.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -496,13 +496,13 @@ void launch_d(const PagesArgs& a, hipStream_t stream) {
 // How many workgroups a row's keys are cut into (n_splits at most, each of min_chunk keys or more, even parts of the
 // row's own length) and the wavefronts of one. Joining costs about 2 us; a workgroup walks 1000 keys in 5 us. So rows are
 // cut until there is one workgroup a CU, and further only to hold the time of a long row among short ones. One token, bf16,
-// cold caches in a graph, us, unsplit / parts of 1024, 512, 256 keys:
-//   20 heads of 64: 1 stream of 447 positions 8.7 / - / - / 8.9 (two parts), 1000 12.8 / - / 11.2 / 9.4, 2000 20.8 / 15.1 /
-//   11.5 / 10.2; 8 of 4000 48.8 / 38.3 / 38.1 / 41.5 (two parts 37.9); 32 of 4000 124 / 121 / 124 / 131;
-//   32/8 heads of 128: 1 of 32000 390 / 34.3 / 39.7 / -; 4 of 32000 412 / 102 / 112 / - (eight parts 95); 16 of 2000 34.3 /
-//   29.9 / 29.7 / 33.3; 32 of 2000 49.8 / 52.5 / 55.2 / 61.0.
-// Wavefronts, us of 2 / 4 / 8: 160 workgroups 12.8 / 10.3 / 9.5, 260 12.3 / 11.1 / 13.6, 520 14.6 / 14.5 / 20.2, 800 17.6 /
-// 20.7 / 27.1, 1280 31.2 / 34.2 / 43.0.
+// cold caches in a graph, all rows of the same length, us, unsplit / parts of 1024, 512, 256 keys:
+//   20 heads of 64: 1 stream of 447 positions 8.8 / - / - / 9.5 (two parts), 1000 11.5 / - / 11.0 / 9.9, 2000 16.9 / 13.8 /
+//   11.5 / 10.7; 8 of 4000 35.2 / 38.6 / 37.1 / 40.2 (two parts, the rule's, 38.9); 32 of 4000 125 / 126 / 123 / 128;
+//   32/8 heads of 128: 1 of 32000 390 / 34.8 / 40.0 / -; 4 of 32000 412 / 102 / 109 / - (eight parts 95, 5.5 TB/s); 16 of 2000
+//   34.4 / 29.8 / 30.2 / 31.4; 32 of 2000 50.5 / 53.0 / 54.3 / 60.6.
+// Wavefronts, rows of 440, us of 2 / 4 / 8: 160 workgroups 13.2 / 10.6 / 10.1, 260 16.0 / 13.9 / 17.5, 520 18.4 / 18.7 / 25.4,
+// 800 23.7 / 26.7 / 33.9, 1280 33.0 / 35.1 / 44.4.
 constexpr int64_t kCus = 256;
 void pages_plan(int64_t B, int64_t sq, int64_t H, int64_t Hk, int64_t D, int64_t max_len, PagesArgs* a) {
   a->G = (int)(H / Hk);

@@ -14,11 +14,14 @@
 //
 // Softmax: p = 2^(c s - m) in fp32 with a reference m per query, taken from the first 32 keys of which one has weight (a score
 // above -inf) and moved only where a lane's 16 probabilities sum to more than 2^15: no maximum is taken otherwise. Sums are of the fp32 probabilities. The products take them in the
-// operands' type, one rounding of half a step (2^-8 or 2^-11 of each; the attention over pages, whose matrix cores
-// idle, takes two operands): a second product would be half as many matrix instructions again.
+// operands' type, one rounding of half a step (2^-8 or 2^-11 of each), as the encoder and long prompts into slots do; the
+// attention over pages and short prompts into slots, whose matrix cores idle, take two operands, the rounded value and what is
+// left. Results in bf16 are 0.0022 (relative, 2-norm) from 64 bits, those of a plain form in fp32, rounded once, 0.0016. Here
+// the second product and the remainders cost, us: 13 tokens 4.63 / 4.76, 1 x 128 over 1500 keys 19.0 / 22.1, the cases below 41 / 53 and
+// 700 / 948, 64 prompts with their writes 108 / 118.
 //
-// Bound: at 128 dims the matrix cores, at 64 the exponentials and what is around them (8 matrix instructions to 16
-// exponentials a lane and step, twice as many at 128), with few blocks the chain of a step. 2 x 8192 tokens of 32/8 heads of 128, causal: 680 .. 715 us, 1.0 PFLOP/s of the
+// Bound: at 128 dims the matrix cores, at 64 the exponentials, the operands' reads from LDS, of which each feeds one matrix
+// instruction of a wavefront's 32 queries (the encoder's form, with 64, has half as many), and with few blocks the chain of a step. 2 x 8192 tokens of 32/8 heads of 128, causal: 680 .. 715 us, 1.0 PFLOP/s of the
 // 1.39 that a library product of 8192^3 reaches; 16 prompts over 1500 keys of 20 heads of 64: 41 us, 390 TFLOP/s.
 // Measured, us, at 64 dims (long batch with its write / cross) and 128:
 //   4 wavefronts, 3 buffers, 3 a SIMD     110 / 41.6    the form taken: other wavefronts of the SIMD fill the softmax's time
@@ -127,7 +130,8 @@ __device__ __forceinline__ Item pick_item(const PackedArgs& a, const Chunk& c, i
 // This workgroup's item, and its group of heads in `sub`; false where it has none. Items of a group of heads are next to
 // each other, on one XCD: those of a sequence read the same keys. The host launches as many workgroups as there may be
 // items; where one chunk holds all sequences their number is known, the first workgroups take them and the CUs get
-// equally many (64 prompts with their writes 109.5 us with the others in between, 108.4 so).
+// equally many. 20 heads of 64, us, with the empty ones in between / so: 64 prompts of 448 tokens 103 / 100, of 30 12.4 / 11.0;
+// 64 tokens over 1500 keys each, 8 prompts 28.4 / 21.3, 16 42.7 / 34.8.
 __device__ __forceinline__ bool find_item(const PackedArgs& a, int rows, int& sub, Item& it) {
   const int n_wg = (int)gridDim.x, groups = a.H / a.nh;
   Chunk c = scan_items(a, rows, 0);

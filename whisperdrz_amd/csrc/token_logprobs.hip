@@ -18,7 +18,8 @@
 // Bound: VALU issue, 17 instructions a token (two of them the exponential's, five the largest term's, which some lane of a
 // wavefront moves at most loads), near the bytes of the logits; for few rows launch, two trips to memory and a handful of
 // barriers. 3584 x 51866 bf16 with 3 alternatives 85 us, 4.4 TB/s (a copy 5.2; 93 us with the masks' instructions where
-// there is no mask); one row of 51866 fp32 in 26 workgroups 11.4 us. 3 or 8 loads in flight a thread 84 and 87 us.
+// there is no mask; logits without a likely token, whose largest moves more often, 102, with a mask 120); one row of 51866
+// fp32 in 26 workgroups 11.4 us. 3 or 8 loads in flight a thread 84 and 87 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -39,7 +40,7 @@ constexpr int kMaxTop = 32;
 constexpr int kMaxSplits = 32;
 constexpr int kList = kThreads * kVec + kVec + kMaxTop;  // tokens listed at most, with those of the round before
 constexpr float kFar = -200.f;    // e^-200 is 0 in fp32, and so are the terms of all logits further down
-constexpr int kCounters = 4096;   // of rows that are split (1024 at most), before their partials
+constexpr int kCounters = 4096;   // of rows that are split (512 at most, each over two workgroups or more), before their partials
 
 // Order of fp32 values as unsigned numbers, above 0 for what can be chosen (-inf cannot).
 __device__ __forceinline__ uint32_t order(float x) {

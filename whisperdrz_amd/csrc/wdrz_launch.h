@@ -347,8 +347,8 @@ struct LogprobArgs {
   int64_t l_stride;
   const uint8_t* blocked;  // bool [rows, V] or nullptr
   int64_t m_stride;
-  const int64_t* tokens;  // [rows] or nullptr
-  float* logprob;         // [rows] or nullptr with tokens
+  const int64_t* tokens;  // [rows]
+  float* logprob;         // [rows]
   float* entropy;         // [rows]
   float* top_logprob;     // [rows, top]
   int64_t* top_id;
