@@ -372,50 +372,59 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void pages_attn_kerne
     if (nan) L = __builtin_nanf("");
     return o;
   };
-  // An infinite value times a probability's two parts, of which the second may be 0 or of the other sign, has become NaN: dims
-  // d .. d + 3 of row r from the values that it sees, each of which has weight. NaN of the scores is in the row's sum as well.
-  auto infinite = [&](int r, int d, f32x4 o) __attribute__((always_inline)) {
-    asm volatile("" ::: "memory");  // rare: stays a branch
-    const int seen = has_new ? n + (r0 + r) / a.G + 1 : n;
-    uint32_t kinds = 0;  // bits 8 e and on of dim d + e: inf, -inf, NaN
+  int odd = 0;  // bit u: this thread's u-th dims have NaN that their row's sum has not
+  auto put = [&](int i, f32x4 o, float L) __attribute__((always_inline)) {
+    const float any = (o[0] + o[1]) + (o[2] + o[3]);
+    odd |= any != any && L == L ? 1 << i / kThreads : 0;
+    const float f = L == 0.f ? 0.f : 1.f / L;  // a row that sees nothing is 0
+    *reinterpret_cast<u32x2*>(out_row(i / (D / 4)) + i % (D / 4) * 8) =
+        u32x2{Pg<T>::pack(o[0] * f, o[1] * f), Pg<T>::pack(o[2] * f, o[3] * f)};
+  };
+  // An infinite value times a probability's two parts, of which the second may be 0 or of the other sign, has become NaN: such
+  // dims again, from the values that their row sees, each of which has weight.
+  auto infinite = [&]() __attribute__((always_inline)) {
+    for (; odd; odd &= odd - 1) {
+      // the arguments anew, so that the loop above holds none of them for this
+      typedef const __attribute__((address_space(4))) PagesArgs* args_t;
+      args_t ap = (args_t)__builtin_amdgcn_kernarg_segment_ptr();
+      asm volatile("" : "+s"(ap));
+      const int n0 = ap->seqlens[b], stream0 = ap->streams ? ap->streams[b] : b, shift = ap->shift;
+      const int32_t* table0 = ap->tables + (int64_t)stream0 * ap->max_pages;
+      const int i = tid + (__ffs(odd) - 1) * kThreads, r = i / (D / 4), d = i % (D / 4) * 4;
+      const char* vn = ap->kn ? ap->vn + (int64_t)b * ap->vns[0] + (int64_t)hk * ap->vns[2] + d * 2 : nullptr;
+      const int seen = ap->kn ? n0 + (r0 + r) / ap->G + 1 : n0;
+      uint32_t kinds = 0;  // bits 8 e and on of dim d + e: inf, -inf, NaN
 #pragma unroll 1
-    for (int key0 = 0; key0 < seen; key0 += kLeast) {  // inside one page
-      const char* vp = a.v_pages + ((((int64_t)table[key0 >> a.shift] * a.Hk + hk) << a.shift) + (key0 & mask)) * kRow + d * 2;
-      u32x2 x[kLeast];
+      for (int key0 = 0; key0 < seen; key0 += kLeast) {  // inside one page
+        const char* vp = ap->v_pages + ((((int64_t)table0[key0 >> shift] * ap->Hk + hk) << shift) + (key0 & ((1 << shift) - 1))) * kRow + d * 2;
+        u32x2 x[kLeast];
 #pragma unroll
-      for (int i = 0; i < kLeast; ++i) {
-        x[i] = u32x2{0, 0};
-        if (key0 + i < seen)
-          x[i] = *reinterpret_cast<const u32x2*>(key0 + i < n ? vp + i * kRow : vnew + (int64_t)(key0 + i - n) * a.vns[1] + d * 2);
+        for (int u = 0; u < kLeast; ++u) {
+          x[u] = u32x2{0, 0};
+          if (key0 + u < seen) x[u] = *reinterpret_cast<const u32x2*>(key0 + u < n0 ? vp + u * kRow : vn + (int64_t)(key0 + u - n0) * ap->vns[1]);
+        }
+#pragma unroll
+        for (int u = 0; u < kLeast; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t v = x[u][e / 2] >> (16 * (e & 1)) & 0xffffu;
+            if ((v & Pg<T>::kExp) == Pg<T>::kExp) kinds |= ((v & 0x7fffu) > Pg<T>::kExp ? 4u : v >> 15 ? 2u : 1u) << (8 * e);
+          }
       }
 #pragma unroll
-      for (int i = 0; i < kLeast; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t u = x[i][e / 2] >> (16 * (e & 1)) & 0xffffu;
-          if ((u & Pg<T>::kExp) == Pg<T>::kExp) kinds |= ((u & 0x7fffu) > Pg<T>::kExp ? 4u : u >> 15 ? 2u : 1u) << (8 * e);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t is = kinds >> (8 * e) & 7u;
+        if (is == 1u || is == 2u) *reinterpret_cast<uint16_t*>(out_row(r) + (d + e) * 2) = (uint16_t)(Pg<T>::kExp | (is == 2u ? 0x8000u : 0u));
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t is = kinds >> (8 * e) & 7u;
-      if (is == 1u) o[e] = INFINITY;
-      if (is == 2u) o[e] = -INFINITY;
-    }
-    return o;
-  };
-  auto put = [&](int r, int d, f32x4 o, float L) __attribute__((always_inline)) {
-    const float any = (o[0] + o[1]) + (o[2] + o[3]);
-    if (any != any && L == L) o = infinite(r, d, o);
-    const float f = L == 0.f ? 0.f : 1.f / L;  // a row that sees nothing is 0
-    *reinterpret_cast<u32x2*>(out_row(r) + d * 2) = u32x2{Pg<T>::pack(o[0] * f, o[1] * f), Pg<T>::pack(o[2] * f, o[3] * f)};
   };
   if (n_split_b == 1) {
     for (int i = tid; i < rows * (D / 4); i += kThreads) {
       float M, L;
       const f32x4 o = joined(i / (D / 4), i % (D / 4) * 4, M, L);
-      put(i / (D / 4), i % (D / 4) * 4, o, L);
+      put(i, o, L);
     }
+    infinite();
     return;
   }
   // ---- several workgroups a row: each publishes its sums, the last to arrive joins them ----
@@ -472,8 +481,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void pages_attn_kerne
           o += x[u] * f;
         }
     }
-    put(r, d, o, L);
+    put(i, o, L);
   }
+  infinite();
   if (tid == 0) __hip_atomic_store(a.ws_count + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
 }
 
