@@ -164,3 +164,15 @@ def test_prompts_without_tokens(cuda, stack, lens, n):
     for i, m in enumerate(lens):
         assert close(got[i], alone(cuda, stack, torch.cat([tokens[a : a + m], step[i]]), xa[i])[-1:])
         a += m
+
+
+def test_tokens_of_32_bits_and_other_tables(cuda, stack):
+    """Tokens and a decoder that the fused first operation does not take have the same logits."""
+    lens, named, told = [16, 33, 17, 5], [0, 1, 1, 6], [16, 33, 17, 3]
+    tokens, new, xa = prompts(cuda, lens, 7)
+    new = torch.tensor(told, device=cuda)
+    at = torch.tensor(named, device=cuda)
+    want, plan = stack.prefill_packed(tokens, new, xa, pool(cuda), at)
+    got, other = stack.prefill_packed(tokens.int(), new.short(), xa, pool(cuda), at.int())
+    assert torch.equal(got.isnan(), want.isnan()) and bool(want[:-2].isfinite().all()) and bool(want[-2:].isnan().all())
+    assert close(got[:-2], want[:-2]) and all(torch.equal(a, b) for a, b in zip(plan, other))

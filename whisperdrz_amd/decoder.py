@@ -518,26 +518,31 @@ class TextDecoderStack(nn.Module):
             raise TypeError(f"xa must be {pool.dtype} and tokens whole numbers, got {xa.dtype} and {tokens.dtype}")
         new_lens = _check_ids("new_lens", new_lens, B, pool.device)
         streams = _check_ids("slot_indices", slot_indices, B, pool.device)
+        cu_audio = torch.arange(0, B * audio + 1, audio, dtype=torch.int32, device=xa.device)
         # a prompt of which tokens are missing counts as -1: it has none, and nor do those behind it
         new_lens = new_lens.masked_fill(new_lens.clamp(min=0).cumsum(0) > tokens.shape[0], -1)
         pool.tables.truncate(0, streams)
         plan = pool.tables.plan(new_lens, tokens.shape[0], streams)
-        # positions from the sums, not the plan's, which are 0 for a prompt that is not served
-        cu, t = plan.cu_seqlens.long(), torch.arange(tokens.shape[0], device=plan.slots.device)
-        prompt = torch.bucketize(t, cu[1:], right=True)
-        positions = t - cu[prompt]
-        none = (prompt == B) | (positions >= self.positional_embedding.shape[0])
-        x = self.token_embedding(tokens) + self.positional_embedding[positions.masked_fill(none, 0)]
-        x = x.masked_fill(none[:, None], float("nan"))[None]
-        cu_audio = audio * torch.arange(B + 1, dtype=torch.int32, device=xa.device)
+        # positions from the sums, not the plan's, which are 0 for a prompt that is not served; n_ctx and on behind the last
+        n_ctx, t = self.positional_embedding.shape[0], torch.arange(tokens.shape[0], device=xa.device)
+        begin = F.pad(plan.cu_seqlens[:-1], (0, 1), value=-n_ctx)
+        positions = t - begin[torch.bucketize(t, plan.cu_seqlens[1:], right=True)]
+        lens = pool.tables.seq_lens.view(1, -1)
+        if tokens.shape[0] <= 1 << 20 and self._fused_prologue(tokens[None], positions[None], None, lens):  # NaN from n_ctx on
+            x, h, _, _ = step_begin(tokens[None], positions[None], self.token_embedding.weight, self.positional_embedding,
+                                    self.blocks[0].attn_ln, None, lens)
+        else:
+            x = self.token_embedding(tokens) + self.positional_embedding[positions.clamp(max=n_ctx - 1)]
+            x = x.masked_fill((positions >= n_ctx)[:, None], float("nan"))[None]
+            h = layer_norm(x, self.blocks[0].attn_ln) if tokens.shape[0] else x
         self_kv = [PackedSelf(c, plan) for c in pool.self_kv]
-        slots = slot_indices.long().masked_fill(plan.starts < 0, -1)  # -1: to no slot
+        slots = torch.where(plan.starts < 0, -1, slot_indices)  # -1: to no slot
         cross_kv = [PackedCross(b.cross_attn, xa, c, slots, plan, cu_audio) for b, c in zip(self.blocks, pool.cross_kv, strict=True)]
         if B == 0 or tokens.shape[0] == 0:  # no prompts, or windows alone
             for c in cross_kv if B else ():
                 c.write()
             return self.token_embedding.weight.new_full((tokens.shape[0], self.token_embedding.num_embeddings), float("nan")), plan
-        h = self._fused_blocks(x, layer_norm(x, self.blocks[0].attn_ln), self_kv, cross_kv, None, [None] * len(self.blocks))
+        h = self._fused_blocks(x, h, self_kv, cross_kv, None, [None] * len(self.blocks))
         return self._logits(h[0]), plan
 
 
