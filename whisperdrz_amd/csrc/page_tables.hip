@@ -7,8 +7,9 @@
 //     need_i = max(0, ceil((lens + m_i) / P) - counts),   off_i = need_0 + .. + need_(i-1)
 // more pages, and gets the stack's entries n_free - 1 - off_i, n_free - 2 - off_i, ..; token t of it stands at
 // position lens + t, slot tables[s][position / P] * P + position % P. Requests are served in their order while
-// pages last: one whose off_i + need_i is above n_free gets nothing, and nor does one that names no stream, a
-// stream that an earlier one named, or a length that the table cannot hold.
+// pages last: one whose off_i + need_i is above n_free gets nothing, which then holds for all behind it that need pages (the
+// sums depend on no answer, and nobody overtakes a long prompt); nor does one that names no stream, a stream that an
+// earlier one named, or a length that the table cannot hold.
 //
 // Bound: launch and a chain of four dependent trips to memory (stream -> its length -> the stack -> the table).
 // One workgroup does the scan, since every request's pages depend on all before it. Plan and truncation of 8 streams 3.5 and
